@@ -233,6 +233,154 @@ typedef struct qsa_b200_topk_args {
  * Needs 4-byte aligned scores, lengths and out. Asynchronous on `stream`. */
 QSA_B200_API int qsa_b200_topk_select(const qsa_b200_topk_args* args, qsa_b200_stream_t stream);
 
+/* ---- The block-scaled cache ----------------------------------------------
+ * Paged E4M3FN caches [num_pages, P, Hkv, 128] with one fp32 scale for each
+ * block of `block_size` consecutive tokens of a page and each KV head:
+ *   stored value = code * scales[page, (t % P) / block_size, g],
+ * scales fp32 [num_pages, P / block_size, Hkv] for K and for V. block_size
+ * divides P; block_size 1 is a scale for every token, P one for every page.
+ * Three entry points serve one attention layer over it: qsa_b200_qk_rope (the
+ * queries), qsa_b200_block_append (new keys and values) and
+ * qsa_b200_block_decode. None has a counterpart in the reference, whose
+ * caches have one scale each (sm89_cutedsl.py:48-62, :79). */
+
+/* Position rotation of a 128-element head. The first rotary_dim elements form
+ * rotary_dim / 2 pairs: pair j is elements (j, j + rotary_dim / 2), or with
+ * `interleaved` (2j, 2j + 1). Pair (a, b) becomes (a c - b s, b c + a s) with
+ * c = table[p * rotary_dim + j], s = table[p * rotary_dim + rotary_dim / 2 + j].
+ * p is the token's position on pair j's axis: the first sections[0] pairs go by
+ * axis 0, the next sections[1] by axis 1, and so on. */
+#define QSA_B200_ROPE_MAX_AXES 4
+typedef struct qsa_b200_rotation {
+  const float* table;       /* fp32 [table_len, rotary_dim]: cosines, then sines; NULL = no rotation */
+  const int32_t* positions; /* [num_axes, tokens], rows axis_stride apart */
+  int64_t axis_stride;      /* elements from one axis to the next, >= tokens with several axes */
+  int32_t table_len;        /* a token with a position outside [0, table_len) gets a row of zeros */
+  int32_t rotary_dim;       /* a multiple of 16 up to 128 */
+  int32_t interleaved;
+  int32_t num_axes;         /* 1 .. QSA_B200_ROPE_MAX_AXES */
+  int32_t sections[QSA_B200_ROPE_MAX_AXES]; /* pairs of each axis, sum rotary_dim / 2 (not read with one axis) */
+} qsa_b200_rotation;
+
+typedef struct qsa_b200_qk_rope_args {
+  const void* q;        /* [tokens, num_q_heads, head_dim] of dtype, heads contiguous */
+  const void* k;        /* optional [tokens, num_kv_heads, head_dim] */
+  void* q_out;          /* shaped like q; may be q itself */
+  void* k_out;          /* shaped like k; may be k itself */
+  const void* q_weight; /* optional [head_dim] of weight_dtype: RMS norm of each query head */
+  const void* k_weight; /* optional [head_dim]: the same for each key head */
+  float eps;            /* >= 0, added to the mean square */
+  int32_t tokens;
+  int32_t num_q_heads;
+  int32_t num_kv_heads; /* 0 without k */
+  int32_t head_dim;     /* must be 128 */
+  int64_t q_stride;     /* elements from one token to the next */
+  int64_t k_stride;
+  int64_t q_out_stride;
+  int64_t k_out_stride;
+  int32_t dtype;        /* QSA_B200_DTYPE_* of q, k and the outputs */
+  int32_t weight_dtype; /* QSA_B200_DTYPE_* of the weights */
+  qsa_b200_rotation rope;
+} qsa_b200_qk_rope_args;
+
+/* RMS norm of every query and key head and the position rotation, in one pass:
+ *   y = x * rsqrt(mean(x^2) + eps) * weight (where a weight is given), rotated,
+ * in fp32 and rounded once to dtype. The outputs may be the inputs (same
+ * pointer and stride); they must not overlap otherwise. Needs 16-byte aligned
+ * tensors with token strides a multiple of 16 bytes, and a 16-byte aligned
+ * table. Asynchronous on `stream`. */
+QSA_B200_API int qsa_b200_qk_rope(const qsa_b200_qk_rope_args* args, qsa_b200_stream_t stream);
+
+typedef struct qsa_b200_block_append_args {
+  const void* k;            /* new keys [tokens, num_kv_heads, head_dim] of input_dtype, heads contiguous */
+  const void* v;            /* new values, same shape, type and strides as k */
+  void* k_cache;            /* fp8 e4m3fn [num_pages, page_size, num_kv_heads, head_dim] */
+  void* v_cache;
+  float* k_scales;          /* fp32 [num_pages, page_size / block_size, num_kv_heads] */
+  float* v_scales;
+  const int32_t* btable;    /* [num_reqs, btable_stride]; first pages_per_req columns = physical pages */
+  const int32_t* reqs;      /* optional [entries]: block-table row of each entry (NULL = identity) */
+  const int32_t* starts;    /* [entries]: logical position of the entry's first new token */
+  const int32_t* cu_tokens; /* optional [entries + 1]: entry e has the tokens cu_tokens[e] .. cu_tokens[e + 1] - 1;
+                               NULL: one token each (tokens == entries) */
+  const void* k_weight;     /* optional [head_dim] of weight_dtype: RMS norm of each key head */
+  float eps;
+  int32_t entries;
+  int32_t tokens;
+  int32_t num_kv_heads;
+  int32_t head_dim;         /* must be 128 */
+  int32_t page_size;
+  int32_t block_size;       /* divides page_size */
+  int32_t pages_per_req;
+  int32_t num_reqs;
+  int64_t num_pages;
+  int64_t btable_stride;
+  int64_t token_stride;     /* elements from one token of k / v to the next */
+  int32_t input_dtype;      /* QSA_B200_DTYPE_* */
+  int32_t weight_dtype;
+  qsa_b200_rotation rope;   /* of the keys; positions NULL = the tokens' logical positions (one axis) */
+} qsa_b200_block_append_args;
+
+/* Appends new keys (normed and rotated on the way, in fp32) and values to the
+ * block-scaled caches. Entry e's tokens go to the logical positions starts[e],
+ * starts[e] + 1, ... of its request. For each block and head that gets a token:
+ *   s = max(s_old, max |x| / 448, 2^-126) over the block's new rows x, with
+ *       s_old the block's scale where it keeps tokens before starts[e], else 0;
+ *   each new row is stored as e4m3fn(x / s), each kept row as
+ *   e4m3fn(code * (s_old / s)); ties to even, saturating at +-448.
+ * Rows at and after the last new token stay as they were. Infinities count
+ * for no maximum and are stored as +-448; NaN stays NaN. Tokens whose page
+ * lies outside the table or the cache are skipped, as are entries with a
+ * negative start or a reqs entry out of range. Two entries that write to one
+ * block race: a page that gets tokens belongs to one request, and a request
+ * comes once in a call. Needs 16-byte aligned k, v, caches and table, token
+ * strides a multiple of 16 bytes. Asynchronous on `stream`. */
+QSA_B200_API int qsa_b200_block_append(const qsa_b200_block_append_args* args, qsa_b200_stream_t stream);
+
+typedef struct qsa_b200_block_decode_args {
+  const void* q;          /* bf16 [rows, num_q_heads, head_dim], contiguous */
+  const void* k_cache;    /* fp8 e4m3fn [num_pages, page_size, num_kv_heads, head_dim] */
+  const void* v_cache;
+  const float* k_scales;  /* fp32 [num_pages, page_size / block_size, num_kv_heads] */
+  const float* v_scales;
+  const int32_t* indices; /* [rows, indices_stride], first `topk` columns = logical tokens, <0 = masked;
+                             NULL = every token in order (topk is then pages_per_req * page_size) */
+  const int32_t* counts;  /* optional [rows]: only the first counts[r] columns may be valid */
+  const int32_t* btable;  /* [num_reqs, btable_stride] */
+  const int32_t* t2r;     /* optional [rows]: row -> block-table row (NULL = identity) */
+  const void* gate;       /* optional bf16 [rows, num_q_heads, head_dim]: out is multiplied by sigmoid(gate) */
+  void* out;              /* bf16 [rows, num_q_heads, head_dim] */
+  float softmax_scale;
+  int32_t rows;
+  int32_t num_q_heads;
+  int32_t num_kv_heads;
+  int32_t head_dim;       /* must be 128 */
+  int32_t page_size;
+  int32_t block_size;     /* divides page_size */
+  int32_t pages_per_req;
+  int32_t num_reqs;
+  int64_t num_pages;      /* num_pages * page_size <= 2^31 - 1 */
+  int32_t topk;           /* not read without indices */
+  int64_t indices_stride;
+  int64_t btable_stride;
+} qsa_b200_block_decode_args;
+
+/* Bytes of device workspace qsa_b200_block_decode needs (256-byte aligned;
+ * split partial results), negative on invalid arguments. */
+QSA_B200_API int64_t qsa_b200_block_decode_workspace_bytes(const qsa_b200_block_decode_args* args);
+
+/* Attention over the block-scaled caches, for row r and query head h of KV
+ * head g = h / (num_q_heads / num_kv_heads), groups of 1 to 32:
+ *   out[r,h] = softmax_t(q[r,h] . K[t,g] ks[t,g] softmax_scale) . V[t,g] vs[t,g]
+ *              (*) sigmoid(gate[r,h])
+ * with the masks of qsa_b200_decode: entries that are negative, past the
+ * count, past the block table or on a page outside the cache do not count,
+ * and what lies in the cache there (NaN too) is not read. A row without a
+ * valid entry gives zeros. The workspace needs no clearing and may be reused
+ * by the next call on the same stream. Asynchronous on `stream`. */
+QSA_B200_API int qsa_b200_block_decode(const qsa_b200_block_decode_args* args, void* workspace, size_t workspace_bytes,
+                                       qsa_b200_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

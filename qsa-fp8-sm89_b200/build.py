@@ -36,8 +36,9 @@ NVCC_FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC,-fvisibilit
               "-Xptxas", "-warn-spills"] + ARCH
 
 CU_SOURCES = ["qsa_capi.cu", "qsa_decode_tc.cu", "qsa_decode_simt.cu", "qsa_noalloc.cu", "qsa_cache_write.cu",
-              "qsa_topk.cu"]
-HEADERS = ["qsa_common.cuh", "qsa_internal.h"]
+              "qsa_topk.cu", "qsa_block_capi.cu", "qsa_qk_rope.cu", "qsa_block_append.cu", "qsa_block_decode.cu"]
+HEADERS = ["qsa_common.cuh", "qsa_internal.h", "qsa_rope.cuh"]
+TORCH_SOURCES = ["qsa_torch_ext.cpp", "qsa_torch_block.cpp"]
 
 LIB = PKG / "libqsa_b200.so"
 TORCH_EXT = PKG / "_qsa_b200_torch.so"
@@ -84,14 +85,14 @@ def _torch_flags():
 
 
 def build_torch_ext(force=False, verbose=False) -> Path:
-    src = CSRC / "qsa_torch_ext.cpp"
-    if not (force or _stale(TORCH_EXT, [src, INCLUDE / "qsa_b200.h", LIB, Path(__file__)])):
+    srcs = [CSRC / s for s in TORCH_SOURCES]
+    if not (force or _stale(TORCH_EXT, [*srcs, INCLUDE / "qsa_b200.h", LIB, Path(__file__)])):
         return TORCH_EXT
     inc, libdir, abi = _torch_flags()
     tmp = BUILD / TORCH_EXT.name
     cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
            *[f"-I{p}" for p in inc], f"-I{CUDA_HOME}/include", f"-I{INCLUDE}",
-           src, "-o", tmp,
+           *srcs, "-o", tmp,
            f"-L{libdir}", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch",
            f"-L{PKG}", "-lqsa_b200",
            f"-Wl,-rpath,{libdir}", "-Wl,-rpath,$ORIGIN"]

@@ -184,6 +184,9 @@ WorkspaceLayout workspace_for(const DecodeParams& p, bool tc) {
 }
 
 }  // namespace
+
+int device_status() { return check_device(); }
+
 }  // namespace qsa
 
 using namespace qsa;

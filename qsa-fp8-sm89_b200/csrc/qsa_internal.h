@@ -113,6 +113,85 @@ struct TopkParams {
 };
 cudaError_t launch_topk(const TopkParams& p, cudaStream_t stream);
 
+// The block-scaled cache: head norm with rotation (qsa_qk_rope.cu), paged
+// append (qsa_block_append.cu) and attention (qsa_block_decode.cu).
+constexpr int kRopeMaxAxes = 4;
+struct RopeParams {
+  const float* table;        // [table_len, rotary] cosines, then sines; null = no rotation
+  const int32_t* positions;  // [axes, tokens]; null = the caller's own position (append)
+  int64_t axis_stride;
+  int table_len;
+  int rotary;  // multiple of 16, <= 128
+  int interleaved;
+  int axes;
+  int ends[kRopeMaxAxes];  // first pair past each axis' section
+  int quads;               // every section is a multiple of 4 pairs
+};
+
+struct QkRopeParams {
+  const void* x[2];  // q, k
+  void* out[2];
+  const void* weight[2];  // may be null
+  int64_t stride[2], out_stride[2];
+  int heads[2];
+  float eps;
+  int tokens;
+  int dtype, weight_dtype;
+  RopeParams rope;
+};
+cudaError_t launch_qk_rope(const QkRopeParams& p, cudaStream_t stream);
+
+struct BlockAppendParams {
+  const void* k;
+  const void* v;
+  uint8_t* k_cache;
+  uint8_t* v_cache;
+  float* k_scales;
+  float* v_scales;
+  const int32_t* btable;
+  const int32_t* reqs;
+  const int32_t* starts;
+  const int32_t* cu_tokens;
+  const void* k_weight;
+  float eps;
+  int entries, tokens, num_kv_heads;
+  int page_size, block_size, pages_per_req, num_reqs;
+  int64_t num_pages, btable_stride, token_stride;
+  int dtype, weight_dtype;
+  RopeParams rope;
+};
+cudaError_t launch_block_append(const BlockAppendParams& p, cudaStream_t stream);
+
+struct BlockDecodeParams {
+  const __nv_bfloat16* q;
+  const __nv_bfloat16* gate;  // may be null
+  __nv_bfloat16* out;
+  const uint8_t* k;
+  const uint8_t* v;
+  const float* k_scales;
+  const float* v_scales;
+  const int32_t* indices;  // null: column t is token t
+  const int32_t* counts;   // may be null
+  const int32_t* btable;
+  const int32_t* t2r;  // may be null
+  float score_scale_log2;  // softmax_scale * log2(e)
+  int rows, num_q_heads, num_kv_heads, group;
+  int page_size, block_size, pages_per_req, num_reqs;
+  int64_t num_pages;
+  int topk;  // columns of a row
+  int64_t indices_stride, btable_stride;
+  // split of the columns over CTAs
+  int chunk_tokens, num_chunks;
+  float* part_o;    // [rows, Hq, num_chunks, 128] normalised partial outputs
+  float* part_lse;  // [rows, Hq, num_chunks] log2-sum-exp2, -inf for an empty chunk
+};
+// Plans the split (chunk_tokens, num_chunks) and gives the workspace's size.
+int64_t block_decode_plan(BlockDecodeParams& p);
+cudaError_t launch_block_decode(const BlockDecodeParams& p, cudaStream_t stream);
+
+// QSA_B200_OK when the current device is an sm_100 part, else QSA_B200_ERR_DEVICE.
+int device_status();
+
 // Top-K entries per work item for a GQA group size (both kernels split rows
 // the same way, so the workspace size depends only on the shape), and the
 // group sizes of the tensor-core kernel.

@@ -54,6 +54,10 @@ EXPORTED = (
     "qsa_b200_decode_noalloc",
     "qsa_b200_cache_write",
     "qsa_b200_topk_select",
+    "qsa_b200_qk_rope",
+    "qsa_b200_block_append",
+    "qsa_b200_block_decode_workspace_bytes",
+    "qsa_b200_block_decode",
 )
 # test hook (include/qsa_b200_testing.h), not part of the decode interface
 TESTING_EXPORTED = ("qsa_b200_testing_set_wait_limit_ns",)
@@ -127,6 +131,113 @@ class TopkArgs(ctypes.Structure):
     ]
 
 
+ROPE_MAX_AXES = 4
+
+
+class Rotation(ctypes.Structure):
+    """Mirror of ``qsa_b200_rotation``."""
+
+    _fields_ = [
+        ("table", c_void_p),
+        ("positions", c_void_p),
+        ("axis_stride", c_int64),
+        ("table_len", c_int32),
+        ("rotary_dim", c_int32),
+        ("interleaved", c_int32),
+        ("num_axes", c_int32),
+        ("sections", c_int32 * ROPE_MAX_AXES),
+    ]
+
+
+class QkRopeArgs(ctypes.Structure):
+    """Mirror of ``qsa_b200_qk_rope_args``."""
+
+    _fields_ = [
+        ("q", c_void_p),
+        ("k", c_void_p),
+        ("q_out", c_void_p),
+        ("k_out", c_void_p),
+        ("q_weight", c_void_p),
+        ("k_weight", c_void_p),
+        ("eps", c_float),
+        ("tokens", c_int32),
+        ("num_q_heads", c_int32),
+        ("num_kv_heads", c_int32),
+        ("head_dim", c_int32),
+        ("q_stride", c_int64),
+        ("k_stride", c_int64),
+        ("q_out_stride", c_int64),
+        ("k_out_stride", c_int64),
+        ("dtype", c_int32),
+        ("weight_dtype", c_int32),
+        ("rope", Rotation),
+    ]
+
+
+class BlockAppendArgs(ctypes.Structure):
+    """Mirror of ``qsa_b200_block_append_args``."""
+
+    _fields_ = [
+        ("k", c_void_p),
+        ("v", c_void_p),
+        ("k_cache", c_void_p),
+        ("v_cache", c_void_p),
+        ("k_scales", c_void_p),
+        ("v_scales", c_void_p),
+        ("btable", c_void_p),
+        ("reqs", c_void_p),
+        ("starts", c_void_p),
+        ("cu_tokens", c_void_p),
+        ("k_weight", c_void_p),
+        ("eps", c_float),
+        ("entries", c_int32),
+        ("tokens", c_int32),
+        ("num_kv_heads", c_int32),
+        ("head_dim", c_int32),
+        ("page_size", c_int32),
+        ("block_size", c_int32),
+        ("pages_per_req", c_int32),
+        ("num_reqs", c_int32),
+        ("num_pages", c_int64),
+        ("btable_stride", c_int64),
+        ("token_stride", c_int64),
+        ("input_dtype", c_int32),
+        ("weight_dtype", c_int32),
+        ("rope", Rotation),
+    ]
+
+
+class BlockDecodeArgs(ctypes.Structure):
+    """Mirror of ``qsa_b200_block_decode_args``."""
+
+    _fields_ = [
+        ("q", c_void_p),
+        ("k_cache", c_void_p),
+        ("v_cache", c_void_p),
+        ("k_scales", c_void_p),
+        ("v_scales", c_void_p),
+        ("indices", c_void_p),
+        ("counts", c_void_p),
+        ("btable", c_void_p),
+        ("t2r", c_void_p),
+        ("gate", c_void_p),
+        ("out", c_void_p),
+        ("softmax_scale", c_float),
+        ("rows", c_int32),
+        ("num_q_heads", c_int32),
+        ("num_kv_heads", c_int32),
+        ("head_dim", c_int32),
+        ("page_size", c_int32),
+        ("block_size", c_int32),
+        ("pages_per_req", c_int32),
+        ("num_reqs", c_int32),
+        ("num_pages", c_int64),
+        ("topk", c_int32),
+        ("indices_stride", c_int64),
+        ("btable_stride", c_int64),
+    ]
+
+
 _configured = False
 
 
@@ -158,6 +269,14 @@ def lib() -> ctypes.CDLL:
         L.qsa_b200_cache_write.restype = c_int
         L.qsa_b200_topk_select.argtypes = [ctypes.POINTER(TopkArgs), c_void_p]
         L.qsa_b200_topk_select.restype = c_int
+        L.qsa_b200_qk_rope.argtypes = [ctypes.POINTER(QkRopeArgs), c_void_p]
+        L.qsa_b200_qk_rope.restype = c_int
+        L.qsa_b200_block_append.argtypes = [ctypes.POINTER(BlockAppendArgs), c_void_p]
+        L.qsa_b200_block_append.restype = c_int
+        L.qsa_b200_block_decode_workspace_bytes.argtypes = [ctypes.POINTER(BlockDecodeArgs)]
+        L.qsa_b200_block_decode_workspace_bytes.restype = c_int64
+        L.qsa_b200_block_decode.argtypes = [ctypes.POINTER(BlockDecodeArgs), c_void_p, c_size_t, c_void_p]
+        L.qsa_b200_block_decode.restype = c_int
         L.qsa_b200_testing_set_wait_limit_ns.argtypes = [ctypes.c_uint64]
         L.qsa_b200_testing_set_wait_limit_ns.restype = ctypes.c_uint64
         _configured = True
@@ -298,6 +417,26 @@ def make_topk_args(scores, k, out, lengths=None) -> TopkArgs:
 def topk_select(args: TopkArgs, stream: int = 0) -> int:
     """Calls ``qsa_b200_topk_select``; returns its status."""
     return int(lib().qsa_b200_topk_select(ctypes.byref(args), c_void_p(stream)))
+
+
+def qk_rope(args: QkRopeArgs, stream: int = 0) -> int:
+    """Calls ``qsa_b200_qk_rope``; returns its status."""
+    return int(lib().qsa_b200_qk_rope(ctypes.byref(args), c_void_p(stream)))
+
+
+def block_append(args: BlockAppendArgs, stream: int = 0) -> int:
+    """Calls ``qsa_b200_block_append``; returns its status."""
+    return int(lib().qsa_b200_block_append(ctypes.byref(args), c_void_p(stream)))
+
+
+def block_decode_workspace_bytes(args: BlockDecodeArgs) -> int:
+    return int(lib().qsa_b200_block_decode_workspace_bytes(ctypes.byref(args)))
+
+
+def block_decode(args: BlockDecodeArgs, workspace=None, workspace_bytes_: int = 0, stream: int = 0) -> int:
+    """Calls ``qsa_b200_block_decode``; returns its status."""
+    ws = None if workspace is None else c_void_p(workspace.data_ptr())
+    return int(lib().qsa_b200_block_decode(ctypes.byref(args), ws, c_size_t(workspace_bytes_), c_void_p(stream)))
 
 
 def device_error(clear: bool = False) -> int:
