@@ -15,7 +15,6 @@ namespace {
 bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 bool dtype_ok(int d) { return d >= QSA_B200_DTYPE_BF16 && d <= QSA_B200_DTYPE_F32; }
 int64_t dtype_bytes(int d) { return d == QSA_B200_DTYPE_F32 ? 4 : 2; }
-int64_t align256(int64_t x) { return (x + 255) / 256 * 256; }
 
 // Checks a rotation and fills its launch parameters. own_positions: the
 // kernel has positions of its own where none are given.
@@ -218,9 +217,7 @@ int qsa_b200_block_decode(const qsa_b200_block_decode_args* a, void* workspace, 
   if (need > 0) {
     if (!workspace || (int64_t)workspace_bytes < need) return QSA_B200_ERR_WORKSPACE;
     if (!aligned(workspace, 256)) return QSA_B200_ERR_MISALIGNED;
-    const int64_t n = (int64_t)p.rows * p.num_q_heads * p.num_chunks;
-    p.part_o = static_cast<float*>(workspace);
-    p.part_lse = reinterpret_cast<float*>(static_cast<char*>(workspace) + align256(n * 128 * 4));
+    block_decode_place(p, workspace);
   }
   return launch_block_decode(p, reinterpret_cast<cudaStream_t>(stream)) == cudaSuccess ? QSA_B200_OK
                                                                                       : QSA_B200_ERR_LAUNCH;

@@ -186,13 +186,23 @@ struct BlockDecodeParams {
   int head_parts, part_heads, virtual_heads, cta_heads;
   // slot / block_size = umulhi(2 slot, block_mul) >> block_shift, exact below 2^31
   uint32_t block_mul, block_shift;
-  // split of the columns over CTAs
-  int chunk_tokens, num_chunks;
-  float* part_o;    // [rows, Hq, num_chunks, 128] normalised partial outputs
-  float* part_lse;  // [rows, Hq, num_chunks] log2-sum-exp2, -inf for an empty chunk
+  // Rows of many columns: units (of a CTA's warps times 16 columns) in the
+  // order row, head group, columns, shared evenly by `ctas` CTAs (workspace).
+  bool planned;
+  struct BlockDecodePlan* plan;  // null: a CTA takes a whole row
+  int64_t* prefix;               // [rows + 1] units of one head group before each row
+  int* lengths;                  // [rows] columns up to the last valid one
+  int* first_row;                // [ctas] row that each CTA begins in
+  float* part_o;                 // [2 ctas, cta_heads, part_heads, 128] normalised results of pieces of rows
+  float* part_lse;               // [2 ctas, cta_heads, part_heads] their log2-sum-exp2, -inf for none
 };
-// Plans the split (chunk_tokens, num_chunks) and gives the workspace's size.
+struct BlockDecodePlan {
+  int64_t units;
+  int ctas;
+};
+// Chooses the split and gives the workspace's size; places it in a workspace.
 int64_t block_decode_plan(BlockDecodeParams& p);
+void block_decode_place(BlockDecodeParams& p, void* workspace);
 cudaError_t launch_block_decode(const BlockDecodeParams& p, cudaStream_t stream);
 
 // QSA_B200_OK when the current device is an sm_100 part, else QSA_B200_ERR_DEVICE.
