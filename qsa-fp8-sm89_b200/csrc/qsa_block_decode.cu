@@ -7,8 +7,10 @@
 // memory), then brings them through a ring of stages by cp.async, 128 (token,
 // KV head) rows of K and of V at a time: 16 tokens of 8 heads, or more tokens
 // of fewer heads. A token's heads are neighbours in the cache, so a warp's loads
-// run along 1 KiB. Each warp multiplies 16 tokens of one head; with fewer than
-// 8 heads the warps of a head join their results in shared memory.
+// run along 1 KiB. Each warp multiplies 16 tokens of one KV head with up to 8
+// query heads: a group of 9 to 16, or 17 to 32, goes as 2 or 4 virtual KV heads
+// whose warps read the same rows of a stage. Warps that have the same heads and
+// other tokens join their results in shared memory.
 //
 // Rows of up to 512 columns are a segment and a CTA each. Longer ones are
 // planned: a scan over the rows' lengths gives every CTA of a grid that fills
@@ -53,14 +55,16 @@ constexpr int kBdWarps = 8;
 constexpr int kBdTile = 16;                         // tokens a warp takes at a time
 constexpr int kBdTable = 2048;                      // slots of a CTA's table
 constexpr int kBdDirect = 512;                      // columns of a row that are not planned
-constexpr int kBdRows = kBdTile * kBdWarps;          // K rows of a stage, and V rows
-constexpr int kStageBytes = 2 * kBdRows * kHeadDim;
 constexpr float kLazy = 8.f;                        // log2 by which a score may pass its reference
 constexpr float kLazyW = 128.f;                     // factor by which a weight may pass its reference
 constexpr float kOneW = 256.f;                      // what stands for W in f16
 constexpr float kLowest = -3.402823466e38f;
 
-__device__ __forceinline__ float sigmoid(float x) { return 1.0f / (1.0f + expf(-x)); }
+// The approximate forms (a few ulp) have no branches: 32 of the exact ones a
+// thread took 3 us at the end of a segment. For x below -88 the divisor is past
+// 2^126, where the approximate quotient is 0, as sigmoid rounds in bf16's range
+// of normal values.
+__device__ __forceinline__ float sigmoid(float x) { return __fdividef(1.0f, 1.0f + __expf(-x)); }
 __device__ __forceinline__ float ex2(float x) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(r) : "f"(x));
@@ -95,6 +99,11 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   return r;
 }
 
+// Of a chain of dependent launches: lets the next kernel start, and waits for
+// all of the one before (nothing where the launch was an ordinary one).
+__device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory"); }
+__device__ __forceinline__ void wait_for_prerequisites() { asm volatile("griddepcontrol.wait;\n" ::: "memory"); }
+
 __device__ __forceinline__ uint32_t pack_f16(float a, float b) {
   const __half2 h = __floats2half2_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&h);
@@ -114,404 +123,372 @@ __device__ __forceinline__ void column_slots(const BlockDecodeParams& p, int64_t
   for (int i = 0; i < N; ++i) t[i] = page[i] < 0 || page[i] >= p.num_pages ? -1 : page[i] * p.page_size + off[i];
 }
 
-// kHeads: query heads of a warp's tile, 8 or 16 (which need the registers of
-// both CTAs). kCh: cache heads of a CTA.
-template <int kHeads, int kCh>
+// kParts: virtual KV heads of a cache head. kCh: cache heads of a CTA.
+template <int kParts, int kCh>
 struct BdCfg {
-  static constexpr int kSets = kHeads / 8;
-  static constexpr int kStages = kHeads == 8 ? 3 : 6;
+  static constexpr int kHeads = kParts * kCh;                // virtual heads of a CTA
+  static constexpr int kSplit = kBdWarps / kHeads;           // warps of a head
+  static constexpr int kUnit = kSplit * kBdTile;             // tokens of a stage; the plan counts in them
+  static constexpr int kRows = kUnit * kCh;                  // its K rows, and V rows: 128 / kParts
+  static constexpr int kStageBytes = 2 * kRows * kHeadDim;
+  static constexpr int kStages = kParts == 1 ? 3 : 6;
   static constexpr int kThreads = 32 * kBdWarps;
-  static constexpr int kCtas = kHeads == 8 ? 2 : 1;  // per SM
-  static constexpr int kScales = kStages * kStageBytes;              // float [stages][K, V][kBdRows]
-  static constexpr int kTable = kScales + kStages * 2 * kBdRows * 4;  // int [kBdTable]
+  static constexpr int kScales = kStages * kStageBytes;             // float [stages][K, V][kRows]
+  static constexpr int kTable = kScales + kStages * 2 * kRows * 4;  // int [kBdTable]
   static constexpr int kSmem = kTable + kBdTable * 4;
-  static constexpr int kLeft = (kHeads * (kHeadDim + 2) * 4 + 127) / 128 * 128;  // a warp's result
-  static_assert(kBdWarps * kLeft <= kScales, "the warps' results fit the ring");
+  static constexpr int kLeft = (8 * (kHeadDim + 2) * 4 + 127) / 128 * 128;  // a warp's result
+  static_assert(kHeads <= kBdWarps && kBdWarps * kLeft <= kScales, "the warps' results fit the ring");
+  static_assert(2 * (kSmem + 1024) <= 228 * 1024, "two CTAs an SM");
 };
 
-template <int kHeads, int kCh>
-__global__ void __launch_bounds__(32 * kBdWarps, BdCfg<kHeads, kCh>::kCtas)
-    qsa_block_decode_kernel(const __grid_constant__ BlockDecodeParams p) {
-  using C = BdCfg<kHeads, kCh>;
-  constexpr int kSets = C::kSets, kStages = C::kStages;
+template <int kParts, int kCh>
+__global__ void __launch_bounds__(32 * kBdWarps, 2) qsa_block_decode_kernel(const __grid_constant__ BlockDecodeParams p) {
+  using C = BdCfg<kParts, kCh>;
+  constexpr int kStages = C::kStages, kUnit = C::kUnit;
   constexpr int kRowStep = kCh * kHeadDim;  // from a token of a stage to the next
   extern __shared__ __align__(128) uint8_t smem[];
   int* table = reinterpret_cast<int*>(smem + C::kTable);
-  float* scales = reinterpret_cast<float*>(smem + C::kScales);
+  const float* scales = reinterpret_cast<const float*>(smem + C::kScales);
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   const int r = lane / 4, c = lane % 4;
   const uint32_t smem_s = smem_u32(smem);
+  const int hgroups = p.num_kv_heads / kCh;
+  const int part = warp / C::kHeads;                // this warp's share of a stage's tokens
+  const int head_in = warp % C::kHeads;             // its virtual head in the CTA
 
-  const int hgroups = p.virtual_heads / p.cta_heads;
-  const int split = kBdWarps / p.cta_heads;  // warps of a head
-  const int part = warp / p.cta_heads;       // this warp's share of the tiles
-  const int unit = split * kBdTile;          // tokens of a stage; the plan counts in them
-
+  launch_dependents();
   // the CTA's range of the plan's units, and its first row
   int64_t at = 0, end = 1;
   int row = (int)(blockIdx.x / hgroups);
   if (p.plan) {
-    const int64_t units = p.plan->units;
-    const int ctas = p.plan->ctas;
-    if ((int)blockIdx.x >= ctas) return;
-    at = blockIdx.x * units / ctas;
-    end = (blockIdx.x + 1) * units / ctas;
-    row = p.first_row[blockIdx.x];
+    wait_for_prerequisites();
+    if ((int)blockIdx.x >= p.plan->ctas) return;
+    at = p.plan->cut[blockIdx.x];
+    end = p.plan->cut[blockIdx.x + 1];
+    row = p.plan->first_row[blockIdx.x];
   }
 
 #pragma unroll 1
   for (bool first = true; at < end; first = false) {
-  // the segment: columns c0 .. c1 - 1 of the row for the head group hg
-  int hg = (int)(blockIdx.x % hgroups), c0 = 0, slot_out = -1;
-  int64_t req = p.t2r ? __ldg(p.t2r + row) : row;
-  int c1 = 0;
-  const int row_now = row;
-  if (p.plan) {
-    const int64_t row_at = p.prefix[row] * hgroups;
-    const int row_units = (int)(p.prefix[row + 1] - p.prefix[row]);
-    const int in_row = (int)(at - row_at);
-    hg = in_row / row_units;
-    const int from = in_row - hg * row_units;
-    const int to = (int)min((int64_t)row_units, from + (end - at));
-    c0 = from * unit;
-    c1 = min((int64_t)to * unit, (int64_t)p.lengths[row]);
-    if (from > 0 || to < row_units) slot_out = 2 * blockIdx.x + (from > 0 ? 0 : 1);
-    at += to - from;
-    if (to == row_units && hg == hgroups - 1) ++row;
-  } else {
-    c1 = p.counts ? min(__ldg(p.counts + row), p.topk) : p.topk;
-    if (req < 0 || req >= p.num_reqs) req = 0, c1 = 0;
-    at = end;
-  }
-  const int gv = hg * p.cta_heads + warp % p.cta_heads;             // (virtual) KV head
-  const int g = gv / p.head_parts;                                  // cache head
-  const int h0 = g * p.group + (gv % p.head_parts) * p.part_heads;  // first query head
-  const int heads = min(p.part_heads, (g + 1) * p.group - h0);
+    // the segment: columns c0 .. c1 - 1 of the row for the head group hg
+    int hg = (int)(blockIdx.x % hgroups), c0 = 0, slot_out = -1;
+    int64_t req = p.t2r ? __ldg(p.t2r + row) : row;
+    int c1 = 0;
+    const int row_now = row;
+    if (p.plan) {
+      const int64_t row_at = p.prefix[row] * hgroups;
+      const int row_units = (int)(p.prefix[row + 1] - p.prefix[row]);
+      const int in_row = (int)(at - row_at);
+      hg = in_row / row_units;
+      const int from = in_row - hg * row_units;
+      const int to = (int)min((int64_t)row_units, from + (end - at));
+      c0 = from * kUnit;
+      c1 = (int)min((int64_t)to * kUnit, (int64_t)p.lengths[row]);
+      if (from > 0 || to < row_units) slot_out = 2 * blockIdx.x + (from > 0 ? 0 : 1);
+      at += to - from;
+      if (to == row_units && hg == hgroups - 1) ++row;
+    } else {
+      c1 = p.counts ? min(__ldg(p.counts + row), p.topk) : p.topk;
+      if (req < 0 || req >= p.num_reqs) req = 0, c1 = 0;
+      at = end;
+    }
+    const int g0 = hg * kCh;                                               // the CTA's first cache head
+    const int in_group = head_in % kParts * p.part_heads;                  // this warp's first query head in its group
+    const int h0 = (g0 + head_in / kParts) * p.group + in_group;
+    const int heads = min(p.part_heads, p.group - in_group);
 
-  // Q fragments: f16 of q 2^e for head r, the order of dims is that of the K
-  // fragments (k-step s: word s of the thread's chunks c and c + 4)
-  uint32_t qf[kSets][8][2];
-  float qs[kSets][2];  // of heads 2c, 2c + 1: 2^-e softmax_scale log2(e)
-#pragma unroll
-  for (int u = 0; u < kSets; ++u) {
-    uint4 w[4] = {};
-    if (u * 8 + r < heads) {
-      const uint4* src = reinterpret_cast<const uint4*>(p.q + ((int64_t)row_now * p.num_q_heads + h0 + u * 8 + r) * kHeadDim);
-      w[0] = src[2 * c], w[1] = src[2 * c + 1], w[2] = src[8 + 2 * c], w[3] = src[8 + 2 * c + 1];
+    // the queries as loaded: head r, 16 dims of either half; converted below,
+    // when the first tiles are under way
+    uint4 q_raw[4] = {};
+    if (r < heads) {
+      const uint4* src = reinterpret_cast<const uint4*>(p.q + ((int64_t)row_now * p.num_q_heads + h0 + r) * kHeadDim);
+      q_raw[0] = __ldg(src + 2 * c), q_raw[1] = __ldg(src + 2 * c + 1);
+      q_raw[2] = __ldg(src + 8 + 2 * c), q_raw[3] = __ldg(src + 8 + 2 * c + 1);
     }
-    float top = 0.f;
-    float2 x[16];
+    uint32_t qf[8][2];  // Q fragments: f16 of q 2^e, in the order of dims of the K fragments
+    float qs[2];        // of heads 2c, 2c + 1: 2^-e softmax_scale log2(e)
+    float o[8][4];      // [dims 16r + 2i, + 1][head 2c, 2c + 1 of either dim]
+    float m[2], l[2], W[2], inv_w[2];  // of heads 2c, 2c + 1
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t b[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        x[4 * i + j] = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&b[j]));
-        top = fmaxf(top, fmaxf(fabsf(x[4 * i + j].x), fabsf(x[4 * i + j].y)));
-      }
-    }
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    int e = 0;  // 2^e maps the largest |q| into [2^14, 2^15)
-    if (top > 0.f && top <= -kLowest) e = min(max(14 + 127 - (int)(__float_as_uint(top) >> 23), -120), 120);
-    const float up = __uint_as_float((uint32_t)(127 + e) << 23);
-    const float down = __uint_as_float((uint32_t)(127 - e) << 23) * p.score_scale_log2;
-    qs[u][0] = __shfl_sync(0xffffffffu, down, 8 * c);
-    qs[u][1] = __shfl_sync(0xffffffffu, down, 8 * c + 4);
-#pragma unroll
-    for (int s = 0; s < 8; ++s) {
-      qf[u][s][0] = pack_f16(x[2 * s].x * up, x[2 * s].y * up);
-      qf[u][s][1] = pack_f16(x[2 * s + 1].x * up, x[2 * s + 1].y * up);
-    }
-  }
-
-  float o[kSets][8][4];  // [head set][dims 16r + 2i, + 1][head 2c, 2c + 1 of either dim]
-  float m[kSets][2], l[kSets][2], W[kSets][2], inv_w[kSets][2];  // of heads 2c, 2c + 1
-#pragma unroll
-  for (int u = 0; u < kSets; ++u) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) m[u][h] = kLowest, l[u][h] = 0.f, W[u][h] = 0.f, inv_w[u][h] = 0.f;  // the first score passes
+    for (int h = 0; h < 2; ++h) m[h] = kLowest, l[h] = 0.f, W[h] = 0.f, inv_w[h] = 0.f;  // the first score passes
 #pragma unroll
     for (int i = 0; i < 8; ++i)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) o[u][i][j] = 0.f;
-  }
+      for (int j = 0; j < 4; ++j) o[i][j] = 0.f;
 
-  // this thread's part of a fetch: 16 bytes of the rows 4i + lane / 8 of its
-  // warp's, and a scale of row tid % 128 (K's in the first warps, V's in the
-  // others). Row (token, head) lies at token * kCh + head; a token's chunks are
-  // stored permuted, K's by (t & 1) << 2, V's by t & 6, so that the 8 threads
-  // of a 16-byte read phase meet no bank twice.
-  const int warp_rows = kBdTile / p.head_parts;  // of the stage's rows
-  const int row0 = warp * warp_rows + lane / 8;
-  const int g0 = hg * p.cta_heads / p.head_parts;  // the CTA's first cache head
-  const int token_bytes = p.num_kv_heads * kHeadDim;
-  const uint8_t* k_src = p.k + (g0 + row0 % kCh) * kHeadDim + lane % 8 * 16;
-  const uint8_t* v_src = p.v + (g0 + row0 % kCh) * kHeadDim + lane % 8 * 16;
-  const int scale_row = tid % kBdRows;
-  const float* s_src = (tid < kBdRows ? p.k_scales : p.v_scales) + g0 + scale_row % kCh;
-  const int token0 = row0 / kCh;
-  const uint32_t k_dst = smem_s + row0 * kHeadDim + ((lane % 8 ^ ((token0 & 1) << 2)) << 4);
-  const uint32_t v_dst = smem_s + (kBdRows + row0) * kHeadDim + ((lane % 8 ^ (token0 & 6)) << 4);
-  const uint32_t s_dst = smem_s + C::kScales + tid * 4;
-  // where this warp's fragments lie in a stage
-  const uint32_t own = (part * kBdTile * kCh + (warp % p.cta_heads) / p.head_parts) * kHeadDim;
-  const uint32_t k_at = own + r * kRowStep + ((c ^ ((r & 1) << 2)) << 4);
-  const uint32_t v_at = own + kBdRows * kHeadDim + 2 * c * kRowStep + ((r ^ (2 * c)) << 4);
-  const uint32_t s_at = part * kBdTile * kCh + (warp % p.cta_heads) / p.head_parts;
+    // this thread's part of a fetch: 16 bytes of the rows 4i + lane / 8 of its
+    // warp's, and a scale of row tid % 128 (K's in the first warps, V's in the
+    // others). Row (token, head) lies at token * kCh + head; a token's chunks
+    // are stored permuted, K's by (t & 1) << 2, V's by t & 6, so that the 8
+    // threads of a 16-byte read phase meet no bank twice.
+    const int row0 = warp * (kBdTile / kParts) + lane / 8;
+    const int token0 = row0 / kCh;
+    const int token_bytes = p.num_kv_heads * kHeadDim;
+    const uint8_t* k_src = p.k + (g0 + row0 % kCh) * kHeadDim + lane % 8 * 16;
+    const uint8_t* v_src = p.v + (g0 + row0 % kCh) * kHeadDim + lane % 8 * 16;
+    const int scale_row = tid % 128;
+    const float* s_src = (tid < 128 ? p.k_scales : p.v_scales) + g0 + scale_row % kCh;
+    const uint32_t k_dst = smem_s + row0 * kHeadDim + ((lane % 8 ^ ((token0 & 1) << 2)) << 4);
+    const uint32_t v_dst = smem_s + (C::kRows + row0) * kHeadDim + ((lane % 8 ^ (token0 & 6)) << 4);
+    const uint32_t s_dst = smem_s + C::kScales + (tid / 128 * C::kRows + scale_row) * 4;
+    // where this warp's fragments and scales lie in a stage
+    const int own = part * kBdTile * kCh + head_in / kParts;
+    const uint32_t k_at = own * kHeadDim + r * kRowStep + ((c ^ ((r & 1) << 2)) << 4);
+    const uint32_t v_at = (C::kRows + own) * kHeadDim + 2 * c * kRowStep + ((r ^ (2 * c)) << 4);
+    const int s_at = own + r * kCh;
 
-  for (int base = c0; base < c1; base += kBdTable) {
-    const int n = min(kBdTable, c1 - base);
-    if (base > c0 || !first) __syncthreads();  // the table's readers are done
-    bool valid = true;
-    // several columns a thread at once: an index, then its page, wait on memory
 #pragma unroll 1
-    for (int i0 = tid; i0 < (n + unit - 1) / unit * unit; i0 += 4 * C::kThreads) {
-      int slot[4];
+    for (int base = c0; base < c1; base += kBdTable) {
+      const int n = min(kBdTable, c1 - base);
+      const int tiles = (n + kUnit - 1) / kUnit;
+      if (base > c0 || !first) __syncthreads();  // the table's readers are done
+      bool valid = true;
+      // several columns a thread at once: an index, then its page, wait on memory
+#pragma unroll 1
+      for (int i0 = tid; i0 < tiles * kUnit; i0 += 8 * C::kThreads) {
+        int slot[8];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int col = i0 + i * C::kThreads;
-        slot[i] = col < n ? (p.indices ? __ldg(p.indices + (int64_t)row_now * p.indices_stride + base + col) : base + col) : -1;
-      }
-      column_slots(p, req, slot);
+        for (int i = 0; i < 8; ++i) {
+          const int col = i0 + i * C::kThreads;
+          slot[i] = col >= n ? -1 : p.indices ? __ldg(p.indices + (int64_t)row_now * p.indices_stride + base + col) : base + col;
+        }
+        column_slots(p, req, slot);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int col = i0 + i * C::kThreads;
-        if (col < (n + unit - 1) / unit * unit) table[col] = slot[i];
-        valid = valid && (slot[i] >= 0 || col >= n);
+        for (int i = 0; i < 8; ++i) {
+          const int col = i0 + i * C::kThreads;
+          if (col < tiles * kUnit) table[col] = slot[i];
+          valid = valid && (slot[i] >= 0 || col >= n);
+        }
       }
-    }
-    const bool clean = __syncthreads_and(valid);  // only the last tile may have masked places
-    const int tiles = (n + unit - 1) / unit;
-    const int whole = clean ? n / unit : 0;  // leading tiles without a masked place
+      const bool clean = __syncthreads_and(valid);  // only the last tile may have masked places
+      const int whole = clean ? n / kUnit : 0;      // leading tiles without one
 
-    auto fetch = [&](int k, int st) {
-      if (k < tiles) {
-        const int* ahead = table + k * unit;
+      auto fetch = [&](int k, int st) {
+        if (k < tiles) {
+          const int* ahead = table + k * kUnit;
+#pragma unroll
+          for (int i = 0; i < 4 / kParts; ++i) {
+            // Row row0 + 4i: with 8 heads the token's other four or the next
+            // token's first, else the same heads 4 / kCh tokens on. The bits
+            // that step adds to the token are none that token0 has, so the
+            // chunk permutation splits into token0's and a constant.
+            const int step = 4 * i / kCh;
+            const int64_t to_head = kCh == 8 ? i % 2 * 4 * kHeadDim : 0;
+            const int slot = ahead[token0 + step];
+            const uint32_t kd = (k_dst ^ ((step & 1) << 6)) + st * C::kStageBytes + i * 4 * kHeadDim;
+            const uint32_t vd = (v_dst ^ ((step & 6) << 4)) + st * C::kStageBytes + i * 4 * kHeadDim;
+            if (k < whole) {
+              cp_async_16_all(kd, k_src + (int64_t)slot * token_bytes + to_head);
+              cp_async_16_all(vd, v_src + (int64_t)slot * token_bytes + to_head);
+            } else {  // masked places read as zeros, whatever the cache holds
+              const int64_t from = (int64_t)max(slot, 0) * token_bytes + to_head;
+              cp_async_16(kd, k_src + from, slot < 0 ? 0u : 16u);
+              cp_async_16(vd, v_src + from, slot < 0 ? 0u : 16u);
+            }
+          }
+          if (kParts == 1 || scale_row < C::kRows) {
+            const int slot = ahead[scale_row / kCh];
+            const uint32_t block = __umulhi(2u * (uint32_t)max(slot, 0), p.block_mul) >> p.block_shift;
+            cp_async_4_or_zero(s_dst + st * 2 * C::kRows * 4, s_src + (int64_t)(int)block * p.num_kv_heads,
+                               slot < 0 ? 0u : 4u);
+          }
+        }
+        cp_async_commit();
+      };
+#pragma unroll
+      for (int st = 0; st < kStages - 1; ++st) fetch(st, st);
+
+      if (base == c0) {
+        float top = 0.f;
+        float2 x[16];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          if (i >= 2 && p.head_parts == 2) break;
-          // Row row0 + 4i: with 8 heads the token's other four or the next
-          // token's first, else the same heads 4 / kCh tokens on. The bits that
-          // step adds to the token are none that token0 has, so the chunk
-          // permutation splits into token0's and a constant.
-          const int step = 4 * i / kCh;
-          const int64_t at = kCh == 8 ? i % 2 * 4 * kHeadDim : 0;
-          const int slot = ahead[token0 + step];
-          const uint32_t kd = (k_dst ^ ((step & 1) << 6)) + st * kStageBytes + i * 4 * kHeadDim;
-          const uint32_t vd = (v_dst ^ ((step & 6) << 4)) + st * kStageBytes + i * 4 * kHeadDim;
-          if (k < whole) {
-            cp_async_16_all(kd, k_src + (int64_t)slot * token_bytes + at);
-            cp_async_16_all(vd, v_src + (int64_t)slot * token_bytes + at);
-          } else {  // masked places read as zeros, whatever the cache holds
-            const int64_t from = (int64_t)max(slot, 0) * token_bytes + at;
-            cp_async_16(kd, k_src + from, slot < 0 ? 0u : 16u);
-            cp_async_16(vd, v_src + from, slot < 0 ? 0u : 16u);
+          const uint32_t b[4] = {q_raw[i].x, q_raw[i].y, q_raw[i].z, q_raw[i].w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            x[4 * i + j] = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&b[j]));
+            top = fmaxf(top, fmaxf(fabsf(x[4 * i + j].x), fabsf(x[4 * i + j].y)));
           }
         }
-        if (scale_row < unit * kCh) {
-          const int slot = ahead[scale_row / kCh];
-          const uint32_t block = __umulhi(2u * (uint32_t)max(slot, 0), p.block_mul) >> p.block_shift;
-          cp_async_4_or_zero(s_dst + st * 2 * kBdRows * 4, s_src + (int64_t)(int)block * p.num_kv_heads,
-                             slot < 0 ? 0u : 4u);
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        int e = 0;  // 2^e maps the largest |q| into [2^14, 2^15)
+        if (top > 0.f && top <= -kLowest) e = min(max(14 + 127 - (int)(__float_as_uint(top) >> 23), -120), 120);
+        const float up = __uint_as_float((uint32_t)(127 + e) << 23);
+        const float down = __uint_as_float((uint32_t)(127 - e) << 23) * p.score_scale_log2;
+        qs[0] = __shfl_sync(0xffffffffu, down, 8 * c);
+        qs[1] = __shfl_sync(0xffffffffu, down, 8 * c + 4);
+#pragma unroll
+        for (int s = 0; s < 8; ++s) {  // k-step s: word s of the thread's chunks c and c + 4
+          qf[s][0] = pack_f16(x[2 * s].x * up, x[2 * s].y * up);
+          qf[s][1] = pack_f16(x[2 * s + 1].x * up, x[2 * s + 1].y * up);
         }
       }
-      cp_async_commit();
-    };
-#pragma unroll
-    for (int st = 0; st < kStages - 1; ++st) fetch(st, st);
 
 #pragma unroll 1
-    for (int k0 = 0; k0 < tiles; k0 += kStages) {
+      for (int k0 = 0; k0 < tiles; k0 += kStages) {
 #pragma unroll
-      for (int st = 0; st < kStages; ++st) {
-        if (k0 + st >= tiles) break;
-        cp_async_wait<kStages - 2>();
-        __syncthreads();  // the tile is there, and every warp has read the one before
-        fetch(k0 + st + kStages - 1, (st + kStages - 1) % kStages);
-        const uint8_t* stage = smem + st * kStageBytes;
-        const float* sc = scales + st * 2 * kBdRows + s_at;
+        for (int st = 0; st < kStages; ++st) {
+          if (k0 + st >= tiles) break;
+          cp_async_wait<kStages - 2>();
+          __syncthreads();  // the tile is there, and every warp has read the one before
+          fetch(k0 + st + kStages - 1, (st + kStages - 1) % kStages);
+          const uint8_t* stage = smem + st * C::kStageBytes;
+          const float* sc = scales + st * 2 * C::kRows + s_at;
 
-        // [head set][token r: heads 2c, 2c+1; token r + 8: the same], in two chains
-        float s[kSets][4] = {}, s1[kSets][4] = {};
+          // [token r: heads 2c, 2c+1; token r + 8: the same], in two chains
+          float s[4] = {}, s1[4] = {};
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const uint4 a4 = *reinterpret_cast<const uint4*>(stage + (k_at ^ (64 * j)));
-          const uint4 b4 = *reinterpret_cast<const uint4*>(stage + (k_at ^ (64 * j)) + 8 * kRowStep);
-          const uint32_t wa[4] = {a4.x, a4.y, a4.z, a4.w}, wb[4] = {b4.x, b4.y, b4.z, b4.w};
+          for (int j = 0; j < 2; ++j) {
+            const uint4 a4 = *reinterpret_cast<const uint4*>(stage + (k_at ^ (64 * j)));
+            const uint4 b4 = *reinterpret_cast<const uint4*>(stage + (k_at ^ (64 * j)) + 8 * kRowStep);
+            const uint32_t wa[4] = {a4.x, a4.y, a4.z, a4.w}, wb[4] = {b4.x, b4.y, b4.z, b4.w};
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint32_t a[4] = {f16_of(wa[i]), f16_of(wb[i]), f16_of(wa[i] >> 16), f16_of(wb[i] >> 16)};
-#pragma unroll
-            for (int u = 0; u < kSets; ++u) mma16816(j ? s1[u] : s[u], a, qf[u][4 * j + i][0], qf[u][4 * j + i][1]);
+            for (int i = 0; i < 4; ++i) {
+              const uint32_t a[4] = {f16_of(wa[i]), f16_of(wb[i]), f16_of(wa[i] >> 16), f16_of(wb[i] >> 16)};
+              mma16816(j ? s1 : s, a, qf[4 * j + i][0], qf[4 * j + i][1]);
+            }
           }
-        }
-#pragma unroll
-        for (int u = 0; u < kSets; ++u)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) s[u][j] += s1[u][j];
-        const float ks[2] = {sc[r * kCh], sc[(8 + r) * kCh]};
-        const float vs[2] = {sc[kBdRows + r * kCh], sc[kBdRows + (8 + r) * kCh]};
-        bool masked[2] = {false, false};
-        if (k0 + st >= whole) {
-          const int* slots = table + (k0 + st) * unit + part * kBdTile;
-          masked[0] = slots[r] < 0, masked[1] = slots[8 + r] < 0;
-        }
+          const float ks[2] = {sc[0], sc[8 * kCh]}, vs[2] = {sc[C::kRows], sc[C::kRows + 8 * kCh]};
+          bool masked[2] = {false, false};
+          if (k0 + st >= whole) {
+            const int* slots = table + (k0 + st) * kUnit + part * kBdTile;
+            masked[0] = slots[r] < 0, masked[1] = slots[8 + r] < 0;
+          }
 
-        // scores over the reference, probabilities, weights over theirs
-        float pr[kSets][4], w[kSets][4];
-        bool pass = false;
-#pragma unroll
-        for (int u = 0; u < kSets; ++u) {
+          // scores over the reference, probabilities, weights over theirs
+          float pr[4], w[4];
+          bool pass = false;
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const int t = j / 2, h = j % 2;
-            float x = fmaf(s[u][j], ks[t] * qs[u][h], -m[u][h]);
+            s[j] += s1[j];
+            float x = fmaf(s[j], ks[t] * qs[h], -m[h]);
             x = masked[t] ? -INFINITY : x;
-            pr[u][j] = ex2(x);
-            w[u][j] = pr[u][j] * (vs[t] * inv_w[u][h]);
-            pass = pass || x > kLazy || fabsf(w[u][j]) > kLazyW * kOneW;
+            pr[j] = ex2(x);
+            w[j] = pr[j] * (vs[t] * inv_w[h]);
+            pass = pass || x > kLazy || fabsf(w[j]) > kLazyW * kOneW;
           }
-        }
-        if (__any_sync(0xffffffffu, pass)) {
-          // move the references, and what was summed against them
-#pragma unroll
-          for (int u = 0; u < kSets; ++u) {
+          if (__any_sync(0xffffffffu, pass)) {
+            // move the references, and what was summed against them
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              const float x0 = masked[0] ? -INFINITY : s[u][h] * (ks[0] * qs[u][h]);
-              const float x1 = masked[1] ? -INFINITY : s[u][2 + h] * (ks[1] * qs[u][h]);
+              const float x0 = masked[0] ? -INFINITY : s[h] * (ks[0] * qs[h]);
+              const float x1 = masked[1] ? -INFINITY : s[2 + h] * (ks[1] * qs[h]);
               float top = fmaxf(x0, x1);
 #pragma unroll
               for (int d = 4; d <= 16; d *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-              const float m_new = fmaxf(m[u][h], top);
-              const float alpha = ex2(m[u][h] - m_new);
-              pr[u][h] = ex2(x0 - m_new), pr[u][2 + h] = ex2(x1 - m_new);
-              const float w0 = pr[u][h] * vs[0], w1 = pr[u][2 + h] * vs[1];
+              const float m_new = fmaxf(m[h], top);
+              const float alpha = ex2(m[h] - m_new);
+              pr[h] = ex2(x0 - m_new), pr[2 + h] = ex2(x1 - m_new);
+              const float w0 = pr[h] * vs[0], w1 = pr[2 + h] * vs[1];
               float w_top = fmaxf(fabsf(w0), fabsf(w1));
 #pragma unroll
               for (int d = 4; d <= 16; d *= 2) w_top = fmaxf(w_top, __shfl_xor_sync(0xffffffffu, w_top, d));
-              const float was = W[u][h] * alpha;
-              W[u][h] = fmaxf(was, w_top);
+              const float was = W[h] * alpha;
+              W[h] = fmaxf(was, w_top);
               // without a weight yet, any that matters passes
-              inv_w[u][h] = W[u][h] > 0.f ? kOneW / W[u][h] : 1e38f;
-              const float f = was > 0.f ? was / W[u][h] : 0.f;
-              m[u][h] = m_new;
-              l[u][h] *= alpha;
-              w[u][h] = w0 * inv_w[u][h], w[u][2 + h] = w1 * inv_w[u][h];
+              inv_w[h] = W[h] > 0.f ? kOneW / W[h] : 1e38f;
+              const float f = was > 0.f ? was / W[h] : 0.f;
+              m[h] = m_new;
+              l[h] *= alpha;
+              w[h] = w0 * inv_w[h], w[2 + h] = w1 * inv_w[h];
 #pragma unroll
-              for (int i = 0; i < 8; ++i) o[u][i][h] *= f, o[u][i][2 + h] *= f;
+              for (int i = 0; i < 8; ++i) o[i][h] *= f, o[i][2 + h] *= f;
             }
           }
-        }
-        uint32_t pf[kSets][2];
+          l[0] += pr[0] + pr[2];
+          l[1] += pr[1] + pr[3];
+          const uint32_t pf[2] = {transpose8x8(pack_f16(w[0], w[1])), transpose8x8(pack_f16(w[2], w[3]))};
+          // V: chunk r of tokens 2c, 2c+1, 8+2c, 9+2c
+          uint32_t vw[4][4];
 #pragma unroll
-        for (int u = 0; u < kSets; ++u) {
-          l[u][0] += pr[u][0] + pr[u][2];
-          l[u][1] += pr[u][1] + pr[u][3];
-          pf[u][0] = transpose8x8(pack_f16(w[u][0], w[u][1]));
-          pf[u][1] = transpose8x8(pack_f16(w[u][2], w[u][3]));
-        }
-        // V: chunk r of tokens 2c, 2c+1, 8+2c, 9+2c
-        uint32_t vw[4][4];
+          for (int j = 0; j < 4; ++j) {
+            const uint4 q4 = *reinterpret_cast<const uint4*>(stage + v_at + ((j / 2) * 8 + j % 2) * kRowStep);
+            vw[j][0] = q4.x, vw[j][1] = q4.y, vw[j][2] = q4.z, vw[j][3] = q4.w;
+          }
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const uint4 q4 = *reinterpret_cast<const uint4*>(stage + v_at + ((j / 2) * 8 + j % 2) * kRowStep);
-          vw[j][0] = q4.x, vw[j][1] = q4.y, vw[j][2] = q4.z, vw[j][3] = q4.w;
-        }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          // a dim's codes of two tokens side by side in the low half
-          const uint32_t sel = i % 2 ? 0x0062 : 0x0040, sel1 = i % 2 ? 0x0073 : 0x0051;
-          const uint32_t a[4] = {f16_of(__byte_perm(vw[0][i / 2], vw[1][i / 2], sel)),
-                                 f16_of(__byte_perm(vw[0][i / 2], vw[1][i / 2], sel1)),
-                                 f16_of(__byte_perm(vw[2][i / 2], vw[3][i / 2], sel)),
-                                 f16_of(__byte_perm(vw[2][i / 2], vw[3][i / 2], sel1))};
-#pragma unroll
-          for (int u = 0; u < kSets; ++u) mma16816(o[u][i], a, pf[u][0], pf[u][1]);
+          for (int i = 0; i < 8; ++i) {
+            // a dim's codes of two tokens side by side in the low half
+            const uint32_t sel = i % 2 ? 0x0062 : 0x0040, sel1 = i % 2 ? 0x0073 : 0x0051;
+            const uint32_t a[4] = {f16_of(__byte_perm(vw[0][i / 2], vw[1][i / 2], sel)),
+                                   f16_of(__byte_perm(vw[0][i / 2], vw[1][i / 2], sel1)),
+                                   f16_of(__byte_perm(vw[2][i / 2], vw[3][i / 2], sel)),
+                                   f16_of(__byte_perm(vw[2][i / 2], vw[3][i / 2], sel1))};
+            mma16816(o[i], a, pf[0], pf[1]);
+          }
         }
       }
+      cp_async_wait<0>();
     }
-    cp_async_wait<0>();
-  }
 
 #pragma unroll
-  for (int u = 0; u < kSets; ++u) {
-#pragma unroll
     for (int h = 0; h < 2; ++h) {
-      W[u][h] *= 1.0f / kOneW;
+      W[h] *= 1.0f / kOneW;
 #pragma unroll
-      for (int d = 4; d <= 16; d *= 2) l[u][h] += __shfl_xor_sync(0xffffffffu, l[u][h], d);
+      for (int d = 4; d <= 16; d *= 2) l[h] += __shfl_xor_sync(0xffffffffu, l[h], d);
     }
-  }
-  if (split > 1) {
-    // the warps of a head join in shared memory: each leaves its result, part
-    // 0 gathers (m and l by head, values by head and dim)
-    __syncthreads();
-    float* left = reinterpret_cast<float*>(smem + warp * C::kLeft);  // [kHeads][2], then [kHeads][128]
-#pragma unroll
-    for (int u = 0; u < kSets; ++u) {
+    if (C::kSplit > 1) {
+      // the warps of a head join in shared memory: each leaves its result, part
+      // 0 gathers (m and l by head, values by head and dim)
+      __syncthreads();
+      float* left = reinterpret_cast<float*>(smem + warp * C::kLeft);  // [8][2], then [8][128]
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const int hh = u * 8 + 2 * c + h;
-        if (r == 0) left[2 * hh] = m[u][h], left[2 * hh + 1] = l[u][h];
+        const int hh = 2 * c + h;
+        if (r == 0) left[2 * hh] = m[h], left[2 * hh + 1] = l[h];
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-          *reinterpret_cast<float2*>(left + 2 * kHeads + hh * kHeadDim + 16 * r + 2 * i) =
-              make_float2(o[u][i][h] * W[u][h], o[u][i][2 + h] * W[u][h]);
+          *reinterpret_cast<float2*>(left + 16 + hh * kHeadDim + 16 * r + 2 * i) = make_float2(o[i][h] * W[h], o[i][2 + h] * W[h]);
       }
-    }
-    __syncthreads();
-    if (part > 0) continue;  // the next table's barrier holds until part 0 has read
-#pragma unroll
-    for (int u = 0; u < kSets; ++u) {
+      __syncthreads();
+      if (part > 0) continue;  // the next segment's barriers hold until part 0 has read
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const int hh = u * 8 + 2 * c + h;
+        const int hh = 2 * c + h;
         float sum = 0.f, top = kLowest;
-        for (int w = 0; w < split; ++w)
-          top = fmaxf(top, reinterpret_cast<const float*>(smem + (warp + w * p.cta_heads) * C::kLeft)[2 * hh]);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) o[u][i][h] = o[u][i][2 + h] = 0.f;
-        for (int w = 0; w < split; ++w) {
-          const float* from = reinterpret_cast<const float*>(smem + (warp + w * p.cta_heads) * C::kLeft);
+        for (int w = 0; w < C::kSplit; ++w)
+          top = fmaxf(top, reinterpret_cast<const float*>(smem + (warp + w * C::kHeads) * C::kLeft)[2 * hh]);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) o[i][h] = o[i][2 + h] = 0.f;
+#pragma unroll 2
+        for (int w = 0; w < C::kSplit; ++w) {
+          const float* from = reinterpret_cast<const float*>(smem + (warp + w * C::kHeads) * C::kLeft);
           const float f = ex2(from[2 * hh] - top);
           sum = fmaf(from[2 * hh + 1], f, sum);
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            const float2 v = *reinterpret_cast<const float2*>(from + 2 * kHeads + hh * kHeadDim + 16 * r + 2 * i);
-            o[u][i][h] = fmaf(f, v.x, o[u][i][h]), o[u][i][2 + h] = fmaf(f, v.y, o[u][i][2 + h]);
+            const float2 v = *reinterpret_cast<const float2*>(from + 16 + hh * kHeadDim + 16 * r + 2 * i);
+            o[i][h] = fmaf(f, v.x, o[i][h]), o[i][2 + h] = fmaf(f, v.y, o[i][2 + h]);
           }
         }
-        m[u][h] = top, l[u][h] = sum, W[u][h] = 1.f;
+        m[h] = top, l[h] = sum, W[h] = 1.f;
       }
     }
-  }
 
 #pragma unroll
-  for (int u = 0; u < kSets; ++u) {
-#pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const int hh = u * 8 + 2 * c + h;
+      const int hh = 2 * c + h;
       if (hh >= heads) continue;
-      const float f = l[u][h] == 0.f ? 0.f : W[u][h] / l[u][h];  // a NaN sum stays one
+      const float f = l[h] == 0.f ? 0.f : W[h] / l[h];  // a NaN sum stays one
       float x[16];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[2 * i] = o[u][i][h] * f, x[2 * i + 1] = o[u][i][2 + h] * f;
-      const int64_t hr = (int64_t)row_now * p.num_q_heads + h0 + hh;
+      for (int i = 0; i < 8; ++i) x[2 * i] = o[i][h] * f, x[2 * i + 1] = o[i][2 + h] * f;
       if (slot_out >= 0) {
-        const int64_t to = ((int64_t)slot_out * p.cta_heads + warp) * p.part_heads + hh;
+        const int64_t to = ((int64_t)slot_out * C::kHeads + head_in) * p.part_heads + hh;
         float4* dst = reinterpret_cast<float4*>(p.part_o + to * kHeadDim + 16 * r);
 #pragma unroll
         for (int i = 0; i < 4; ++i) dst[i] = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
-        if (r == 0) p.part_lse[to] = l[u][h] == 0.f ? -INFINITY : m[u][h] + log2f(l[u][h]);
+        if (r == 0) p.part_lse[to] = l[h] == 0.f ? -INFINITY : m[h] + log2f(l[h]);
         continue;
       }
+      const int64_t hr = (int64_t)row_now * p.num_q_heads + h0 + hh;
       if (p.gate) {
         const uint4* src = reinterpret_cast<const uint4*>(p.gate + hr * kHeadDim + 16 * r);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const uint4 w4 = src[i];
+          const uint4 w4 = __ldg(src + i);
           const uint32_t b[4] = {w4.x, w4.y, w4.z, w4.w};
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
@@ -531,13 +508,13 @@ __global__ void __launch_bounds__(32 * kBdWarps, BdCfg<kHeads, kCh>::kCtas)
       dst[1] = make_uint4(b[4], b[5], b[6], b[7]);
     }
   }
-  }  // segments
 }
 
 // Valid length of each row for the plan: its count, or the place past its last
 // index that is not negative. A CTA a row, from the row's end.
 constexpr int kLenThreads = 256;
 __global__ void __launch_bounds__(kLenThreads) qsa_block_lengths_kernel(const __grid_constant__ BlockDecodeParams p) {
+  launch_dependents();
   const int row = blockIdx.x;
   const int count = p.counts ? min(max(__ldg(p.counts + row), 0), p.topk) : p.topk;
   const int32_t* list = p.indices + (int64_t)row * p.indices_stride;
@@ -564,8 +541,11 @@ __global__ void __launch_bounds__(kLenThreads) qsa_block_lengths_kernel(const __
 // place has one: its zeros), the number of CTAs that share them, and the row
 // that each begins in. One CTA; a thread takes consecutive rows.
 constexpr int kPlanThreads = 1024;
+constexpr int kPlanWaves = 1;
 constexpr int kPlanUnits = 8;  // units a CTA gets at least, so that small work has few pieces
 __global__ void __launch_bounds__(kPlanThreads) qsa_block_plan_kernel(const __grid_constant__ BlockDecodeParams p, int max_ctas) {
+  launch_dependents();
+  wait_for_prerequisites();
   const int t = threadIdx.x;
   const int unit = kBdWarps / p.cta_heads * kBdTile;
   const int hgroups = p.virtual_heads / p.cta_heads;
@@ -602,59 +582,75 @@ __global__ void __launch_bounds__(kPlanThreads) qsa_block_plan_kernel(const __gr
   const int64_t units = total * hgroups;
   const int ctas = (int)min((int64_t)max_ctas, (units + kPlanUnits - 1) / kPlanUnits);
   int64_t before = run - mine + (t >= 32 ? sums[t / 32 - 1] : 0);
-  if (t == 0) p.plan->units = units, p.plan->ctas = ctas, p.prefix[0] = 0;
   for (int r = r0; r < r1; ++r) {
-    const int64_t n = max(1, (int)(((int64_t)p.lengths[r] + unit - 1) / unit));
-    // CTAs whose first unit, b units / ctas, lies in this row
-    const int64_t lo = before * hgroups, hi = (before + n) * hgroups;
-    for (int64_t b = (lo * ctas + units - 1) / units; b < ctas && b * units / ctas < hi; ++b)
-      if (b * units / ctas >= lo) p.first_row[b] = r;
-    before += n;
-    p.prefix[r + 1] = before;
+    p.prefix[r] = before;
+    before += max(1, (int)(((int64_t)p.lengths[r] + unit - 1) / unit));
+  }
+  if (t == 0) p.plan->ctas = ctas, p.prefix[p.rows] = total;
+  __syncthreads();
+  // CTA b begins at unit b units / ctas, in the last row that begins before it
+  for (int b = t; b <= ctas; b += kPlanThreads) {
+    const int64_t x = b * units / ctas;
+    int lo = 0, hi = p.rows - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) / 2;
+      if (p.prefix[mid] * hgroups <= x) lo = mid;
+      else hi = mid - 1;
+    }
+    p.plan->cut[b] = x;
+    p.plan->first_row[b] = lo;
+    // what is joined at this cut: a row and head group that it is the first to
+    // cut; its last piece is of the last CTA that begins before its end
+    const int64_t row_at = p.prefix[lo] * hgroups, row_units = p.prefix[lo + 1] - p.prefix[lo];
+    const int hg = (int)(x - row_at) / (int)row_units;
+    const int64_t begin = row_at + hg * row_units;
+    const bool first = b > 0 && b < ctas && x > begin && (b - 1) * units / ctas <= begin;
+    p.plan->joins[b] = first ? make_int4(lo, hg, (int)(((begin + row_units) * ctas - 1) / units), 0) : make_int4(-1, 0, 0, 0);
   }
 }
 
-// Joins the pieces of one (row, query head) a warp, in the plan's order; a row
-// that one CTA took whole is done.
-__global__ void __launch_bounds__(256) qsa_block_join_kernel(const __grid_constant__ BlockDecodeParams p) {
+// Joins the pieces of the rows that the plan cut, in the plan's order. CTA
+// (b - 1, y) takes what is joined at the cut before planned CTA b, for virtual
+// head y of its group; a warp a query head.
+__global__ void __launch_bounds__(256, 6) qsa_block_join_kernel(const __grid_constant__ BlockDecodeParams p) {
+  wait_for_prerequisites();
+  const int b = blockIdx.x + 1;
+  const int ctas = p.plan->ctas;
+  const int4 what = p.plan->joins[b];
+  if (b >= ctas || what.x < 0) return;
+  const int row = what.x, hg = what.y, last = what.z;
   const int lane = threadIdx.x % 32;
-  const int64_t hr = (int64_t)blockIdx.x * 8 + threadIdx.x / 32;
-  if (hr >= (int64_t)p.rows * p.num_q_heads) return;
-  const int row = (int)(hr / p.num_q_heads), h = (int)(hr % p.num_q_heads);
-  const int in_group = h % p.group;
-  const int gv = h / p.group * p.head_parts + in_group / p.part_heads;
-  const int hgroups = p.virtual_heads / p.cta_heads;
-  const int64_t units = p.plan->units, ctas = p.plan->ctas;
-  const int64_t n = p.prefix[row + 1] - p.prefix[row];
-  const int64_t x0 = p.prefix[row] * hgroups + gv / p.cta_heads * n;
-  // unit x is CTA b's where b units / ctas <= x < (b + 1) units / ctas
-  const int b0 = (int)(((x0 + 1) * ctas - 1) / units), b1 = (int)(((x0 + n) * ctas - 1) / units);
-  if (b0 == b1) return;
-  auto piece = [&](int b) -> int64_t {  // the first piece is its CTA's second kind
-    return ((int64_t)(2 * b + (b == b0 ? 1 : 0)) * p.cta_heads + gv % p.cta_heads) * p.part_heads + in_group % p.part_heads;
-  };
-  float top = -INFINITY;
-  for (int b = b0 + lane; b <= b1; b += 32) top = fmaxf(top, p.part_lse[piece(b)]);
+  const int gv = hg * p.cta_heads + blockIdx.y;
+  const int in_group = gv % p.head_parts * p.part_heads;
+  const int heads = min(p.part_heads, p.group - in_group);
+  for (int hh = threadIdx.x / 32; hh < heads; hh += 8) {
+    // the first piece is its CTA's second kind
+    auto piece = [&](int at) -> int64_t {
+      return ((int64_t)(2 * at + (at == b - 1 ? 1 : 0)) * p.cta_heads + blockIdx.y) * p.part_heads + hh;
+    };
+    float top = -INFINITY;
+    for (int at = b - 1 + lane; at <= last; at += 32) top = fmaxf(top, p.part_lse[piece(at)]);
 #pragma unroll
-  for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-  float acc[4] = {0.f, 0.f, 0.f, 0.f}, sum = 0.f;
-#pragma unroll 4
-  for (int b = b0; b <= b1; ++b) {
-    const int64_t from = piece(b);
-    const float lse = p.part_lse[from];
-    const float4 v = *reinterpret_cast<const float4*>(p.part_o + from * kHeadDim + lane * 4);
-    const float w = lse == -INFINITY ? 0.f : exp2f(lse - top);
-    sum += w;
-    acc[0] = fmaf(w, v.x, acc[0]), acc[1] = fmaf(w, v.y, acc[1]);
-    acc[2] = fmaf(w, v.z, acc[2]), acc[3] = fmaf(w, v.w, acc[3]);
+    for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+    float acc[4] = {0.f, 0.f, 0.f, 0.f}, sum = 0.f;
+#pragma unroll 8
+    for (int at = b - 1; at <= last; ++at) {
+      const int64_t from = piece(at);
+      const float lse = p.part_lse[from];
+      const float4 v = *reinterpret_cast<const float4*>(p.part_o + from * kHeadDim + lane * 4);
+      const float w = lse == -INFINITY ? 0.f : exp2f(lse - top);
+      sum += w;
+      acc[0] = fmaf(w, v.x, acc[0]), acc[1] = fmaf(w, v.y, acc[1]);
+      acc[2] = fmaf(w, v.z, acc[2]), acc[3] = fmaf(w, v.w, acc[3]);
+    }
+    const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+    const int64_t off = ((int64_t)row * p.num_q_heads + gv / p.head_parts * p.group + in_group + hh) * kHeadDim + lane * 4;
+#pragma unroll
+    for (int d = 0; d < 4; ++d) acc[d] *= inv * (p.gate ? sigmoid(__bfloat162float(p.gate[off + d])) : 1.f);
+    const __nv_bfloat162 a = __floats2bfloat162_rn(acc[0], acc[1]), c = __floats2bfloat162_rn(acc[2], acc[3]);
+    *reinterpret_cast<uint2*>(p.out + off) =
+        make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&c));
   }
-  const float inv = sum == 0.f ? 0.f : 1.0f / sum;
-  const int64_t off = hr * kHeadDim + lane * 4;
-#pragma unroll
-  for (int d = 0; d < 4; ++d) acc[d] *= inv * (p.gate ? sigmoid(__bfloat162float(p.gate[off + d])) : 1.f);
-  const __nv_bfloat162 a = __floats2bfloat162_rn(acc[0], acc[1]), b = __floats2bfloat162_rn(acc[2], acc[3]);
-  *reinterpret_cast<uint2*>(p.out + off) =
-      make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
 }
 
 int sm_count() {
@@ -670,11 +666,28 @@ int sm_count() {
 }
 
 int64_t align256(int64_t x) { return (x + 255) / 256 * 256; }
-int planned_ctas(const BlockDecodeParams& p) { return sm_count() * (p.part_heads > 8 ? BdCfg<16, 1>::kCtas : BdCfg<8, 1>::kCtas); }
+int planned_ctas() { return min(2 * kPlanWaves * sm_count(), kPlanMaxCtas); }
 
-template <int kHeads, int kCh>
+// Launches a kernel that waits for its prerequisites itself (early = true: it
+// may start before the stream's last kernel has ended).
+template <typename Kernel, typename... Args>
+cudaError_t start(Kernel kernel, dim3 grid, int threads, int smem, bool early, cudaStream_t stream, Args... args) {
+  cudaLaunchConfig_t config = {};
+  config.gridDim = grid;
+  config.blockDim = dim3(threads);
+  config.dynamicSmemBytes = smem;
+  config.stream = stream;
+  cudaLaunchAttribute attr = {};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = &attr;
+  config.numAttrs = early ? 1 : 0;
+  return cudaLaunchKernelEx(&config, kernel, args...);
+}
+
+template <int kParts, int kCh>
 cudaError_t launch(const BlockDecodeParams& p, cudaStream_t stream) {
-  using C = BdCfg<kHeads, kCh>;
+  using C = BdCfg<kParts, kCh>;
   // the shared memory beyond the default limit, once per device
   static std::atomic<uint64_t> ready{0};
   int dev = 0;
@@ -682,35 +695,38 @@ cudaError_t launch(const BlockDecodeParams& p, cudaStream_t stream) {
   if (e != cudaSuccess) return e;
   const uint64_t bit = 1ull << (dev & 63);
   if (!(ready.load(std::memory_order_acquire) & bit)) {
-    e = cudaFuncSetAttribute(qsa_block_decode_kernel<kHeads, kCh>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+    e = cudaFuncSetAttribute(qsa_block_decode_kernel<kParts, kCh>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
     if (e != cudaSuccess) return e;
     ready.fetch_or(bit, std::memory_order_acq_rel);
   }
-  const int64_t grid = p.plan ? planned_ctas(p) : (int64_t)p.rows * (p.virtual_heads / p.cta_heads);
+  const int64_t grid = p.plan ? planned_ctas() : (int64_t)p.rows * (p.num_kv_heads / kCh);
   if (grid > 0x7fffffffll) return cudaErrorInvalidValue;
-  qsa_block_decode_kernel<kHeads, kCh><<<(unsigned)grid, C::kThreads, C::kSmem, stream>>>(p);
-  return cudaGetLastError();
+  return start(qsa_block_decode_kernel<kParts, kCh>, dim3((unsigned)grid), C::kThreads, C::kSmem, p.plan != nullptr, stream, p);
 }
 
-template <int kHeads>
-cudaError_t launch(const BlockDecodeParams& p, cudaStream_t stream) {
-  switch (p.cta_heads / p.head_parts) {
-    case 1: return launch<kHeads, 1>(p, stream);
-    case 2: return launch<kHeads, 2>(p, stream);
-    case 4: return launch<kHeads, 4>(p, stream);
-    default: return launch<kHeads, 8>(p, stream);
+cudaError_t launch_main(const BlockDecodeParams& p, cudaStream_t stream) {
+  switch (p.head_parts * 16 + p.cta_heads / p.head_parts) {
+    case 16 + 1: return launch<1, 1>(p, stream);
+    case 16 + 2: return launch<1, 2>(p, stream);
+    case 16 + 4: return launch<1, 4>(p, stream);
+    case 16 + 8: return launch<1, 8>(p, stream);
+    case 32 + 1: return launch<2, 1>(p, stream);
+    case 32 + 2: return launch<2, 2>(p, stream);
+    case 32 + 4: return launch<2, 4>(p, stream);
+    case 64 + 1: return launch<4, 1>(p, stream);
+    case 64 + 2: return launch<4, 2>(p, stream);
+    default: return cudaErrorInvalidValue;
   }
 }
 
 }  // namespace
 
 int64_t block_decode_plan(BlockDecodeParams& p) {
-  // a group above 16 goes as two virtual KV heads
-  p.head_parts = p.group > 16 ? 2 : 1;
+  p.head_parts = p.group <= 8 ? 1 : p.group <= 16 ? 2 : 4;
   p.part_heads = (p.group + p.head_parts - 1) / p.head_parts;
   p.virtual_heads = p.num_kv_heads * p.head_parts;
-  p.cta_heads = 1;
-  while (p.cta_heads < 8 && p.virtual_heads % (2 * p.cta_heads) == 0) p.cta_heads *= 2;
+  p.cta_heads = p.head_parts;
+  while (p.cta_heads < kBdWarps && p.virtual_heads % (2 * p.cta_heads) == 0) p.cta_heads *= 2;
   // mul = ceil(2^(31 + shift) / block) with block <= 2^shift: n mul exceeds
   // n 2^(31 + shift) / block by less than n, so n / block is exact for n < 2^31
   uint32_t shift = 0;
@@ -719,14 +735,14 @@ int64_t block_decode_plan(BlockDecodeParams& p) {
   p.block_mul = (uint32_t)((((uint64_t)1 << (31 + shift)) + p.block_size - 1) / p.block_size);
   p.planned = p.topk > kBdDirect;
   if (!p.planned) return 0;
-  const int64_t pieces = 2ll * planned_ctas(p) * p.cta_heads * p.part_heads;
+  const int64_t pieces = 2ll * planned_ctas() * p.cta_heads * p.part_heads;
   return align256(pieces * kHeadDim * 4) + align256(pieces * 4) + align256((int64_t)sizeof(BlockDecodePlan)) +
-         align256(8ll * (p.rows + 1)) + align256(4ll * p.rows) + align256(4ll * planned_ctas(p));
+         align256(8ll * (p.rows + 1)) + align256(4ll * p.rows);
 }
 
 void block_decode_place(BlockDecodeParams& p, void* workspace) {
   char* at = static_cast<char*>(workspace);
-  const int64_t pieces = 2ll * planned_ctas(p) * p.cta_heads * p.part_heads;
+  const int64_t pieces = 2ll * planned_ctas() * p.cta_heads * p.part_heads;
   auto take = [&](int64_t bytes) {
     char* here = at;
     at += align256(bytes);
@@ -737,19 +753,16 @@ void block_decode_place(BlockDecodeParams& p, void* workspace) {
   p.plan = reinterpret_cast<BlockDecodePlan*>(take(sizeof(BlockDecodePlan)));
   p.prefix = reinterpret_cast<int64_t*>(take(8ll * (p.rows + 1)));
   p.lengths = reinterpret_cast<int*>(take(4ll * p.rows));
-  p.first_row = reinterpret_cast<int*>(take(4ll * planned_ctas(p)));
 }
 
 cudaError_t launch_block_decode(const BlockDecodeParams& p, cudaStream_t stream) {
-  if (p.plan) {
-    if (p.indices) qsa_block_lengths_kernel<<<p.rows, kLenThreads, 0, stream>>>(p);
-    qsa_block_plan_kernel<<<1, kPlanThreads, 0, stream>>>(p, planned_ctas(p));
-  }
-  cudaError_t e = p.part_heads > 8 ? launch<16>(p, stream) : launch<8>(p, stream);
-  if (e != cudaSuccess || !p.plan) return e;
-  const int64_t warps = (int64_t)p.rows * p.num_q_heads;
-  qsa_block_join_kernel<<<(unsigned)((warps + 7) / 8), 256, 0, stream>>>(p);
-  return cudaGetLastError();
+  if (!p.plan) return launch_main(p, stream);
+  cudaError_t e = cudaSuccess;
+  if (p.indices) e = start(qsa_block_lengths_kernel, dim3(p.rows), kLenThreads, 0, false, stream, p);
+  if (e == cudaSuccess) e = start(qsa_block_plan_kernel, dim3(1), kPlanThreads, 0, p.indices != nullptr, stream, p, planned_ctas());
+  if (e == cudaSuccess) e = launch_main(p, stream);
+  if (e == cudaSuccess) e = start(qsa_block_join_kernel, dim3(planned_ctas() - 1, p.cta_heads), 256, 0, true, stream, p);
+  return e;
 }
 
 }  // namespace qsa

@@ -192,13 +192,15 @@ struct BlockDecodeParams {
   struct BlockDecodePlan* plan;  // null: a CTA takes a whole row
   int64_t* prefix;               // [rows + 1] units of one head group before each row
   int* lengths;                  // [rows] columns up to the last valid one
-  int* first_row;                // [ctas] row that each CTA begins in
   float* part_o;                 // [2 ctas, cta_heads, part_heads, 128] normalised results of pieces of rows
   float* part_lse;               // [2 ctas, cta_heads, part_heads] their log2-sum-exp2, -inf for none
 };
+constexpr int kPlanMaxCtas = 2048;
 struct BlockDecodePlan {
-  int64_t units;
   int ctas;
+  int4 joins[kPlanMaxCtas + 1];     // row, head group and last CTA of what is joined at a CTA's begin, or -1
+  int first_row[kPlanMaxCtas + 1];  // row that each CTA begins in
+  int64_t cut[kPlanMaxCtas + 1];    // its first unit
 };
 // Chooses the split and gives the workspace's size; places it in a workspace.
 int64_t block_decode_plan(BlockDecodeParams& p);
