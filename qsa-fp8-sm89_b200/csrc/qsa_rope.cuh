@@ -1,9 +1,11 @@
 // One 128-element head by a half warp: load, RMS norm, position rotation.
 //
-// Lane l of the 16 holds elements 8l .. 8l+7. A norm is then 8 products and
-// 4 shuffles; the partner of element d in a rotation of half h = rotary / 2
-// is element d + h, 8 | h, so whole lanes exchange: lane l and lane l + h/8
-// (adjacent pairs stay inside a lane). Everything is fp32; the caller rounds.
+// Lane l of the 16 holds two pieces of 4 elements. Where pairs are (j, j + R/2)
+// of R rotated elements, lanes below R/8 hold elements 4l .. 4l+3 and R/2 + 4l
+// .. + 3, which are the two sides of pairs 4l .. 4l+3; the others, and all lanes
+// where pairs are neighbours, hold elements 8l .. 8l+7. A rotation then needs
+// no exchange between lanes, and four cosines and sines a lane in either form.
+// A norm takes 4 shuffles. Everything is fp32; the caller rounds.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -18,76 +20,82 @@ namespace qsa {
 
 constexpr int kRowLanes = 16;  // lanes of a row, 8 elements each
 
-// 8 consecutive elements as loaded (16 bytes, or 32 in fp32), widened later
-// so that several rows' loads can be in flight together
+// First elements of a lane's two pieces.
+struct Pieces {
+  int a, b;
+};
+__device__ __forceinline__ Pieces lane_pieces(const RopeParams& p, int l) {
+  if (p.table && !p.interleaved && l < (p.rotary >> 3)) return {4 * l, (p.rotary >> 1) + 4 * l};
+  return {8 * l, 8 * l + 4};
+}
+
+// A lane's 8 elements as loaded, widened later so that several rows' loads can
+// be in flight together.
 template <typename T>
 struct Raw8 {
-  uint4 w[sizeof(T) / 2];
+  typename std::conditional<sizeof(T) == 4, uint4, uint2>::type a, b;
 };
 
 template <typename T>
-__device__ __forceinline__ void load8(const T* src, Raw8<T>& r) {
-  const uint4* p = reinterpret_cast<const uint4*>(src);
-#pragma unroll
-  for (int i = 0; i < (int)(sizeof(T) / 2); ++i) r.w[i] = p[i];
+__device__ __forceinline__ void load8(const T* row, Pieces at, Raw8<T>& r) {
+  using W = decltype(r.a);
+  r.a = *reinterpret_cast<const W*>(row + at.a);
+  r.b = *reinterpret_cast<const W*>(row + at.b);
+}
+
+__device__ __forceinline__ void widen4(const uint4& w, float* x, float) {
+  x[0] = __uint_as_float(w.x), x[1] = __uint_as_float(w.y), x[2] = __uint_as_float(w.z), x[3] = __uint_as_float(w.w);
+}
+__device__ __forceinline__ void widen4(const uint2& w, float* x, __nv_bfloat16) {
+  const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w.x));
+  const float2 g = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w.y));
+  x[0] = f.x, x[1] = f.y, x[2] = g.x, x[3] = g.y;
+}
+__device__ __forceinline__ void widen4(const uint2& w, float* x, __half) {
+  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w.x));
+  const float2 g = __half22float2(*reinterpret_cast<const __half2*>(&w.y));
+  x[0] = f.x, x[1] = f.y, x[2] = g.x, x[3] = g.y;
 }
 
 template <typename T>
 __device__ __forceinline__ void widen8(const Raw8<T>& r, float (&x)[8]) {
-  if constexpr (sizeof(T) == 4) {
-    const uint32_t w[8] = {r.w[0].x, r.w[0].y, r.w[0].z, r.w[0].w, r.w[1].x, r.w[1].y, r.w[1].z, r.w[1].w};
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = __uint_as_float(w[i]);
-  } else {
-    const uint32_t w[4] = {r.w[0].x, r.w[0].y, r.w[0].z, r.w[0].w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      float2 f;
-      if constexpr (std::is_same<T, __nv_bfloat16>::value)
-        f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[i]));
-      else
-        f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-      x[2 * i] = f.x;
-      x[2 * i + 1] = f.y;
-    }
-  }
+  widen4(r.a, x, T());
+  widen4(r.b, x + 4, T());
+}
+
+__device__ __forceinline__ void store4(float* dst, const float* x) {
+  *reinterpret_cast<float4*>(dst) = make_float4(x[0], x[1], x[2], x[3]);
+}
+__device__ __forceinline__ void store4(__nv_bfloat16* dst, const float* x) {
+  const __nv_bfloat162 a = __floats2bfloat162_rn(x[0], x[1]), b = __floats2bfloat162_rn(x[2], x[3]);
+  *reinterpret_cast<uint2*>(dst) =
+      make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+}
+__device__ __forceinline__ void store4(__half* dst, const float* x) {
+  const __half2 a = __floats2half2_rn(x[0], x[1]), b = __floats2half2_rn(x[2], x[3]);
+  *reinterpret_cast<uint2*>(dst) =
+      make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
 }
 
 template <typename T>
-__device__ __forceinline__ void store8(T* dst, const float (&x)[8]) {
-  uint4* p = reinterpret_cast<uint4*>(dst);
-  if constexpr (sizeof(T) == 4) {
-    p[0] = make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
-    p[1] = make_uint4(__float_as_uint(x[4]), __float_as_uint(x[5]), __float_as_uint(x[6]), __float_as_uint(x[7]));
-  } else {
-    uint32_t w[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-        const __nv_bfloat162 h = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
-        w[i] = *reinterpret_cast<const uint32_t*>(&h);
-      } else {
-        const __half2 h = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
-        w[i] = *reinterpret_cast<const uint32_t*>(&h);
-      }
-    }
-    *p = make_uint4(w[0], w[1], w[2], w[3]);
-  }
+__device__ __forceinline__ void store8(T* row, Pieces at, const float (&x)[8]) {
+  store4(row + at.a, x);
+  store4(row + at.b, x + 4);
 }
 
-// Elements 8l .. 8l+7 of a norm weight.
-__device__ __forceinline__ void load_weight8(const void* weight, int dtype, int l, float (&w)[8]) {
+// A lane's elements of a norm weight.
+__device__ __forceinline__ void load_weight8(const void* weight, int dtype, Pieces at, float (&w)[8]) {
   if (dtype == QSA_B200_DTYPE_F32) {
     Raw8<float> r;
-    load8(static_cast<const float*>(weight) + 8 * l, r);
+    load8(static_cast<const float*>(weight), at, r);
     widen8(r, w);
   } else if (dtype == QSA_B200_DTYPE_F16) {
     Raw8<__half> r;
-    load8(static_cast<const __half*>(weight) + 8 * l, r);
+    load8(static_cast<const __half*>(weight), at, r);
     widen8(r, w);
   } else {
     Raw8<__nv_bfloat16> r;
-    load8(static_cast<const __nv_bfloat16*>(weight) + 8 * l, r);
+    load8(static_cast<const __nv_bfloat16*>(weight), at, r);
     widen8(r, w);
   }
 }
@@ -104,88 +112,64 @@ __device__ __forceinline__ void rms_norm8(float (&x)[8], const float (&w)[8], fl
   for (int i = 0; i < 8; ++i) x[i] = x[i] * r * w[i];
 }
 
-// A lane's cosines and sines: for adjacent pairs the first four are its four
-// pairs', for split halves element i's pair (8 (l mod h/8) + i).
-struct Turn8 {
-  float c[8], s[8];
-  bool in;  // the token's positions lie inside the table
+// The cosines and sines of a lane's pairs 4l .. 4l+3.
+struct Turn4 {
+  float c[4], s[4];
+  bool turns;  // the lane holds rotated elements
+  bool in;     // the token's positions lie inside the table
 };
 
-// Position of the token on the axis of pair j. `own`: the position where the
-// rotation has no list of positions.
-__device__ __forceinline__ int rope_position(const RopeParams& p, int64_t token, int64_t own, int j) {
-  if (!p.positions) return own > 0x7fffffffll ? 0x7fffffff : (int)own;
+// Axis of pair j.
+__device__ __forceinline__ int rope_axis(const RopeParams& p, int j) {
   int axis = 0;
-  if (p.axes > 1) {
 #pragma unroll
-    for (int a = 0; a < kRopeMaxAxes - 1; ++a) axis += (a + 1 < p.axes && j >= p.ends[a]) ? 1 : 0;
-  }
+  for (int a = 0; a < kRopeMaxAxes - 1; ++a) axis += (a + 1 < p.axes && j >= p.ends[a]) ? 1 : 0;
+  return axis;
+}
+
+// The token's position on an axis; `own` where the rotation has no list.
+__device__ __forceinline__ int rope_position(const RopeParams& p, int64_t token, int64_t own, int axis) {
+  if (!p.positions) return own > 0x7fffffffll ? 0x7fffffff : (int)own;
   return __ldg(p.positions + axis * p.axis_stride + token);
 }
 
-// Must run in every lane of the half warp (lanes past the rotated elements
-// get the identity). Reads nothing outside the table.
-__device__ __forceinline__ void load_turn8(const RopeParams& p, int64_t token, int64_t own, int l, Turn8& t) {
-#pragma unroll
-  for (int i = 0; i < 8; ++i) t.c[i] = 1.f, t.s[i] = 0.f;
+// Reads nothing outside the table.
+__device__ __forceinline__ void load_turn4(const RopeParams& p, int64_t token, int64_t own, int l, Turn4& t) {
   t.in = true;
-  const int half = p.rotary >> 1;
-  const int lanes = p.rotary >> 3;  // lanes that hold rotated elements
-  if (p.axes == 1) {
-    const int pos = rope_position(p, token, own, 0);
-    t.in = pos >= 0 && pos < p.table_len;
-  } else {
-    for (int a = 0; a < p.axes; ++a) {
-      const int pos = __ldg(p.positions + a * p.axis_stride + token);
-      t.in = t.in && pos >= 0 && pos < p.table_len;
-    }
+  for (int a = 0; a < p.axes; ++a) {
+    const int pos = rope_position(p, token, own, a);
+    t.in = t.in && pos >= 0 && pos < p.table_len;
   }
-  if (!t.in || l >= lanes) return;
-  const int n = p.interleaved ? 4 : 8;                          // pairs of this lane
-  const int j0 = p.interleaved ? 4 * l : 8 * (l % (lanes >> 1));  // the first of them
+  t.turns = t.in && l < (p.rotary >> 3);
+  if (!t.turns) return;
+  const int half = p.rotary >> 1;
   if (p.quads) {
-#pragma unroll
-    for (int i = 0; i < 8; i += 4) {
-      if (i >= n) break;
-      const float* row = p.table + (int64_t)rope_position(p, token, own, j0 + i) * p.rotary + j0 + i;
-      const float4 c = __ldg(reinterpret_cast<const float4*>(row));
-      const float4 s = __ldg(reinterpret_cast<const float4*>(row + half));
-      t.c[i] = c.x, t.c[i + 1] = c.y, t.c[i + 2] = c.z, t.c[i + 3] = c.w;
-      t.s[i] = s.x, t.s[i + 1] = s.y, t.s[i + 2] = s.z, t.s[i + 3] = s.w;
-    }
+    const float* row = p.table + (int64_t)rope_position(p, token, own, rope_axis(p, 4 * l)) * p.rotary + 4 * l;
+    const float4 c = __ldg(reinterpret_cast<const float4*>(row));
+    const float4 s = __ldg(reinterpret_cast<const float4*>(row + half));
+    t.c[0] = c.x, t.c[1] = c.y, t.c[2] = c.z, t.c[3] = c.w;
+    t.s[0] = s.x, t.s[1] = s.y, t.s[2] = s.z, t.s[3] = s.w;
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      if (i >= n) break;
-      const float* row = p.table + (int64_t)rope_position(p, token, own, j0 + i) * p.rotary + j0 + i;
+    for (int i = 0; i < 4; ++i) {
+      const float* row = p.table + (int64_t)rope_position(p, token, own, rope_axis(p, 4 * l + i)) * p.rotary + 4 * l + i;
       t.c[i] = __ldg(row);
       t.s[i] = __ldg(row + half);
     }
   }
 }
 
-// Rotates the half warp's row. Every lane of the warp takes part in the
-// exchange.
-__device__ __forceinline__ void rotate8(const RopeParams& p, const Turn8& t, int l, float (&x)[8]) {
-  if (p.interleaved) {
-    if (l < (p.rotary >> 3)) {
+__device__ __forceinline__ void rotate8(const RopeParams& p, const Turn4& t, float (&x)[8]) {
+  auto turn = [&](float& a, float& b, int i) {
+    const float u = a * t.c[i] - b * t.s[i], v = b * t.c[i] + a * t.s[i];
+    a = u, b = v;
+  };
+  if (t.turns && p.interleaved) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float a = x[2 * i], b = x[2 * i + 1];
-        x[2 * i] = a * t.c[i] - b * t.s[i];
-        x[2 * i + 1] = b * t.c[i] + a * t.s[i];
-      }
-    }
-  } else {
-    const int hl = p.rotary >> 4;  // lanes of one half
-    const int partner = l < hl ? l + hl : l < 2 * hl ? l - hl : l;
-    const float sign = l < hl ? -1.f : 1.f;
+    for (int i = 0; i < 4; ++i) turn(x[2 * i], x[2 * i + 1], i);
+  } else if (t.turns) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float other = __shfl_sync(0xffffffffu, x[i], partner, kRowLanes);
-      // past the rotated elements 0 * infinity would be NaN
-      x[i] = l < 2 * hl ? x[i] * t.c[i] + sign * other * t.s[i] : x[i];
-    }
+    for (int i = 0; i < 4; ++i) turn(x[i], x[4 + i], i);
   }
   if (!t.in) {
 #pragma unroll
