@@ -6,11 +6,13 @@
 //
 // Bound by HBM: a new row is read once (128 elements) and written once (128
 // bytes). A block belongs to one request, so one group of warps owns a (block,
-// KV head, K or V) and needs no atomics. A warp holds 16 rows of it in
-// registers as fp32, a half warp a row (qsa_rope.cuh), from their loads over
-// the block's maximum to their stores: one warp for blocks of up to 16 tokens,
-// 2 to 8 for up to 128, which share their maxima in shared memory. Larger
-// blocks are read twice, 128 rows at a time.
+// KV head, K or V) and needs no atomics. A warp holds 8 rows of it in registers
+// as fp32, a half warp a row (qsa_rope.cuh), from their loads over the block's
+// maximum to their stores; up to 8 warps share a block of up to 64 tokens and
+// exchange their maxima in shared memory. Larger blocks are read twice, 64 rows
+// at a time. A group goes through up to 8 heads of its block: where it lies and
+// the cosines and sines of its rows are looked up once for them, and a head's
+// rows are loaded while the one before is worked on.
 //
 // Entry e has at most floor(n_e / B) + 2 blocks of B tokens, so its blocks get
 // the slots floor(cu[e] / B) + 2e + j, which never overlap and end below
@@ -27,254 +29,366 @@ namespace qsa {
 namespace {
 
 constexpr int kApWarps = 8;
-constexpr int kApSteps = 8;                   // row pairs that a warp holds
+constexpr int kApSteps = 4;                   // row pairs that a warp holds
 constexpr int kApRows = 2 * kApSteps;
+constexpr int kApHeads = 8;                   // heads that a group goes through, at most
 constexpr float kMinScale = 1.17549435e-38f;  // 2^-126: 1 / scale stays finite
+
+// x / s rounded to nearest, inv = 1 / s within a few ulp: a product and a
+// residual step. (An IEEE division for each element costs several times as
+// much; without the step, ties of x / s fall to the other side more often.)
+__device__ __forceinline__ float divide(float x, float s, float inv) {
+  const float q = x * inv;
+  return fmaf(fmaf(-q, s, x), inv, q);
+}
 
 __device__ __forceinline__ uint32_t to_e4m3(const float* x) {
   return (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(x[0], x[1]), __NV_SATFINITE, __NV_E4M3) |
          (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(x[2], x[3]), __NV_SATFINITE, __NV_E4M3) << 16;
 }
 
+// Whole numbers stay in 32 bits (a 64-bit division is over 100 instructions,
+// and a warp makes several): logical positions are below 2^32 where a start
+// and a count of tokens, both below 2^31, are added.
 struct ApBlock {
-  int64_t token;  // first new token of the block
-  int64_t pos;    // its logical position
-  int kept;       // rows of the block before it that stay
-  int count;      // new rows, 0: there is no such block
-  int64_t req;    // block-table row
+  int token;     // first new token of the block
+  uint32_t pos;  // its logical position
+  int kept;      // rows of the block before it that stay
+  int count;     // new rows, 0: there is no such block
+  int req;       // block-table row
 };
 
 // The block of a slot, but for its page.
-__device__ __forceinline__ ApBlock find_block(const BlockAppendParams& p, int64_t slot, int lane) {
-  const int B = p.block_size;
-  int e = 0;
-  int64_t j = 0, first = slot, count = 1;
+__device__ __forceinline__ ApBlock find_block(const BlockAppendParams& p, uint32_t slot, int lane) {
+  const uint32_t B = p.block_size;
+  int e = 0, first = (int)slot, count = 1;
+  uint32_t j = 0;
+  bool is = true;
   if (p.cu_tokens) {
     // the last entry whose first slot, floor(cu[e] / B) + 2e, is <= slot
     for (int n = p.entries; n > 1;) {
       const int step = (n + 31) / 32;
       const int at = e + lane * step;
-      const bool below = lane * step < n && (int64_t)(__ldg(p.cu_tokens + at) / B) + 2 * (int64_t)at <= slot;
+      const bool below = lane * step < n && (uint32_t)max(__ldg(p.cu_tokens + at), 0) / B + 2u * at <= slot;
       const int k = max(__popc(__ballot_sync(0xffffffffu, below)) - 1, 0);
       e += k * step;
       n = min(step, n - k * step);
     }
     first = min(max(__ldg(p.cu_tokens + e), 0), p.tokens);
     count = min(max(__ldg(p.cu_tokens + e + 1), 0), p.tokens) - first;
-    j = slot - (first / B + 2 * (int64_t)e);
+    const uint32_t slot0 = (uint32_t)first / B + 2u * e;
+    is = count > 0 && slot >= slot0;
+    j = slot - slot0;
   } else {
     e = (int)slot;
   }
-  const int64_t start = __ldg(p.starts + e);
+  const int start = __ldg(p.starts + e);
   ApBlock b;
   b.req = p.reqs ? __ldg(p.reqs + e) : e;
-  const int64_t base = (start / B + j) * B;  // logical position of the block's row 0
-  const int64_t from = max(base, start), to = min(base + B, start + count);
-  b.token = first + (from - start);
-  b.pos = from;
-  b.kept = (int)(from - base);
-  b.count = count <= 0 || j < 0 || start < 0 || from >= to ? 0 : (int)(to - from);
+  const uint32_t lead = (uint32_t)max(start, 0) % B;  // rows of the first block that stay
+  const uint32_t skip = j == 0 ? 0 : j * B - lead;    // new tokens before this block
+  b.kept = j == 0 ? (int)lead : 0;
+  b.token = first + (int)skip;
+  b.pos = (uint32_t)start + skip;
+  b.count = is && start >= 0 && j <= (uint32_t)count / B + 1 && skip < (uint32_t)count
+                ? (int)min(B - (uint32_t)b.kept, (uint32_t)count - skip)
+                : 0;
   return b;
 }
 
-// Physical slot of the block's row 0, -1 where it has no page.
-__device__ __forceinline__ int64_t block_slot(const BlockAppendParams& p, const ApBlock& b) {
-  const int64_t base = b.pos - b.kept;
-  const int64_t lp = base / p.page_size;
-  if (b.count == 0 || b.req < 0 || b.req >= p.num_reqs || lp >= p.pages_per_req) return -1;
-  const int64_t page = __ldg(p.btable + b.req * p.btable_stride + lp);
-  return page < 0 || page >= p.num_pages ? -1 : page * p.page_size + base % p.page_size;
+// Physical page of a block, -1 where it has none; off: its row 0 in the page.
+__device__ __forceinline__ int block_page(const BlockAppendParams& p, const ApBlock& b, uint32_t& off) {
+  const uint32_t base = b.pos - b.kept;
+  const uint32_t lp = base / (uint32_t)p.page_size;
+  off = base - lp * p.page_size;
+  if (b.count == 0 || b.req < 0 || b.req >= p.num_reqs || lp >= (uint32_t)p.pages_per_req) return -1;
+  const int page = __ldg(p.btable + b.req * p.btable_stride + lp);
+  return page < 0 || page >= p.num_pages ? -1 : page;
 }
 
-// kHold: the group's warps hold all rows of a block.
-template <typename T, bool kHold>
-__global__ void __launch_bounds__(32 * kApWarps, 2)
-    qsa_block_append_kernel(const __grid_constant__ BlockAppendParams p, int64_t items, int group) {
-  __shared__ float tops[kApWarps];
+enum { kPlain = 0, kHalves = 1, kNeighbours = 2 };  // no rotation; its pairs
+
+// One group's blocks: see the kernel. kTurn: the rows are rotated.
+template <typename T, bool kHold, int kTurn>
+__device__ __forceinline__ void append_block(const BlockAppendParams& p, const ApBlock& b, bool is_k, int g0, int group,
+                                             int per, float (*tops)[kApWarps]) {
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int l = lane % kRowLanes, side = lane / kRowLanes;
-  const int64_t item = (int64_t)blockIdx.x * (kApWarps / group) + warp / group;
-  // neighbours are the heads of one block: their rows of the rotation's table
-  // are the same
-  const int g = (int)(item % p.num_kv_heads);
-  const bool is_k = item / p.num_kv_heads % 2 == 0;
-  ApBlock b = {};
-  if (item < items) b = find_block(p, item / p.num_kv_heads / 2, lane);
-  const bool norm = is_k && p.k_weight, turn = is_k && p.rope.table;
-  RopeParams rope = p.rope;
-  if (!turn) rope.table = nullptr;
-  const Pieces pieces = lane_pieces(rope, l);
-  const T* src = static_cast<const T*>(is_k ? p.k : p.v) + (int64_t)g * kHeadDim;
+  const bool norm = is_k && p.k_weight;
+  const int turning = kTurn == kPlain ? 0 : p.rope.rotary >> 3;  // lanes that hold rotated elements
+  const bool halves = kTurn == kHalves && l < turning;
+  const Pieces pieces = halves ? Pieces{4 * l, (p.rope.rotary >> 1) + 4 * l} : Pieces{8 * l, 8 * l + 4};
+  const T* src = static_cast<const T*>(is_k ? p.k : p.v);
+
+  // The half warp's rows of the block's new ones: row0, row0 + 2, ... Past the
+  // last row the last one is read again, which changes no maximum.
+  const int row0 = warp % group * kApRows + side;
+  auto clamped = [&](int row) { return b.count > 0 ? b.token + min(row, b.count - 1) : 0; };
+  const T* rows[kApSteps];
+#pragma unroll
+  for (int i = 0; i < kApSteps; ++i) rows[i] = src + (int64_t)clamped(row0 + 2 * i) * p.token_stride;
+  auto load = [&](int g, Raw8<T> (&raw)[kApSteps]) {
+    g = min(g, p.num_kv_heads - 1);
+#pragma unroll
+    for (int i = 0; i < kApSteps; ++i) load8(rows[i] + g * kHeadDim, pieces, raw[i]);
+  };
+  Raw8<T> raw[kApSteps];
+  load(g0, raw);
   float w[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) w[i] = 1.f;
   if (norm) load_weight8(p.k_weight, p.weight_dtype, pieces, w);
+  uint32_t off;
+  const int page = block_page(p, b, off);
+  const int step = p.num_kv_heads * kHeadDim;
+  uint8_t* cache = (is_k ? p.k_cache : p.v_cache) + ((int64_t)max(page, 0) * p.page_size + off) * step;
+  float* scales = (is_k ? p.k_scales : p.v_scales) +
+                  ((int64_t)max(page, 0) * (p.page_size / p.block_size) + off / (uint32_t)p.block_size) * p.num_kv_heads;
+  const int kept = page < 0 ? 0 : b.kept;
 
-  // Row pairs row0, row0 + 2, ... of the block's new rows: zeros past the last
-  const int row0 = warp % group * kApRows + side;
-  auto load = [&](int first, Raw8<T> (&raw)[kApSteps]) {
-#pragma unroll
-    for (int i = 0; i < kApSteps; ++i) {
-      raw[i] = {};
-      if (first + 2 * i < b.count) load8(src + (b.token + first + 2 * i) * p.token_stride, pieces, raw[i]);
+  // The rotation of a row: the lane's cosines and sines; false outside the table
+  auto load_turn = [&](int row, float4& c, float4& sn) {
+    bool in = true;
+    const int64_t token = clamped(row);
+    const uint32_t own = b.pos + min(row, max(b.count - 1, 0));
+    for (int a = 0; a < p.rope.axes; ++a) {
+      const int pos = rope_position(p.rope, token, own, a);
+      in = in && pos >= 0 && pos < p.rope.table_len;
     }
+    if (!in || l >= turning) return in;
+    const int half = p.rope.rotary >> 1;
+    if (p.rope.quads) {
+      const float* at = p.rope.table + (int64_t)rope_position(p.rope, token, own, rope_axis(p.rope, 4 * l)) * p.rope.rotary + 4 * l;
+      c = __ldg(reinterpret_cast<const float4*>(at));
+      sn = __ldg(reinterpret_cast<const float4*>(at + half));
+    } else {
+      float v[8];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float* at = p.rope.table + (int64_t)rope_position(p.rope, token, own, rope_axis(p.rope, 4 * l + i)) * p.rope.rotary + 4 * l + i;
+        v[i] = __ldg(at), v[4 + i] = __ldg(at + half);
+      }
+      c = make_float4(v[0], v[1], v[2], v[3]), sn = make_float4(v[4], v[5], v[6], v[7]);
+    }
+    return in;
   };
-  auto value = [&](int row, const Raw8<T>& raw, float (&x)[8]) {
-    widen8(raw, x);
+  float4 cs[kTurn == kPlain || !kHold ? 1 : kApSteps], sn[kTurn == kPlain || !kHold ? 1 : kApSteps];
+  uint32_t inside = 0xffffffffu;  // bit i: row i's positions lie inside the table
+  if (kTurn != kPlain && kHold) {
+#pragma unroll
+    for (int i = 0; i < kApSteps; ++i)
+      if (!load_turn(row0 + 2 * i, cs[i], sn[i])) inside &= ~(1u << i);
+  }
+  auto value = [&](const Raw8<T>& from, const float4& c, const float4& s, bool in, float (&x)[8]) {
+    widen8(from, x);
     if (norm) rms_norm8(x, w, p.eps);
-    if (turn && row < b.count) {
-      Turn4 t;
-      load_turn4(rope, b.token + row, b.pos + row, l, t);
-      rotate8(rope, t, x);
+    if constexpr (kTurn != kPlain) {
+      const float cc[4] = {c.x, c.y, c.z, c.w}, ss[4] = {s.x, s.y, s.z, s.w};
+      if (l < turning) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float &u = x[kTurn == kHalves ? i : 2 * i], &v = x[kTurn == kHalves ? 4 + i : 2 * i + 1];
+          const float y = u * cc[i] - v * ss[i];
+          v = v * cc[i] + u * ss[i];
+          u = y;
+        }
+      }
+      if (!in) {
+#pragma unroll
+        for (int d = 0; d < 8; ++d) x[d] = 0.f;
+      }
     }
   };
-  // the largest |x|, over the group; NaN counts for none, infinity neither
-  auto largest = [&](float top, bool again) {
+  auto row_top = [&](const float (&x)[8], float top) {  // NaN counts for none
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    if (group > 1) {
-      if (again) __syncthreads();
-      if (lane == 0) tops[warp] = top;
-      __syncthreads();
-      for (int i = 0; i < group; ++i) top = fmaxf(top, tops[warp / group * group + i]);
-    }
+    for (int d = 0; d < 8; ++d) top = fmaxf(top, fabsf(x[d]));
     return top;
   };
+  auto finite_top = [&](const float (&x)[8], float top) {
+#pragma unroll
+    for (int d = 0; d < 8; ++d) top = fabsf(x[d]) <= FLT_MAX ? fmaxf(top, fabsf(x[d])) : top;
+    return top;
+  };
+  // largest of values that are not negative: their bits order as they do
+  auto warp_max = [](float v) { return __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(v))); };
+  auto group_max = [&](int slot) { return warp_max(tops[slot][warp / group * group + lane % group]); };
 
-  Raw8<T> raw[kApSteps];
-  load(row0, raw);
-  const int64_t slot = block_slot(p, b);
-  const int64_t step = (int64_t)p.num_kv_heads * kHeadDim;
-  uint8_t* dst = (is_k ? p.k_cache : p.v_cache) + max(slot, (int64_t)0) * step + (int64_t)g * kHeadDim;
-  float* scale = (is_k ? p.k_scales : p.v_scales) + max(slot, (int64_t)0) / p.block_size * p.num_kv_heads + g;
-  const int kept = slot < 0 ? 0 : b.kept;
-  const float old = kept > 0 ? *scale : 0.f;
-  uint2 codes[kApSteps];  // of kept rows
-  if (kHold && kept > 0) {
-#pragma unroll
-    for (int i = 0; i < kApSteps; ++i)
-      if (row0 + 2 * i < kept) codes[i] = *reinterpret_cast<const uint2*>(dst + (row0 + 2 * i) * step + 8 * l);
-  }
-
-  float x[kHold ? kApSteps : 1][8];
-  float top = 0.f;
-  if constexpr (kHold) {
-#pragma unroll
-    for (int i = 0; i < kApSteps; ++i) {
-      value(row0 + 2 * i, raw[i], x[i]);
-#pragma unroll
-      for (int d = 0; d < 8; ++d) top = fmaxf(top, fabsf(x[i][d]));
-    }
-  } else {
-    for (int first = row0; first - row0 < b.count; first += kApWarps * kApRows) {
-      if (first > row0) load(first, raw);
-#pragma unroll
-      for (int i = 0; i < kApSteps; ++i) {
-        value(first + 2 * i, raw[i], x[0]);
-#pragma unroll
-        for (int d = 0; d < 8; ++d)
-          if (fabsf(x[0][d]) <= FLT_MAX) top = fmaxf(top, fabsf(x[0][d]));
-      }
-    }
-  }
-  top = largest(top, false);
-  const bool infinite = top > FLT_MAX;
-  if constexpr (kHold) {
-    if (__syncthreads_or(infinite)) {  // rare, and then for the whole CTA
-      float finite = 0.f;
+#pragma unroll 1
+  for (int h = 0; h < per; ++h) {  // as often for every warp of the CTA
+    const int g = g0 + h;
+    const bool live = page >= 0 && g < p.num_kv_heads;
+    uint8_t* dst = cache + g * kHeadDim;
+    float* scale = scales + g;
+    const float old = live && kept > 0 ? *scale : 0.f;
+    uint2 codes[kApSteps];  // of kept rows
+    if (kHold && live && kept > 0) {
 #pragma unroll
       for (int i = 0; i < kApSteps; ++i)
-#pragma unroll
-        for (int d = 0; d < 8; ++d)
-          if (fabsf(x[i][d]) <= FLT_MAX) finite = fmaxf(finite, fabsf(x[i][d]));
-      top = largest(finite, true);
+        if (row0 + 2 * i < kept) codes[i] = *reinterpret_cast<const uint2*>(dst + (int64_t)(row0 + 2 * i) * step + 8 * l);
     }
-  }
-  if (slot < 0) return;
-  const float s = fmaxf(old, fmaxf(__fdiv_rn(top, 448.f), kMinScale));
-  const float inv = __fdiv_rn(1.f, s);
-  // x / s rounded to nearest: a product with the reciprocal and a residual step
-  // (an IEEE division for each element costs several times as much; without
-  // the step, ties of x / s fall to the other side more often)
-  auto store = [&](int row, float (&v)[8]) {
+    float x[kHold ? kApSteps : 1][8];
+    float top = 0.f;
+    // larger blocks: the rows again, 64 at a time, through `with`
+    auto each_row = [&](auto with) {
+      for (int first = row0; first - row0 < b.count; first += kApWarps * kApRows) {
 #pragma unroll
-    for (int d = 0; d < 8; ++d) {
-      const float q = v[d] * inv;
-      const float r = fmaf(-q, s, v[d]);
-      v[d] = fabsf(q) <= FLT_MAX ? fmaf(r, inv, q) : q;
-    }
-    uint8_t* to = dst + (b.kept + row) * step;
-    const uint32_t u0 = to_e4m3(v), u1 = to_e4m3(v + 4);
-    if (pieces.b == pieces.a + 4) {
-      *reinterpret_cast<uint2*>(to + pieces.a) = make_uint2(u0, u1);
+        for (int i = 0; i < kApSteps; ++i) {
+          load8(src + (int64_t)clamped(first + 2 * i) * p.token_stride + min(g, p.num_kv_heads - 1) * kHeadDim, pieces, raw[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < kApSteps; ++i) {
+          const bool in = kTurn == kPlain || load_turn(first + 2 * i, cs[0], sn[0]);
+          value(raw[i], cs[0], sn[0], in, x[0]);
+          with(first + 2 * i);
+        }
+      }
+    };
+    if constexpr (kHold) {
+#pragma unroll
+      for (int i = 0; i < kApSteps; ++i) {
+        const int j = kTurn == kPlain ? 0 : i;
+        value(raw[i], cs[j], sn[j], (inside >> i) & 1u, x[i]);
+        top = row_top(x[i], top);
+      }
+      if (h + 1 < per) load(g + 1, raw);
     } else {
-      *reinterpret_cast<uint32_t*>(to + pieces.a) = u0;
-      *reinterpret_cast<uint32_t*>(to + pieces.b) = u1;
+      each_row([&](int) { top = finite_top(x[0], top); });
     }
-  };
-  if constexpr (kHold) {
+    top = warp_max(top);
+    bool infinite = top > FLT_MAX;
+    if (group > 1) {
+      // the buffers alternate: a warp that sets one again has passed the
+      // barrier after the last readings of it
+      if (lane == 0) tops[h % 2][warp] = top;
+      infinite = __syncthreads_or(infinite);
+      top = group_max(h % 2);
+    }
+    if constexpr (kHold) {
+      if (infinite) {  // rare: once more, without the infinities
+        top = 0.f;
 #pragma unroll
-    for (int i = 0; i < kApSteps; ++i)
-      if (row0 + 2 * i < b.count) store(row0 + 2 * i, x[i]);
-  } else {
-    for (int first = row0; first - row0 < b.count; first += kApWarps * kApRows) {
-      load(first, raw);
-#pragma unroll
-      for (int i = 0; i < kApSteps; ++i) {
-        value(first + 2 * i, raw[i], x[0]);
-        if (first + 2 * i < b.count) store(first + 2 * i, x[0]);
+        for (int i = 0; i < kApSteps; ++i) top = finite_top(x[i], top);
+        top = warp_max(top);
+        if (group > 1) {
+          if (lane == 0) tops[2][warp] = top;
+          __syncthreads();
+          top = group_max(2);
+        }
       }
+    } else {
+      infinite = true;  // not known: only the finite ones were looked at
     }
-  }
-  if (old == s) return;
-  const float ratio = __fdiv_rn(old, s);
-  auto rescale = [&](int row, uint2 was) {
-    const uint32_t c[2] = {was.x, was.y};
-    float v[8];
+    if (!live) continue;
+    const float s = fmaxf(old, fmaxf(divide(top, 448.f, 1.0f / 448.f), kMinScale));
+    const float inv = __fdividef(1.f, s);  // s is below 2^126
+    auto store = [&](int row, float (&v)[8]) {
+      if (infinite) {  // an infinity's residual would be NaN
 #pragma unroll
-    for (int d = 0; d < 4; ++d) {
-      const float2 f = e4m3x2_to_f32x2((uint16_t)(c[d / 2] >> (16 * (d % 2))));
-      v[2 * d] = f.x * ratio;
-      v[2 * d + 1] = f.y * ratio;
-    }
-    *reinterpret_cast<uint2*>(dst + row * step + 8 * l) = make_uint2(to_e4m3(v), to_e4m3(v + 4));
-  };
-  if constexpr (kHold) {
+        for (int d = 0; d < 8; ++d) v[d] = fabsf(v[d]) > FLT_MAX ? v[d] : divide(v[d], s, inv);
+      } else {
 #pragma unroll
-    for (int i = 0; i < kApSteps; ++i)
-      if (row0 + 2 * i < kept) rescale(row0 + 2 * i, codes[i]);
-  } else {
-    for (int first = row0; first < kept; first += kApWarps * kApRows)
+        for (int d = 0; d < 8; ++d) v[d] = divide(v[d], s, inv);
+      }
+      uint8_t* to = dst + (int64_t)(b.kept + row) * step;
+      const uint32_t u0 = to_e4m3(v), u1 = to_e4m3(v + 4);
+      if (halves) {
+        *reinterpret_cast<uint32_t*>(to + pieces.a) = u0;
+        *reinterpret_cast<uint32_t*>(to + pieces.b) = u1;
+      } else {
+        *reinterpret_cast<uint2*>(to + pieces.a) = make_uint2(u0, u1);
+      }
+    };
+    if constexpr (kHold) {
 #pragma unroll
       for (int i = 0; i < kApSteps; ++i)
-        if (first + 2 * i < kept)
-          rescale(first + 2 * i, *reinterpret_cast<const uint2*>(dst + (first + 2 * i) * step + 8 * l));
+        if (row0 + 2 * i < b.count) store(row0 + 2 * i, x[i]);
+    } else {
+      each_row([&](int row) {
+        if (row < b.count) store(row, x[0]);
+      });
+    }
+    if (old == s) continue;
+    const float ratio = divide(old, s, inv);
+    auto rescale = [&](int row, uint2 was) {
+      const uint32_t c[2] = {was.x, was.y};
+      float v[8];
+#pragma unroll
+      for (int d = 0; d < 4; ++d) {
+        const float2 f = e4m3x2_to_f32x2((uint16_t)(c[d / 2] >> (16 * (d % 2))));
+        v[2 * d] = f.x * ratio;
+        v[2 * d + 1] = f.y * ratio;
+      }
+      *reinterpret_cast<uint2*>(dst + (int64_t)row * step + 8 * l) = make_uint2(to_e4m3(v), to_e4m3(v + 4));
+    };
+    if constexpr (kHold) {
+      if (kept > 0) {
+#pragma unroll
+        for (int i = 0; i < kApSteps; ++i)
+          if (row0 + 2 * i < kept) rescale(row0 + 2 * i, codes[i]);
+      }
+    } else {
+      for (int row = row0; row < kept; row += 2)
+        if ((row - row0) / 2 % (kApWarps * kApSteps) < kApSteps)
+          rescale(row, *reinterpret_cast<const uint2*>(dst + (int64_t)row * step + 8 * l));
+    }
+    if (warp % group == 0 && lane == 0) *scale = s;
   }
-  if (warp % group == 0 && lane == 0) *scale = s;
+}
+
+// kHold: the group's warps hold all rows of a block. per: heads of a group.
+template <typename T, bool kHold, int kTurn>
+__global__ void __launch_bounds__(32 * kApWarps, 2)
+    qsa_block_append_kernel(const __grid_constant__ BlockAppendParams p, uint32_t items, int group, int per) {
+  __shared__ float tops[3][kApWarps];
+  const uint32_t parts = (p.num_kv_heads + per - 1) / per;
+  // K's groups come first, then V's: a CTA's warps do the same work
+  const uint32_t item = blockIdx.x * (kApWarps / group) + threadIdx.x / 32 / group;
+  const bool is_k = blockIdx.y == 0;
+  const uint32_t slot = item / parts;
+  const int g0 = (int)(item - slot * parts) * per;
+  ApBlock b = {};
+  if (item < items) b = find_block(p, slot, threadIdx.x % 32);
+  if (is_k)
+    append_block<T, kHold, kTurn>(p, b, true, g0, group, per, tops);
+  else
+    append_block<T, kHold, kPlain>(p, b, false, g0, group, per, tops);
+}
+
+template <typename T, bool kHold>
+cudaError_t launch(const BlockAppendParams& p, int64_t slots, cudaStream_t stream) {
+  int group = 1;
+  while (group < kApWarps && group * kApRows < p.block_size) group *= 2;
+  // more heads a group while 148 SMs of 16 warps are filled twice
+  int per = 1;
+  while (per < kApHeads && per < p.num_kv_heads && slots * 2 * ((p.num_kv_heads + 2 * per - 1) / (2 * per)) * group >= 148 * 32)
+    per *= 2;
+  const int64_t items = slots * ((p.num_kv_heads + per - 1) / per);
+  const int64_t blocks = (items * group + kApWarps - 1) / kApWarps;
+  if (items > 0xffffffffll - kApWarps || blocks > 0x7fffffffll) return cudaErrorInvalidValue;
+  const dim3 grid((unsigned)blocks, 2);
+  const int threads = 32 * kApWarps;
+  if (!p.rope.table)
+    qsa_block_append_kernel<T, kHold, kPlain><<<grid, threads, 0, stream>>>(p, (uint32_t)items, group, per);
+  else if (!p.rope.interleaved)
+    qsa_block_append_kernel<T, kHold, kHalves><<<grid, threads, 0, stream>>>(p, (uint32_t)items, group, per);
+  else
+    qsa_block_append_kernel<T, kHold, kNeighbours><<<grid, threads, 0, stream>>>(p, (uint32_t)items, group, per);
+  return cudaGetLastError();
 }
 
 template <typename T>
-cudaError_t launch(const BlockAppendParams& p, int64_t items, cudaStream_t stream) {
-  int group = 1;
-  while (group < kApWarps && group * kApRows < p.block_size) group *= 2;
-  const int64_t grid = (items * group + kApWarps - 1) / kApWarps;
-  if (grid > 0x7fffffffll) return cudaErrorInvalidValue;
-  if (p.block_size <= kApWarps * kApRows)
-    qsa_block_append_kernel<T, true><<<(unsigned)grid, 32 * kApWarps, 0, stream>>>(p, items, group);
-  else
-    qsa_block_append_kernel<T, false><<<(unsigned)grid, 32 * kApWarps, 0, stream>>>(p, items, group);
-  return cudaGetLastError();
+cudaError_t launch_type(const BlockAppendParams& p, int64_t slots, cudaStream_t stream) {
+  return p.block_size <= kApWarps * kApRows ? launch<T, true>(p, slots, stream) : launch<T, false>(p, slots, stream);
 }
 
 }  // namespace
 
 cudaError_t launch_block_append(const BlockAppendParams& p, cudaStream_t stream) {
   const int64_t slots = p.cu_tokens ? (int64_t)(p.tokens / p.block_size) + 2 * (int64_t)p.entries : p.entries;
-  const int64_t items = slots * p.num_kv_heads * 2;
   switch (p.dtype) {
-    case QSA_B200_DTYPE_BF16: return launch<__nv_bfloat16>(p, items, stream);
-    case QSA_B200_DTYPE_F16: return launch<__half>(p, items, stream);
-    default: return launch<float>(p, items, stream);
+    case QSA_B200_DTYPE_BF16: return launch_type<__nv_bfloat16>(p, slots, stream);
+    case QSA_B200_DTYPE_F16: return launch_type<__half>(p, slots, stream);
+    default: return launch_type<float>(p, slots, stream);
   }
 }
 

@@ -22,7 +22,7 @@ __global__ void __launch_bounds__(kQrThreads) qsa_qk_rope_kernel(const __grid_co
   const int parts = q_parts + (p.heads[1] + per - 1) / per;
   const int64_t at = (int64_t)blockIdx.x * (kQrThreads / kRowLanes) + threadIdx.x / kRowLanes;
   const bool live = at < (int64_t)p.tokens * parts;  // every lane goes through the norm's exchanges
-  const int64_t token = live ? at / parts : 0;
+  const int64_t token = live ? (at <= 0xffffffffll ? (uint32_t)at / (uint32_t)parts : at / parts) : 0;
   const int part = live ? (int)(at - token * parts) : 0;
   const int which = part >= q_parts ? 1 : 0;
   const int h0 = (part - which * q_parts) * per;

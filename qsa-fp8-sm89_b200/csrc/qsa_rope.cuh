@@ -128,13 +128,13 @@ __device__ __forceinline__ int rope_axis(const RopeParams& p, int j) {
 }
 
 // The token's position on an axis; `own` where the rotation has no list.
-__device__ __forceinline__ int rope_position(const RopeParams& p, int64_t token, int64_t own, int axis) {
-  if (!p.positions) return own > 0x7fffffffll ? 0x7fffffff : (int)own;
+__device__ __forceinline__ int rope_position(const RopeParams& p, int64_t token, uint32_t own, int axis) {
+  if (!p.positions) return (int)min(own, 0x7fffffffu);
   return __ldg(p.positions + axis * p.axis_stride + token);
 }
 
 // Reads nothing outside the table.
-__device__ __forceinline__ void load_turn4(const RopeParams& p, int64_t token, int64_t own, int l, Turn4& t) {
+__device__ __forceinline__ void load_turn4(const RopeParams& p, int64_t token, uint32_t own, int l, Turn4& t) {
   t.in = true;
   for (int a = 0; a < p.axes; ++a) {
     const int pos = rope_position(p, token, own, a);
