@@ -10,7 +10,8 @@
 // as fp32, a half warp a row (qsa_rope.cuh), from their loads over the block's
 // maximum to their stores; up to 8 warps share a block of up to 64 tokens and
 // exchange their maxima in shared memory. Larger blocks are read twice, 64 rows
-// at a time. A group goes through up to 8 heads of its block: where it lies and
+// at a time; blocks of up to 4 tokens go several to a warp, each row with the
+// scale of its own block. A group goes through up to 8 heads of its block: where it lies and
 // the cosines and sines of its rows are looked up once for them, and a head's
 // rows are loaded while the one before is worked on.
 //
@@ -20,6 +21,7 @@
 // slot finds its entry by a search that splits the list 32 ways a step. The new
 // rows' loads go out before the block table is read, and a kept block's codes
 // before it is known whether its scale grows.
+#include <atomic>
 #include <cfloat>
 
 #include "qsa_common.cuh"
@@ -31,6 +33,7 @@ namespace {
 constexpr int kApWarps = 8;
 constexpr int kApSteps = 4;                   // row pairs that a warp holds
 constexpr int kApRows = 2 * kApSteps;
+constexpr int kApStages = 2;                  // heads whose rows are under way or at hand
 constexpr int kApHeads = 8;                   // heads that a group goes through, at most
 constexpr float kMinScale = 1.17549435e-38f;  // 2^-126: 1 / scale stays finite
 
@@ -58,9 +61,8 @@ struct ApBlock {
   int req;       // block-table row
 };
 
-// The block of a slot, but for its page.
-__device__ __forceinline__ ApBlock find_block(const BlockAppendParams& p, uint32_t slot, int lane) {
-  const uint32_t B = p.block_size;
+// The block of a slot, but for its page. B: tokens of a block.
+__device__ __forceinline__ ApBlock find_block(const BlockAppendParams& p, uint32_t slot, int lane, uint32_t B) {
   int e = 0, first = (int)slot, count = 1;
   uint32_t j = 0;
   bool is = true;
@@ -108,10 +110,91 @@ __device__ __forceinline__ int block_page(const BlockAppendParams& p, const ApBl
 
 enum { kPlain = 0, kHalves = 1, kNeighbours = 2 };  // no rotation; its pairs
 
+// A lane's cosines and sines of a row; false where a position lies outside the
+// table.
+__device__ __forceinline__ bool row_turn(const RopeParams& p, int64_t token, uint32_t own, int l, int turning, float4& c,
+                                         float4& s) {
+  bool in = true;
+  for (int a = 0; a < p.axes; ++a) {
+    const int pos = rope_position(p, token, own, a);
+    in = in && pos >= 0 && pos < p.table_len;
+  }
+  if (!in || l >= turning) return in;
+  const int half = p.rotary >> 1;
+  if (p.quads) {
+    const float* at = p.table + (int64_t)rope_position(p, token, own, rope_axis(p, 4 * l)) * p.rotary + 4 * l;
+    c = __ldg(reinterpret_cast<const float4*>(at));
+    s = __ldg(reinterpret_cast<const float4*>(at + half));
+  } else {
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float* at = p.table + (int64_t)rope_position(p, token, own, rope_axis(p, 4 * l + i)) * p.rotary + 4 * l + i;
+      v[i] = __ldg(at), v[4 + i] = __ldg(at + half);
+    }
+    c = make_float4(v[0], v[1], v[2], v[3]), s = make_float4(v[4], v[5], v[6], v[7]);
+  }
+  return in;
+}
+
+template <int kTurn>
+__device__ __forceinline__ void turn_row(const float4& c, const float4& s, bool in, bool turns, float (&x)[8]) {
+  if constexpr (kTurn != kPlain) {
+    const float cc[4] = {c.x, c.y, c.z, c.w}, ss[4] = {s.x, s.y, s.z, s.w};
+    if (turns) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float &u = x[kTurn == kHalves ? i : 2 * i], &v = x[kTurn == kHalves ? 4 + i : 2 * i + 1];
+        const float y = u * cc[i] - v * ss[i];
+        v = v * cc[i] + u * ss[i];
+        u = y;
+      }
+    }
+    if (!in) {
+#pragma unroll
+      for (int d = 0; d < 8; ++d) x[d] = 0.f;
+    }
+  }
+}
+
+// Eight values over their scale, as codes.
+__device__ __forceinline__ uint2 quantise8(float (&v)[8], float s, float inv, bool infinite) {
+  if (infinite) {  // an infinity's residual would be NaN
+#pragma unroll
+    for (int d = 0; d < 8; ++d) v[d] = fabsf(v[d]) > FLT_MAX ? v[d] : divide(v[d], s, inv);
+  } else {
+#pragma unroll
+    for (int d = 0; d < 8; ++d) v[d] = divide(v[d], s, inv);
+  }
+  return make_uint2(to_e4m3(v), to_e4m3(v + 4));
+}
+
+// Eight codes over a larger scale.
+__device__ __forceinline__ uint2 rescale8(uint2 was, float ratio) {
+  const uint32_t c[2] = {was.x, was.y};
+  float v[8];
+#pragma unroll
+  for (int d = 0; d < 4; ++d) {
+    const float2 f = e4m3x2_to_f32x2((uint16_t)(c[d / 2] >> (16 * (d % 2))));
+    v[2 * d] = f.x * ratio;
+    v[2 * d + 1] = f.y * ratio;
+  }
+  return make_uint2(to_e4m3(v), to_e4m3(v + 4));
+}
+
+__device__ __forceinline__ void store_codes(uint8_t* row, Pieces at, bool halves, uint2 codes) {
+  if (halves) {
+    *reinterpret_cast<uint32_t*>(row + at.a) = codes.x;
+    *reinterpret_cast<uint32_t*>(row + at.b) = codes.y;
+  } else {  // the two pieces are one
+    *reinterpret_cast<uint2*>(row + at.a) = codes;
+  }
+}
+
 // One group's blocks: see the kernel. kTurn: the rows are rotated.
 template <typename T, bool kHold, int kTurn>
 __device__ __forceinline__ void append_block(const BlockAppendParams& p, const ApBlock& b, bool is_k, int g0, int group,
-                                             int per, float (*tops)[kApWarps]) {
+                                             int per, float (*tops)[kApWarps], T* ring) {
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int l = lane % kRowLanes, side = lane / kRowLanes;
   const bool norm = is_k && p.k_weight;
@@ -124,16 +207,36 @@ __device__ __forceinline__ void append_block(const BlockAppendParams& p, const A
   // last row the last one is read again, which changes no maximum.
   const int row0 = warp % group * kApRows + side;
   auto clamped = [&](int row) { return b.count > 0 ? b.token + min(row, b.count - 1) : 0; };
+  // without halves the two pieces are one
+  auto load_row = [&](const T* row, Raw8<T>& r) {
+    if constexpr (kTurn == kHalves || sizeof(T) == 4) {
+      load8(row, pieces, r);
+    } else {
+      const uint4 v = *reinterpret_cast<const uint4*>(row + 8 * l);
+      r.a = make_uint2(v.x, v.y), r.b = make_uint2(v.z, v.w);
+    }
+  };
   const T* rows[kApSteps];
 #pragma unroll
   for (int i = 0; i < kApSteps; ++i) rows[i] = src + (int64_t)clamped(row0 + 2 * i) * p.token_stride;
-  auto load = [&](int g, Raw8<T> (&raw)[kApSteps]) {
-    g = min(g, p.num_kv_heads - 1);
+  // head h's rows into its stage of the warp's ring
+  auto fetch = [&](int h) {
+    if (h < per) {
+      const int g = min(g0 + h, p.num_kv_heads - 1);
+      T* to = ring + (h % kApStages * kApRows + side * kApSteps) * kHeadDim;
 #pragma unroll
-    for (int i = 0; i < kApSteps; ++i) load8(rows[i] + g * kHeadDim, pieces, raw[i]);
+      for (int i = 0; i < kApSteps; ++i)
+#pragma unroll
+        for (int c = l * 16; c < kHeadDim * (int)sizeof(T); c += kRowLanes * 16)
+          cp_async_16(smem_u32(to + i * kHeadDim) + c, reinterpret_cast<const uint8_t*>(rows[i] + g * kHeadDim) + c, 16u);
+    }
+    cp_async_commit();
   };
   Raw8<T> raw[kApSteps];
-  load(g0, raw);
+  if constexpr (kHold) {
+#pragma unroll
+    for (int h = 0; h < kApStages - 1; ++h) fetch(h);
+  }
   float w[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) w[i] = 1.f;
@@ -146,58 +249,24 @@ __device__ __forceinline__ void append_block(const BlockAppendParams& p, const A
                   ((int64_t)max(page, 0) * (p.page_size / p.block_size) + off / (uint32_t)p.block_size) * p.num_kv_heads;
   const int kept = page < 0 ? 0 : b.kept;
 
-  // The rotation of a row: the lane's cosines and sines; false outside the table
   auto load_turn = [&](int row, float4& c, float4& sn) {
-    bool in = true;
-    const int64_t token = clamped(row);
-    const uint32_t own = b.pos + min(row, max(b.count - 1, 0));
-    for (int a = 0; a < p.rope.axes; ++a) {
-      const int pos = rope_position(p.rope, token, own, a);
-      in = in && pos >= 0 && pos < p.rope.table_len;
-    }
-    if (!in || l >= turning) return in;
-    const int half = p.rope.rotary >> 1;
-    if (p.rope.quads) {
-      const float* at = p.rope.table + (int64_t)rope_position(p.rope, token, own, rope_axis(p.rope, 4 * l)) * p.rope.rotary + 4 * l;
-      c = __ldg(reinterpret_cast<const float4*>(at));
-      sn = __ldg(reinterpret_cast<const float4*>(at + half));
-    } else {
-      float v[8];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float* at = p.rope.table + (int64_t)rope_position(p.rope, token, own, rope_axis(p.rope, 4 * l + i)) * p.rope.rotary + 4 * l + i;
-        v[i] = __ldg(at), v[4 + i] = __ldg(at + half);
-      }
-      c = make_float4(v[0], v[1], v[2], v[3]), sn = make_float4(v[4], v[5], v[6], v[7]);
-    }
-    return in;
+    return row_turn(p.rope, clamped(row), b.pos + min(row, max(b.count - 1, 0)), l, turning, c, sn);
   };
-  float4 cs[kTurn == kPlain || !kHold ? 1 : kApSteps], sn[kTurn == kPlain || !kHold ? 1 : kApSteps];
+  // the lane's cosines and sines of its rows wait in shared memory
+  float4* turns = reinterpret_cast<float4*>(ring + kApStages * kApRows * kHeadDim) + lane;
   uint32_t inside = 0xffffffffu;  // bit i: row i's positions lie inside the table
   if (kTurn != kPlain && kHold) {
 #pragma unroll
-    for (int i = 0; i < kApSteps; ++i)
-      if (!load_turn(row0 + 2 * i, cs[i], sn[i])) inside &= ~(1u << i);
+    for (int i = 0; i < kApSteps; ++i) {
+      float4 c = {}, sn = {};
+      if (!load_turn(row0 + 2 * i, c, sn)) inside &= ~(1u << i);
+      turns[(2 * i) * 32] = c, turns[(2 * i + 1) * 32] = sn;
+    }
   }
   auto value = [&](const Raw8<T>& from, const float4& c, const float4& s, bool in, float (&x)[8]) {
     widen8(from, x);
     if (norm) rms_norm8(x, w, p.eps);
-    if constexpr (kTurn != kPlain) {
-      const float cc[4] = {c.x, c.y, c.z, c.w}, ss[4] = {s.x, s.y, s.z, s.w};
-      if (l < turning) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float &u = x[kTurn == kHalves ? i : 2 * i], &v = x[kTurn == kHalves ? 4 + i : 2 * i + 1];
-          const float y = u * cc[i] - v * ss[i];
-          v = v * cc[i] + u * ss[i];
-          u = y;
-        }
-      }
-      if (!in) {
-#pragma unroll
-        for (int d = 0; d < 8; ++d) x[d] = 0.f;
-      }
-    }
+    turn_row<kTurn>(c, s, in, l < turning, x);
   };
   auto row_top = [&](const float (&x)[8], float top) {  // NaN counts for none
 #pragma unroll
@@ -233,24 +302,31 @@ __device__ __forceinline__ void append_block(const BlockAppendParams& p, const A
       for (int first = row0; first - row0 < b.count; first += kApWarps * kApRows) {
 #pragma unroll
         for (int i = 0; i < kApSteps; ++i) {
-          load8(src + (int64_t)clamped(first + 2 * i) * p.token_stride + min(g, p.num_kv_heads - 1) * kHeadDim, pieces, raw[i]);
+          load_row(src + (int64_t)clamped(first + 2 * i) * p.token_stride + min(g, p.num_kv_heads - 1) * kHeadDim, raw[i]);
         }
 #pragma unroll
         for (int i = 0; i < kApSteps; ++i) {
-          const bool in = kTurn == kPlain || load_turn(first + 2 * i, cs[0], sn[0]);
-          value(raw[i], cs[0], sn[0], in, x[0]);
+          float4 c = {}, sn = {};
+          const bool in = kTurn == kPlain || load_turn(first + 2 * i, c, sn);
+          value(raw[i], c, sn, in, x[0]);
           with(first + 2 * i);
         }
       }
     };
     if constexpr (kHold) {
+      cp_async_wait<kApStages - 2>();
+      __syncwarp();  // the head's rows are there, and every lane has read the one's before
+      fetch(h + kApStages - 1);
+#pragma unroll
+      for (int i = 0; i < kApSteps; ++i)
+        load_row(ring + (h % kApStages * kApRows + side * kApSteps + i) * kHeadDim, raw[i]);
 #pragma unroll
       for (int i = 0; i < kApSteps; ++i) {
-        const int j = kTurn == kPlain ? 0 : i;
-        value(raw[i], cs[j], sn[j], (inside >> i) & 1u, x[i]);
+        float4 c = {}, sn = {};
+        if (kTurn != kPlain) c = turns[(2 * i) * 32], sn = turns[(2 * i + 1) * 32];
+        value(raw[i], c, sn, (inside >> i) & 1u, x[i]);
         top = row_top(x[i], top);
       }
-      if (h + 1 < per) load(g + 1, raw);
     } else {
       each_row([&](int) { top = finite_top(x[0], top); });
     }
@@ -282,21 +358,7 @@ __device__ __forceinline__ void append_block(const BlockAppendParams& p, const A
     const float s = fmaxf(old, fmaxf(divide(top, 448.f, 1.0f / 448.f), kMinScale));
     const float inv = __fdividef(1.f, s);  // s is below 2^126
     auto store = [&](int row, float (&v)[8]) {
-      if (infinite) {  // an infinity's residual would be NaN
-#pragma unroll
-        for (int d = 0; d < 8; ++d) v[d] = fabsf(v[d]) > FLT_MAX ? v[d] : divide(v[d], s, inv);
-      } else {
-#pragma unroll
-        for (int d = 0; d < 8; ++d) v[d] = divide(v[d], s, inv);
-      }
-      uint8_t* to = dst + (int64_t)(b.kept + row) * step;
-      const uint32_t u0 = to_e4m3(v), u1 = to_e4m3(v + 4);
-      if (halves) {
-        *reinterpret_cast<uint32_t*>(to + pieces.a) = u0;
-        *reinterpret_cast<uint32_t*>(to + pieces.b) = u1;
-      } else {
-        *reinterpret_cast<uint2*>(to + pieces.a) = make_uint2(u0, u1);
-      }
+      store_codes(dst + (int64_t)(b.kept + row) * step, pieces, halves, quantise8(v, s, inv, infinite));
     };
     if constexpr (kHold) {
 #pragma unroll
@@ -310,15 +372,7 @@ __device__ __forceinline__ void append_block(const BlockAppendParams& p, const A
     if (old == s) continue;
     const float ratio = divide(old, s, inv);
     auto rescale = [&](int row, uint2 was) {
-      const uint32_t c[2] = {was.x, was.y};
-      float v[8];
-#pragma unroll
-      for (int d = 0; d < 4; ++d) {
-        const float2 f = e4m3x2_to_f32x2((uint16_t)(c[d / 2] >> (16 * (d % 2))));
-        v[2 * d] = f.x * ratio;
-        v[2 * d + 1] = f.y * ratio;
-      }
-      *reinterpret_cast<uint2*>(dst + (int64_t)row * step + 8 * l) = make_uint2(to_e4m3(v), to_e4m3(v + 4));
+      *reinterpret_cast<uint2*>(dst + (int64_t)row * step + 8 * l) = rescale8(was, ratio);
     };
     if constexpr (kHold) {
       if (kept > 0) {
@@ -331,15 +385,137 @@ __device__ __forceinline__ void append_block(const BlockAppendParams& p, const A
         if ((row - row0) / 2 % (kApWarps * kApSteps) < kApSteps)
           rescale(row, *reinterpret_cast<const uint2*>(dst + (int64_t)row * step + 8 * l));
     }
+    __syncwarp();  // the old scale is read before a lane writes it
     if (warp % group == 0 && lane == 0) *scale = s;
   }
 }
 
+// Blocks of up to 4 tokens: a warp takes as many as its 8 rows hold, b being
+// their run (a block of `run` = 8 / block_size * block_size tokens to
+// find_block). Each row has a scale, and a page, of its own block.
+template <typename T, int kTurn>
+__device__ __forceinline__ void append_packed(const BlockAppendParams& p, const ApBlock& b, bool is_k, int g0, int per) {
+  const int lane = threadIdx.x % 32, l = lane % kRowLanes, side = lane / kRowLanes;
+  const bool norm = is_k && p.k_weight;
+  const int turning = kTurn == kPlain ? 0 : p.rope.rotary >> 3;
+  const bool halves = kTurn == kHalves && l < turning;
+  const Pieces pieces = halves ? Pieces{4 * l, (p.rope.rotary >> 1) + 4 * l} : Pieces{8 * l, 8 * l + 4};
+  const int B = p.block_size;
+  const uint32_t half_mask = 0xffffu << (16 * side);
+  if (b.count == 0 || b.req < 0 || b.req >= p.num_reqs) return;
+
+  // the half warp's new rows side, side + 2, ...: where they are and go
+  const T* src[kApSteps];
+  int64_t row_at[kApSteps], scale_at[kApSteps];  // -1: not written
+  int block[kApSteps];                           // in the run
+  float4 cs[kTurn == kPlain ? 1 : kApSteps], sn[kTurn == kPlain ? 1 : kApSteps];
+  uint32_t inside = 0xffffffffu;
+#pragma unroll
+  for (int i = 0; i < kApSteps; ++i) {
+    const int row = side + 2 * i, in_run = min(row, b.count - 1);
+    const int token = b.token + in_run;
+    const uint32_t pos = b.pos + in_run;
+    src[i] = static_cast<const T*>(is_k ? p.k : p.v) + (int64_t)token * p.token_stride;
+    const uint32_t lp = pos / (uint32_t)p.page_size, off = pos - lp * p.page_size;
+    const int page = lp < (uint32_t)p.pages_per_req ? __ldg(p.btable + b.req * p.btable_stride + lp) : -1;
+    const bool goes = row < b.count && page >= 0 && page < p.num_pages;
+    row_at[i] = goes ? (int64_t)page * p.page_size + off : -1;
+    scale_at[i] = goes ? (int64_t)page * (p.page_size / B) + off / (uint32_t)B : -1;
+    block[i] = (b.kept + in_run) / B;
+    if (kTurn != kPlain && !row_turn(p.rope, token, pos, l, turning, cs[i], sn[i])) inside &= ~(1u << i);
+  }
+  float w[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) w[i] = 1.f;
+  if (norm) load_weight8(p.k_weight, p.weight_dtype, pieces, w);
+  const int lead = b.kept % B, lead_block = b.kept / B;  // rows that the first new row's block keeps
+  uint8_t* cache = is_k ? p.k_cache : p.v_cache;
+  float* scales = is_k ? p.k_scales : p.v_scales;
+
+#pragma unroll 1
+  for (int g = g0; g < min(g0 + per, p.num_kv_heads); ++g) {
+    Raw8<T> raw[kApSteps];
+    float old[kApSteps];
+#pragma unroll
+    for (int i = 0; i < kApSteps; ++i) {
+      load8(src[i] + g * kHeadDim, pieces, raw[i]);
+      old[i] = lead > 0 && block[i] == lead_block && scale_at[i] >= 0 ? scales[scale_at[i] * p.num_kv_heads + g] : 0.f;
+    }
+    float x[kApSteps][8], top[2 * kApSteps];  // of every row of the warp
+    bool infinite = false;
+#pragma unroll
+    for (int i = 0; i < kApSteps; ++i) {
+      const int j = kTurn == kPlain ? 0 : i;
+      widen8(raw[i], x[i]);
+      if (norm) rms_norm8(x[i], w, p.eps);
+      turn_row<kTurn>(cs[j], sn[j], (inside >> i) & 1u, l < turning, x[i]);
+      float v = 0.f;  // NaN counts for none
+#pragma unroll
+      for (int d = 0; d < 8; ++d) v = fmaxf(v, fabsf(x[i][d]));
+      infinite = infinite || v > FLT_MAX;
+      top[i] = v;
+    }
+    if (__any_sync(0xffffffffu, infinite)) {  // rare: infinities count for none
+      infinite = true;
+#pragma unroll
+      for (int i = 0; i < kApSteps; ++i) {
+        top[i] = 0.f;
+#pragma unroll
+        for (int d = 0; d < 8; ++d) top[i] = fabsf(x[i][d]) <= FLT_MAX ? fmaxf(top[i], fabsf(x[i][d])) : top[i];
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kApSteps; ++i) {
+      top[i] = __uint_as_float(__reduce_max_sync(half_mask, __float_as_uint(top[i])));
+      top[kApSteps + i] = __shfl_xor_sync(0xffffffffu, top[i], 16);
+    }
+    __syncwarp();  // the old scales are read before a lane writes them
+#pragma unroll
+    for (int i = 0; i < kApSteps; ++i) {
+      // the maximum of the row's block, whose other rows are this half's or the
+      // other's; rows past the last one repeat it
+      float v = top[i];
+      if (B > 1) {
+#pragma unroll
+        for (int k = 0; k < kApSteps; ++k) {
+          if (block[k] == block[i]) v = fmaxf(v, top[k]);
+          const int other = (b.kept + min(1 - side + 2 * k, b.count - 1)) / B;
+          if (other == block[i]) v = fmaxf(v, top[kApSteps + k]);
+        }
+      }
+      const float s = fmaxf(old[i], fmaxf(divide(v, 448.f, 1.0f / 448.f), kMinScale));
+      const float inv = __fdividef(1.f, s);
+      if (row_at[i] < 0) continue;
+      store_codes(cache + (row_at[i] * p.num_kv_heads + g) * kHeadDim, pieces, halves, quantise8(x[i], s, inv, infinite));
+      // the first row of a block that goes sees to its scale and its kept rows
+      const int row = side + 2 * i;
+      const bool begins = row == 0 || (b.kept + row) % B == 0;
+      if (!begins || old[i] == s) continue;
+      if (row == 0 && lead > 0) {
+        const float ratio = divide(old[i], s, inv);
+        for (int back = 1; back <= lead; ++back) {
+          uint2* at = reinterpret_cast<uint2*>(cache + ((row_at[i] - back) * p.num_kv_heads + g) * kHeadDim + 8 * l);
+          *at = rescale8(*at, ratio);
+        }
+      }
+      if (l == 0) scales[scale_at[i] * p.num_kv_heads + g] = s;
+    }
+  }
+}
+
+// A warp's shared memory: its ring, and four cosines and sines a lane and row.
+template <typename T>
+__host__ __device__ constexpr int ap_warp_bytes() {
+  return kApStages * kApRows * kHeadDim * (int)sizeof(T) + kApSteps * 2 * 32 * 16;
+}
+
 // kHold: the group's warps hold all rows of a block. per: heads of a group.
 template <typename T, bool kHold, int kTurn>
-__global__ void __launch_bounds__(32 * kApWarps, 2)
+__global__ void __launch_bounds__(32 * kApWarps, sizeof(T) == 2 && kTurn == kPlain ? 3 : 2)
     qsa_block_append_kernel(const __grid_constant__ BlockAppendParams p, uint32_t items, int group, int per) {
   __shared__ float tops[3][kApWarps];
+  extern __shared__ __align__(128) uint8_t smem[];
+  T* ring = reinterpret_cast<T*>(smem + threadIdx.x / 32 * ap_warp_bytes<T>());
   const uint32_t parts = (p.num_kv_heads + per - 1) / per;
   // K's groups come first, then V's: a CTA's warps do the same work
   const uint32_t item = blockIdx.x * (kApWarps / group) + threadIdx.x / 32 / group;
@@ -347,11 +523,44 @@ __global__ void __launch_bounds__(32 * kApWarps, 2)
   const uint32_t slot = item / parts;
   const int g0 = (int)(item - slot * parts) * per;
   ApBlock b = {};
-  if (item < items) b = find_block(p, slot, threadIdx.x % 32);
+  if (item < items) b = find_block(p, slot, threadIdx.x % 32, p.block_size);
   if (is_k)
-    append_block<T, kHold, kTurn>(p, b, true, g0, group, per, tops);
+    append_block<T, kHold, kTurn>(p, b, true, g0, group, per, tops, ring);
   else
-    append_block<T, kHold, kPlain>(p, b, false, g0, group, per, tops);
+    append_block<T, kHold, kPlain>(p, b, false, g0, group, per, tops, ring);
+}
+
+template <typename T, int kTurn>
+__global__ void __launch_bounds__(32 * kApWarps, 2)
+    qsa_block_append_packed_kernel(const __grid_constant__ BlockAppendParams p, uint32_t items, int run, int per) {
+  const uint32_t parts = (p.num_kv_heads + per - 1) / per;
+  const uint32_t item = blockIdx.x * kApWarps + threadIdx.x / 32;
+  if (item >= items) return;
+  const uint32_t slot = item / parts;
+  const int g0 = (int)(item - slot * parts) * per;
+  const ApBlock b = find_block(p, slot, threadIdx.x % 32, run);
+  if (blockIdx.y == 0)
+    append_packed<T, kTurn>(p, b, true, g0, per);
+  else
+    append_packed<T, kPlain>(p, b, false, g0, per);
+}
+
+template <typename T, bool kHold, int kTurn>
+cudaError_t launch(const BlockAppendParams& p, uint32_t items, dim3 grid, int group, int per, cudaStream_t stream) {
+  constexpr int kSmem = kHold ? kApWarps * ap_warp_bytes<T>() : 0;
+  // shared memory beyond the default limit, once per device
+  static std::atomic<uint64_t> ready{0};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const uint64_t bit = 1ull << (dev & 63);
+  if (kSmem > 0 && !(ready.load(std::memory_order_acquire) & bit)) {
+    e = cudaFuncSetAttribute(qsa_block_append_kernel<T, kHold, kTurn>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+    if (e != cudaSuccess) return e;
+    ready.fetch_or(bit, std::memory_order_acq_rel);
+  }
+  qsa_block_append_kernel<T, kHold, kTurn><<<grid, 32 * kApWarps, kSmem, stream>>>(p, items, group, per);
+  return cudaGetLastError();
 }
 
 template <typename T, bool kHold>
@@ -366,29 +575,45 @@ cudaError_t launch(const BlockAppendParams& p, int64_t slots, cudaStream_t strea
   const int64_t blocks = (items * group + kApWarps - 1) / kApWarps;
   if (items > 0xffffffffll - kApWarps || blocks > 0x7fffffffll) return cudaErrorInvalidValue;
   const dim3 grid((unsigned)blocks, 2);
+  if (!p.rope.table) return launch<T, kHold, kPlain>(p, (uint32_t)items, grid, group, per, stream);
+  if (!p.rope.interleaved) return launch<T, kHold, kHalves>(p, (uint32_t)items, grid, group, per, stream);
+  return launch<T, kHold, kNeighbours>(p, (uint32_t)items, grid, group, per, stream);
+}
+
+template <typename T>
+cudaError_t launch_packed(const BlockAppendParams& p, int64_t slots, int run, cudaStream_t stream) {
+  int per = 1;
+  while (per < kApHeads && per < p.num_kv_heads && slots * 2 * ((p.num_kv_heads + 2 * per - 1) / (2 * per)) >= 148 * 32) per *= 2;
+  const int64_t items = slots * ((p.num_kv_heads + per - 1) / per);
+  const int64_t blocks = (items + kApWarps - 1) / kApWarps;
+  if (items > 0xffffffffll - kApWarps || blocks > 0x7fffffffll) return cudaErrorInvalidValue;
+  const dim3 grid((unsigned)blocks, 2);
   const int threads = 32 * kApWarps;
   if (!p.rope.table)
-    qsa_block_append_kernel<T, kHold, kPlain><<<grid, threads, 0, stream>>>(p, (uint32_t)items, group, per);
+    qsa_block_append_packed_kernel<T, kPlain><<<grid, threads, 0, stream>>>(p, (uint32_t)items, run, per);
   else if (!p.rope.interleaved)
-    qsa_block_append_kernel<T, kHold, kHalves><<<grid, threads, 0, stream>>>(p, (uint32_t)items, group, per);
+    qsa_block_append_packed_kernel<T, kHalves><<<grid, threads, 0, stream>>>(p, (uint32_t)items, run, per);
   else
-    qsa_block_append_kernel<T, kHold, kNeighbours><<<grid, threads, 0, stream>>>(p, (uint32_t)items, group, per);
+    qsa_block_append_packed_kernel<T, kNeighbours><<<grid, threads, 0, stream>>>(p, (uint32_t)items, run, per);
   return cudaGetLastError();
 }
 
 template <typename T>
-cudaError_t launch_type(const BlockAppendParams& p, int64_t slots, cudaStream_t stream) {
+cudaError_t launch_type(const BlockAppendParams& p, cudaStream_t stream) {
+  // blocks of up to 4 tokens leave half of a warp's 8 rows empty, or more
+  const int run = p.block_size <= kApRows / 2 ? kApRows / p.block_size * p.block_size : p.block_size;
+  const int64_t slots = p.cu_tokens ? (int64_t)(p.tokens / run) + 2 * (int64_t)p.entries : p.entries;
+  if (run > p.block_size) return launch_packed<T>(p, slots, run, stream);
   return p.block_size <= kApWarps * kApRows ? launch<T, true>(p, slots, stream) : launch<T, false>(p, slots, stream);
 }
 
 }  // namespace
 
 cudaError_t launch_block_append(const BlockAppendParams& p, cudaStream_t stream) {
-  const int64_t slots = p.cu_tokens ? (int64_t)(p.tokens / p.block_size) + 2 * (int64_t)p.entries : p.entries;
   switch (p.dtype) {
-    case QSA_B200_DTYPE_BF16: return launch_type<__nv_bfloat16>(p, slots, stream);
-    case QSA_B200_DTYPE_F16: return launch_type<__half>(p, slots, stream);
-    default: return launch_type<float>(p, slots, stream);
+    case QSA_B200_DTYPE_BF16: return launch_type<__nv_bfloat16>(p, stream);
+    case QSA_B200_DTYPE_F16: return launch_type<__half>(p, stream);
+    default: return launch_type<float>(p, stream);
   }
 }
 

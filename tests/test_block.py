@@ -370,6 +370,11 @@ APPEND_CASES = {
     "odd_blocks": (24, 12, 5, 32, True, None, True, [0, 11, 12, 37], [25, 2, 12, 40]),
     "one_scale_a_page": (64, 64, 1, 0, False, None, False, [0, 60, 63], [64, 5, 130]),
     "large_blocks": (128, 128, 2, 128, False, (16, 24, 24), True, [0, 100], [300, 29]),
+    "pages_of_one": (1, 1, 2, 128, False, None, True, [0, 5, 3], [9, 1, 17]),
+    "runs_over_pages": (12, 4, 3, 64, True, None, True, [0, 11, 13, 2], [30, 7, 12, 1]),
+    "pairs_one_token_each": (16, 2, 9, 128, False, None, True, [0, 1, 14, 15, 17], None),
+    "many_entries": (16, 8, 1, 128, False, None, True, [(7 * i) % 40 for i in range(80)], [(5 * i) % 11 for i in range(80)]),
+    "blocks_past_the_held": (256, 256, 2, 128, False, None, True, [0, 200, 255], [300, 3, 70]),
     "tiny_blocks": (48, 3, 4, 16, False, (1, 7), False, [2, 0, 46], [50, 4, 5]),
 }
 
