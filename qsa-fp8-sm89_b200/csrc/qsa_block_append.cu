@@ -63,27 +63,21 @@ struct ApBlock {
 
 // The block of a slot, but for its page. B: tokens of a block.
 __device__ __forceinline__ ApBlock find_block(const BlockAppendParams& p, uint32_t slot, int lane, uint32_t B) {
-  int e = 0, first = (int)slot, count = 1;
-  uint32_t j = 0;
-  bool is = true;
-  if (p.cu_tokens) {
-    // the last entry whose first slot, floor(cu[e] / B) + 2e, is <= slot
-    for (int n = p.entries; n > 1;) {
-      const int step = (n + 31) / 32;
-      const int at = e + lane * step;
-      const bool below = lane * step < n && (uint32_t)max(__ldg(p.cu_tokens + at), 0) / B + 2u * at <= slot;
-      const int k = max(__popc(__ballot_sync(0xffffffffu, below)) - 1, 0);
-      e += k * step;
-      n = min(step, n - k * step);
-    }
-    first = min(max(__ldg(p.cu_tokens + e), 0), p.tokens);
-    count = min(max(__ldg(p.cu_tokens + e + 1), 0), p.tokens) - first;
-    const uint32_t slot0 = (uint32_t)first / B + 2u * e;
-    is = count > 0 && slot >= slot0;
-    j = slot - slot0;
-  } else {
-    e = (int)slot;
+  int e = 0;
+  // the last entry whose first slot, floor(cu[e] / B) + 2e, is <= slot
+  for (int n = p.entries; n > 1;) {
+    const int step = (n + 31) / 32;
+    const int at = e + lane * step;
+    const bool below = lane * step < n && (uint32_t)max(__ldg(p.cu_tokens + at), 0) / B + 2u * at <= slot;
+    const int k = max(__popc(__ballot_sync(0xffffffffu, below)) - 1, 0);
+    e += k * step;
+    n = min(step, n - k * step);
   }
+  const int first = min(max(__ldg(p.cu_tokens + e), 0), p.tokens);
+  const int count = min(max(__ldg(p.cu_tokens + e + 1), 0), p.tokens) - first;
+  const uint32_t slot0 = (uint32_t)first / B + 2u * e;
+  const bool is = count > 0 && slot >= slot0;
+  const uint32_t j = slot - slot0;
   const int start = __ldg(p.starts + e);
   ApBlock b;
   b.req = p.reqs ? __ldg(p.reqs + e) : e;
@@ -545,6 +539,100 @@ __global__ void __launch_bounds__(32 * kApWarps, 2)
     append_packed<T, kPlain>(p, b, false, g0, per);
 }
 
+// One token an entry, a decode step's append: a warp takes an entry and head, its
+// lower half warp the key, the upper one the value. The call is bound by the
+// latency of what hangs together (start, page, old scale), so the row's load
+// goes out first.
+template <typename T, int kTurn>
+__global__ void __launch_bounds__(32 * kApWarps) qsa_block_append_one_kernel(const __grid_constant__ BlockAppendParams p) {
+  const int lane = threadIdx.x % 32, l = lane % kRowLanes, side = lane / kRowLanes;
+  const uint32_t item = blockIdx.x * kApWarps + threadIdx.x / 32;
+  const uint32_t e = item / (uint32_t)p.num_kv_heads;
+  const int g = (int)(item - e * p.num_kv_heads);
+  if (e >= (uint32_t)p.entries) return;
+  const bool is_k = side == 0;
+  const int turning = kTurn == kPlain ? 0 : p.rope.rotary >> 3;
+  const bool halves = kTurn == kHalves && is_k && l < turning;
+  const Pieces pieces = halves ? Pieces{4 * l, (p.rope.rotary >> 1) + 4 * l} : Pieces{8 * l, 8 * l + 4};
+  Raw8<T> raw;
+  load8(static_cast<const T*>(is_k ? p.k : p.v) + (int64_t)e * p.token_stride + g * kHeadDim, pieces, raw);
+  const int start = __ldg(p.starts + e);
+  const int req = p.reqs ? __ldg(p.reqs + e) : (int)e;
+  const int B = p.block_size;
+  const int lp = max(start, 0) / p.page_size, off = max(start, 0) - lp * p.page_size;
+  int page = -1;
+  if (start >= 0 && req >= 0 && req < p.num_reqs && lp < p.pages_per_req) page = __ldg(p.btable + req * p.btable_stride + lp);
+  const bool goes = page >= 0 && page < p.num_pages;
+  float4 c = {}, sn = {};
+  bool in = true;
+  if (kTurn != kPlain && is_k) in = row_turn(p.rope, e, max(start, 0), l, turning, c, sn);
+  float w[8], x[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) w[i] = 1.f;
+  if (p.k_weight) load_weight8(p.k_weight, p.weight_dtype, pieces, w);
+  float* scale = (is_k ? p.k_scales : p.v_scales) +
+                 ((int64_t)max(page, 0) * (p.page_size / B) + off / B) * p.num_kv_heads + g;
+  const int lead = off % B;  // rows that the block keeps
+  const float old = goes && lead > 0 ? *scale : 0.f;
+
+  widen8(raw, x);
+  if (p.k_weight) {
+    float y[8];
+#pragma unroll
+    for (int d = 0; d < 8; ++d) y[d] = x[d];
+    rms_norm8(y, w, p.eps);
+#pragma unroll
+    for (int d = 0; d < 8; ++d) x[d] = is_k ? y[d] : x[d];
+  }
+  if (is_k) turn_row<kTurn>(c, sn, in, l < turning, x);
+  float top = 0.f, finite = 0.f;
+#pragma unroll
+  for (int d = 0; d < 8; ++d) {
+    top = fmaxf(top, fabsf(x[d]));
+    finite = fabsf(x[d]) <= FLT_MAX ? fmaxf(finite, fabsf(x[d])) : finite;
+  }
+#pragma unroll
+  for (int o = kRowLanes / 2; o > 0; o >>= 1) {
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    finite = fmaxf(finite, __shfl_xor_sync(0xffffffffu, finite, o));
+  }
+  if (!goes) return;  // the whole warp: one page for both
+  const float s = fmaxf(old, fmaxf(divide(finite, 448.f, 1.0f / 448.f), kMinScale));
+  const float inv = __fdividef(1.f, s);
+  const int step = p.num_kv_heads * kHeadDim;
+  uint8_t* row = (is_k ? p.k_cache : p.v_cache) + ((int64_t)page * p.page_size + off) * step + g * kHeadDim;
+  store_codes(row, pieces, halves, quantise8(x, s, inv, top > FLT_MAX));
+  if (old != s) {
+    const float ratio = divide(old, s, inv);
+    for (int back = 1; back <= lead; back += 8) {
+      uint2 codes[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (back + i <= lead) codes[i] = *reinterpret_cast<const uint2*>(row - (int64_t)(back + i) * step + 8 * l);
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (back + i <= lead) *reinterpret_cast<uint2*>(row - (int64_t)(back + i) * step + 8 * l) = rescale8(codes[i], ratio);
+    }
+  }
+  __syncwarp();  // the old scales are read before a lane writes them
+  if (old != s && l == 0) *scale = s;
+}
+
+template <typename T>
+cudaError_t launch_one(const BlockAppendParams& p, cudaStream_t stream) {
+  const int64_t items = (int64_t)p.entries * p.num_kv_heads;
+  if (items > 0xffffffffll - kApWarps) return cudaErrorInvalidValue;
+  const unsigned grid = (unsigned)((items + kApWarps - 1) / kApWarps);
+  const int threads = 32 * kApWarps;
+  if (!p.rope.table)
+    qsa_block_append_one_kernel<T, kPlain><<<grid, threads, 0, stream>>>(p);
+  else if (!p.rope.interleaved)
+    qsa_block_append_one_kernel<T, kHalves><<<grid, threads, 0, stream>>>(p);
+  else
+    qsa_block_append_one_kernel<T, kNeighbours><<<grid, threads, 0, stream>>>(p);
+  return cudaGetLastError();
+}
+
 template <typename T, bool kHold, int kTurn>
 cudaError_t launch(const BlockAppendParams& p, uint32_t items, dim3 grid, int group, int per, cudaStream_t stream) {
   constexpr int kSmem = kHold ? kApWarps * ap_warp_bytes<T>() : 0;
@@ -600,9 +688,10 @@ cudaError_t launch_packed(const BlockAppendParams& p, int64_t slots, int run, cu
 
 template <typename T>
 cudaError_t launch_type(const BlockAppendParams& p, cudaStream_t stream) {
+  if (!p.cu_tokens) return launch_one<T>(p, stream);
   // blocks of up to 4 tokens leave half of a warp's 8 rows empty, or more
   const int run = p.block_size <= kApRows / 2 ? kApRows / p.block_size * p.block_size : p.block_size;
-  const int64_t slots = p.cu_tokens ? (int64_t)(p.tokens / run) + 2 * (int64_t)p.entries : p.entries;
+  const int64_t slots = (int64_t)(p.tokens / run) + 2 * (int64_t)p.entries;
   if (run > p.block_size) return launch_packed<T>(p, slots, run, stream);
   return p.block_size <= kApWarps * kApRows ? launch<T, true>(p, slots, stream) : launch<T, false>(p, slots, stream);
 }
