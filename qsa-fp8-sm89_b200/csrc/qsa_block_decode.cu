@@ -263,34 +263,39 @@ __global__ void __launch_bounds__(32 * kBdWarps, 2) qsa_block_decode_kernel(cons
       const bool clean = __syncthreads_and(valid);  // only the last tile may have masked places
       const int whole = clean ? n / kUnit : 0;      // leading tiles without one
 
+      // Row row0 + 4i of a stage: with 8 heads the token's other four or the
+      // next token's first, else the same heads 4 / kCh tokens on. The bits that
+      // step adds to the token are none that token0 has, so the chunk
+      // permutation splits into token0's and a constant.
       auto fetch = [&](int k, int st) {
-        if (k < tiles) {
-          const int* ahead = table + k * kUnit;
+        const int* ahead = table + k * kUnit;
+        if (__builtin_expect(k < whole, 1)) {
 #pragma unroll
           for (int i = 0; i < 4 / kParts; ++i) {
-            // Row row0 + 4i: with 8 heads the token's other four or the next
-            // token's first, else the same heads 4 / kCh tokens on. The bits
-            // that step adds to the token are none that token0 has, so the
-            // chunk permutation splits into token0's and a constant.
             const int step = 4 * i / kCh;
-            const int64_t to_head = kCh == 8 ? i % 2 * 4 * kHeadDim : 0;
+            const int64_t from = (int64_t)ahead[token0 + step] * token_bytes;
+            const int to_head = kCh == 8 ? i % 2 * 4 * kHeadDim : 0;
+            cp_async_16_all((k_dst ^ ((step & 1) << 6)) + st * C::kStageBytes + i * 4 * kHeadDim, k_src + from + to_head);
+            cp_async_16_all((v_dst ^ ((step & 6) << 4)) + st * C::kStageBytes + i * 4 * kHeadDim, v_src + from + to_head);
+          }
+          if (kParts == 1 || scale_row < C::kRows) {
+            const uint32_t block = __umulhi(2u * (uint32_t)ahead[scale_row / kCh], p.block_mul) >> p.block_shift;
+            cp_async_4_or_zero(s_dst + st * 2 * C::kRows * 4, s_src + (int64_t)(int)block * p.num_kv_heads, 4u);
+          }
+        } else if (k < tiles) {  // masked places read as zeros, whatever the cache holds
+#pragma unroll 1
+          for (int i = 0; i < 4 / kParts; ++i) {
+            const int step = 4 * i / kCh;
             const int slot = ahead[token0 + step];
-            const uint32_t kd = (k_dst ^ ((step & 1) << 6)) + st * C::kStageBytes + i * 4 * kHeadDim;
-            const uint32_t vd = (v_dst ^ ((step & 6) << 4)) + st * C::kStageBytes + i * 4 * kHeadDim;
-            if (k < whole) {
-              cp_async_16_all(kd, k_src + (int64_t)slot * token_bytes + to_head);
-              cp_async_16_all(vd, v_src + (int64_t)slot * token_bytes + to_head);
-            } else {  // masked places read as zeros, whatever the cache holds
-              const int64_t from = (int64_t)max(slot, 0) * token_bytes + to_head;
-              cp_async_16(kd, k_src + from, slot < 0 ? 0u : 16u);
-              cp_async_16(vd, v_src + from, slot < 0 ? 0u : 16u);
-            }
+            const int64_t from = (int64_t)max(slot, 0) * token_bytes + (kCh == 8 ? i % 2 * 4 * kHeadDim : 0);
+            const uint32_t bytes = slot < 0 ? 0u : 16u;
+            cp_async_16((k_dst ^ ((step & 1) << 6)) + st * C::kStageBytes + i * 4 * kHeadDim, k_src + from, bytes);
+            cp_async_16((v_dst ^ ((step & 6) << 4)) + st * C::kStageBytes + i * 4 * kHeadDim, v_src + from, bytes);
           }
           if (kParts == 1 || scale_row < C::kRows) {
             const int slot = ahead[scale_row / kCh];
             const uint32_t block = __umulhi(2u * (uint32_t)max(slot, 0), p.block_mul) >> p.block_shift;
-            cp_async_4_or_zero(s_dst + st * 2 * C::kRows * 4, s_src + (int64_t)(int)block * p.num_kv_heads,
-                               slot < 0 ? 0u : 4u);
+            cp_async_4_or_zero(s_dst + st * 2 * C::kRows * 4, s_src + (int64_t)(int)block * p.num_kv_heads, slot < 0 ? 0u : 4u);
           }
         }
         cp_async_commit();
@@ -357,8 +362,7 @@ __global__ void __launch_bounds__(32 * kBdWarps, 2) qsa_block_decode_kernel(cons
           }
 
           // scores over the reference, probabilities, weights over theirs
-          float pr[4], w[4];
-          bool pass = false;
+          float pr[4], w[4], x_top = -INFINITY, w_abs = 0.f;
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const int t = j / 2, h = j % 2;
@@ -367,9 +371,10 @@ __global__ void __launch_bounds__(32 * kBdWarps, 2) qsa_block_decode_kernel(cons
             x = masked[t] ? -INFINITY : x;
             pr[j] = ex2(x);
             w[j] = pr[j] * (vs[t] * inv_w[h]);
-            pass = pass || x > kLazy || fabsf(w[j]) > kLazyW * kOneW;
+            x_top = fmaxf(x_top, x);
+            w_abs = fmaxf(w_abs, fabsf(w[j]));
           }
-          if (__any_sync(0xffffffffu, pass)) {
+          if (__any_sync(0xffffffffu, x_top > kLazy || w_abs > kLazyW * kOneW)) {
             // move the references, and what was summed against them
 #pragma unroll
             for (int h = 0; h < 2; ++h) {

@@ -107,7 +107,12 @@ __device__ __forceinline__ void rms_norm8(float (&x)[8], const float (&w)[8], fl
   for (int i = 0; i < 8; ++i) s = fmaf(x[i], x[i], s);
 #pragma unroll
   for (int o = kRowLanes / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-  const float r = rsqrtf(fmaf(s, 1.0f / 128.0f, eps));
+  // one Newton step from the 2 ulp of rsqrtf to nearly the nearest value: what a
+  // row is off by shifts all its codes where it is quantised
+  const float v = fmaf(s, 1.0f / 128.0f, eps);
+  float r = rsqrtf(v);
+  const float t = v * r, e = fmaf(-fmaf(v, r, -t), r, fmaf(-t, r, 1.0f));  // 1 - v r r
+  if (r > 0.f && r <= 3.4e38f) r = fmaf(0.5f * r, e, r);
 #pragma unroll
   for (int i = 0; i < 8; ++i) x[i] = x[i] * r * w[i];
 }
