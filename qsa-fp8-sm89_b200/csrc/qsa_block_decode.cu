@@ -54,6 +54,7 @@ namespace {
 constexpr int kBdWarps = 8;
 constexpr int kBdTile = 16;                         // tokens a warp takes at a time
 constexpr int kBdTable = 2048;                      // slots of a CTA's table
+constexpr int kBdColumns = 8;                       // columns that a thread looks up at once
 constexpr int kBdDirect = 512;                      // columns of a row that are not planned
 constexpr float kLazy = 8.f;                        // log2 by which a score may pass its reference
 constexpr float kLazyW = 128.f;                     // factor by which a weight may pass its reference
@@ -107,20 +108,6 @@ __device__ __forceinline__ void wait_for_prerequisites() { asm volatile("griddep
 __device__ __forceinline__ uint32_t pack_f16(float a, float b) {
   const __half2 h = __floats2half2_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&h);
-}
-
-// Logical tokens (negative: masked) to physical slots, -1 where masked.
-template <int N>
-__device__ __forceinline__ void column_slots(const BlockDecodeParams& p, int64_t req, int (&t)[N]) {
-  int page[N], off[N];
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const int lp = t[i] / p.page_size;
-    off[i] = t[i] - lp * p.page_size;
-    page[i] = t[i] >= 0 && lp < p.pages_per_req ? __ldg(p.btable + req * p.btable_stride + lp) : -1;
-  }
-#pragma unroll
-  for (int i = 0; i < N; ++i) t[i] = page[i] < 0 || page[i] >= p.num_pages ? -1 : page[i] * p.page_size + off[i];
 }
 
 // kParts: virtual KV heads of a cache head. kCh: cache heads of a CTA.
@@ -243,21 +230,32 @@ __global__ void __launch_bounds__(32 * kBdWarps, 2) qsa_block_decode_kernel(cons
       const int tiles = (n + kUnit - 1) / kUnit;
       if (base > c0 || !first) __syncthreads();  // the table's readers are done
       bool valid = true;
-      // several columns a thread at once: an index, then its page, wait on memory
+      // several columns a thread at once: an index, then its page, wait on
+      // memory. Steps past the last column are left by the whole CTA.
 #pragma unroll 1
-      for (int i0 = tid; i0 < tiles * kUnit; i0 += 8 * C::kThreads) {
-        int slot[8];
+      for (int i0 = 0; i0 < tiles * kUnit; i0 += kBdColumns * C::kThreads) {
+        int t[kBdColumns], off[kBdColumns], page[kBdColumns];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int col = i0 + i * C::kThreads;
-          slot[i] = col >= n ? -1 : p.indices ? __ldg(p.indices + (int64_t)row_now * p.indices_stride + base + col) : base + col;
+        for (int i = 0; i < kBdColumns; ++i) {
+          const int col = i0 + i * C::kThreads + tid;
+          t[i] = base + col;
+          if (p.indices && i0 + i * C::kThreads < n) t[i] = col < n ? __ldg(p.indices + (int64_t)row_now * p.indices_stride + t[i]) : -1;
         }
-        column_slots(p, req, slot);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int col = i0 + i * C::kThreads;
-          if (col < tiles * kUnit) table[col] = slot[i];
-          valid = valid && (slot[i] >= 0 || col >= n);
+        for (int i = 0; i < kBdColumns; ++i) {
+          if (i0 + i * C::kThreads >= n) break;
+          const int col = i0 + i * C::kThreads + tid;
+          const uint32_t lp = __umulhi(2u * (uint32_t)max(t[i], 0), p.page_mul) >> p.page_shift;
+          off[i] = t[i] - (int)lp * p.page_size;
+          page[i] = col < n && t[i] >= 0 && (int)lp < p.pages_per_req ? __ldg(p.btable + req * p.btable_stride + lp) : -1;
+        }
+#pragma unroll
+        for (int i = 0; i < kBdColumns; ++i) {
+          const int col = i0 + i * C::kThreads + tid;
+          if (i0 + i * C::kThreads >= tiles * kUnit) break;
+          const bool in = i0 + i * C::kThreads < n && page[i] >= 0 && page[i] < p.num_pages;
+          if (col < tiles * kUnit) table[col] = in ? page[i] * p.page_size + off[i] : -1;
+          valid = valid && (in || col >= n);
         }
       }
       const bool clean = __syncthreads_and(valid);  // only the last tile may have masked places
@@ -732,12 +730,15 @@ int64_t block_decode_plan(BlockDecodeParams& p) {
   p.virtual_heads = p.num_kv_heads * p.head_parts;
   p.cta_heads = p.head_parts;
   while (p.cta_heads < kBdWarps && p.virtual_heads % (2 * p.cta_heads) == 0) p.cta_heads *= 2;
-  // mul = ceil(2^(31 + shift) / block) with block <= 2^shift: n mul exceeds
-  // n 2^(31 + shift) / block by less than n, so n / block is exact for n < 2^31
-  uint32_t shift = 0;
-  while ((1ll << shift) < p.block_size) ++shift;
-  p.block_shift = shift;
-  p.block_mul = (uint32_t)((((uint64_t)1 << (31 + shift)) + p.block_size - 1) / p.block_size);
+  // mul = ceil(2^(31 + shift) / d) with d <= 2^shift: n mul exceeds
+  // n 2^(31 + shift) / d by less than n, so n / d is exact for n < 2^31
+  auto reciprocal = [](uint32_t d, uint32_t& mul, uint32_t& shift) {
+    shift = 0;
+    while ((1ll << shift) < d) ++shift;
+    mul = (uint32_t)((((uint64_t)1 << (31 + shift)) + d - 1) / d);
+  };
+  reciprocal(p.block_size, p.block_mul, p.block_shift);
+  reciprocal(p.page_size, p.page_mul, p.page_shift);
   p.planned = p.topk > kBdDirect;
   if (!p.planned) return 0;
   const int64_t pieces = 2ll * planned_ctas() * p.cta_heads * p.part_heads;

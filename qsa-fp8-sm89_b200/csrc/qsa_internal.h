@@ -184,8 +184,9 @@ struct BlockDecodeParams {
   // heads each (the last one may have fewer); a CTA takes cta_heads of the
   // virtual_heads of a row.
   int head_parts, part_heads, virtual_heads, cta_heads;
-  // slot / block_size = umulhi(2 slot, block_mul) >> block_shift, exact below 2^31
-  uint32_t block_mul, block_shift;
+  // slot / block_size = umulhi(2 slot, block_mul) >> block_shift, exact below
+  // 2^31; token / page_size likewise
+  uint32_t block_mul, block_shift, page_mul, page_shift;
   // Rows of many columns: units (of a CTA's warps times 16 columns) in the
   // order row, head group, columns, shared evenly by `ctas` CTAs (workspace).
   bool planned;
