@@ -544,8 +544,8 @@ __global__ void __launch_bounds__(kLenThreads) qsa_block_lengths_kernel(const __
 // place has one: its zeros), the number of CTAs that share them, and the row
 // that each begins in. One CTA; a thread takes consecutive rows.
 constexpr int kPlanThreads = 1024;
-constexpr int kPlanWaves = 1;
-constexpr int kPlanUnits = 8;  // units a CTA gets at least, so that small work has few pieces
+constexpr int kJoinFew = 8;      // pieces that a warp joins
+constexpr int kPlanTokens = 128;  // columns a CTA gets at least (and two units), so that small work has few pieces
 __global__ void __launch_bounds__(kPlanThreads) qsa_block_plan_kernel(const __grid_constant__ BlockDecodeParams p, int max_ctas) {
   launch_dependents();
   wait_for_prerequisites();
@@ -563,6 +563,8 @@ __global__ void __launch_bounds__(kPlanThreads) qsa_block_plan_kernel(const __gr
     mine += max(1, (int)(((int64_t)len + unit - 1) / unit));
   }
   __shared__ int64_t sums[kPlanThreads / 32];
+  __shared__ int listed[2];
+  if (t < 2) listed[t] = 0;
   int64_t run = mine;
 #pragma unroll
   for (int d = 1; d < 32; d *= 2) {
@@ -583,7 +585,8 @@ __global__ void __launch_bounds__(kPlanThreads) qsa_block_plan_kernel(const __gr
   __syncthreads();
   const int64_t total = sums[kPlanThreads / 32 - 1];
   const int64_t units = total * hgroups;
-  const int ctas = (int)min((int64_t)max_ctas, (units + kPlanUnits - 1) / kPlanUnits);
+  const int least = max(kPlanTokens / unit, 2);
+  const int ctas = (int)min((int64_t)max_ctas, (units + least - 1) / least);
   int64_t before = run - mine + (t >= 32 ? sums[t / 32 - 1] : 0);
   for (int r = r0; r < r1; ++r) {
     p.prefix[r] = before;
@@ -602,57 +605,103 @@ __global__ void __launch_bounds__(kPlanThreads) qsa_block_plan_kernel(const __gr
     }
     p.plan->cut[b] = x;
     p.plan->first_row[b] = lo;
-    // what is joined at this cut: a row and head group that it is the first to
-    // cut; its last piece is of the last CTA that begins before its end
+    // a row and head group that this cut is the first to cut is joined: its last
+    // piece is of the last CTA that begins before its end
     const int64_t row_at = p.prefix[lo] * hgroups, row_units = p.prefix[lo + 1] - p.prefix[lo];
     const int hg = (int)(x - row_at) / (int)row_units;
     const int64_t begin = row_at + hg * row_units;
-    const bool first = b > 0 && b < ctas && x > begin && (b - 1) * units / ctas <= begin;
-    p.plan->joins[b] = first ? make_int4(lo, hg, (int)(((begin + row_units) * ctas - 1) / units), 0) : make_int4(-1, 0, 0, 0);
+    if (b > 0 && b < ctas && x > begin && (b - 1) * units / ctas <= begin) {
+      const int last = (int)(((begin + row_units) * ctas - 1) / units);
+      const bool many = last - b + 2 > kJoinFew;
+      const int at = atomicAdd(&listed[many], 1);  // the order of the list does not matter
+      p.plan->joins[many ? kPlanMaxCtas - 1 - at : at] = make_int4(lo, hg, b, last);
+    }
   }
+  __syncthreads();
+  if (t < 2) p.plan->num_joins[t] = listed[t];
 }
 
-// Joins the pieces of the rows that the plan cut, in the plan's order. CTA
-// (b - 1, y) takes what is joined at the cut before planned CTA b, for virtual
-// head y of its group; a warp a query head.
-__global__ void __launch_bounds__(256, 6) qsa_block_join_kernel(const __grid_constant__ BlockDecodeParams p) {
+// Joins the pieces of the rows that the plan cut, in the plan's order: a warp a
+// query head where they are few, a CTA a query head where a long row was cut
+// into many (256 pieces one after the other took a warp 40 us).
+constexpr int kJoinThreads = 256, kJoinCtas = 6;  // CTAs an SM
+__global__ void __launch_bounds__(kJoinThreads, kJoinCtas) qsa_block_join_kernel(const __grid_constant__ BlockDecodeParams p) {
+  __shared__ float tops[8], sums[8];
+  __shared__ float4 accs[8][32];
   wait_for_prerequisites();
-  const int b = blockIdx.x + 1;
-  const int ctas = p.plan->ctas;
-  const int4 what = p.plan->joins[b];
-  if (b >= ctas || what.x < 0) return;
-  const int row = what.x, hg = what.y, last = what.z;
-  const int lane = threadIdx.x % 32;
-  const int gv = hg * p.cta_heads + blockIdx.y;
-  const int in_group = gv % p.head_parts * p.part_heads;
-  const int heads = min(p.part_heads, p.group - in_group);
-  for (int hh = threadIdx.x / 32; hh < heads; hh += 8) {
-    // the first piece is its CTA's second kind
-    auto piece = [&](int at) -> int64_t {
-      return ((int64_t)(2 * at + (at == b - 1 ? 1 : 0)) * p.cta_heads + blockIdx.y) * p.part_heads + hh;
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  const int heads = p.cta_heads * p.part_heads;  // of a head group, with those that a part lacks
+  // One query head: `pieces` of the CTAs from what.z - 1 on, every `step`-th from `first`
+  struct Sum {
+    float top, sum;
+    float4 acc;
+  };
+  auto locate = [&](const int4& what, int head, int& in_group) {
+    const int gv = what.y * p.cta_heads + head / p.part_heads;
+    in_group = gv % p.head_parts * p.part_heads + head % p.part_heads;
+    return ((int64_t)what.x * p.num_q_heads + gv / p.head_parts * p.group + in_group) * kHeadDim + lane * 4;
+  };
+  auto gather = [&](const int4& what, int head, int first, int step) {
+    auto piece = [&](int at) -> int64_t {  // the first piece is its CTA's second kind
+      return (int64_t)(2 * at + (at == what.z - 1 ? 1 : 0)) * heads + head;
     };
-    float top = -INFINITY;
-    for (int at = b - 1 + lane; at <= last; at += 32) top = fmaxf(top, p.part_lse[piece(at)]);
+    Sum s = {-INFINITY, 0.f, make_float4(0.f, 0.f, 0.f, 0.f)};
+    for (int at = what.z - 1 + first + lane * step; at <= what.w; at += 32 * step) s.top = fmaxf(s.top, p.part_lse[piece(at)]);
 #pragma unroll
-    for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-    float acc[4] = {0.f, 0.f, 0.f, 0.f}, sum = 0.f;
-#pragma unroll 8
-    for (int at = b - 1; at <= last; ++at) {
+    for (int d = 16; d > 0; d >>= 1) s.top = fmaxf(s.top, __shfl_xor_sync(0xffffffffu, s.top, d));
+#pragma unroll 4
+    for (int at = what.z - 1 + first; at <= what.w; at += step) {
       const int64_t from = piece(at);
       const float lse = p.part_lse[from];
       const float4 v = *reinterpret_cast<const float4*>(p.part_o + from * kHeadDim + lane * 4);
-      const float w = lse == -INFINITY ? 0.f : exp2f(lse - top);
-      sum += w;
-      acc[0] = fmaf(w, v.x, acc[0]), acc[1] = fmaf(w, v.y, acc[1]);
-      acc[2] = fmaf(w, v.z, acc[2]), acc[3] = fmaf(w, v.w, acc[3]);
+      const float w = lse == -INFINITY ? 0.f : exp2f(lse - s.top);
+      s.sum += w;
+      s.acc.x = fmaf(w, v.x, s.acc.x), s.acc.y = fmaf(w, v.y, s.acc.y);
+      s.acc.z = fmaf(w, v.z, s.acc.z), s.acc.w = fmaf(w, v.w, s.acc.w);
     }
-    const float inv = sum == 0.f ? 0.f : 1.0f / sum;
-    const int64_t off = ((int64_t)row * p.num_q_heads + gv / p.head_parts * p.group + in_group + hh) * kHeadDim + lane * 4;
+    return s;
+  };
+  auto finish = [&](const Sum& s, int64_t off) {
+    const float inv = s.sum == 0.f ? 0.f : 1.0f / s.sum;
+    float x[4] = {s.acc.x * inv, s.acc.y * inv, s.acc.z * inv, s.acc.w * inv};
+    if (p.gate) {
 #pragma unroll
-    for (int d = 0; d < 4; ++d) acc[d] *= inv * (p.gate ? sigmoid(__bfloat162float(p.gate[off + d])) : 1.f);
-    const __nv_bfloat162 a = __floats2bfloat162_rn(acc[0], acc[1]), c = __floats2bfloat162_rn(acc[2], acc[3]);
+      for (int d = 0; d < 4; ++d) x[d] *= sigmoid(__bfloat162float(p.gate[off + d]));
+    }
+    const __nv_bfloat162 a = __floats2bfloat162_rn(x[0], x[1]), b = __floats2bfloat162_rn(x[2], x[3]);
     *reinterpret_cast<uint2*>(p.out + off) =
-        make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&c));
+        make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+  };
+  int in_group;
+  const int few = p.plan->num_joins[0] * heads, many = p.plan->num_joins[1] * heads;
+  for (int item = blockIdx.x * 8 + warp; item < few; item += gridDim.x * 8) {
+    const int4 what = p.plan->joins[item / heads];
+    const int64_t off = locate(what, item % heads, in_group);
+    if (in_group < p.group) finish(gather(what, item % heads, 0, 1), off);
+  }
+  for (int item = blockIdx.x; item < many; item += gridDim.x) {
+    const int4 what = p.plan->joins[kPlanMaxCtas - 1 - item / heads];
+    const int64_t off = locate(what, item % heads, in_group);
+    if (in_group >= p.group) continue;
+    const Sum mine = gather(what, item % heads, warp, 8);
+    if (lane == 0) tops[warp] = mine.top, sums[warp] = mine.sum;
+    accs[warp][lane] = mine.acc;
+    __syncthreads();
+    if (warp == 0) {
+      Sum all = {-INFINITY, 0.f, make_float4(0.f, 0.f, 0.f, 0.f)};
+#pragma unroll
+      for (int i = 0; i < 8; ++i) all.top = fmaxf(all.top, tops[i]);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float w = tops[i] == -INFINITY ? 0.f : exp2f(tops[i] - all.top);
+        all.sum = fmaf(w, sums[i], all.sum);
+        const float4 v = accs[i][lane];
+        all.acc.x = fmaf(w, v.x, all.acc.x), all.acc.y = fmaf(w, v.y, all.acc.y);
+        all.acc.z = fmaf(w, v.z, all.acc.z), all.acc.w = fmaf(w, v.w, all.acc.w);
+      }
+      finish(all, off);
+    }
+    __syncthreads();
   }
 }
 
@@ -669,7 +718,7 @@ int sm_count() {
 }
 
 int64_t align256(int64_t x) { return (x + 255) / 256 * 256; }
-int planned_ctas() { return min(2 * kPlanWaves * sm_count(), kPlanMaxCtas); }
+int planned_ctas() { return min(2 * sm_count(), kPlanMaxCtas); }
 
 // Launches a kernel that waits for its prerequisites itself (early = true: it
 // may start before the stream's last kernel has ended).
@@ -767,7 +816,7 @@ cudaError_t launch_block_decode(const BlockDecodeParams& p, cudaStream_t stream)
   if (p.indices) e = start(qsa_block_lengths_kernel, dim3(p.rows), kLenThreads, 0, false, stream, p);
   if (e == cudaSuccess) e = start(qsa_block_plan_kernel, dim3(1), kPlanThreads, 0, p.indices != nullptr, stream, p, planned_ctas());
   if (e == cudaSuccess) e = launch_main(p, stream);
-  if (e == cudaSuccess) e = start(qsa_block_join_kernel, dim3(planned_ctas() - 1, p.cta_heads), 256, 0, true, stream, p);
+  if (e == cudaSuccess) e = start(qsa_block_join_kernel, dim3(kJoinCtas * sm_count()), kJoinThreads, 0, true, stream, p);
   return e;
 }
 

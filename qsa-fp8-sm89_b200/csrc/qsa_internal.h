@@ -196,10 +196,12 @@ struct BlockDecodeParams {
   float* part_o;                 // [2 ctas, cta_heads, part_heads, 128] normalised results of pieces of rows
   float* part_lse;               // [2 ctas, cta_heads, part_heads] their log2-sum-exp2, -inf for none
 };
-constexpr int kPlanMaxCtas = 2048;
+constexpr int kPlanMaxCtas = 1024;
 struct BlockDecodePlan {
   int ctas;
-  int4 joins[kPlanMaxCtas + 1];     // row, head group and last CTA of what is joined at a CTA's begin, or -1
+  int num_joins[2];                 // rows and head groups of few pieces, and of many
+  int4 joins[kPlanMaxCtas];         // row, head group, CTAs of the second and the last piece: the few
+                                    // from the front, the many from the back
   int first_row[kPlanMaxCtas + 1];  // row that each CTA begins in
   int64_t cut[kPlanMaxCtas + 1];    // its first unit
 };
