@@ -792,3 +792,122 @@ def test_operators_refuse_what_does_not_fit():
     assert qsa_block_decode(q[:0], *caches, bt, None).shape == (0, 8, D)
     none = torch.empty(4, 0, dtype=torch.int32, device="cuda")
     assert not qsa_block_decode(q, *caches, bt, i32(0, 0, 1, 1), none).any()
+
+
+@pytest.mark.gpu
+def test_the_serving_example_runs_the_operators_together():
+    """Against fp32 from the projections, so with the codes' own error: a value
+    is off by up to 2^-4 of itself (2^-4 / sqrt(3) / 2 or so on average) and a
+    score by the same of |q||k| / sqrt(128), of some tens of terms."""
+    import importlib.util
+
+    from conftest import REPO
+
+    spec = importlib.util.spec_from_file_location("block_cache_serving", REPO / "examples" / "block_cache_serving.py")
+    example = importlib.util.module_from_spec(spec)
+    import sys
+
+    sys.modules[spec.name] = example
+    spec.loader.exec_module(example)
+    for kw in (dict(), dict(requests=3, steps=2, hq=12, hkv=2, page=24, block=8, topk=7, seed=1)):
+        dense, sparse = example.serve(**kw)
+        assert dense < 0.08 and sparse < 0.08, (dense, sparse)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("group,hkv", [(1, 8), (8, 1), (5, 3), (4, 6), (12, 2), (16, 4), (9, 1), (20, 1), (32, 2), (17, 8)])
+@pytest.mark.parametrize("dense", [False, True])
+def test_block_decode_planned_rows(group, hkv, dense):
+    """Rows of more than 512 columns: shared evenly by the GPU's CTAs, cut and
+    joined, for every layout of heads; empty and short rows between long ones."""
+    from qsa_b200 import qsa_block_decode
+
+    gen = torch.Generator().manual_seed(100 * group + hkv)
+    rows, reqs, page, block, ppr = 7, 3, 16, 4, 130
+    ctx = ppr * page
+    q, gate, k, v, ks, vs, btable, t2r = _decode_inputs(gen, rows, reqs, group * hkv, hkv, page, block, ppr)
+    counts = torch.tensor([1501, 0, 1, ctx, 17, 0, 777], dtype=torch.int32)
+    indices = None
+    if not dense:
+        indices = torch.argsort(torch.rand(rows, ctx, generator=gen), 1)[:, :1600].to(torch.int32)
+        indices[torch.rand(rows, 1600, generator=gen) < 0.02] = -1
+        indices[4] = -1
+    c = lambda t: None if t is None else t.cuda()
+    args = [c(t) for t in (q, k, v, ks, vs, btable, t2r, indices)]
+    out = qsa_block_decode(*args, gate=c(gate), counts=c(counts))
+    again = qsa_block_decode(*args, gate=c(gate), counts=c(counts))
+    torch.cuda.synchronize()
+    assert torch.equal(out, again)
+    _decode_check(out, q, k, v, ks, vs, btable, t2r, indices, counts, gate)
+    assert not out[1].any() and not out[5].any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("group,hkv", [(4, 8), (3, 1), (10, 2)])
+def test_block_decode_one_long_row_in_many_pieces(group, hkv):
+    from qsa_b200 import qsa_block_decode
+
+    gen = torch.Generator().manual_seed(group)
+    page, ppr = 64, 130
+    q, gate, k, v, ks, vs, btable, _ = _decode_inputs(gen, 2, 2, group * hkv, hkv, page, page, ppr)
+    counts = torch.tensor([8317, 3], dtype=torch.int32)
+    c = lambda t: t.cuda()
+    out = qsa_block_decode(c(q), c(k), c(v), c(ks), c(vs), c(btable), None, gate=c(gate), counts=c(counts))
+    torch.cuda.synchronize()
+    _decode_check(out, q, k, v, ks, vs, btable, None, None, counts, gate)
+
+
+@pytest.mark.gpu
+def test_c_abi_calls_with_a_callers_workspace():
+    """The C entry points on raw pointers: the torch operators' results, and
+    refusals of a missing, small or misaligned workspace."""
+    from qsa_b200 import capi, qsa_block_decode, qsa_qk_rope
+
+    gen = torch.Generator().manual_seed(51)
+    rows, hkv, group, page, ppr = 3, 2, 4, 16, 60
+    q, gate, k, v, ks, vs, btable, _ = (t.cuda() for t in _decode_inputs(gen, rows, rows, 8, hkv, page, page, ppr))
+    counts = torch.tensor([950, 0, 600], dtype=torch.int32, device="cuda")
+    want = qsa_block_decode(q, k, v, ks, vs, btable, None, gate=gate, counts=counts)
+    out = torch.empty_like(q)
+    ptr = lambda t: ctypes.c_void_p(t.data_ptr())
+    a = capi.BlockDecodeArgs(q=ptr(q), k_cache=ptr(k), v_cache=ptr(v), k_scales=ptr(ks), v_scales=ptr(vs), counts=ptr(counts),
+                             btable=ptr(btable), gate=ptr(gate), out=ptr(out), softmax_scale=D ** -0.5, rows=rows,
+                             num_q_heads=8, num_kv_heads=hkv, head_dim=D, page_size=page, block_size=page,
+                             pages_per_req=ppr, num_reqs=rows, num_pages=k.shape[0], btable_stride=ppr)
+    need = capi.block_decode_workspace_bytes(a)
+    assert need > 0
+    ws = torch.randint(0, 256, (need + 256,), dtype=torch.uint8, device="cuda")  # needs no clearing
+    stream = torch.cuda.current_stream().cuda_stream
+    assert capi.block_decode(a, None, 0, stream) == capi.ERR_WORKSPACE
+    assert capi.block_decode(a, ws, need - 1, stream) == capi.ERR_WORKSPACE
+    assert capi.block_decode(a, ws[16:], need, stream) == capi.ERR_MISALIGNED
+    for _ in range(2):
+        assert capi.block_decode(a, ws, need, stream) == capi.OK
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)
+
+    table = rope_table(1000, 128).cuda()
+    y = torch.empty_like(q)
+    r = capi.QkRopeArgs(q=ptr(q), q_out=ptr(y), tokens=rows, num_q_heads=8, head_dim=D, q_stride=8 * D, q_out_stride=8 * D,
+                        dtype=capi.DTYPE_BF16)
+    r.rope.table, r.rope.positions = ptr(table), ptr(counts)
+    r.rope.table_len, r.rope.rotary_dim, r.rope.num_axes = 1000, 128, 1
+    assert capi.qk_rope(r, stream) == capi.OK
+    want, _ = qsa_qk_rope(q, None, table, counts)
+    torch.cuda.synchronize()
+    assert torch.equal(y, want)
+
+
+@pytest.mark.gpu
+def test_strides_that_break_a_vector_load_are_refused():
+    from qsa_b200 import block_cache, qsa_block_append, qsa_qk_rope
+
+    wide = torch.zeros(4, 2 * D + 4, device="cuda", dtype=torch.bfloat16)
+    x = wide[:, :2 * D].unflatten(1, (2, D))  # token stride 260 elements: 520 bytes
+    with pytest.raises(RuntimeError, match="aligned"):
+        qsa_qk_rope(x)
+    with pytest.raises(RuntimeError, match="aligned"):
+        qsa_block_append(x, x, *block_cache(4, 4, 2), torch.zeros(4, 1, device="cuda", dtype=torch.int32),
+                         torch.zeros(4, device="cuda", dtype=torch.int32))
+    with pytest.raises(RuntimeError, match="contiguous heads"):
+        qsa_qk_rope(torch.zeros(4, D, 2, device="cuda").transpose(1, 2))
