@@ -7,10 +7,10 @@
 // memory), then brings them through a ring of stages by cp.async, 128 (token,
 // KV head) rows of K and of V at a time: 16 tokens of 8 heads, or more tokens
 // of fewer heads. A token's heads are neighbours in the cache, so a warp's loads
-// run along 1 KiB. Each warp multiplies 16 tokens of one KV head with up to 8
-// query heads: a group of 9 to 16, or 17 to 32, goes as 2 or 4 virtual KV heads
-// whose warps read the same rows of a stage. Warps that have the same heads and
-// other tokens join their results in shared memory.
+// run along 1 KiB. Each warp multiplies 16 tokens of one KV head with a set of
+// up to 8 query heads, or two sets: a larger group goes as 2 or 4 virtual KV
+// heads whose warps read the same rows of a stage. Warps that have the same
+// heads and other tokens join their results in shared memory.
 //
 // Rows of up to 512 columns are a segment and a CTA each. Longer ones are
 // planned: a scan over the rows' lengths gives every CTA of a grid that fills
@@ -55,6 +55,7 @@ constexpr int kBdWarps = 8;
 constexpr int kBdTile = 16;                         // tokens a warp takes at a time
 constexpr int kBdTable = 2048;                      // slots of a CTA's table
 constexpr int kBdColumns = 8;                       // columns that a thread looks up at once
+constexpr int64_t kBdTwoSets = 1 << 19;             // (row, column, KV head)s from which a warp takes 16 query heads
 constexpr int kBdDirect = 512;                      // columns of a row that are not planned
 constexpr float kLazy = 8.f;                        // log2 by which a score may pass its reference
 constexpr float kLazyW = 128.f;                     // factor by which a weight may pass its reference
@@ -110,27 +111,30 @@ __device__ __forceinline__ uint32_t pack_f16(float a, float b) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// kParts: virtual KV heads of a cache head. kCh: cache heads of a CTA.
-template <int kParts, int kCh>
+// kSets: sets of 8 query heads of a warp. kParts: virtual KV heads of a cache
+// head. kCh: cache heads of a CTA.
+template <int kSets, int kParts, int kCh>
 struct BdCfg {
   static constexpr int kHeads = kParts * kCh;                // virtual heads of a CTA
   static constexpr int kSplit = kBdWarps / kHeads;           // warps of a head
   static constexpr int kUnit = kSplit * kBdTile;             // tokens of a stage; the plan counts in them
   static constexpr int kRows = kUnit * kCh;                  // its K rows, and V rows: 128 / kParts
   static constexpr int kStageBytes = 2 * kRows * kHeadDim;
-  static constexpr int kStages = kParts == 1 ? 3 : 6;
+  static constexpr int kStages = kParts == 4 ? 6 : (kSets == 1 ? 3 : 2) * kParts;
   static constexpr int kThreads = 32 * kBdWarps;
   static constexpr int kScales = kStages * kStageBytes;             // float [stages][K, V][kRows]
   static constexpr int kTable = kScales + kStages * 2 * kRows * 4;  // int [kBdTable]
-  static constexpr int kSmem = kTable + kBdTable * 4;
-  static constexpr int kLeft = (8 * (kHeadDim + 2) * 4 + 127) / 128 * 128;  // a warp's result
-  static_assert(kHeads <= kBdWarps && kBdWarps * kLeft <= kScales, "the warps' results fit the ring");
+  // with two sets of heads the Q fragments lie here: uint4 [heads][k-steps][lanes]
+  static constexpr int kQ = kTable + kBdTable * 4;
+  static constexpr int kSmem = kQ + (kSets == 1 ? 0 : kHeads * 8 * 32 * 16);
+  static constexpr int kLeft = (8 * kSets * (kHeadDim + 2) * 4 + 127) / 128 * 128;  // a warp's result
+  static_assert(kHeads <= kBdWarps && kBdWarps * kLeft <= kSmem, "the warps' results fit in what is free at a segment's end");
   static_assert(2 * (kSmem + 1024) <= 228 * 1024, "two CTAs an SM");
 };
 
-template <int kParts, int kCh>
+template <int kSets, int kParts, int kCh>
 __global__ void __launch_bounds__(32 * kBdWarps, 2) qsa_block_decode_kernel(const __grid_constant__ BlockDecodeParams p) {
-  using C = BdCfg<kParts, kCh>;
+  using C = BdCfg<kSets, kParts, kCh>;
   constexpr int kStages = C::kStages, kUnit = C::kUnit;
   constexpr int kRowStep = kCh * kHeadDim;  // from a token of a stage to the next
   extern __shared__ __align__(128) uint8_t smem[];
@@ -184,24 +188,35 @@ __global__ void __launch_bounds__(32 * kBdWarps, 2) qsa_block_decode_kernel(cons
     const int h0 = (g0 + head_in / kParts) * p.group + in_group;
     const int heads = min(p.part_heads, p.group - in_group);
 
-    // the queries as loaded: head r, 16 dims of either half; converted below,
-    // when the first tiles are under way
-    uint4 q_raw[4] = {};
-    if (r < heads) {
-      const uint4* src = reinterpret_cast<const uint4*>(p.q + ((int64_t)row_now * p.num_q_heads + h0 + r) * kHeadDim);
-      q_raw[0] = __ldg(src + 2 * c), q_raw[1] = __ldg(src + 2 * c + 1);
-      q_raw[2] = __ldg(src + 8 + 2 * c), q_raw[3] = __ldg(src + 8 + 2 * c + 1);
+    // the queries as loaded: head r of a set, 16 dims of either half; converted
+    // below, when the first tiles are under way
+    uint4 q_raw[4];
+    auto load_q = [&](int u) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) q_raw[i] = make_uint4(0u, 0u, 0u, 0u);
+      if (u * 8 + r < heads) {
+        const uint4* src = reinterpret_cast<const uint4*>(p.q + ((int64_t)row_now * p.num_q_heads + h0 + u * 8 + r) * kHeadDim);
+        q_raw[0] = __ldg(src + 2 * c), q_raw[1] = __ldg(src + 2 * c + 1);
+        q_raw[2] = __ldg(src + 8 + 2 * c), q_raw[3] = __ldg(src + 8 + 2 * c + 1);
+      }
+    };
+    load_q(0);
+    // Q fragments: f16 of q 2^e, in the order of dims of the K fragments. One
+    // set of heads has them in registers, two leave them in shared memory
+    uint32_t qf[kSets == 1 ? 8 : 1][2];
+    uint4* q_here = reinterpret_cast<uint4*>(smem + C::kQ) + head_in * 8 * 32 + lane;
+    float qs[kSets][2];   // of heads 2c, 2c + 1 of the set: 2^-e softmax_scale log2(e)
+    float o[kSets][8][4]; // [set][dims 16r + 2i, + 1][head 2c, 2c + 1 of either dim]
+    float m[kSets][2], l[kSets][2], W[kSets][2], inv_w[kSets][2];  // of heads 2c, 2c + 1
+#pragma unroll
+    for (int u = 0; u < kSets; ++u) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) m[u][h] = kLowest, l[u][h] = 0.f, W[u][h] = 0.f, inv_w[u][h] = 0.f;  // the first score passes
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[u][i][j] = 0.f;
     }
-    uint32_t qf[8][2];  // Q fragments: f16 of q 2^e, in the order of dims of the K fragments
-    float qs[2];        // of heads 2c, 2c + 1: 2^-e softmax_scale log2(e)
-    float o[8][4];      // [dims 16r + 2i, + 1][head 2c, 2c + 1 of either dim]
-    float m[2], l[2], W[2], inv_w[2];  // of heads 2c, 2c + 1
-#pragma unroll
-    for (int h = 0; h < 2; ++h) m[h] = kLowest, l[h] = 0.f, W[h] = 0.f, inv_w[h] = 0.f;  // the first score passes
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) o[i][j] = 0.f;
 
     // this thread's part of a fetch: 16 bytes of the rows 4i + lane / 8 of its
     // warp's, and a scale of row tid % 128 (K's in the first warps, V's in the
@@ -302,29 +317,38 @@ __global__ void __launch_bounds__(32 * kBdWarps, 2) qsa_block_decode_kernel(cons
       for (int st = 0; st < kStages - 1; ++st) fetch(st, st);
 
       if (base == c0) {
-        float top = 0.f;
-        float2 x[16];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t b[4] = {q_raw[i].x, q_raw[i].y, q_raw[i].z, q_raw[i].w};
+        for (int u = 0; u < kSets; ++u) {
+          if (u > 0) load_q(u);
+          float top = 0.f;
+          float2 x[16];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            x[4 * i + j] = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&b[j]));
-            top = fmaxf(top, fmaxf(fabsf(x[4 * i + j].x), fabsf(x[4 * i + j].y)));
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t b[4] = {q_raw[i].x, q_raw[i].y, q_raw[i].z, q_raw[i].w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              x[4 * i + j] = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&b[j]));
+              top = fmaxf(top, fmaxf(fabsf(x[4 * i + j].x), fabsf(x[4 * i + j].y)));
+            }
           }
-        }
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        int e = 0;  // 2^e maps the largest |q| into [2^14, 2^15)
-        if (top > 0.f && top <= -kLowest) e = min(max(14 + 127 - (int)(__float_as_uint(top) >> 23), -120), 120);
-        const float up = __uint_as_float((uint32_t)(127 + e) << 23);
-        const float down = __uint_as_float((uint32_t)(127 - e) << 23) * p.score_scale_log2;
-        qs[0] = __shfl_sync(0xffffffffu, down, 8 * c);
-        qs[1] = __shfl_sync(0xffffffffu, down, 8 * c + 4);
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+          int e = 0;  // 2^e maps the largest |q| into [2^14, 2^15)
+          if (top > 0.f && top <= -kLowest) e = min(max(14 + 127 - (int)(__float_as_uint(top) >> 23), -120), 120);
+          const float up = __uint_as_float((uint32_t)(127 + e) << 23);
+          const float down = __uint_as_float((uint32_t)(127 - e) << 23) * p.score_scale_log2;
+          qs[u][0] = __shfl_sync(0xffffffffu, down, 8 * c);
+          qs[u][1] = __shfl_sync(0xffffffffu, down, 8 * c + 4);
 #pragma unroll
-        for (int s = 0; s < 8; ++s) {  // k-step s: word s of the thread's chunks c and c + 4
-          qf[s][0] = pack_f16(x[2 * s].x * up, x[2 * s].y * up);
-          qf[s][1] = pack_f16(x[2 * s + 1].x * up, x[2 * s + 1].y * up);
+          for (int s = 0; s < 8; ++s) {  // k-step s: word s of the thread's chunks c and c + 4
+            const uint32_t f0 = pack_f16(x[2 * s].x * up, x[2 * s].y * up);
+            const uint32_t f1 = pack_f16(x[2 * s + 1].x * up, x[2 * s + 1].y * up);
+            if constexpr (kSets == 1) {
+              qf[s][0] = f0, qf[s][1] = f1;
+            } else {  // the same for every part; the loop's first barrier is between this and its reading
+              if (part == 0) reinterpret_cast<uint2*>(q_here + s * 32)[u] = make_uint2(f0, f1);
+            }
+          }
         }
       }
 
@@ -339,8 +363,9 @@ __global__ void __launch_bounds__(32 * kBdWarps, 2) qsa_block_decode_kernel(cons
           const uint8_t* stage = smem + st * C::kStageBytes;
           const float* sc = scales + st * 2 * C::kRows + s_at;
 
-          // [token r: heads 2c, 2c+1; token r + 8: the same], in two chains
-          float s[4] = {}, s1[4] = {};
+          // [set][token r: heads 2c, 2c+1; token r + 8: the same], of one set in
+          // two chains
+          float s[2][4] = {};
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
             const uint4 a4 = *reinterpret_cast<const uint4*>(stage + (k_at ^ (64 * j)));
@@ -349,8 +374,18 @@ __global__ void __launch_bounds__(32 * kBdWarps, 2) qsa_block_decode_kernel(cons
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               const uint32_t a[4] = {f16_of(wa[i]), f16_of(wb[i]), f16_of(wa[i] >> 16), f16_of(wb[i] >> 16)};
-              mma16816(j ? s1 : s, a, qf[4 * j + i][0], qf[4 * j + i][1]);
+              if constexpr (kSets == 1) {
+                mma16816(s[j], a, qf[4 * j + i][0], qf[4 * j + i][1]);
+              } else {
+                const uint4 q4 = q_here[(4 * j + i) * 32];
+                mma16816(s[0], a, q4.x, q4.y);
+                mma16816(s[1], a, q4.z, q4.w);
+              }
             }
+          }
+          if constexpr (kSets == 1) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) s[0][j] += s[1][j];
           }
           const float ks[2] = {sc[0], sc[8 * kCh]}, vs[2] = {sc[C::kRows], sc[C::kRows + 8 * kCh]};
           bool masked[2] = {false, false};
@@ -360,49 +395,52 @@ __global__ void __launch_bounds__(32 * kBdWarps, 2) qsa_block_decode_kernel(cons
           }
 
           // scores over the reference, probabilities, weights over theirs
-          float pr[4], w[4], x_top = -INFINITY, w_abs = 0.f;
+          uint32_t pf[kSets][2];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int t = j / 2, h = j % 2;
-            s[j] += s1[j];
-            float x = fmaf(s[j], ks[t] * qs[h], -m[h]);
-            x = masked[t] ? -INFINITY : x;
-            pr[j] = ex2(x);
-            w[j] = pr[j] * (vs[t] * inv_w[h]);
-            x_top = fmaxf(x_top, x);
-            w_abs = fmaxf(w_abs, fabsf(w[j]));
-          }
-          if (__any_sync(0xffffffffu, x_top > kLazy || w_abs > kLazyW * kOneW)) {
-            // move the references, and what was summed against them
+          for (int u = 0; u < kSets; ++u) {
+            float pr[4], w[4], x_top = -INFINITY, w_abs = 0.f;
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const float x0 = masked[0] ? -INFINITY : s[h] * (ks[0] * qs[h]);
-              const float x1 = masked[1] ? -INFINITY : s[2 + h] * (ks[1] * qs[h]);
-              float top = fmaxf(x0, x1);
-#pragma unroll
-              for (int d = 4; d <= 16; d *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-              const float m_new = fmaxf(m[h], top);
-              const float alpha = ex2(m[h] - m_new);
-              pr[h] = ex2(x0 - m_new), pr[2 + h] = ex2(x1 - m_new);
-              const float w0 = pr[h] * vs[0], w1 = pr[2 + h] * vs[1];
-              float w_top = fmaxf(fabsf(w0), fabsf(w1));
-#pragma unroll
-              for (int d = 4; d <= 16; d *= 2) w_top = fmaxf(w_top, __shfl_xor_sync(0xffffffffu, w_top, d));
-              const float was = W[h] * alpha;
-              W[h] = fmaxf(was, w_top);
-              // without a weight yet, any that matters passes
-              inv_w[h] = W[h] > 0.f ? kOneW / W[h] : 1e38f;
-              const float f = was > 0.f ? was / W[h] : 0.f;
-              m[h] = m_new;
-              l[h] *= alpha;
-              w[h] = w0 * inv_w[h], w[2 + h] = w1 * inv_w[h];
-#pragma unroll
-              for (int i = 0; i < 8; ++i) o[i][h] *= f, o[i][2 + h] *= f;
+            for (int j = 0; j < 4; ++j) {
+              const int t = j / 2, h = j % 2;
+              float x = fmaf(s[u][j], ks[t] * qs[u][h], -m[u][h]);
+              x = masked[t] ? -INFINITY : x;
+              pr[j] = ex2(x);
+              w[j] = pr[j] * (vs[t] * inv_w[u][h]);
+              x_top = fmaxf(x_top, x);
+              w_abs = fmaxf(w_abs, fabsf(w[j]));
             }
+            if (__any_sync(0xffffffffu, x_top > kLazy || w_abs > kLazyW * kOneW)) {
+              // move the references, and what was summed against them
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const float x0 = masked[0] ? -INFINITY : s[u][h] * (ks[0] * qs[u][h]);
+                const float x1 = masked[1] ? -INFINITY : s[u][2 + h] * (ks[1] * qs[u][h]);
+                float top = fmaxf(x0, x1);
+#pragma unroll
+                for (int d = 4; d <= 16; d *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+                const float m_new = fmaxf(m[u][h], top);
+                const float alpha = ex2(m[u][h] - m_new);
+                pr[h] = ex2(x0 - m_new), pr[2 + h] = ex2(x1 - m_new);
+                const float w0 = pr[h] * vs[0], w1 = pr[2 + h] * vs[1];
+                float w_top = fmaxf(fabsf(w0), fabsf(w1));
+#pragma unroll
+                for (int d = 4; d <= 16; d *= 2) w_top = fmaxf(w_top, __shfl_xor_sync(0xffffffffu, w_top, d));
+                const float was = W[u][h] * alpha;
+                W[u][h] = fmaxf(was, w_top);
+                // without a weight yet, any that matters passes
+                inv_w[u][h] = W[u][h] > 0.f ? kOneW / W[u][h] : 1e38f;
+                const float f = was > 0.f ? was / W[u][h] : 0.f;
+                m[u][h] = m_new;
+                l[u][h] *= alpha;
+                w[h] = w0 * inv_w[u][h], w[2 + h] = w1 * inv_w[u][h];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) o[u][i][h] *= f, o[u][i][2 + h] *= f;
+              }
+            }
+            l[u][0] += pr[0] + pr[2];
+            l[u][1] += pr[1] + pr[3];
+            pf[u][0] = transpose8x8(pack_f16(w[0], w[1])), pf[u][1] = transpose8x8(pack_f16(w[2], w[3]));
           }
-          l[0] += pr[0] + pr[2];
-          l[1] += pr[1] + pr[3];
-          const uint32_t pf[2] = {transpose8x8(pack_f16(w[0], w[1])), transpose8x8(pack_f16(w[2], w[3]))};
           // V: chunk r of tokens 2c, 2c+1, 8+2c, 9+2c
           uint32_t vw[4][4];
 #pragma unroll
@@ -418,7 +456,8 @@ __global__ void __launch_bounds__(32 * kBdWarps, 2) qsa_block_decode_kernel(cons
                                    f16_of(__byte_perm(vw[0][i / 2], vw[1][i / 2], sel1)),
                                    f16_of(__byte_perm(vw[2][i / 2], vw[3][i / 2], sel)),
                                    f16_of(__byte_perm(vw[2][i / 2], vw[3][i / 2], sel1))};
-            mma16816(o[i], a, pf[0], pf[1]);
+#pragma unroll
+            for (int u = 0; u < kSets; ++u) mma16816(o[u][i], a, pf[u][0], pf[u][1]);
           }
         }
       }
@@ -426,89 +465,102 @@ __global__ void __launch_bounds__(32 * kBdWarps, 2) qsa_block_decode_kernel(cons
     }
 
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      W[h] *= 1.0f / kOneW;
+    for (int u = 0; u < kSets; ++u) {
 #pragma unroll
-      for (int d = 4; d <= 16; d *= 2) l[h] += __shfl_xor_sync(0xffffffffu, l[h], d);
+      for (int h = 0; h < 2; ++h) {
+        W[u][h] *= 1.0f / kOneW;
+#pragma unroll
+        for (int d = 4; d <= 16; d *= 2) l[u][h] += __shfl_xor_sync(0xffffffffu, l[u][h], d);
+      }
     }
     if (C::kSplit > 1) {
       // the warps of a head join in shared memory: each leaves its result, part
       // 0 gathers (m and l by head, values by head and dim)
       __syncthreads();
-      float* left = reinterpret_cast<float*>(smem + warp * C::kLeft);  // [8][2], then [8][128]
+      float* left = reinterpret_cast<float*>(smem + warp * C::kLeft);  // [heads][2], then [heads][128]
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int hh = 2 * c + h;
-        if (r == 0) left[2 * hh] = m[h], left[2 * hh + 1] = l[h];
+      for (int u = 0; u < kSets; ++u) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          *reinterpret_cast<float2*>(left + 16 + hh * kHeadDim + 16 * r + 2 * i) = make_float2(o[i][h] * W[h], o[i][2 + h] * W[h]);
+        for (int h = 0; h < 2; ++h) {
+          const int hh = u * 8 + 2 * c + h;
+          if (r == 0) left[2 * hh] = m[u][h], left[2 * hh + 1] = l[u][h];
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            *reinterpret_cast<float2*>(left + 16 * kSets + hh * kHeadDim + 16 * r + 2 * i) =
+                make_float2(o[u][i][h] * W[u][h], o[u][i][2 + h] * W[u][h]);
+        }
       }
       __syncthreads();
       if (part > 0) continue;  // the next segment's barriers hold until part 0 has read
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int hh = 2 * c + h;
-        float sum = 0.f, top = kLowest;
+      for (int u = 0; u < kSets; ++u) {
 #pragma unroll
-        for (int w = 0; w < C::kSplit; ++w)
-          top = fmaxf(top, reinterpret_cast<const float*>(smem + (warp + w * C::kHeads) * C::kLeft)[2 * hh]);
+        for (int h = 0; h < 2; ++h) {
+          const int hh = u * 8 + 2 * c + h;
+          float sum = 0.f, top = kLowest;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) o[i][h] = o[i][2 + h] = 0.f;
+          for (int w = 0; w < C::kSplit; ++w)
+            top = fmaxf(top, reinterpret_cast<const float*>(smem + (warp + w * C::kHeads) * C::kLeft)[2 * hh]);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) o[u][i][h] = o[u][i][2 + h] = 0.f;
 #pragma unroll 2
-        for (int w = 0; w < C::kSplit; ++w) {
-          const float* from = reinterpret_cast<const float*>(smem + (warp + w * C::kHeads) * C::kLeft);
-          const float f = ex2(from[2 * hh] - top);
-          sum = fmaf(from[2 * hh + 1], f, sum);
+          for (int w = 0; w < C::kSplit; ++w) {
+            const float* from = reinterpret_cast<const float*>(smem + (warp + w * C::kHeads) * C::kLeft);
+            const float f = ex2(from[2 * hh] - top);
+            sum = fmaf(from[2 * hh + 1], f, sum);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const float2 v = *reinterpret_cast<const float2*>(from + 16 + hh * kHeadDim + 16 * r + 2 * i);
-            o[i][h] = fmaf(f, v.x, o[i][h]), o[i][2 + h] = fmaf(f, v.y, o[i][2 + h]);
+            for (int i = 0; i < 8; ++i) {
+              const float2 v = *reinterpret_cast<const float2*>(from + 16 * kSets + hh * kHeadDim + 16 * r + 2 * i);
+              o[u][i][h] = fmaf(f, v.x, o[u][i][h]), o[u][i][2 + h] = fmaf(f, v.y, o[u][i][2 + h]);
+            }
           }
+          m[u][h] = top, l[u][h] = sum, W[u][h] = 1.f;
         }
-        m[h] = top, l[h] = sum, W[h] = 1.f;
       }
     }
 
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int hh = 2 * c + h;
-      if (hh >= heads) continue;
-      const float f = l[h] == 0.f ? 0.f : W[h] / l[h];  // a NaN sum stays one
-      float x[16];
+    for (int u = 0; u < kSets; ++u) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[2 * i] = o[i][h] * f, x[2 * i + 1] = o[i][2 + h] * f;
-      if (slot_out >= 0) {
-        const int64_t to = ((int64_t)slot_out * C::kHeads + head_in) * p.part_heads + hh;
-        float4* dst = reinterpret_cast<float4*>(p.part_o + to * kHeadDim + 16 * r);
+      for (int h = 0; h < 2; ++h) {
+        const int hh = u * 8 + 2 * c + h;
+        if (hh >= heads) continue;
+        const float f = l[u][h] == 0.f ? 0.f : W[u][h] / l[u][h];  // a NaN sum stays one
+        float x[16];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) dst[i] = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
-        if (r == 0) p.part_lse[to] = l[h] == 0.f ? -INFINITY : m[h] + log2f(l[h]);
-        continue;
-      }
-      const int64_t hr = (int64_t)row_now * p.num_q_heads + h0 + hh;
-      if (p.gate) {
-        const uint4* src = reinterpret_cast<const uint4*>(p.gate + hr * kHeadDim + 16 * r);
+        for (int i = 0; i < 8; ++i) x[2 * i] = o[u][i][h] * f, x[2 * i + 1] = o[u][i][2 + h] * f;
+        if (slot_out >= 0) {
+          const int64_t to = ((int64_t)slot_out * C::kHeads + head_in) * p.part_heads + hh;
+          float4* dst = reinterpret_cast<float4*>(p.part_o + to * kHeadDim + 16 * r);
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const uint4 w4 = __ldg(src + i);
-          const uint32_t b[4] = {w4.x, w4.y, w4.z, w4.w};
+          for (int i = 0; i < 4; ++i) dst[i] = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+          if (r == 0) p.part_lse[to] = l[u][h] == 0.f ? -INFINITY : m[u][h] + log2f(l[u][h]);
+          continue;
+        }
+        const int64_t hr = (int64_t)row_now * p.num_q_heads + h0 + hh;
+        if (p.gate) {
+          const uint4* src = reinterpret_cast<const uint4*>(p.gate + hr * kHeadDim + 16 * r);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float2 gt = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&b[j]));
-            x[8 * i + 2 * j] *= sigmoid(gt.x), x[8 * i + 2 * j + 1] *= sigmoid(gt.y);
+          for (int i = 0; i < 2; ++i) {
+            const uint4 w4 = __ldg(src + i);
+            const uint32_t b[4] = {w4.x, w4.y, w4.z, w4.w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const float2 gt = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&b[j]));
+              x[8 * i + 2 * j] *= sigmoid(gt.x), x[8 * i + 2 * j + 1] *= sigmoid(gt.y);
+            }
           }
         }
-      }
-      uint32_t b[8];
+        uint32_t b[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const __nv_bfloat162 v = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
-        b[i] = *reinterpret_cast<const uint32_t*>(&v);
+        for (int i = 0; i < 8; ++i) {
+          const __nv_bfloat162 v = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+          b[i] = *reinterpret_cast<const uint32_t*>(&v);
+        }
+        uint4* dst = reinterpret_cast<uint4*>(p.out + hr * kHeadDim + 16 * r);
+        dst[0] = make_uint4(b[0], b[1], b[2], b[3]);
+        dst[1] = make_uint4(b[4], b[5], b[6], b[7]);
       }
-      uint4* dst = reinterpret_cast<uint4*>(p.out + hr * kHeadDim + 16 * r);
-      dst[0] = make_uint4(b[0], b[1], b[2], b[3]);
-      dst[1] = make_uint4(b[4], b[5], b[6], b[7]);
     }
   }
 }
@@ -737,9 +789,9 @@ cudaError_t start(Kernel kernel, dim3 grid, int threads, int smem, bool early, c
   return cudaLaunchKernelEx(&config, kernel, args...);
 }
 
-template <int kParts, int kCh>
+template <int kSets, int kParts, int kCh>
 cudaError_t launch(const BlockDecodeParams& p, cudaStream_t stream) {
-  using C = BdCfg<kParts, kCh>;
+  using C = BdCfg<kSets, kParts, kCh>;
   // the shared memory beyond the default limit, once per device
   static std::atomic<uint64_t> ready{0};
   int dev = 0;
@@ -747,26 +799,34 @@ cudaError_t launch(const BlockDecodeParams& p, cudaStream_t stream) {
   if (e != cudaSuccess) return e;
   const uint64_t bit = 1ull << (dev & 63);
   if (!(ready.load(std::memory_order_acquire) & bit)) {
-    e = cudaFuncSetAttribute(qsa_block_decode_kernel<kParts, kCh>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+    e = cudaFuncSetAttribute(qsa_block_decode_kernel<kSets, kParts, kCh>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
     if (e != cudaSuccess) return e;
     ready.fetch_or(bit, std::memory_order_acq_rel);
   }
   const int64_t grid = p.plan ? planned_ctas() : (int64_t)p.rows * (p.num_kv_heads / kCh);
   if (grid > 0x7fffffffll) return cudaErrorInvalidValue;
-  return start(qsa_block_decode_kernel<kParts, kCh>, dim3((unsigned)grid), C::kThreads, C::kSmem, p.plan != nullptr, stream, p);
+  return start(qsa_block_decode_kernel<kSets, kParts, kCh>, dim3((unsigned)grid), C::kThreads, C::kSmem, p.plan != nullptr, stream, p);
 }
 
 cudaError_t launch_main(const BlockDecodeParams& p, cudaStream_t stream) {
-  switch (p.head_parts * 16 + p.cta_heads / p.head_parts) {
-    case 16 + 1: return launch<1, 1>(p, stream);
-    case 16 + 2: return launch<1, 2>(p, stream);
-    case 16 + 4: return launch<1, 4>(p, stream);
-    case 16 + 8: return launch<1, 8>(p, stream);
-    case 32 + 1: return launch<2, 1>(p, stream);
-    case 32 + 2: return launch<2, 2>(p, stream);
-    case 32 + 4: return launch<2, 4>(p, stream);
-    case 64 + 1: return launch<4, 1>(p, stream);
-    case 64 + 2: return launch<4, 2>(p, stream);
+  const int ch = p.cta_heads / p.head_parts;
+  switch ((p.part_heads > 8 ? 64 : 0) + p.head_parts * 8 + ch) {
+    case 8 + 1: return launch<1, 1, 1>(p, stream);
+    case 8 + 2: return launch<1, 1, 2>(p, stream);
+    case 8 + 4: return launch<1, 1, 4>(p, stream);
+    case 8 + 8: return launch<1, 1, 8>(p, stream);
+    case 16 + 1: return launch<1, 2, 1>(p, stream);
+    case 16 + 2: return launch<1, 2, 2>(p, stream);
+    case 16 + 4: return launch<1, 2, 4>(p, stream);
+    case 32 + 1: return launch<1, 4, 1>(p, stream);
+    case 32 + 2: return launch<1, 4, 2>(p, stream);
+    case 72 + 1: return launch<2, 1, 1>(p, stream);
+    case 72 + 2: return launch<2, 1, 2>(p, stream);
+    case 72 + 4: return launch<2, 1, 4>(p, stream);
+    case 72 + 8: return launch<2, 1, 8>(p, stream);
+    case 80 + 1: return launch<2, 2, 1>(p, stream);
+    case 80 + 2: return launch<2, 2, 2>(p, stream);
+    case 80 + 4: return launch<2, 2, 4>(p, stream);
     default: return cudaErrorInvalidValue;
   }
 }
@@ -774,7 +834,12 @@ cudaError_t launch_main(const BlockDecodeParams& p, cudaStream_t stream) {
 }  // namespace
 
 int64_t block_decode_plan(BlockDecodeParams& p) {
-  p.head_parts = p.group <= 8 ? 1 : p.group <= 16 ? 2 : 4;
+  // A group above 8: two sets of heads a warp share the conversions (128 rows of
+  // 2000 tokens, 16 heads for each of 8 KV heads: 138 us against 170), but make a
+  // tile's work longer, which shows where a CTA has few tiles (61 rows of 3000
+  // tokens on average, 20 heads for one KV head: 61 us against 52)
+  const bool large = (int64_t)p.rows * p.num_kv_heads * p.topk >= kBdTwoSets;
+  p.head_parts = p.group <= 8 ? 1 : p.group <= 16 ? (large ? 1 : 2) : (large ? 2 : 4);
   p.part_heads = (p.group + p.head_parts - 1) / p.head_parts;
   p.virtual_heads = p.num_kv_heads * p.head_parts;
   p.cta_heads = p.head_parts;

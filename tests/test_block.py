@@ -911,3 +911,24 @@ def test_strides_that_break_a_vector_load_are_refused():
                          torch.zeros(4, device="cuda", dtype=torch.int32))
     with pytest.raises(RuntimeError, match="contiguous heads"):
         qsa_qk_rope(torch.zeros(4, D, 2, device="cuda").transpose(1, 2))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("group,hkv", [(16, 8), (12, 4), (9, 2), (11, 1), (17, 8), (32, 2), (20, 1), (31, 4)])
+@pytest.mark.parametrize("columns", [500, 1900])
+def test_block_decode_wide_groups_over_much_work(group, hkv, columns):
+    """Enough work for a warp to take 16 query heads (2^19 rows, columns and KV
+    heads): some of the rows, the first and the last among them."""
+    from qsa_b200 import qsa_block_decode
+
+    gen = torch.Generator().manual_seed(group + columns)
+    rows, reqs, page, block, ppr = (1 << 19) // (hkv * columns) + 2, 3, 16, 8, 125
+    q, gate, k, v, ks, vs, btable, t2r = _decode_inputs(gen, rows, reqs, group * hkv, hkv, page, block, ppr)
+    indices = torch.randint(0, ppr * page, (rows, columns), generator=gen, dtype=torch.int32)
+    counts = torch.randint(0, columns + 1, (rows,), generator=gen, dtype=torch.int32)
+    counts[0], counts[1], counts[-1] = columns, 0, 33
+    c = lambda t: t.cuda()
+    out = qsa_block_decode(*(c(t) for t in (q, k, v, ks, vs, btable, t2r, indices)), gate=c(gate), counts=c(counts))
+    torch.cuda.synchronize()
+    pick = [0, 1, rows // 3, rows // 2, rows - 1]
+    _decode_check(out, q, k, v, ks, vs, btable, t2r, indices, counts, gate, rows=pick)
