@@ -102,55 +102,6 @@ __device__ __forceinline__ int block_page(const BlockAppendParams& p, const ApBl
   return page < 0 || page >= p.num_pages ? -1 : page;
 }
 
-enum { kPlain = 0, kHalves = 1, kNeighbours = 2 };  // no rotation; its pairs
-
-// A lane's cosines and sines of a row; false where a position lies outside the
-// table.
-__device__ __forceinline__ bool row_turn(const RopeParams& p, int64_t token, uint32_t own, int l, int turning, float4& c,
-                                         float4& s) {
-  bool in = true;
-  for (int a = 0; a < p.axes; ++a) {
-    const int pos = rope_position(p, token, own, a);
-    in = in && pos >= 0 && pos < p.table_len;
-  }
-  if (!in || l >= turning) return in;
-  const int half = p.rotary >> 1;
-  if (p.quads) {
-    const float* at = p.table + (int64_t)rope_position(p, token, own, rope_axis(p, 4 * l)) * p.rotary + 4 * l;
-    c = __ldg(reinterpret_cast<const float4*>(at));
-    s = __ldg(reinterpret_cast<const float4*>(at + half));
-  } else {
-    float v[8];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float* at = p.table + (int64_t)rope_position(p, token, own, rope_axis(p, 4 * l + i)) * p.rotary + 4 * l + i;
-      v[i] = __ldg(at), v[4 + i] = __ldg(at + half);
-    }
-    c = make_float4(v[0], v[1], v[2], v[3]), s = make_float4(v[4], v[5], v[6], v[7]);
-  }
-  return in;
-}
-
-template <int kTurn>
-__device__ __forceinline__ void turn_row(const float4& c, const float4& s, bool in, bool turns, float (&x)[8]) {
-  if constexpr (kTurn != kPlain) {
-    const float cc[4] = {c.x, c.y, c.z, c.w}, ss[4] = {s.x, s.y, s.z, s.w};
-    if (turns) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        float &u = x[kTurn == kHalves ? i : 2 * i], &v = x[kTurn == kHalves ? 4 + i : 2 * i + 1];
-        const float y = u * cc[i] - v * ss[i];
-        v = v * cc[i] + u * ss[i];
-        u = y;
-      }
-    }
-    if (!in) {
-#pragma unroll
-      for (int d = 0; d < 8; ++d) x[d] = 0.f;
-    }
-  }
-}
-
 // Eight values over their scale, as codes.
 __device__ __forceinline__ uint2 quantise8(float (&v)[8], float s, float inv, bool infinite) {
   if (infinite) {  // an infinity's residual would be NaN
@@ -194,7 +145,7 @@ __device__ __forceinline__ void append_block(const BlockAppendParams& p, const A
   const bool norm = is_k && p.k_weight;
   const int turning = kTurn == kPlain ? 0 : p.rope.rotary >> 3;  // lanes that hold rotated elements
   const bool halves = kTurn == kHalves && l < turning;
-  const Pieces pieces = halves ? Pieces{4 * l, (p.rope.rotary >> 1) + 4 * l} : Pieces{8 * l, 8 * l + 4};
+  const Pieces pieces = lane_pieces<kTurn>(l, p.rope.rotary);
   const T* src = static_cast<const T*>(is_k ? p.k : p.v);
 
   // The half warp's rows of the block's new ones: row0, row0 + 2, ... Past the
@@ -243,8 +194,8 @@ __device__ __forceinline__ void append_block(const BlockAppendParams& p, const A
                   ((int64_t)max(page, 0) * (p.page_size / p.block_size) + off / (uint32_t)p.block_size) * p.num_kv_heads;
   const int kept = page < 0 ? 0 : b.kept;
 
-  auto load_turn = [&](int row, float4& c, float4& sn) {
-    return row_turn(p.rope, clamped(row), b.pos + min(row, max(b.count - 1, 0)), l, turning, c, sn);
+  auto turn_of = [&](int row, float4& c, float4& sn) {
+    return load_turn(p.rope, clamped(row), b.pos + min(row, max(b.count - 1, 0)), l, turning, c, sn);
   };
   // the lane's cosines and sines of its rows wait in shared memory
   float4* turns = reinterpret_cast<float4*>(ring + kApStages * kApRows * kHeadDim) + lane;
@@ -253,7 +204,7 @@ __device__ __forceinline__ void append_block(const BlockAppendParams& p, const A
 #pragma unroll
     for (int i = 0; i < kApSteps; ++i) {
       float4 c = {}, sn = {};
-      if (!load_turn(row0 + 2 * i, c, sn)) inside &= ~(1u << i);
+      if (!turn_of(row0 + 2 * i, c, sn)) inside &= ~(1u << i);
       turns[(2 * i) * 32] = c, turns[(2 * i + 1) * 32] = sn;
     }
   }
@@ -301,7 +252,7 @@ __device__ __forceinline__ void append_block(const BlockAppendParams& p, const A
 #pragma unroll
         for (int i = 0; i < kApSteps; ++i) {
           float4 c = {}, sn = {};
-          const bool in = kTurn == kPlain || load_turn(first + 2 * i, c, sn);
+          const bool in = kTurn == kPlain || turn_of(first + 2 * i, c, sn);
           value(raw[i], c, sn, in, x[0]);
           with(first + 2 * i);
         }
@@ -393,7 +344,7 @@ __device__ __forceinline__ void append_packed(const BlockAppendParams& p, const 
   const bool norm = is_k && p.k_weight;
   const int turning = kTurn == kPlain ? 0 : p.rope.rotary >> 3;
   const bool halves = kTurn == kHalves && l < turning;
-  const Pieces pieces = halves ? Pieces{4 * l, (p.rope.rotary >> 1) + 4 * l} : Pieces{8 * l, 8 * l + 4};
+  const Pieces pieces = lane_pieces<kTurn>(l, p.rope.rotary);
   const int B = p.block_size;
   const uint32_t half_mask = 0xffffu << (16 * side);
   if (b.count == 0 || b.req < 0 || b.req >= p.num_reqs) return;
@@ -416,7 +367,7 @@ __device__ __forceinline__ void append_packed(const BlockAppendParams& p, const 
     row_at[i] = goes ? (int64_t)page * p.page_size + off : -1;
     scale_at[i] = goes ? (int64_t)page * (p.page_size / B) + off / (uint32_t)B : -1;
     block[i] = (b.kept + in_run) / B;
-    if (kTurn != kPlain && !row_turn(p.rope, token, pos, l, turning, cs[i], sn[i])) inside &= ~(1u << i);
+    if (kTurn != kPlain && !load_turn(p.rope, token, pos, l, turning, cs[i], sn[i])) inside &= ~(1u << i);
   }
   float w[8];
 #pragma unroll
@@ -553,7 +504,7 @@ __global__ void __launch_bounds__(32 * kApWarps) qsa_block_append_one_kernel(con
   const bool is_k = side == 0;
   const int turning = kTurn == kPlain ? 0 : p.rope.rotary >> 3;
   const bool halves = kTurn == kHalves && is_k && l < turning;
-  const Pieces pieces = halves ? Pieces{4 * l, (p.rope.rotary >> 1) + 4 * l} : Pieces{8 * l, 8 * l + 4};
+  const Pieces pieces = halves ? lane_pieces<kTurn>(l, p.rope.rotary) : Pieces{8 * l, 8 * l + 4};
   Raw8<T> raw;
   load8(static_cast<const T*>(is_k ? p.k : p.v) + (int64_t)e * p.token_stride + g * kHeadDim, pieces, raw);
   const int start = __ldg(p.starts + e);
@@ -565,7 +516,7 @@ __global__ void __launch_bounds__(32 * kApWarps) qsa_block_append_one_kernel(con
   const bool goes = page >= 0 && page < p.num_pages;
   float4 c = {}, sn = {};
   bool in = true;
-  if (kTurn != kPlain && is_k) in = row_turn(p.rope, e, max(start, 0), l, turning, c, sn);
+  if (kTurn != kPlain && is_k) in = load_turn(p.rope, e, max(start, 0), l, turning, c, sn);
   float w[8], x[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) w[i] = 1.f;

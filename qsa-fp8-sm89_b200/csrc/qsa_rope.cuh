@@ -20,12 +20,15 @@ namespace qsa {
 
 constexpr int kRowLanes = 16;  // lanes of a row, 8 elements each
 
+enum { kPlain = 0, kHalves = 1, kNeighbours = 2 };  // no rotation; its pairs
+
 // First elements of a lane's two pieces.
 struct Pieces {
   int a, b;
 };
-__device__ __forceinline__ Pieces lane_pieces(const RopeParams& p, int l) {
-  if (p.table && !p.interleaved && l < (p.rotary >> 3)) return {4 * l, (p.rotary >> 1) + 4 * l};
+template <int kTurn>
+__device__ __forceinline__ Pieces lane_pieces(int l, int rotary) {
+  if (kTurn == kHalves && l < (rotary >> 3)) return {4 * l, (rotary >> 1) + 4 * l};
   return {8 * l, 8 * l + 4};
 }
 
@@ -100,8 +103,9 @@ __device__ __forceinline__ void load_weight8(const void* weight, int dtype, Piec
   }
 }
 
-// x *= rsqrt(mean(x^2) + eps) * w over the half warp's 128 elements.
-__device__ __forceinline__ void rms_norm8(float (&x)[8], const float (&w)[8], float eps) {
+// x *= rsqrt(mean(x^2) + eps) * w over the half warp's 128 elements, where
+// `norms` (every lane goes through the exchanges).
+__device__ __forceinline__ void rms_norm8(float (&x)[8], const float (&w)[8], float eps, bool norms = true) {
   float s = 0.f;
 #pragma unroll
   for (int i = 0; i < 8; ++i) s = fmaf(x[i], x[i], s);
@@ -113,16 +117,10 @@ __device__ __forceinline__ void rms_norm8(float (&x)[8], const float (&w)[8], fl
   float r = rsqrtf(v);
   const float t = v * r, e = fmaf(-fmaf(v, r, -t), r, fmaf(-t, r, 1.0f));  // 1 - v r r
   if (r > 0.f && r <= 3.4e38f) r = fmaf(0.5f * r, e, r);
+  if (!norms) r = 1.f;
 #pragma unroll
   for (int i = 0; i < 8; ++i) x[i] = x[i] * r * w[i];
 }
-
-// The cosines and sines of a lane's pairs 4l .. 4l+3.
-struct Turn4 {
-  float c[4], s[4];
-  bool turns;  // the lane holds rotated elements
-  bool in;     // the token's positions lie inside the table
-};
 
 // Axis of pair j.
 __device__ __forceinline__ int rope_axis(const RopeParams& p, int j) {
@@ -138,47 +136,52 @@ __device__ __forceinline__ int rope_position(const RopeParams& p, int64_t token,
   return __ldg(p.positions + axis * p.axis_stride + token);
 }
 
-// Reads nothing outside the table.
-__device__ __forceinline__ void load_turn4(const RopeParams& p, int64_t token, uint32_t own, int l, Turn4& t) {
-  t.in = true;
+// The cosines and sines of a lane's pairs 4l .. 4l+3; false where a position
+// lies outside the table (nothing is read there). turning: lanes that hold
+// rotated elements.
+__device__ __forceinline__ bool load_turn(const RopeParams& p, int64_t token, uint32_t own, int l, int turning, float4& c,
+                                          float4& s) {
+  bool in = true;
   for (int a = 0; a < p.axes; ++a) {
     const int pos = rope_position(p, token, own, a);
-    t.in = t.in && pos >= 0 && pos < p.table_len;
+    in = in && pos >= 0 && pos < p.table_len;
   }
-  t.turns = t.in && l < (p.rotary >> 3);
-  if (!t.turns) return;
+  if (!in || l >= turning) return in;
   const int half = p.rotary >> 1;
   if (p.quads) {
-    const float* row = p.table + (int64_t)rope_position(p, token, own, rope_axis(p, 4 * l)) * p.rotary + 4 * l;
-    const float4 c = __ldg(reinterpret_cast<const float4*>(row));
-    const float4 s = __ldg(reinterpret_cast<const float4*>(row + half));
-    t.c[0] = c.x, t.c[1] = c.y, t.c[2] = c.z, t.c[3] = c.w;
-    t.s[0] = s.x, t.s[1] = s.y, t.s[2] = s.z, t.s[3] = s.w;
+    const float* at = p.table + (int64_t)rope_position(p, token, own, rope_axis(p, 4 * l)) * p.rotary + 4 * l;
+    c = __ldg(reinterpret_cast<const float4*>(at));
+    s = __ldg(reinterpret_cast<const float4*>(at + half));
   } else {
+    float v[8];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float* row = p.table + (int64_t)rope_position(p, token, own, rope_axis(p, 4 * l + i)) * p.rotary + 4 * l + i;
-      t.c[i] = __ldg(row);
-      t.s[i] = __ldg(row + half);
+      const float* at = p.table + (int64_t)rope_position(p, token, own, rope_axis(p, 4 * l + i)) * p.rotary + 4 * l + i;
+      v[i] = __ldg(at), v[4 + i] = __ldg(at + half);
     }
+    c = make_float4(v[0], v[1], v[2], v[3]), s = make_float4(v[4], v[5], v[6], v[7]);
   }
+  return in;
 }
 
-__device__ __forceinline__ void rotate8(const RopeParams& p, const Turn4& t, float (&x)[8]) {
-  auto turn = [&](float& a, float& b, int i) {
-    const float u = a * t.c[i] - b * t.s[i], v = b * t.c[i] + a * t.s[i];
-    a = u, b = v;
-  };
-  if (t.turns && p.interleaved) {
+// A row outside the table becomes zeros. turns: the lane holds rotated elements.
+template <int kTurn>
+__device__ __forceinline__ void turn_row(const float4& c, const float4& s, bool in, bool turns, float (&x)[8]) {
+  if constexpr (kTurn != kPlain) {
+    const float cc[4] = {c.x, c.y, c.z, c.w}, ss[4] = {s.x, s.y, s.z, s.w};
+    if (turns) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) turn(x[2 * i], x[2 * i + 1], i);
-  } else if (t.turns) {
+      for (int i = 0; i < 4; ++i) {
+        float &u = x[kTurn == kHalves ? i : 2 * i], &v = x[kTurn == kHalves ? 4 + i : 2 * i + 1];
+        const float y = u * cc[i] - v * ss[i];
+        v = v * cc[i] + u * ss[i];
+        u = y;
+      }
+    }
+    if (!in) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) turn(x[i], x[4 + i], i);
-  }
-  if (!t.in) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = 0.f;
+      for (int d = 0; d < 8; ++d) x[d] = 0.f;
+    }
   }
 }
 
