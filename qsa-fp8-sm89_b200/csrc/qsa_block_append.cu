@@ -193,6 +193,7 @@ __device__ __forceinline__ void append_block(const BlockAppendParams& p, const A
   float* scales = (is_k ? p.k_scales : p.v_scales) +
                   ((int64_t)max(page, 0) * (p.page_size / p.block_size) + off / (uint32_t)p.block_size) * p.num_kv_heads;
   const int kept = page < 0 ? 0 : b.kept;
+  const bool all_rows = __all_sync(0xffffffffu, row0 + 2 * (kApSteps - 1) < b.count);
 
   auto turn_of = [&](int row, float4& c, float4& sn) {
     return load_turn(p.rope, clamped(row), b.pos + min(row, max(b.count - 1, 0)), l, turning, c, sn);
@@ -208,10 +209,10 @@ __device__ __forceinline__ void append_block(const BlockAppendParams& p, const A
       turns[(2 * i) * 32] = c, turns[(2 * i + 1) * 32] = sn;
     }
   }
-  auto value = [&](const Raw8<T>& from, const float4& c, const float4& s, bool in, float (&x)[8]) {
-    widen8(from, x);
+  auto normed = [&](float (&x)[kApSteps][8]) {
+#pragma unroll
+    for (int i = 0; i < kApSteps; ++i) widen8(raw[i], x[i]);
     if (norm) rms_norm8(x, w, p.eps);
-    turn_row<kTurn>(c, s, in, l < turning, x);
   };
   auto row_top = [&](const float (&x)[8], float top) {  // NaN counts for none
 #pragma unroll
@@ -240,7 +241,7 @@ __device__ __forceinline__ void append_block(const BlockAppendParams& p, const A
       for (int i = 0; i < kApSteps; ++i)
         if (row0 + 2 * i < kept) codes[i] = *reinterpret_cast<const uint2*>(dst + (int64_t)(row0 + 2 * i) * step + 8 * l);
     }
-    float x[kHold ? kApSteps : 1][8];
+    float x[kApSteps][8];
     float top = 0.f;
     // larger blocks: the rows again, 64 at a time, through `with`
     auto each_row = [&](auto with) {
@@ -249,12 +250,13 @@ __device__ __forceinline__ void append_block(const BlockAppendParams& p, const A
         for (int i = 0; i < kApSteps; ++i) {
           load_row(src + (int64_t)clamped(first + 2 * i) * p.token_stride + min(g, p.num_kv_heads - 1) * kHeadDim, raw[i]);
         }
+        normed(x);
 #pragma unroll
         for (int i = 0; i < kApSteps; ++i) {
           float4 c = {}, sn = {};
           const bool in = kTurn == kPlain || turn_of(first + 2 * i, c, sn);
-          value(raw[i], c, sn, in, x[0]);
-          with(first + 2 * i);
+          turn_row<kTurn>(c, sn, in, l < turning, x[i]);
+          with(first + 2 * i, x[i]);
         }
       }
     };
@@ -265,15 +267,23 @@ __device__ __forceinline__ void append_block(const BlockAppendParams& p, const A
 #pragma unroll
       for (int i = 0; i < kApSteps; ++i)
         load_row(ring + (h % kApStages * kApRows + side * kApSteps + i) * kHeadDim, raw[i]);
+      normed(x);
+      // all lanes hold rotated elements: nothing to choose between the rows
+      auto turn = [&](bool turns_too) {
 #pragma unroll
-      for (int i = 0; i < kApSteps; ++i) {
-        float4 c = {}, sn = {};
-        if (kTurn != kPlain) c = turns[(2 * i) * 32], sn = turns[(2 * i + 1) * 32];
-        value(raw[i], c, sn, (inside >> i) & 1u, x[i]);
-        top = row_top(x[i], top);
-      }
+        for (int i = 0; i < kApSteps; ++i) {
+          float4 c = {}, sn = {};
+          if (kTurn != kPlain) c = turns[(2 * i) * 32], sn = turns[(2 * i + 1) * 32];
+          turn_row<kTurn>(c, sn, (inside >> i) & 1u, turns_too, x[i]);
+          top = row_top(x[i], top);
+        }
+      };
+      if (turning == kRowLanes)
+        turn(true);
+      else
+        turn(l < turning);
     } else {
-      each_row([&](int) { top = finite_top(x[0], top); });
+      each_row([&](int, const float(&v)[8]) { top = finite_top(v, top); });
     }
     top = warp_max(top);
     bool infinite = top > FLT_MAX;
@@ -306,12 +316,18 @@ __device__ __forceinline__ void append_block(const BlockAppendParams& p, const A
       store_codes(dst + (int64_t)(b.kept + row) * step, pieces, halves, quantise8(v, s, inv, infinite));
     };
     if constexpr (kHold) {
+      if (all_rows && !infinite) {
 #pragma unroll
-      for (int i = 0; i < kApSteps; ++i)
-        if (row0 + 2 * i < b.count) store(row0 + 2 * i, x[i]);
+        for (int i = 0; i < kApSteps; ++i)
+          store_codes(dst + (int64_t)(b.kept + row0 + 2 * i) * step, pieces, halves, quantise8(x[i], s, inv, false));
+      } else {
+#pragma unroll
+        for (int i = 0; i < kApSteps; ++i)
+          if (row0 + 2 * i < b.count) store(row0 + 2 * i, x[i]);
+      }
     } else {
-      each_row([&](int row) {
-        if (row < b.count) store(row, x[0]);
+      each_row([&](int row, float(&v)[8]) {
+        if (row < b.count) store(row, v);
       });
     }
     if (old == s) continue;
@@ -389,10 +405,11 @@ __device__ __forceinline__ void append_packed(const BlockAppendParams& p, const 
     float x[kApSteps][8], top[2 * kApSteps];  // of every row of the warp
     bool infinite = false;
 #pragma unroll
+    for (int i = 0; i < kApSteps; ++i) widen8(raw[i], x[i]);
+    if (norm) rms_norm8(x, w, p.eps);
+#pragma unroll
     for (int i = 0; i < kApSteps; ++i) {
       const int j = kTurn == kPlain ? 0 : i;
-      widen8(raw[i], x[i]);
-      if (norm) rms_norm8(x[i], w, p.eps);
       turn_row<kTurn>(cs[j], sn[j], (inside >> i) & 1u, l < turning, x[i]);
       float v = 0.f;  // NaN counts for none
 #pragma unroll
@@ -528,12 +545,12 @@ __global__ void __launch_bounds__(32 * kApWarps) qsa_block_append_one_kernel(con
 
   widen8(raw, x);
   if (p.k_weight) {
-    float y[8];
+    float y[1][8];
 #pragma unroll
-    for (int d = 0; d < 8; ++d) y[d] = x[d];
+    for (int d = 0; d < 8; ++d) y[0][d] = x[d];
     rms_norm8(y, w, p.eps);
 #pragma unroll
-    for (int d = 0; d < 8; ++d) x[d] = is_k ? y[d] : x[d];
+    for (int d = 0; d < 8; ++d) x[d] = is_k ? y[0][d] : x[d];
   }
   if (is_k) turn_row<kTurn>(c, sn, in, l < turning, x);
   float top = 0.f, finite = 0.f;

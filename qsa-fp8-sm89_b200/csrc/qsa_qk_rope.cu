@@ -24,7 +24,7 @@ constexpr int kQrHeads = 8;  // heads of a half warp, at most
 
 // kTurn: the rotation's pairs, or none. kNorm: some heads are normed.
 template <typename T, int kTurn, bool kNorm>
-__global__ void __launch_bounds__(kQrThreads, 9) qsa_qk_rope_kernel(const __grid_constant__ QkRopeParams p, int per) {
+__global__ void __launch_bounds__(kQrThreads, sizeof(T) == 4 ? 8 : 9) qsa_qk_rope_kernel(const __grid_constant__ QkRopeParams p, int per) {
   constexpr int kBatch = 2;
   const int l = threadIdx.x % kRowLanes;
   const int q_parts = (p.heads[0] + per - 1) / per;
@@ -57,13 +57,14 @@ __global__ void __launch_bounds__(kQrThreads, 9) qsa_qk_rope_kernel(const __grid
       if (!kFull) raw[i] = {};
       if (kFull || b + i < n) load8(src + (b + i) * 128, pieces, raw[i]);
     }
+    float x[kBatch][8];
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) widen8(raw[i], x[i]);
+    if constexpr (kNorm) rms_norm8(x, w, p.eps, weight != nullptr);
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) {
-      float x[8];
-      widen8(raw[i], x);
-      if constexpr (kNorm) rms_norm8(x, w, p.eps, weight != nullptr);
-      turn_row<kTurn>(c, sn, in, l < turning, x);
-      if (kFull || b + i < n) store8(dst + (b + i) * 128, pieces, x);
+      turn_row<kTurn>(c, sn, in, l < turning, x[i]);
+      if (kFull || b + i < n) store8(dst + (b + i) * 128, pieces, x[i]);
     }
   };
   int b = 0;

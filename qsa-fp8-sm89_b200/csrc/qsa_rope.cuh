@@ -103,23 +103,34 @@ __device__ __forceinline__ void load_weight8(const void* weight, int dtype, Piec
   }
 }
 
-// x *= rsqrt(mean(x^2) + eps) * w over the half warp's 128 elements, where
-// `norms` (every lane goes through the exchanges).
-__device__ __forceinline__ void rms_norm8(float (&x)[8], const float (&w)[8], float eps, bool norms = true) {
-  float s = 0.f;
+// x *= rsqrt(mean(x^2) + eps) * w over the half warp's 128 elements, for N rows
+// whose exchanges run side by side. Every lane goes through them; where `norms` is
+// false it keeps its rows.
+template <int N>
+__device__ __forceinline__ void rms_norm8(float (&x)[N][8], const float (&w)[8], float eps, bool norms = true) {
+  float s[N];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) s = fmaf(x[i], x[i], s);
+  for (int n = 0; n < N; ++n) {
+    s[n] = 0.f;
 #pragma unroll
-  for (int o = kRowLanes / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-  // one Newton step from the 2 ulp of rsqrtf to nearly the nearest value: what a
-  // row is off by shifts all its codes where it is quantised
-  const float v = fmaf(s, 1.0f / 128.0f, eps);
-  float r = rsqrtf(v);
-  const float t = v * r, e = fmaf(-fmaf(v, r, -t), r, fmaf(-t, r, 1.0f));  // 1 - v r r
-  if (r > 0.f && r <= 3.4e38f) r = fmaf(0.5f * r, e, r);
-  if (!norms) r = 1.f;
+    for (int i = 0; i < 8; ++i) s[n] = fmaf(x[n][i], x[n][i], s[n]);
+  }
 #pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] = x[i] * r * w[i];
+  for (int o = kRowLanes / 2; o > 0; o >>= 1)
+#pragma unroll
+    for (int n = 0; n < N; ++n) s[n] += __shfl_xor_sync(0xffffffffu, s[n], o);
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    // one Newton step from the 2 ulp of rsqrtf to nearly the nearest value: what a
+    // row is off by shifts all its codes where it is quantised
+    const float v = fmaf(s[n], 1.0f / 128.0f, eps);
+    float r = rsqrtf(v);
+    const float t = v * r, e = fmaf(-fmaf(v, r, -t), r, fmaf(-t, r, 1.0f));  // 1 - v r r
+    if (r > 0.f && r <= 3.4e38f) r = fmaf(0.5f * r, e, r);
+    if (!norms) r = 1.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[n][i] = x[n][i] * r * w[i];
+  }
 }
 
 // Axis of pair j.
