@@ -103,6 +103,26 @@ __device__ __forceinline__ void load_weight8(const void* weight, int dtype, Piec
   }
 }
 
+// Two fp32 operations an instruction; each half is rounded as by itself.
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};\n" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpair(uint64_t v, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;\n" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;\n" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;\n" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+
 // x *= rsqrt(mean(x^2) + eps) * w over the half warp's 128 elements, for N rows
 // whose exchanges run side by side. Every lane goes through them; where `norms` is
 // false it keeps its rows.
@@ -111,9 +131,15 @@ __device__ __forceinline__ void rms_norm8(float (&x)[N][8], const float (&w)[8],
   float s[N];
 #pragma unroll
   for (int n = 0; n < N; ++n) {
-    s[n] = 0.f;
+    uint64_t sum = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) s[n] = fmaf(x[n][i], x[n][i], s[n]);
+    for (int i = 0; i < 8; i += 2) {
+      const uint64_t v = pair(x[n][i], x[n][i + 1]);
+      sum = fma2(v, v, sum);
+    }
+    float even, odd;
+    unpair(sum, even, odd);
+    s[n] = even + odd;
   }
 #pragma unroll
   for (int o = kRowLanes / 2; o > 0; o >>= 1)
@@ -129,7 +155,8 @@ __device__ __forceinline__ void rms_norm8(float (&x)[N][8], const float (&w)[8],
     if (r > 0.f && r <= 3.4e38f) r = fmaf(0.5f * r, e, r);
     if (!norms) r = 1.f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[n][i] = x[n][i] * r * w[i];
+    for (int i = 0; i < 8; i += 2)
+      unpair(mul2(mul2(pair(x[n][i], x[n][i + 1]), pair(r, r)), pair(w[i], w[i + 1])), x[n][i], x[n][i + 1]);
   }
 }
 
@@ -180,10 +207,18 @@ template <int kTurn>
 __device__ __forceinline__ void turn_row(const float4& c, const float4& s, bool in, bool turns, float (&x)[8]) {
   if constexpr (kTurn != kPlain) {
     const float cc[4] = {c.x, c.y, c.z, c.w}, ss[4] = {s.x, s.y, s.z, s.w};
-    if (turns) {
+    if (turns && kTurn == kHalves) {
+#pragma unroll
+      for (int i = 0; i < 4; i += 2) {
+        const uint64_t u = pair(x[i], x[i + 1]), v = pair(x[4 + i], x[5 + i]);
+        const uint64_t co = pair(cc[i], cc[i + 1]);
+        unpair(fma2(u, co, mul2(v, pair(-ss[i], -ss[i + 1]))), x[i], x[i + 1]);
+        unpair(fma2(v, co, mul2(u, pair(ss[i], ss[i + 1]))), x[4 + i], x[5 + i]);
+      }
+    } else if (turns) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        float &u = x[kTurn == kHalves ? i : 2 * i], &v = x[kTurn == kHalves ? 4 + i : 2 * i + 1];
+        float &u = x[2 * i], &v = x[2 * i + 1];
         const float y = u * cc[i] - v * ss[i];
         v = v * cc[i] + u * ss[i];
         u = y;
