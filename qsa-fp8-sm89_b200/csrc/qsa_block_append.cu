@@ -21,6 +21,17 @@
 // slot finds its entry by a search that splits the list 32 ways a step. The new
 // rows' loads go out before the block table is read, and a kept block's codes
 // before it is known whether its scale grows.
+//
+// Prompts of 52224 tokens in all, 8 KV heads, blocks of 64: 348 MB in 96 us, 3.6
+// TB/s; 37 % of DRAM, 59 % of the issue slots with 16 warps an SM (128
+// registers): what bounds it is the arithmetic's latency. Without norm and rotation
+// 71 us. The steps: two passes over the rows 348; rows held in registers 299;
+// loads without guards, the pairing known at compile time 158; no IEEE division,
+// one redux a maximum 139; rows through cp.async a head ahead 108 (two or three
+// heads ahead: the same); the norm's exchanges side by side 104; no branches
+// around whole blocks 98; packed fp32 arithmetic 96. 3 CTAs of 80 registers an SM
+// pay only where nothing rotates (76 against 79).
+// 256 entries of one token: 5.7 us. Blocks above 64 tokens read twice: 201 us.
 #include <atomic>
 #include <cfloat>
 

@@ -9,11 +9,12 @@
 // the norm are template parameters: 43 M instead of 55 M instructions at the size
 // below. 9 CTAs of 128 threads an SM (56 registers).
 //
-// 16384 tokens of 32 + 8 heads of bf16, 2 x 168 MB and the table's 8 MB: 67.7 us,
+// 16384 tokens of 32 + 8 heads of bf16, 2 x 168 MB and the table's 8 MB: 67.8 us,
 // 5.1 TB/s (a plain copy: 6.5). 4 heads at a time and 256 threads: 71.7; 8 CTAs
 // an SM: 70; 10: 68.1, with spills; loads ahead of the table's rows and a batch
-// ahead: 73 to 86. 256 tokens: 8.7 us, the launch and two rounds to memory.
-// 1531 tokens with three axes: 10.5 us (4 heads at a time: 14.6).
+// ahead: 73 to 86. Warps wait for memory most of the time (56 % of DRAM, 62 % of
+// the issue slots). 256 tokens: 9 us, the launch and two rounds to memory. 1531
+// tokens of fp32 with three axes: 10.2 us (4 heads at a time: 14.6).
 #include "qsa_rope.cuh"
 
 namespace qsa {
