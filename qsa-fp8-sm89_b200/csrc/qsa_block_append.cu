@@ -31,7 +31,9 @@
 // heads ahead: the same); the norm's exchanges side by side 104; no branches
 // around whole blocks 98; packed fp32 arithmetic 96. 3 CTAs of 80 registers an SM
 // pay only where nothing rotates (76 against 79).
-// 256 entries of one token: 5.7 us. Blocks above 64 tokens read twice: 201 us.
+// 256 entries of one token: 5.7 us. Blocks above 64 tokens read twice: 200 us;
+// blocks of 1 token 125 us, of 2 to 4 tokens 163 (each row's scale, its page and
+// its place are its own, so the registers hold no row ahead).
 #include <atomic>
 #include <cfloat>
 
@@ -369,8 +371,11 @@ __device__ __forceinline__ void append_block(const BlockAppendParams& p, const A
 // Blocks of up to 4 tokens: a warp takes as many as its 8 rows hold, b being
 // their run (a block of `run` = 8 / block_size * block_size tokens to
 // find_block). Each row has a scale, and a page, of its own block.
-template <typename T, int kTurn>
-__device__ __forceinline__ void append_packed(const BlockAppendParams& p, const ApBlock& b, bool is_k, int g0, int per) {
+// kSingle: blocks of one token, so that rows have nothing to do with each other
+// and nothing is kept. turns: the lane's cosines and sines of its rows wait here.
+template <typename T, int kTurn, bool kSingle>
+__device__ __forceinline__ void append_packed(const BlockAppendParams& p, const ApBlock& b, bool is_k, int g0, int per,
+                                              float4* turns) {
   const int lane = threadIdx.x % 32, l = lane % kRowLanes, side = lane / kRowLanes;
   const bool norm = is_k && p.k_weight;
   const int turning = kTurn == kPlain ? 0 : p.rope.rotary >> 3;
@@ -383,9 +388,11 @@ __device__ __forceinline__ void append_packed(const BlockAppendParams& p, const 
   // the half warp's new rows side, side + 2, ...: where they are and go
   const T* src[kApSteps];
   int64_t row_at[kApSteps], scale_at[kApSteps];  // -1: not written
-  int block[kApSteps];                           // in the run
-  float4 cs[kTurn == kPlain ? 1 : kApSteps], sn[kTurn == kPlain ? 1 : kApSteps];
   uint32_t inside = 0xffffffffu;
+  // byte i: which of the half warp's rows (bits 0 .. 3) and of the other's are
+  // of row i's block; bit i: row i is its block's first new one, and its block
+  // keeps rows (known ahead: a head's work has no divisions)
+  uint32_t same = 0, begins = 0, leads = 0;
 #pragma unroll
   for (int i = 0; i < kApSteps; ++i) {
     const int row = side + 2 * i, in_run = min(row, b.count - 1);
@@ -397,43 +404,66 @@ __device__ __forceinline__ void append_packed(const BlockAppendParams& p, const 
     const bool goes = row < b.count && page >= 0 && page < p.num_pages;
     row_at[i] = goes ? (int64_t)page * p.page_size + off : -1;
     scale_at[i] = goes ? (int64_t)page * (p.page_size / B) + off / (uint32_t)B : -1;
-    block[i] = (b.kept + in_run) / B;
-    if (kTurn != kPlain && !load_turn(p.rope, token, pos, l, turning, cs[i], sn[i])) inside &= ~(1u << i);
+    if constexpr (!kSingle) {
+      const int block = (b.kept + in_run) / B;
+#pragma unroll
+      for (int k = 0; k < kApSteps; ++k) {
+        const int mine = (b.kept + min(side + 2 * k, b.count - 1)) / B, other = (b.kept + min(1 - side + 2 * k, b.count - 1)) / B;
+        same |= (mine == block ? 1u : 0u) << (8 * i + k) | (other == block ? 1u : 0u) << (8 * i + 4 + k);
+      }
+      if (row == 0 || (b.kept + row) % B == 0) begins |= 1u << i;
+      if (b.kept % B > 0 && block == b.kept / B) leads |= 1u << i;
+    }
+    if (kTurn != kPlain) {
+      float4 c = {}, sn = {};
+      if (!load_turn(p.rope, token, pos, l, turning, c, sn)) inside &= ~(1u << i);
+      turns[(2 * i) * 32] = c, turns[(2 * i + 1) * 32] = sn;  // read by this lane alone
+    }
   }
   float w[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) w[i] = 1.f;
   if (norm) load_weight8(p.k_weight, p.weight_dtype, pieces, w);
-  const int lead = b.kept % B, lead_block = b.kept / B;  // rows that the first new row's block keeps
+  const int lead = kSingle ? 0 : b.kept % B;  // rows that the first new row's block keeps
   uint8_t* cache = is_k ? p.k_cache : p.v_cache;
   float* scales = is_k ? p.k_scales : p.v_scales;
 
-#pragma unroll 1
-  for (int g = g0; g < min(g0 + per, p.num_kv_heads); ++g) {
-    Raw8<T> raw[kApSteps];
-    float old[kApSteps];
+  const int g1 = min(g0 + per, p.num_kv_heads);
+  Raw8<T> raw[kApSteps];
+  auto load = [&](int g) {
 #pragma unroll
-    for (int i = 0; i < kApSteps; ++i) {
-      load8(src[i] + g * kHeadDim, pieces, raw[i]);
-      old[i] = lead > 0 && block[i] == lead_block && scale_at[i] >= 0 ? scales[scale_at[i] * p.num_kv_heads + g] : 0.f;
+    for (int i = 0; i < kApSteps; ++i) load8(src[i] + g * kHeadDim, pieces, raw[i]);
+  };
+  constexpr bool kAhead = kSingle;  // otherwise there are no registers for it
+  if (kAhead) load(g0);
+#pragma unroll 1
+  for (int g = g0; g < g1; ++g) {
+    if (!kAhead) load(g);
+    float old[kApSteps];
+    if constexpr (!kSingle) {
+#pragma unroll
+      for (int i = 0; i < kApSteps; ++i)
+        old[i] = (leads >> i & 1u) && scale_at[i] >= 0 ? scales[scale_at[i] * p.num_kv_heads + g] : 0.f;
     }
     float x[kApSteps][8], top[2 * kApSteps];  // of every row of the warp
     bool infinite = false;
 #pragma unroll
     for (int i = 0; i < kApSteps; ++i) widen8(raw[i], x[i]);
+    if (kAhead && g + 1 < g1) load(g + 1);  // under way while this head is worked on
     if (norm) rms_norm8(x, w, p.eps);
 #pragma unroll
     for (int i = 0; i < kApSteps; ++i) {
-      const int j = kTurn == kPlain ? 0 : i;
-      turn_row<kTurn>(cs[j], sn[j], (inside >> i) & 1u, l < turning, x[i]);
+      float4 c = {}, sn = {};
+      if (kTurn != kPlain) c = turns[(2 * i) * 32], sn = turns[(2 * i + 1) * 32];
+      turn_row<kTurn>(c, sn, (inside >> i) & 1u, l < turning, x[i]);
       float v = 0.f;  // NaN counts for none
 #pragma unroll
       for (int d = 0; d < 8; ++d) v = fmaxf(v, fabsf(x[i][d]));
       infinite = infinite || v > FLT_MAX;
       top[i] = v;
     }
-    if (__any_sync(0xffffffffu, infinite)) {  // rare: infinities count for none
-      infinite = true;
+    infinite = __any_sync(0xffffffffu, infinite);
+    if (infinite) {  // rare: infinities count for none
 #pragma unroll
       for (int i = 0; i < kApSteps; ++i) {
         top[i] = 0.f;
@@ -444,7 +474,23 @@ __device__ __forceinline__ void append_packed(const BlockAppendParams& p, const 
 #pragma unroll
     for (int i = 0; i < kApSteps; ++i) {
       top[i] = __uint_as_float(__reduce_max_sync(half_mask, __float_as_uint(top[i])));
-      top[kApSteps + i] = __shfl_xor_sync(0xffffffffu, top[i], 16);
+      if (!kSingle) top[kApSteps + i] = __shfl_xor_sync(0xffffffffu, top[i], 16);
+    }
+    if constexpr (kSingle) {
+      float s[kApSteps], inv[kApSteps];
+#pragma unroll
+      for (int i = 0; i < kApSteps; ++i) {
+        s[i] = fmaxf(divide(top[i], 448.f, 1.0f / 448.f), kMinScale);
+        inv[i] = __fdividef(1.f, s[i]);
+      }
+#pragma unroll
+      for (int i = 0; i < kApSteps; ++i) {
+        const uint2 codes = quantise8(x[i], s[i], inv[i], infinite);
+        if (row_at[i] < 0) continue;
+        store_codes(cache + (row_at[i] * p.num_kv_heads + g) * kHeadDim, pieces, halves, codes);
+        if (l == 0) scales[row_at[i] * p.num_kv_heads + g] = s[i];  // a row is a block
+      }
+      continue;
     }
     __syncwarp();  // the old scales are read before a lane writes them
 #pragma unroll
@@ -452,23 +498,15 @@ __device__ __forceinline__ void append_packed(const BlockAppendParams& p, const 
       // the maximum of the row's block, whose other rows are this half's or the
       // other's; rows past the last one repeat it
       float v = top[i];
-      if (B > 1) {
 #pragma unroll
-        for (int k = 0; k < kApSteps; ++k) {
-          if (block[k] == block[i]) v = fmaxf(v, top[k]);
-          const int other = (b.kept + min(1 - side + 2 * k, b.count - 1)) / B;
-          if (other == block[i]) v = fmaxf(v, top[kApSteps + k]);
-        }
-      }
+      for (int k = 0; k < 2 * kApSteps; ++k) v = same >> (8 * i + k) & 1u ? fmaxf(v, top[k]) : v;
       const float s = fmaxf(old[i], fmaxf(divide(v, 448.f, 1.0f / 448.f), kMinScale));
       const float inv = __fdividef(1.f, s);
       if (row_at[i] < 0) continue;
       store_codes(cache + (row_at[i] * p.num_kv_heads + g) * kHeadDim, pieces, halves, quantise8(x[i], s, inv, infinite));
       // the first row of a block that goes sees to its scale and its kept rows
-      const int row = side + 2 * i;
-      const bool begins = row == 0 || (b.kept + row) % B == 0;
-      if (!begins || old[i] == s) continue;
-      if (row == 0 && lead > 0) {
+      if (!(begins >> i & 1u) || old[i] == s) continue;
+      if (i == 0 && side == 0 && lead > 0) {
         const float ratio = divide(old[i], s, inv);
         for (int back = 1; back <= lead; ++back) {
           uint2* at = reinterpret_cast<uint2*>(cache + ((row_at[i] - back) * p.num_kv_heads + g) * kHeadDim + 8 * l);
@@ -507,9 +545,11 @@ __global__ void __launch_bounds__(32 * kApWarps, sizeof(T) == 2 && kTurn == kPla
     append_block<T, kHold, kPlain>(p, b, false, g0, group, per, tops, ring);
 }
 
-template <typename T, int kTurn>
+template <typename T, int kTurn, bool kSingle>
 __global__ void __launch_bounds__(32 * kApWarps, 2)
     qsa_block_append_packed_kernel(const __grid_constant__ BlockAppendParams p, uint32_t items, int run, int per) {
+  __shared__ float4 turns[kTurn == kPlain ? 1 : kApWarps * kApSteps * 2 * 32];
+  float4* own_turns = turns + (kTurn == kPlain ? 0 : threadIdx.x / 32 * kApSteps * 2 * 32 + threadIdx.x % 32);
   const uint32_t parts = (p.num_kv_heads + per - 1) / per;
   const uint32_t item = blockIdx.x * kApWarps + threadIdx.x / 32;
   if (item >= items) return;
@@ -517,9 +557,9 @@ __global__ void __launch_bounds__(32 * kApWarps, 2)
   const int g0 = (int)(item - slot * parts) * per;
   const ApBlock b = find_block(p, slot, threadIdx.x % 32, run);
   if (blockIdx.y == 0)
-    append_packed<T, kTurn>(p, b, true, g0, per);
+    append_packed<T, kTurn, kSingle>(p, b, true, g0, per, own_turns);
   else
-    append_packed<T, kPlain>(p, b, false, g0, per);
+    append_packed<T, kPlain, kSingle>(p, b, false, g0, per, own_turns);
 }
 
 // One token an entry, a decode step's append: a warp takes an entry and head, its
@@ -651,7 +691,7 @@ cudaError_t launch(const BlockAppendParams& p, int64_t slots, cudaStream_t strea
   return launch<T, kHold, kNeighbours>(p, (uint32_t)items, grid, group, per, stream);
 }
 
-template <typename T>
+template <typename T, bool kSingle>
 cudaError_t launch_packed(const BlockAppendParams& p, int64_t slots, int run, cudaStream_t stream) {
   int per = 1;
   while (per < kApHeads && per < p.num_kv_heads && slots * 2 * ((p.num_kv_heads + 2 * per - 1) / (2 * per)) >= 148 * 32) per *= 2;
@@ -661,11 +701,11 @@ cudaError_t launch_packed(const BlockAppendParams& p, int64_t slots, int run, cu
   const dim3 grid((unsigned)blocks, 2);
   const int threads = 32 * kApWarps;
   if (!p.rope.table)
-    qsa_block_append_packed_kernel<T, kPlain><<<grid, threads, 0, stream>>>(p, (uint32_t)items, run, per);
+    qsa_block_append_packed_kernel<T, kPlain, kSingle><<<grid, threads, 0, stream>>>(p, (uint32_t)items, run, per);
   else if (!p.rope.interleaved)
-    qsa_block_append_packed_kernel<T, kHalves><<<grid, threads, 0, stream>>>(p, (uint32_t)items, run, per);
+    qsa_block_append_packed_kernel<T, kHalves, kSingle><<<grid, threads, 0, stream>>>(p, (uint32_t)items, run, per);
   else
-    qsa_block_append_packed_kernel<T, kNeighbours><<<grid, threads, 0, stream>>>(p, (uint32_t)items, run, per);
+    qsa_block_append_packed_kernel<T, kNeighbours, kSingle><<<grid, threads, 0, stream>>>(p, (uint32_t)items, run, per);
   return cudaGetLastError();
 }
 
@@ -675,7 +715,8 @@ cudaError_t launch_type(const BlockAppendParams& p, cudaStream_t stream) {
   // blocks of up to 4 tokens leave half of a warp's 8 rows empty, or more
   const int run = p.block_size <= kApRows / 2 ? kApRows / p.block_size * p.block_size : p.block_size;
   const int64_t slots = (int64_t)(p.tokens / run) + 2 * (int64_t)p.entries;
-  if (run > p.block_size) return launch_packed<T>(p, slots, run, stream);
+  if (run > p.block_size)
+    return p.block_size == 1 ? launch_packed<T, true>(p, slots, run, stream) : launch_packed<T, false>(p, slots, run, stream);
   return p.block_size <= kApWarps * kApRows ? launch<T, true>(p, slots, stream) : launch<T, false>(p, slots, stream);
 }
 
