@@ -932,3 +932,66 @@ def test_block_decode_wide_groups_over_much_work(group, hkv, columns):
     torch.cuda.synchronize()
     pick = [0, 1, rows // 3, rows // 2, rows - 1]
     _decode_check(out, q, k, v, ks, vs, btable, t2r, indices, counts, gate, rows=pick)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("hkv", [5, 8])
+@pytest.mark.parametrize("page,block", [(16, 1), (16, 2), (12, 4), (16, 16), (64, 64), (128, 128)])
+def test_block_append_of_much_work_holds_what_small_calls_hold(page, block, hkv, dtype):
+    """A large call, whose warps go through several heads of a block, against a
+    call for each request, whose warps take one: the same bits."""
+    from qsa_b200 import qsa_block_append
+
+    gen = torch.Generator().manual_seed(page + block + hkv)
+    n = 40
+    counts = torch.randint(1, 600, (n,), generator=gen)
+    starts = torch.randint(0, 90, (n,), generator=gen).to(torch.int32).cuda()
+    cu = torch.cat([torch.zeros(1, dtype=torch.int64), counts.cumsum(0)]).to(torch.int32)
+    ppr = -(-700 // page)
+    pages = n * ppr
+    btable = torch.randperm(pages, generator=gen).view(n, ppr).to(torch.int32).cuda()
+    kv = torch.randn(int(cu[-1]), 2 * hkv, D, generator=gen).to(dtype).cuda()
+    w = (1 + 0.3 * torch.randn(D, generator=gen)).to(dtype).cuda()
+    table = rope_table(700, 64).cuda()
+    codes, scales = _caches(gen, pages, page, block, hkv)
+    results = []
+    for parts in ([(0, n)], [(e, e + 1) for e in range(n)]):
+        kc, vc = (c.clone().cuda().view(torch.float8_e4m3fn) for c in codes)
+        ks, vs = (s.clone().cuda() for s in scales)
+        for a, b in parts:
+            x = kv[int(cu[a]):int(cu[b])]
+            qsa_block_append(x[:, :hkv], x[:, hkv:], kc, vc, ks, vs, btable, starts[a:b].clone(),
+                             reqs=torch.arange(a, b, dtype=torch.int32, device="cuda"),
+                             cu_tokens=(cu[a:b + 1] - cu[a]).cuda(), table=table, k_weight=w)
+        results.append([u8(kc), u8(vc), ks.cpu().numpy(), vs.cpu().numpy()])
+    for large, small in zip(*results):
+        assert np.array_equal(large, small)
+    assert not np.array_equal(results[0][0], codes[0].numpy())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("tokens,hq,hkv,rotary,interleaved,norm", [
+    (2101, 32, 8, 128, False, True), (30011, 5, 3, 64, False, True), (12007, 13, 0, 128, True, True),
+    (9001, 17, 1, 32, True, False), (6007, 24, 4, 0, False, True)])
+def test_qk_rope_of_much_work_gives_what_small_calls_give(tokens, hq, hkv, rotary, interleaved, norm, dtype):
+    """A large call, whose half warps go through several heads of a token,
+    against calls on slices, whose half warps take one: the same bits."""
+    from qsa_b200 import qsa_qk_rope
+
+    gen = torch.Generator(device="cuda").manual_seed(tokens)
+    qkv = torch.randn(tokens, hq + hkv, D, generator=gen, device="cuda").to(dtype)
+    k = qkv[:, hq:] if hkv else None
+    w = (1 + 0.3 * torch.randn(D, generator=gen, device="cuda")).to(dtype) if norm else None
+    table = rope_table(512, rotary).cuda() if rotary else None
+    positions = torch.randint(-1, 513, (tokens,), generator=gen, device="cuda", dtype=torch.int32) if rotary else None
+    opts = dict(q_weight=w, interleaved=interleaved)
+    large = qsa_qk_rope(qkv[:, :hq], k, table, positions, **opts)
+    step = 18000 // (hq + hkv)
+    for a in range(0, tokens, step):
+        at = slice(a, min(a + step, tokens))
+        small = qsa_qk_rope(qkv[at, :hq], None if k is None else k[at], table,
+                            None if positions is None else positions[at].clone(), **opts)
+        for x, y in zip(large, small):
+            assert (x is None and y is None) or torch.equal(x[at], y)
