@@ -43,7 +43,10 @@
 // Softmax with lazy references: scores are taken against a reference m that
 // moves only when one passes it by 8, weights p vs against a reference W that
 // moves when one passes 128 W (2^15 in f16), so that scales may spread over any
-// range. The usual tile needs one vote and no reduction.
+// range. The usual tile needs one vote and no reduction. W is 2^-112 at least: a
+// block of zero values has the scale 2^-126, and 2^8 over that passes fp32's range.
+// With all scales at 2^-126 a weight keeps its 11 bits down to a probability of
+// 2^-8 and is off by 2^-19 of the largest below that.
 //
 // Times: 8 rows of 90001 to 131072 tokens, 64 query on 8 KV heads: 287 us, 6.3
 // TB/s of cache (a plain copy: 6.5; after some 10 ms of it the 1000 W limit lowers
@@ -68,6 +71,7 @@ constexpr int kBdDirect = 512;                      // columns of a row that are
 constexpr float kLazy = 8.f;                        // log2 by which a score may pass its reference
 constexpr float kLazyW = 128.f;                     // factor by which a weight may pass its reference
 constexpr float kOneW = 256.f;                      // what stands for W in f16
+constexpr float kLeastW = 0x1p-112f;                // kOneW / W stays finite
 constexpr float kLowest = -3.402823466e38f;
 
 // The approximate forms (a few ulp) have no branches: 32 of the exact ones a
@@ -434,9 +438,8 @@ __global__ void __launch_bounds__(32 * kBdWarps, 2) qsa_block_decode_kernel(cons
 #pragma unroll
                 for (int d = 4; d <= 16; d *= 2) w_top = fmaxf(w_top, __shfl_xor_sync(0xffffffffu, w_top, d));
                 const float was = W[u][h] * alpha;
-                W[u][h] = fmaxf(was, w_top);
-                // without a weight yet, any that matters passes
-                inv_w[u][h] = W[u][h] > 0.f ? kOneW / W[u][h] : 1e38f;
+                W[u][h] = fmaxf(fmaxf(was, w_top), kLeastW);
+                inv_w[u][h] = kOneW / W[u][h];
                 const float f = was > 0.f ? was / W[u][h] : 0.f;
                 m[u][h] = m_new;
                 l[u][h] *= alpha;

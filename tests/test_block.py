@@ -995,3 +995,81 @@ def test_qk_rope_of_much_work_gives_what_small_calls_give(tokens, hq, hkv, rotar
                             None if positions is None else positions[at].clone(), **opts)
         for x, y in zip(large, small):
             assert (x is None and y is None) or torch.equal(x[at], y)
+
+
+# ------------------------------------- GPU: what the writer stores, attended ----
+# tokens of each request, and the ranges of them whose values are zero
+ZERO_CONTEXTS = [(1, [(0, 1)]), (40, [(0, 40)]), (46, [(0, 16)]), (114, [(0, 64)]), (228, [(0, 128)]), (150, [(134, 150)]),
+                 (33, [(32, 33)]), (505, [(0, 256), (300, 505)]), (7, [(0, 5)])]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("group,hkv", [(4, 8), (4, 1), (3, 2), (20, 1), (12, 2), (16, 8)])
+@pytest.mark.parametrize("page,block", [(16, 16), (8, 1)])
+@pytest.mark.parametrize("columns", [512, 800, "two sets"])
+@pytest.mark.parametrize("dense", [False, True])
+def test_zero_values_appended_and_attended(group, hkv, page, block, columns, dense):
+    """Values of zero get the writer's smallest scale, 2^-126: their average
+    is zero, and beside other values they only count in the softmax's sum. Every
+    second KV head keeps ordinary values."""
+    from qsa_b200 import block_cache, qsa_block_append, qsa_block_decode
+
+    gen = torch.Generator().manual_seed(group + hkv + page)
+    counts = [n for n, _ in ZERO_CONTEXTS]
+    rows = len(counts)
+    used = -(-max(counts) // page)
+    if columns == "two sets":  # from 2^19 (row, column, KV head)s on a warp takes 16 query heads
+        columns = (1 << 19) // (rows * hkv) + page
+    ppr = -(-columns // page)
+    btable = torch.full((rows, ppr), -1, dtype=torch.int32)
+    btable[:, :used] = torch.randperm(rows * used, generator=gen).view(rows, used).to(torch.int32)
+    kv = torch.randn(sum(counts), 2 * hkv, D, generator=gen)
+    at = 0
+    for n, zeros in ZERO_CONTEXTS:
+        for a, b in zeros:
+            kv[at + a:at + b, hkv::2] = 0.0
+        at += n
+    kv = kv.to(torch.bfloat16).cuda()
+    cache = block_cache(rows * used, page, hkv, block)
+    cu = torch.tensor([0] + list(np.cumsum(counts)), dtype=torch.int32, device="cuda")
+    qsa_block_append(kv[:, :hkv], kv[:, hkv:], *cache, btable.cuda(), torch.zeros(rows, dtype=torch.int32, device="cuda"),
+                     cu_tokens=cu)
+    assert (cache[3] == 2.0 ** -126).any()
+    q = _bf16(torch.randn(rows, group * hkv, D, generator=gen))
+    gate = _bf16(torch.randn(rows, group * hkv, D, generator=gen))
+    n = torch.tensor(counts, dtype=torch.int32)
+    indices = None
+    if not dense:
+        indices = torch.arange(columns, dtype=torch.int32).repeat(rows, 1)
+        indices = torch.where(indices < n[:, None], indices, -1)
+    out = qsa_block_decode(q.cuda(), *cache, btable.cuda(), None, None if dense else indices.cuda(), gate=gate.cuda(),
+                           counts=n.cuda() if dense else None)
+    torch.cuda.synchronize()
+    ref = _decode_check(out, q, *(t.cpu() for t in cache), btable, None, None if dense else indices[:, :max(counts)],
+                        n if dense else None, gate)
+    zero = (ref == 0).all(-1)
+    assert zero[:2, :group].all() and not out.cpu()[torch.from_numpy(zero)].any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("group,hkv", [(4, 8), (5, 1), (16, 8), (20, 2)])
+@pytest.mark.parametrize("columns", [512, 800])
+def test_block_decode_value_scales_from_zero_to_large(group, hkv, columns):
+    """Value scales of 0, 2^-126 and 2^-121 beside ordinary and large ones, a
+    tiny one in front of every row, and rows of tiny ones alone."""
+    from qsa_b200 import qsa_block_decode
+
+    gen = torch.Generator().manual_seed(group + hkv)
+    rows, page = 8, 16
+    ppr = columns // page
+    q, gate, k, v, ks, vs, btable, _ = _decode_inputs(gen, rows, rows, group * hkv, hkv, page, page, ppr)
+    choice = torch.tensor([0.0, 2.0 ** -126, 2.0 ** -121, 2.0 ** -100, 0.02, 8.0, 300.0])
+    vs = choice[torch.randint(0, len(choice), vs.shape, generator=gen)]
+    first = btable[:, 0].long()
+    vs[first] = choice[torch.randint(0, 3, (rows, 1, hkv), generator=gen)]
+    vs[btable[6].long()], vs[btable[7].long()] = 2.0 ** -126, 2.0 ** -121
+    counts = torch.tensor([1, 16, 17, 40, 200, columns, columns - 3, 130], dtype=torch.int32)
+    c = lambda t: t.cuda()
+    out = qsa_block_decode(c(q), c(k), c(v), c(ks), c(vs), c(btable), None, gate=c(gate), counts=c(counts))
+    torch.cuda.synchronize()
+    _decode_check(out, q, k, v, ks, vs, btable, None, None, counts, gate)
