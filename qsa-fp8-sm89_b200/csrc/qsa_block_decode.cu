@@ -417,7 +417,9 @@ __global__ void __launch_bounds__(32 * kBdWarps, 2) qsa_block_decode_kernel(cons
               float x = fmaf(s[u][j], ks[t] * qs[u][h], -m[u][h]);
               x = masked[t] ? -INFINITY : x;
               pr[j] = ex2(x);
-              w[j] = pr[j] * (vs[t] * inv_w[u][h]);
+              // a scale over a far smaller reference may pass fp32's range; of a
+              // probability of 0 it must not
+              w[j] = (pr[j] * vs[t]) * inv_w[u][h];
               x_top = fmaxf(x_top, x);
               w_abs = fmaxf(w_abs, fabsf(w[j]));
             }

@@ -1073,3 +1073,32 @@ def test_block_decode_value_scales_from_zero_to_large(group, hkv, columns):
     out = qsa_block_decode(c(q), c(k), c(v), c(ks), c(vs), c(btable), None, gate=c(gate), counts=c(counts))
     torch.cuda.synchronize()
     _decode_check(out, q, k, v, ks, vs, btable, None, None, counts, gate)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("group,hkv", [(4, 8), (5, 1), (16, 8), (20, 2)])
+@pytest.mark.parametrize("columns", [512, 800])
+@pytest.mark.parametrize("tiny", [0.0, 2.0 ** -126])
+def test_block_decode_a_large_scale_of_no_probability(group, hkv, columns, tiny):
+    """Tokens whose scores lie some 300 powers of two below the others' have
+    the probability 0, whatever the scale of their values."""
+    from qsa_b200 import qsa_block_decode
+
+    gen = torch.Generator().manual_seed(group + hkv)
+    rows, page = 4, 16
+    ppr = columns // page
+    q, gate, k, v, ks, vs, btable, _ = _decode_inputs(gen, rows, rows, group * hkv, hkv, page, page, ppr)
+    # along dim 0 a query of 2000 meets +-32 * 0.02: scores of about +-113, 163 powers of two either way
+    q[..., 0] = 2000.0
+    k[..., 0] = -32.0
+    ks[:] = 0.02
+    vs[:] = 1024.0
+    first = btable[:, :1].long()
+    k[first, :, :, 0] = 32.0
+    vs[first] = tiny
+    counts = torch.tensor([16, 17, 200, columns], dtype=torch.int32)
+    c = lambda t: t.cuda()
+    out = qsa_block_decode(c(q), c(k), c(v), c(ks), c(vs), c(btable), None, gate=c(gate), counts=c(counts))
+    torch.cuda.synchronize()
+    _decode_check(out, q, k, v, ks, vs, btable, None, None, counts, gate)
+    assert tiny > 0 or not out.any()
