@@ -360,7 +360,8 @@ typedef struct qsa_b200_block_decode_args {
   int32_t pages_per_req;
   int32_t num_reqs;
   int64_t num_pages;      /* num_pages * page_size <= 2^31 - 1 */
-  int32_t topk;           /* not read without indices */
+  int32_t topk;           /* not read without indices; a row's columns (topk, or pages_per_req * page_size) are
+                             up to 2^31 - 2049, and times num_kv_heads below 2^36 */
   int64_t indices_stride;
   int64_t btable_stride;
 } qsa_b200_block_decode_args;

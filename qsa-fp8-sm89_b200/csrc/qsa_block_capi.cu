@@ -63,9 +63,11 @@ int check_block_decode(const qsa_b200_block_decode_args* a, BlockDecodeParams* p
     return QSA_B200_ERR_BAD_SHAPE;
   if (a->indices && (a->topk < 0 || a->indices_stride < a->topk)) return QSA_B200_ERR_BAD_SHAPE;
   if (a->head_dim != 128 || a->num_q_heads / a->num_kv_heads > 32) return QSA_B200_ERR_UNSUPPORTED;
-  // token slots and columns are held as int32
-  if (a->num_pages > 0x7fffffffll / a->page_size ||
-      (!a->indices && (int64_t)a->pages_per_req * a->page_size > 0x7fffffffll))
+  // token slots, columns and the tiles of a row over its (up to 4 virtual) KV
+  // heads are held as int32
+  const int64_t columns = a->indices ? a->topk : (int64_t)a->pages_per_req * a->page_size;
+  if (a->num_pages > 0x7fffffffll / a->page_size || columns > kBlockMaxColumns ||
+      (columns / 128 + 1) * 4 > 0x7fffffffll / a->num_kv_heads)
     return QSA_B200_ERR_UNSUPPORTED;
   if ((int64_t)a->rows * a->num_q_heads > 0x7fffffffll) return QSA_B200_ERR_BAD_SHAPE;
   if (a->rows > 0) {

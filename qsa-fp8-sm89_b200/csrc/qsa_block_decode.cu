@@ -65,6 +65,7 @@ namespace {
 constexpr int kBdWarps = 8;
 constexpr int kBdTile = 16;                         // tokens a warp takes at a time
 constexpr int kBdTable = 2048;                      // slots of a CTA's table
+static_assert(kBlockMaxColumns + kBdTable <= 0x7fffffffll, "the columns' counter");
 constexpr int kBdColumns = 8;                       // columns that a thread looks up at once
 constexpr int64_t kBdTwoSets = 1 << 19;             // (row, column, KV head)s from which a warp takes 16 query heads
 constexpr int kBdDirect = 512;                      // columns of a row that are not planned

@@ -196,6 +196,9 @@ struct BlockDecodeParams {
   float* part_o;                 // [2 ctas, cta_heads, part_heads, 128] normalised results of pieces of rows
   float* part_lse;               // [2 ctas, cta_heads, part_heads] their log2-sum-exp2, -inf for none
 };
+// Columns of a row: they are counted in int32, a CTA's table of slots at a time,
+// which may begin up to a table past the last one.
+constexpr int kBlockMaxColumns = 0x7fffffff - 2048;
 constexpr int kPlanMaxCtas = 1024;
 struct BlockDecodePlan {
   int ctas;

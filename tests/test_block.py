@@ -1102,3 +1102,24 @@ def test_block_decode_a_large_scale_of_no_probability(group, hkv, columns, tiny)
     torch.cuda.synchronize()
     _decode_check(out, q, k, v, ks, vs, btable, None, None, counts, gate)
     assert tiny > 0 or not out.any()
+
+
+def test_block_decode_refuses_columns_past_its_counters():
+    """Columns are counted in int32, 2048 at a time, and so are the tiles of a
+    row over its KV heads: what would overflow is refused, the largest is not."""
+    from qsa_b200 import capi
+
+    ppr = (2 ** 31 - 2048) // 16
+    for over, ok in [
+        (dict(indices=None, pages_per_req=ppr, btable_stride=ppr), False),  # 2^31 - 2048 columns
+        (dict(indices=None, pages_per_req=ppr - 1, btable_stride=ppr), True),
+        (dict(topk=2 ** 31 - 1, indices_stride=2 ** 31 - 1), False),
+        (dict(topk=2 ** 31 - 2048, indices_stride=2 ** 31 - 1), False),
+        (dict(topk=2 ** 31 - 2049, indices_stride=2 ** 31 - 1), True),
+        (dict(topk=2 ** 30, indices_stride=2 ** 30, num_q_heads=128, num_kv_heads=128), False),
+        (dict(topk=2 ** 30, indices_stride=2 ** 30, num_q_heads=63, num_kv_heads=63), True),
+    ]:
+        need = capi.block_decode_workspace_bytes(_decode_args(**over))
+        assert need > 0 if ok else need == capi.ERR_UNSUPPORTED, (over, need)
+        if not ok:
+            assert capi.block_decode(_decode_args(**over)) == capi.ERR_UNSUPPORTED
