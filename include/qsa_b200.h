@@ -238,7 +238,8 @@ QSA_B200_API int qsa_b200_topk_select(const qsa_b200_topk_args* args, qsa_b200_s
  * block of `block_size` consecutive tokens of a page and each KV head:
  *   stored value = code * scales[page, (t % P) / block_size, g],
  * scales fp32 [num_pages, P / block_size, Hkv] for K and for V. block_size
- * divides P; block_size 1 is a scale for every token, P one for every page.
+ * divides P; block_size 1 is a scale for every token, P one for every page. Up to
+ * (2^31 - 1) / 128 heads of a kind.
  * Three entry points serve one attention layer over it: qsa_b200_qk_rope (the
  * queries), qsa_b200_block_append (new keys and values) and
  * qsa_b200_block_decode. None has a counterpart in the reference, whose

@@ -62,7 +62,8 @@ int check_block_decode(const qsa_b200_block_decode_args* a, BlockDecodeParams* p
   if (a->rows < 0 || a->num_q_heads < 1 || a->num_kv_heads < 1 || a->num_q_heads % a->num_kv_heads != 0)
     return QSA_B200_ERR_BAD_SHAPE;
   if (a->indices && (a->topk < 0 || a->indices_stride < a->topk)) return QSA_B200_ERR_BAD_SHAPE;
-  if (a->head_dim != 128 || a->num_q_heads / a->num_kv_heads > 32) return QSA_B200_ERR_UNSUPPORTED;
+  if (a->head_dim != 128 || a->num_q_heads / a->num_kv_heads > 32 || a->num_kv_heads > kBlockMaxHeads)
+    return QSA_B200_ERR_UNSUPPORTED;
   // token slots, columns and the tiles of a row over its (up to 4 virtual) KV
   // heads are held as int32
   const int64_t columns = a->indices ? a->topk : (int64_t)a->pages_per_req * a->page_size;
@@ -117,7 +118,8 @@ int qsa_b200_qk_rope(const qsa_b200_qk_rope_args* a, qsa_b200_stream_t stream) {
   if (!a) return QSA_B200_ERR_NULL_POINTER;
   if (a->tokens < 0 || a->num_q_heads < 1 || a->num_kv_heads < 0 || (a->k && a->num_kv_heads < 1))
     return QSA_B200_ERR_BAD_SHAPE;
-  if (a->head_dim != 128 || !dtype_ok(a->dtype) || ((a->q_weight || a->k_weight) && !dtype_ok(a->weight_dtype)))
+  if (a->head_dim != 128 || !dtype_ok(a->dtype) || ((a->q_weight || a->k_weight) && !dtype_ok(a->weight_dtype)) ||
+      a->num_q_heads > kBlockMaxHeads || a->num_kv_heads > kBlockMaxHeads)
     return QSA_B200_ERR_UNSUPPORTED;
   if (!(a->eps >= 0.f) || !std::isfinite(a->eps)) return QSA_B200_ERR_BAD_VALUE;
   const int64_t q_row = (int64_t)a->num_q_heads * 128, k_row = (int64_t)a->num_kv_heads * 128;
@@ -155,7 +157,8 @@ int qsa_b200_block_append(const qsa_b200_block_append_args* a, qsa_b200_stream_t
   if (st != QSA_B200_OK) return st;
   if (a->entries < 0 || a->tokens < 0 || a->num_kv_heads < 1 || (!a->cu_tokens && a->tokens != a->entries))
     return QSA_B200_ERR_BAD_SHAPE;
-  if (a->head_dim != 128 || !dtype_ok(a->input_dtype) || (a->k_weight && !dtype_ok(a->weight_dtype)))
+  if (a->head_dim != 128 || !dtype_ok(a->input_dtype) || (a->k_weight && !dtype_ok(a->weight_dtype)) ||
+      a->num_kv_heads > kBlockMaxHeads)
     return QSA_B200_ERR_UNSUPPORTED;
   if (!(a->eps >= 0.f) || !std::isfinite(a->eps)) return QSA_B200_ERR_BAD_VALUE;
   if (a->token_stride < (int64_t)a->num_kv_heads * 128) return QSA_B200_ERR_BAD_SHAPE;

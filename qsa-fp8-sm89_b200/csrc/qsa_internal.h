@@ -116,6 +116,7 @@ cudaError_t launch_topk(const TopkParams& p, cudaStream_t stream);
 // The block-scaled cache: head norm with rotation (qsa_qk_rope.cu), paged
 // append (qsa_block_append.cu) and attention (qsa_block_decode.cu).
 constexpr int kRopeMaxAxes = 4;
+constexpr int kBlockMaxHeads = 0x7fffffff / 128;  // elements of a token's heads are counted in int32
 struct RopeParams {
   const float* table;        // [table_len, rotary] cosines, then sines; null = no rotation
   const int32_t* positions;  // [axes, tokens]; null = the caller's own position (append)

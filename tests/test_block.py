@@ -1123,3 +1123,17 @@ def test_block_decode_refuses_columns_past_its_counters():
         assert need > 0 if ok else need == capi.ERR_UNSUPPORTED, (over, need)
         if not ok:
             assert capi.block_decode(_decode_args(**over)) == capi.ERR_UNSUPPORTED
+
+
+def test_block_operators_refuse_heads_past_32_bits():
+    """A token's heads are counted in int32 elements: up to 2^24 - 1 of them."""
+    from qsa_b200 import capi
+
+    n, stride = 1 << 24, 1 << 31
+    assert capi.qk_rope(_rope_args(num_q_heads=n, q_stride=stride, q_out_stride=stride)) == capi.ERR_UNSUPPORTED
+    assert capi.qk_rope(_rope_args(num_kv_heads=n, k_stride=stride, k_out_stride=stride)) == capi.ERR_UNSUPPORTED
+    assert capi.qk_rope(_rope_args(num_q_heads=n - 1, q_stride=stride, q_out_stride=stride, tokens=0)) == capi.OK
+    assert capi.block_append(_append_args(num_kv_heads=n, token_stride=stride)) == capi.ERR_UNSUPPORTED
+    assert capi.block_append(_append_args(num_kv_heads=n - 1, token_stride=stride, tokens=0)) == capi.OK
+    assert capi.block_decode(_decode_args(num_q_heads=n, num_kv_heads=n)) == capi.ERR_UNSUPPORTED
+    assert capi.block_decode_workspace_bytes(_decode_args(num_q_heads=n - 1, num_kv_heads=n - 1)) == 0
