@@ -1137,3 +1137,89 @@ def test_block_operators_refuse_heads_past_32_bits():
     assert capi.block_append(_append_args(num_kv_heads=n - 1, token_stride=stride, tokens=0)) == capi.OK
     assert capi.block_decode(_decode_args(num_q_heads=n, num_kv_heads=n)) == capi.ERR_UNSUPPORTED
     assert capi.block_decode_workspace_bytes(_decode_args(num_q_heads=n - 1, num_kv_heads=n - 1)) == 0
+
+
+def _edge_rows(gen, cu, hkv, dtype, with_max):
+    """New rows [tokens, hkv, 128] of an append: in about a third of the (entry,
+    head)s some rows hold infinities, NaN, zeros, the type's largest value or
+    values near its smallest normal one."""
+    total = int(cu[-1])
+    x = torch.randn(total, hkv, D, generator=gen)
+    info = torch.finfo(dtype)
+    for e in range(len(cu) - 1):
+        for g in range(hkv):
+            if torch.rand((), generator=gen) > 0.35:
+                continue
+            for t in range(int(cu[e]), int(cu[e + 1])):
+                if torch.rand((), generator=gen) > 0.2:
+                    continue
+                kind, d = (int(torch.randint(0, n, (), generator=gen)) for n in (7 if with_max else 6, D))
+                if kind == 0:
+                    x[t, g, d] = float("inf")
+                elif kind == 1:
+                    x[t, g, d], x[t, g, (d + 5) % D] = -float("inf"), float("inf")
+                elif kind == 2:
+                    x[t, g, d] = float("nan")
+                elif kind == 3:
+                    x[t, g] = float("inf")
+                elif kind == 4:
+                    x[t, g] = 0.0
+                elif kind == 5:
+                    x[t, g] *= info.tiny
+                else:
+                    x[t, g, d] = info.max
+    return x.to(dtype)
+
+
+# page, block, entries of a large call (whose warps go through several heads), most tokens of an entry
+EDGE_FORMS = [(8, 1, 260, 12), (16, 2, 260, 12), (12, 4, 260, 12), (16, 16, 160, 40), (64, 64, 40, 90), (256, 256, 38, 300)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("page,block,many,longest", EDGE_FORMS)
+@pytest.mark.parametrize("large", [False, True])
+@pytest.mark.parametrize("turned", ["plain", "rotated", "normed"])
+def test_block_append_edge_values_in_every_form(page, block, many, longest, large, turned, dtype):
+    """Infinities, NaN, zeros and extremes among the new rows of a call with
+    cu_tokens, in some heads of some blocks, and NaN among the kept codes."""
+    from qsa_b200 import qsa_block_append
+
+    gen = torch.Generator().manual_seed(1000 * block + 10 * large + len(turned))
+    hkv, n = (8, many) if large else (3, 24)
+    counts = torch.randint(0, longest + 1, (n,), generator=gen)
+    if block > 64 and large:  # mostly short, so that the 64-bit check stays quick
+        counts = torch.where(torch.rand(n, generator=gen) < 0.85, counts % 7, counts)
+    starts = torch.randint(0, 2 * block, (n,), generator=gen)
+    cu = torch.cat([torch.zeros(1, dtype=torch.int64), counts.cumsum(0)]).to(torch.int32)
+    ppr = -(-(2 * block + longest) // page)
+    pages = n * ppr
+    btable = torch.randperm(pages, generator=gen).view(n, ppr).to(torch.int32)
+    k_new = _edge_rows(gen, cu, hkv, dtype, turned != "normed")  # squares of the largest values pass fp32
+    v_new = _edge_rows(gen, cu, hkv, dtype, True)
+    w = (1 + 0.3 * torch.randn(D, generator=gen)).to(dtype) if turned == "normed" else None
+    table = None if turned == "plain" else rope_table(2 * block + longest, 64 if turned == "normed" else D)
+    codes, scales = _caches(gen, pages, page, block, hkv)
+    for e in range(n):
+        for t in range(int(starts[e]) - int(starts[e]) % block, int(starts[e])):
+            if torch.rand((), generator=gen) < 0.2:
+                codes[:, btable[e, t // page], t % page, int(torch.randint(0, hkv, (), generator=gen)), t % D] = 0x7F + 0x80 * (t % 2)
+    kc, vc = (c.cuda().view(torch.float8_e4m3fn) for c in codes)
+    ks, vs = (s.cuda() for s in scales)
+    kv = torch.cat([k_new, v_new], 1).cuda()
+    dev = lambda t: None if t is None else t.cuda()
+    qsa_block_append(kv[:, :hkv], kv[:, hkv:], kc, vc, ks, vs, btable.cuda(), starts.to(torch.int32).cuda(),
+                     cu_tokens=cu.cuda(), table=dev(table), k_weight=dev(w), eps=1e-5)
+    torch.cuda.synchronize()
+    pos = np.concatenate([np.arange(s, s + c) for s, c in zip(starts.tolist(), counts.tolist())])
+    with np.errstate(invalid="ignore"):
+        k, _ = B.norm_rotate(np64(k_new), None if w is None else np64(w), 1e-5, None if table is None else np64(table), pos)
+        want = B.append(k, np64(v_new), codes[0].numpy(), codes[1].numpy(), scales[0].numpy(), scales[1].numpy(),
+                        btable.numpy(), starts.tolist(), None, cu.numpy())
+    for side in want:
+        assert np.isnan(side["values"][side["written"]]).any()
+    assert np.isinf(want[1]["values"][want[1]["written"]]).any()
+    # as in the test of ordinary values
+    key_err = 0.0 if turned == "plain" else 16 * U
+    _check_append((u8(kc), ks.cpu().numpy()), want[0], codes[0].numpy(), scales[0].numpy(), key_err * 2 * 448, key_err * 2 + 2 * U)
+    _check_append((u8(vc), vs.cpu().numpy()), want[1], codes[1].numpy(), scales[1].numpy(), 0.0, 2 * U)
