@@ -50,7 +50,7 @@
 //
 // Times: 8 rows of 90001 to 131072 tokens, 64 query on 8 KV heads: 287 us, 6.3
 // TB/s of cache (a plain copy: 6.5; after some 10 ms of it the 1000 W limit lowers
-// the clock and it takes 310 to 325 us); 512 rows of 64 to 2048 selected tokens:
+// the clock and it takes 310 to 335 us); 512 rows of 64 to 2048 selected tokens:
 // 234 us, 5.0 TB/s, 217 of them this kernel, where each row's start waits for its
 // ring to fill, the rest planning and joining; 256 rows of 512: 57 us, 5.0 TB/s,
 // one wave whose start and end (5 and 4 us) nothing covers; 4 rows of 64: 12 us,

@@ -181,9 +181,9 @@ struct BlockDecodeParams {
   int64_t num_pages;
   int topk;  // columns of a row
   int64_t indices_stride, btable_stride;
-  // A group above 16 goes as head_parts virtual KV heads of part_heads query
-  // heads each (the last one may have fewer); a CTA takes cta_heads of the
-  // virtual_heads of a row.
+  // A group above 8 (above 16 where there is much work) goes as head_parts
+  // virtual KV heads of part_heads query heads each (the last one may have
+  // fewer); a CTA takes cta_heads of the virtual_heads of a row.
   int head_parts, part_heads, virtual_heads, cta_heads;
   // slot / block_size = umulhi(2 slot, block_mul) >> block_shift, exact below
   // 2^31; token / page_size likewise

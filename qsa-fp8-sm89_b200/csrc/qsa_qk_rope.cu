@@ -13,8 +13,11 @@
 // 5.1 TB/s (a plain copy: 6.5). 4 heads at a time and 256 threads: 71.7; 8 CTAs
 // an SM: 70; 10: 68.1, with spills; loads ahead of the table's rows and a batch
 // ahead: 73 to 86. Warps wait for memory most of the time (56 % of DRAM, 62 % of
-// the issue slots). 256 tokens: 9 us, the launch and two rounds to memory. 1531
-// tokens of fp32 with three axes: 10.2 us (4 heads at a time: 14.6).
+// the issue slots). 256 tokens of 64 + 8 heads of f16: 6.2 us one after the other
+// in a graph, 12.3 with a cold L2: a half warp's heads are loaded after its position
+// and its table row, three rounds to memory. 1531 tokens of 24 + 4 heads of fp32 with
+// three axes: 8.1 us and 14 to 16 (from Python back to back 10.2; 4 heads at a
+// time: 14.6).
 #include "qsa_rope.cuh"
 
 namespace qsa {

@@ -3,8 +3,9 @@ block of consecutive tokens and KV head.
 
     stored value = code * scales[page, (t % P) // block, g]
 
-Three calls serve one attention layer over it, each one launch (the decode up
-to two), asynchronous on the current CUDA stream, CUDA tensors only:
+Three calls serve one attention layer over it, asynchronous on the current
+CUDA stream, CUDA tensors only. Each is one launch; the decode of rows of more
+than 512 columns is three, or four with ``indices``:
 
 * ``qsa_qk_rope``: RMS norm of every query and key head and the position
   rotation, over one or several position axes, in one pass;
