@@ -383,6 +383,155 @@ QSA_B200_API int64_t qsa_b200_block_decode_workspace_bytes(const qsa_b200_block_
 QSA_B200_API int qsa_b200_block_decode(const qsa_b200_block_decode_args* args, void* workspace, size_t workspace_bytes,
                                        qsa_b200_stream_t stream);
 
+/* ---- The latent cache ------------------------------------------------------
+ * Keys and values of all heads come from one vector a token: `rank` latent
+ * values, which are key and value, and 64 rotated values, which are key only.
+ * A paged cache keeps E4M3FN codes of the latent, the rotated part in bf16 and
+ * one fp32 scale a token:
+ *   key = scale * (codes, rope)      value = scale * codes.
+ * qsa_b200_latent_append writes scales that are powers of two from 2^-60 to
+ * 2^60; readers take any scale clamped to that range, and NaN as NaN. Four
+ * entry points serve one attention layer over it: qsa_b200_latent_append,
+ * qsa_b200_latent_read, qsa_b200_latent_decode (the absorbed form) and
+ * qsa_b200_latent_prefill (the expanded form, which needs no cache). None has a
+ * counterpart in the reference, whose caches hold a key and a value for each KV
+ * head (sm89_cutedsl.py:48-62). */
+typedef struct qsa_b200_latent_cache {
+  void* codes;           /* fp8 e4m3fn [num_pages, page_size, rank] */
+  void* rope;            /* bf16 [num_pages, page_size, rope_dim] */
+  float* scales;         /* fp32 [num_pages, page_size] */
+  const int32_t* btable; /* [num_reqs, btable_stride]; first pages_per_req columns = physical pages */
+  int32_t rank;          /* 128, 256, 384 or 512 */
+  int32_t rope_dim;      /* must be 64 */
+  int32_t page_size;
+  int32_t pages_per_req; /* pages_per_req * page_size and num_pages * page_size up to 2^31 - 1024 */
+  int32_t num_reqs;
+  int64_t num_pages;
+  int64_t btable_stride;
+} qsa_b200_latent_cache;
+
+typedef struct qsa_b200_latent_append_args {
+  qsa_b200_latent_cache cache;
+  const void* c;            /* new latents [tokens, rank] of input_dtype, rows c_stride elements apart */
+  const void* r;            /* their rotated part, before the rotation [tokens, rope_dim], rows r_stride apart */
+  const int32_t* starts;    /* [entries]: logical position of the entry's first new token */
+  const int32_t* reqs;      /* optional [entries]: block-table row of each entry (NULL = identity) */
+  const int32_t* cu_tokens; /* optional [entries + 1]: entry e has the tokens cu_tokens[e] .. cu_tokens[e + 1] - 1;
+                               NULL: one token each (tokens == entries) */
+  const void* c_weight;     /* optional [rank] of weight_dtype: RMS norm of the latent */
+  float eps;
+  int32_t entries;
+  int32_t tokens;
+  int32_t input_dtype;      /* QSA_B200_DTYPE_* */
+  int32_t weight_dtype;
+  int64_t c_stride;
+  int64_t r_stride;
+  qsa_b200_rotation rotation; /* of r: one axis, rotary_dim up to 64; positions NULL = the tokens' logical positions */
+} qsa_b200_latent_append_args;
+
+/* Appends new tokens to the latent cache, in fp32 up to the stored roundings.
+ * Entry e's tokens go to the logical positions starts[e], starts[e] + 1, ... of
+ * its request:
+ *   y     = c * rsqrt(mean(c^2) + eps) * c_weight   (c itself without a weight)
+ *   scale = 2^e, e the least with max|y| <= 448 * 2^e, from -60 to 60
+ *   codes = e4m3fn(y / scale), ties to even, saturating at +-448
+ *   rope  = bf16(rotated r / scale)
+ * Infinities of y count for no maximum and are stored as +-448. A token with a
+ * NaN in y gets the scale NaN and zero codes. A position outside the rotation
+ * table gives a zero rotated part. Tokens outside the block table or the cache
+ * are skipped, as are entries with a negative start or a reqs entry out of
+ * range. A cache place is named once in a call. Needs 16-byte aligned c, r,
+ * codes, rope, c_weight and table, strides a multiple of 16 bytes.
+ * Asynchronous on `stream`. */
+QSA_B200_API int qsa_b200_latent_append(const qsa_b200_latent_append_args* args, qsa_b200_stream_t stream);
+
+typedef struct qsa_b200_latent_read_args {
+  qsa_b200_latent_cache cache;
+  void* c;                  /* [tokens, rank] of output_dtype, contiguous */
+  void* r;                  /* [tokens, rope_dim] of output_dtype, contiguous */
+  const int32_t* starts;    /* [entries] */
+  const int32_t* reqs;      /* optional [entries] */
+  const int32_t* cu_tokens; /* optional [entries + 1]; NULL: one token each (tokens == entries) */
+  int32_t entries;
+  int32_t tokens;
+  int32_t output_dtype;     /* QSA_B200_DTYPE_* */
+} qsa_b200_latent_read_args;
+
+/* Reads tokens back: scale * codes and scale * rope, rounded once. Entry e's
+ * rows are the logical positions starts[e], starts[e] + 1, ... of its request,
+ * laid out as in qsa_b200_latent_append. Positions outside the block table or
+ * the cache give zeros; rows that no entry names are left as they are. Needs
+ * 16-byte aligned tensors. Asynchronous on `stream`. */
+QSA_B200_API int qsa_b200_latent_read(const qsa_b200_latent_read_args* args, qsa_b200_stream_t stream);
+
+#define QSA_B200_LATENT_MAX_NODES 256
+typedef struct qsa_b200_latent_decode_args {
+  qsa_b200_latent_cache cache;
+  const void* q;          /* bf16 [rows, nodes, heads, rank + rope_dim], contiguous, in the latent's space */
+  void* out;              /* bf16 [rows, nodes, heads, rank], contiguous */
+  const int32_t* indices; /* [rows, indices_stride], first `topk` columns = logical tokens, <0 = masked;
+                             NULL = every token in order */
+  const int32_t* counts;  /* optional [rows]: only the first counts[r] columns (without indices: tokens) may be valid */
+  const int32_t* t2r;     /* optional [rows]: row -> block-table row (NULL = identity) */
+  const int32_t* tree;    /* optional [rows, nodes, tree_words], contiguous: what each node sees of the row's nodes */
+  float softmax_scale;
+  int32_t rows;
+  int32_t nodes;          /* query tokens of a row, 1 .. QSA_B200_LATENT_MAX_NODES; 1 with indices */
+  int32_t heads;          /* 1 .. 128 */
+  int32_t topk;           /* not read without indices; up to 2^31 - 1024 */
+  int32_t tree_words;     /* >= (nodes + 31) / 32 */
+  int64_t indices_stride;
+} qsa_b200_latent_decode_args;
+
+/* Bytes of device workspace qsa_b200_latent_decode needs (256-byte aligned),
+ * negative on invalid arguments. */
+QSA_B200_API int64_t qsa_b200_latent_decode_workspace_bytes(const qsa_b200_latent_decode_args* args);
+
+/* Attention in the latent's space (the absorbed form), for row r, node i, head h:
+ *   out[r,i,h] = softmax_t(q[r,i,h] . key_t * softmax_scale) . value_t
+ * over the tokens that the node sees. With one node: the first counts[r]
+ * columns (all without counts). With several, the row's nodes are the last
+ * `nodes` of its counts[r] tokens; each node sees the tokens before them and,
+ * of the nodes, those j whose bit j % 32 is set in word j / 32 of its tree
+ * words, or without a tree nodes 0 to i. Masked entries (those, and as in
+ * qsa_b200_decode negative ones and ones on a page outside the table or the
+ * cache) do not count, and what the cache holds there is not read, apart from
+ * tokens that another node of the row sees. A node without a visible token
+ * gives zeros. The workspace needs no clearing and may be reused by the next
+ * call on the same stream. Needs 16-byte aligned tensors. Asynchronous on
+ * `stream`. */
+QSA_B200_API int qsa_b200_latent_decode(const qsa_b200_latent_decode_args* args, void* workspace, size_t workspace_bytes,
+                                        qsa_b200_stream_t stream);
+
+typedef struct qsa_b200_latent_prefill_args {
+  const void* q;       /* [q_tokens, heads, 192]: 128 values, then the 64 rotated ones */
+  const void* k;       /* [k_tokens, heads, 128] */
+  const void* k_rope;  /* [k_tokens, 64], for all heads */
+  const void* v;       /* [k_tokens, heads, 128] */
+  void* out;           /* [q_tokens, heads, 128], contiguous */
+  const int32_t* cu_q; /* [entries + 1]: entry e has the query tokens cu_q[e] .. cu_q[e + 1] - 1 */
+  const int32_t* cu_k; /* [entries + 1]: and the key tokens cu_k[e] .. cu_k[e + 1] - 1 */
+  float softmax_scale;
+  int32_t entries;
+  int32_t q_tokens;
+  int32_t k_tokens;
+  int32_t heads;
+  int32_t causal;      /* query i of n sees the keys up to i + (m - n) of m */
+  int32_t dtype;       /* QSA_B200_DTYPE_BF16 or _F16, of all tensors */
+  int64_t q_stride, q_head_stride; /* elements from one token, and one head, to the next */
+  int64_t k_stride, k_head_stride;
+  int64_t v_stride, v_head_stride;
+  int64_t k_rope_stride;
+} qsa_b200_latent_prefill_args;
+
+/* Attention of prompts in the expanded form, for query token i of an entry and
+ * head h over the entry's visible keys j:
+ *   out[i,h] = softmax_j((q[i,h,:128] . k[j,h] + q[i,h,128:] . k_rope[j]) * softmax_scale) . v[j,h]
+ * A query without a visible key gives zeros; query tokens that no entry names
+ * are left as they are. Needs 16-byte aligned tensors and strides (at least the
+ * rows they separate) a multiple of 16 bytes. Asynchronous on `stream`. */
+QSA_B200_API int qsa_b200_latent_prefill(const qsa_b200_latent_prefill_args* args, qsa_b200_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -214,6 +214,78 @@ int64_t block_decode_plan(BlockDecodeParams& p);
 void block_decode_place(BlockDecodeParams& p, void* workspace);
 cudaError_t launch_block_decode(const BlockDecodeParams& p, cudaStream_t stream);
 
+// The latent cache: append and read (qsa_latent_cache.cu), absorbed attention
+// (qsa_latent_decode.cu), expanded attention of prompts (qsa_latent_prefill.cu).
+constexpr int kLatentRope = 64;
+constexpr int kLatentMaxTokens = 0x7fffffff - 1023;  // tokens and slots are counted in int32, a tile past the last one
+constexpr float kLatentLeastScale = 0x1p-60f, kLatentMostScale = 0x1p60f;
+struct LatentCache {
+  uint8_t* codes;
+  __nv_bfloat16* rope;
+  float* scales;
+  const int32_t* btable;
+  int rank, page_size, pages_per_req, num_reqs;
+  int64_t num_pages, btable_stride;
+  // token / page_size = umulhi(2 token, page_mul) >> page_shift, exact below 2^31
+  uint32_t page_mul, page_shift;
+};
+// The tokens that entries name: cu_tokens may be null (one each).
+struct LatentTokens {
+  const int32_t* starts;
+  const int32_t* reqs;
+  const int32_t* cu_tokens;
+  int entries, tokens;
+};
+struct LatentAppendParams {
+  LatentCache cache;
+  LatentTokens list;
+  const void* c;
+  const void* r;
+  const void* c_weight;
+  float eps;
+  int dtype, weight_dtype;
+  int64_t c_stride, r_stride;
+  RopeParams rope;
+};
+cudaError_t launch_latent_append(const LatentAppendParams& p, cudaStream_t stream);
+
+struct LatentReadParams {
+  LatentCache cache;
+  LatentTokens list;
+  void* c;
+  void* r;
+  int dtype;
+};
+cudaError_t launch_latent_read(const LatentReadParams& p, cudaStream_t stream);
+
+struct LatentDecodeParams {
+  LatentCache cache;
+  const __nv_bfloat16* q;
+  __nv_bfloat16* out;
+  const int32_t* indices;
+  const int32_t* counts;
+  const int32_t* t2r;
+  const int32_t* tree;
+  float score_scale_log2;  // softmax_scale * log2(e)
+  int rows, nodes, heads, topk, tree_words;
+  int64_t indices_stride;
+};
+cudaError_t launch_latent_decode(const LatentDecodeParams& p, cudaStream_t stream);
+
+struct LatentPrefillParams {
+  const void* q;
+  const void* k;
+  const void* k_rope;
+  const void* v;
+  void* out;
+  const int32_t* cu_q;
+  const int32_t* cu_k;
+  float score_scale_log2;
+  int entries, q_tokens, k_tokens, heads, causal, dtype;
+  int64_t q_stride, q_head_stride, k_stride, k_head_stride, v_stride, v_head_stride, k_rope_stride;
+};
+cudaError_t launch_latent_prefill(const LatentPrefillParams& p, cudaStream_t stream);
+
 // QSA_B200_OK when the current device is an sm_100 part, else QSA_B200_ERR_DEVICE.
 int device_status();
 

@@ -58,6 +58,11 @@ EXPORTED = (
     "qsa_b200_block_append",
     "qsa_b200_block_decode_workspace_bytes",
     "qsa_b200_block_decode",
+    "qsa_b200_latent_append",
+    "qsa_b200_latent_read",
+    "qsa_b200_latent_decode_workspace_bytes",
+    "qsa_b200_latent_decode",
+    "qsa_b200_latent_prefill",
 )
 # test hook (include/qsa_b200_testing.h), not part of the decode interface
 TESTING_EXPORTED = ("qsa_b200_testing_set_wait_limit_ns",)
@@ -238,6 +243,111 @@ class BlockDecodeArgs(ctypes.Structure):
     ]
 
 
+class LatentCache(ctypes.Structure):
+    """Mirror of ``qsa_b200_latent_cache``."""
+
+    _fields_ = [
+        ("codes", c_void_p),
+        ("rope", c_void_p),
+        ("scales", c_void_p),
+        ("btable", c_void_p),
+        ("rank", c_int32),
+        ("rope_dim", c_int32),
+        ("page_size", c_int32),
+        ("pages_per_req", c_int32),
+        ("num_reqs", c_int32),
+        ("num_pages", c_int64),
+        ("btable_stride", c_int64),
+    ]
+
+
+class LatentAppendArgs(ctypes.Structure):
+    """Mirror of ``qsa_b200_latent_append_args``."""
+
+    _fields_ = [
+        ("cache", LatentCache),
+        ("c", c_void_p),
+        ("r", c_void_p),
+        ("starts", c_void_p),
+        ("reqs", c_void_p),
+        ("cu_tokens", c_void_p),
+        ("c_weight", c_void_p),
+        ("eps", c_float),
+        ("entries", c_int32),
+        ("tokens", c_int32),
+        ("input_dtype", c_int32),
+        ("weight_dtype", c_int32),
+        ("c_stride", c_int64),
+        ("r_stride", c_int64),
+        ("rotation", Rotation),
+    ]
+
+
+class LatentReadArgs(ctypes.Structure):
+    """Mirror of ``qsa_b200_latent_read_args``."""
+
+    _fields_ = [
+        ("cache", LatentCache),
+        ("c", c_void_p),
+        ("r", c_void_p),
+        ("starts", c_void_p),
+        ("reqs", c_void_p),
+        ("cu_tokens", c_void_p),
+        ("entries", c_int32),
+        ("tokens", c_int32),
+        ("output_dtype", c_int32),
+    ]
+
+
+class LatentDecodeArgs(ctypes.Structure):
+    """Mirror of ``qsa_b200_latent_decode_args``."""
+
+    _fields_ = [
+        ("cache", LatentCache),
+        ("q", c_void_p),
+        ("out", c_void_p),
+        ("indices", c_void_p),
+        ("counts", c_void_p),
+        ("t2r", c_void_p),
+        ("tree", c_void_p),
+        ("softmax_scale", c_float),
+        ("rows", c_int32),
+        ("nodes", c_int32),
+        ("heads", c_int32),
+        ("topk", c_int32),
+        ("tree_words", c_int32),
+        ("indices_stride", c_int64),
+    ]
+
+
+class LatentPrefillArgs(ctypes.Structure):
+    """Mirror of ``qsa_b200_latent_prefill_args``."""
+
+    _fields_ = [
+        ("q", c_void_p),
+        ("k", c_void_p),
+        ("k_rope", c_void_p),
+        ("v", c_void_p),
+        ("out", c_void_p),
+        ("cu_q", c_void_p),
+        ("cu_k", c_void_p),
+        ("softmax_scale", c_float),
+        ("entries", c_int32),
+        ("q_tokens", c_int32),
+        ("k_tokens", c_int32),
+        ("heads", c_int32),
+        ("causal", c_int32),
+        ("dtype", c_int32),
+        ("q_stride", c_int64),
+        ("q_head_stride", c_int64),
+        ("k_stride", c_int64),
+        ("k_head_stride", c_int64),
+        ("v_stride", c_int64),
+        ("v_head_stride", c_int64),
+        ("k_rope_stride", c_int64),
+    ]
+
+
 _configured = False
 
 
@@ -277,6 +387,13 @@ def lib() -> ctypes.CDLL:
         L.qsa_b200_block_decode_workspace_bytes.restype = c_int64
         L.qsa_b200_block_decode.argtypes = [ctypes.POINTER(BlockDecodeArgs), c_void_p, c_size_t, c_void_p]
         L.qsa_b200_block_decode.restype = c_int
+        for name, args in (("append", LatentAppendArgs), ("read", LatentReadArgs), ("prefill", LatentPrefillArgs)):
+            f = getattr(L, f"qsa_b200_latent_{name}")
+            f.argtypes, f.restype = [ctypes.POINTER(args), c_void_p], c_int
+        L.qsa_b200_latent_decode_workspace_bytes.argtypes = [ctypes.POINTER(LatentDecodeArgs)]
+        L.qsa_b200_latent_decode_workspace_bytes.restype = c_int64
+        L.qsa_b200_latent_decode.argtypes = [ctypes.POINTER(LatentDecodeArgs), c_void_p, c_size_t, c_void_p]
+        L.qsa_b200_latent_decode.restype = c_int
         L.qsa_b200_testing_set_wait_limit_ns.argtypes = [ctypes.c_uint64]
         L.qsa_b200_testing_set_wait_limit_ns.restype = ctypes.c_uint64
         _configured = True
@@ -437,6 +554,31 @@ def block_decode(args: BlockDecodeArgs, workspace=None, workspace_bytes_: int = 
     """Calls ``qsa_b200_block_decode``; returns its status."""
     ws = None if workspace is None else c_void_p(workspace.data_ptr())
     return int(lib().qsa_b200_block_decode(ctypes.byref(args), ws, c_size_t(workspace_bytes_), c_void_p(stream)))
+
+
+def latent_append(args: LatentAppendArgs, stream: int = 0) -> int:
+    """Calls ``qsa_b200_latent_append``; returns its status."""
+    return int(lib().qsa_b200_latent_append(ctypes.byref(args), c_void_p(stream)))
+
+
+def latent_read(args: LatentReadArgs, stream: int = 0) -> int:
+    """Calls ``qsa_b200_latent_read``; returns its status."""
+    return int(lib().qsa_b200_latent_read(ctypes.byref(args), c_void_p(stream)))
+
+
+def latent_decode_workspace_bytes(args: LatentDecodeArgs) -> int:
+    return int(lib().qsa_b200_latent_decode_workspace_bytes(ctypes.byref(args)))
+
+
+def latent_decode(args: LatentDecodeArgs, workspace=None, workspace_bytes_: int = 0, stream: int = 0) -> int:
+    """Calls ``qsa_b200_latent_decode``; returns its status."""
+    ws = None if workspace is None else c_void_p(workspace.data_ptr())
+    return int(lib().qsa_b200_latent_decode(ctypes.byref(args), ws, c_size_t(workspace_bytes_), c_void_p(stream)))
+
+
+def latent_prefill(args: LatentPrefillArgs, stream: int = 0) -> int:
+    """Calls ``qsa_b200_latent_prefill``; returns its status."""
+    return int(lib().qsa_b200_latent_prefill(ctypes.byref(args), c_void_p(stream)))
 
 
 def device_error(clear: bool = False) -> int:
