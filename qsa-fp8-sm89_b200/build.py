@@ -38,7 +38,7 @@ NVCC_FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC,-fvisibilit
 CU_SOURCES = ["qsa_capi.cu", "qsa_decode_tc.cu", "qsa_decode_simt.cu", "qsa_noalloc.cu", "qsa_cache_write.cu",
               "qsa_topk.cu", "qsa_block_capi.cu", "qsa_qk_rope.cu", "qsa_block_append.cu", "qsa_block_decode.cu",
               "qsa_latent_capi.cu", "qsa_latent_cache.cu", "qsa_latent_decode.cu", "qsa_latent_prefill.cu"]
-HEADERS = ["qsa_common.cuh", "qsa_internal.h", "qsa_rope.cuh", "qsa_latent.cuh"]
+HEADERS = ["qsa_common.cuh", "qsa_internal.h", "qsa_rope.cuh", "qsa_latent.cuh", "qsa_latent_tc.cuh"]
 TORCH_SOURCES = ["qsa_torch_ext.cpp", "qsa_torch_block.cpp", "qsa_torch_latent.cpp"]
 
 LIB = PKG / "libqsa_b200.so"

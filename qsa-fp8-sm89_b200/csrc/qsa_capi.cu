@@ -186,6 +186,7 @@ WorkspaceLayout workspace_for(const DecodeParams& p, bool tc) {
 }  // namespace
 
 int device_status() { return check_device(); }
+int* error_word() { return device_error_word(); }
 
 }  // namespace qsa
 

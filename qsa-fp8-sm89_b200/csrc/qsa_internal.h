@@ -77,6 +77,9 @@ struct DecodeParams {
   uint64_t wait_limit_ns;
 };
 
+// Device address of the current device's error word.
+int* error_word();
+
 // Wait limit the launches of this process use (the test hook's value, else
 // the 1 s default).
 uint64_t wait_limit_ns();
@@ -269,7 +272,19 @@ struct LatentDecodeParams {
   float score_scale_log2;  // softmax_scale * log2(e)
   int rows, nodes, heads, topk, tree_words;
   int64_t indices_stride;
+  // The split: a CTA takes one of the row_tiles 64-row parts of a row's (node,
+  // head) pairs, over the columns that its group (of `groups`) has.
+  int row_tiles, groups;
+  int planned;    // groups share all rows' tiles evenly (workspace); else group g has row g
+  int2* begins;   // [groups] row and tile that each group begins with
+  float* part_o;  // [2 groups, row_tiles, 64, rank] results of pieces of rows
+  float* part_lse;  // [2 groups, row_tiles, 64] their log2-sum-exp2, -inf for none
+  int* err;
+  uint64_t wait_limit_ns;
 };
+// Chooses the split and gives the workspace's size; places it in a workspace.
+int64_t latent_decode_plan(LatentDecodeParams& p);
+void latent_decode_place(LatentDecodeParams& p, void* workspace);
 cudaError_t launch_latent_decode(const LatentDecodeParams& p, cudaStream_t stream);
 
 struct LatentPrefillParams {
@@ -283,6 +298,8 @@ struct LatentPrefillParams {
   float score_scale_log2;
   int entries, q_tokens, k_tokens, heads, causal, dtype;
   int64_t q_stride, q_head_stride, k_stride, k_head_stride, v_stride, v_head_stride, k_rope_stride;
+  int* err;
+  uint64_t wait_limit_ns;
 };
 cudaError_t launch_latent_prefill(const LatentPrefillParams& p, cudaStream_t stream);
 

@@ -169,17 +169,24 @@ int64_t qsa_b200_latent_decode_workspace_bytes(const qsa_b200_latent_decode_args
   LatentDecodeParams p;
   const int st = check_decode(a, &p);
   if (st != QSA_B200_OK) return st;
-  return 0;
+  return p.rows == 0 ? 0 : latent_decode_plan(p);
 }
 
 int qsa_b200_latent_decode(const qsa_b200_latent_decode_args* a, void* workspace, size_t workspace_bytes,
                            qsa_b200_stream_t stream) {
-  (void)workspace, (void)workspace_bytes;
   LatentDecodeParams p;
   int st = check_decode(a, &p);
   if (st != QSA_B200_OK || p.rows == 0) return st;
   st = device_status();
   if (st != QSA_B200_OK) return st;
+  const int64_t need = latent_decode_plan(p);
+  if (need > 0) {
+    if (!workspace || (int64_t)workspace_bytes < need) return QSA_B200_ERR_WORKSPACE;
+    if (!aligned(workspace, 256)) return QSA_B200_ERR_MISALIGNED;
+    latent_decode_place(p, workspace);
+  }
+  p.err = error_word();
+  p.wait_limit_ns = wait_limit_ns();
   return launched(launch_latent_decode(p, reinterpret_cast<cudaStream_t>(stream)));
 }
 
@@ -221,6 +228,8 @@ int qsa_b200_latent_prefill(const qsa_b200_latent_prefill_args* a, qsa_b200_stre
   p.v_stride = a->v_stride;
   p.v_head_stride = a->v_head_stride;
   p.k_rope_stride = a->k_rope_stride;
+  p.err = error_word();
+  p.wait_limit_ns = wait_limit_ns();
   return launched(launch_latent_prefill(p, reinterpret_cast<cudaStream_t>(stream)));
 }
 

@@ -1,93 +1,841 @@
 // Attention in the latent's space over the latent cache (the absorbed form).
 //
-// A warp takes one query head of one node and goes through its columns, a token
-// at a time: lane l holds elements 4l .. 4l+3 of each 128 of the latent and two
-// rotated ones. Softmax by a running maximum and sum, all in fp32.
+//   out[r,i,h] = softmax_t(q[r,i,h] . key_t scale) . value_t,
+//   key_t = s_t (codes_t, rope_t),  value_t = s_t codes_t
+//
+// A row's (node, head) pairs share every token, 64 of them a CTA, so that the
+// tokens are an operand of large tensor-core products and are fetched once:
+//   S   = Q K^T     128 lanes x 128 tokens. Q lies in tensor memory as two
+//                   E4M3 terms a value, q 2^a = t0 + t1 / 16, in neighbouring
+//                   lanes: a product of codes with codes needs no conversion of
+//                   the cache, and a warp's lane pair has both terms' scores of
+//                   one head: a shuffle joins them, and each lane goes on with
+//                   64 of the 128 tokens. The rotated part is a bf16 product
+//                   into the same accumulator (q 2^a exact in bf16, zeros in the
+//                   lanes of the second terms).
+//   O^T = V^T P^T   128 values of the latent x 64 pairs, four times for a rank of
+//                   512. V^T is the same codes in shared memory, read the other
+//                   way; P is two E4M3 terms a weight. A transposed O takes 256
+//                   columns of tensor memory for 64 pairs (O itself would need
+//                   all 512 for its 128 lanes).
+// q: the terms are exact for a bf16 value within 2^13 of the head's largest and
+// off by 2^-21 of the largest at most below. P: a weight is rounded to bf16's 8
+// bits, which two terms hold down to 2^-8 of the reference's, to steps of 2^-15 of
+// that below; the sum of weights takes the bf16 value, so that most of this
+// rounding cancels in the quotient.
+//
+// Softmax. With s_t a weight on the codes is w_t = 2^(score_t + log2 s_t - r): one
+// running reference r of score + log2 s bounds all that goes into E4M3, and the
+// softmax's own sum is l = sum w_t / s_t. Scales within 2^-60 .. 2^60 keep both in
+// fp32's range. r moves only when a tile passes it by 2.8 (2^6 2^2.8 < 448), and
+// then O is rescaled in tensor memory; the usual tile needs one vote.
+//
+// Warps: four loaders bring 128-token tiles, 128 bytes of each token at a
+// time, into a ring of 16 KiB slots by cp.async (gathered rows in the 128-byte
+// swizzle that the matrix unit reads); one issues the products; four do the
+// softmax and the results. The product of scores of tile i + 1 runs while tile i's
+// softmax does, and P V of tile i after it.
+//
+// Work: group g of CTAs (one CTA for each 64 pairs of a row, so that the CTAs that
+// read the same tokens run side by side) has an even share of all rows' tiles: at
+// most two pieces of rows and any whole rows between. Pieces are joined by their
+// log-sums in a second kernel. Few short rows are a CTA each.
+//
+// Every wait is bounded; a CTA that gives up records it in the device error word,
+// waits for its own copies and products, frees its tensor memory and returns.
+#include <atomic>
+
 #include "qsa_latent.cuh"
+#include "qsa_latent_tc.cuh"
 
 namespace qsa {
 namespace {
 
-constexpr int kLdWarps = 4;
+constexpr int kLdPairs = 64;     // (node, head) pairs of a CTA
+constexpr int kLdTile = 128;     // tokens of a tile
+constexpr int kLdSlot = kLdTile * 128;
+constexpr int kLdSlots = 11;
+constexpr int kLdMeta = 4;       // tiles whose scales are held
+constexpr int kLdLag = 6;        // slots under way before a loader looks back
+constexpr int kLdLoader0 = 4, kLdMmaWarp = 8;
+// Three warpgroups: softmax, loaders, and the warp of the products with three idle
+// ones. The softmax takes registers that the others hand back: 240 + 2 x 128 of
+// the 3 x 168 that the block is launched with.
+constexpr int kLdThreads = 384;
+constexpr int64_t kLdDirectTiles = 4;  // tiles of a row that is not split
+constexpr float kLdOne = 6.f;    // log2 of the weight at the reference
+constexpr float kLdLazy = 2.8f;  // log2 by which a weight may pass it
+constexpr float kLowest = -3.402823466e38f;
+constexpr uint64_t kLdDrainNs = 1000000000ull;
 
-template <int kChunks>
-__global__ void __launch_bounds__(32 * kLdWarps) qsa_latent_decode_kernel(const __grid_constant__ LatentDecodeParams p) {
-  constexpr int kRank = 128 * kChunks;
-  const int lane = threadIdx.x % 32;
-  const int64_t at = (int64_t)blockIdx.x * kLdWarps + threadIdx.x / 32;  // (row, node, head)
-  if (at >= (int64_t)p.rows * p.nodes * p.heads) return;
-  const int row = (int)(at / (p.nodes * p.heads));
-  const int node = (int)(at / p.heads) % p.nodes;
-  const __nv_bfloat16* q = p.q + at * (kRank + kLatentRope);
-  float x[kChunks][4], o[kChunks][4] = {};
-#pragma unroll
-  for (int i = 0; i < kChunks; ++i) latent_load4(q + 128 * i + 4 * lane, x[i]);
-  const uint32_t qr = __ldg(reinterpret_cast<const uint32_t*>(q + kRank) + lane);
-  const float q0 = __uint_as_float(qr << 16), q1 = __uint_as_float(qr & 0xffff0000u);
+// Scales of a tile: s, log2 s, 1 / s, each in two halves of 64 tokens that a lane
+// pair reads at once, apart by a bank group.
+constexpr int kLdHalf = 68;
+struct LdMeta {
+  float s[2 * kLdHalf], lg[2 * kLdHalf], inv[2 * kLdHalf];
+};
 
+constexpr int kLdQr = 0;                           // rotated queries: 128 rows of 64 bf16
+constexpr int kLdP = kLdQr + 16384;                // weights: two terms of 64 rows of 128 tokens
+constexpr int kLdRing = kLdP + 16384;
+constexpr int kLdMetaAt = kLdRing + kLdSlots * kLdSlot;
+constexpr int kLdRow = kLdMetaAt + kLdMeta * (int)sizeof(LdMeta);  // float [64]: factors of heads
+constexpr int kLdBars = kLdRow + kLdPairs * 4;
+constexpr int kLdNumBars = 2 * kLdSlots + 2 * kLdMeta + 7;
+constexpr int kLdMisc = kLdBars + kLdNumBars * 8;  // tensor memory address, abort flag, group's range
+constexpr int kLdSmem = kLdMisc + 64 + 1024;
+static_assert(kLdSmem <= 232448 && kLdBars % 8 == 0 && kLdMisc % 8 == 0 && kLdMetaAt % 16 == 0, "shared memory");
+
+constexpr uint32_t kLdTmemS = 128, kLdTmemO = 256;  // columns; Q from 0
+
+// Columns of a row that may hold a token.
+__device__ __forceinline__ int ld_columns(const LatentDecodeParams& p, int row, int& count) {
   const int64_t req = p.t2r ? (int64_t)__ldg(p.t2r + row) : (int64_t)row;
   const int capacity = p.indices ? p.topk : p.cache.pages_per_req * p.cache.page_size;
-  const int count = p.counts ? max(__ldg(p.counts + row), 0) : capacity;
-  const int columns = req >= 0 && req < p.cache.num_reqs ? min(count, capacity) : 0;
-  const int own = p.nodes > 1 ? count - p.nodes : 0x7fffffff;  // the first node's place
-  float m = -INFINITY, l = 0.f;
-  for (int col = 0; col < columns; ++col) {
-    if (p.nodes > 1 && col >= own) {
-      const int d = col - own;
-      const bool seen = p.tree ? (__ldg(p.tree + ((int64_t)row * p.nodes + node) * p.tree_words + d / 32) >> (d % 32)) & 1 : d <= node;
-      if (!seen) continue;
+  count = p.counts ? max(__ldg(p.counts + row), 0) : capacity;
+  return req >= 0 && req < p.cache.num_reqs ? min(count, capacity) : 0;
+}
+__device__ __forceinline__ int ld_tiles(const LatentDecodeParams& p, int row) {
+  int count;
+  return (ld_columns(p, row, count) + kLdTile - 1) / kLdTile;
+}
+
+// The segments of a group: tiles from .. to - 1 of a row.
+struct LdWalk {
+  int row, from, to;
+  int64_t left;
+  bool whole;
+  __device__ __forceinline__ bool next(const LatentDecodeParams& p) {
+    // `row` and `from` name where the group's next tile lies, at or after it
+    while (left > 0) {
+      const int tiles = ld_tiles(p, row);
+      if (tiles > from) {
+        to = from + (int)min((int64_t)(tiles - from), left);
+        whole = from == 0 && to == tiles;
+        left -= to - from;
+        return true;
+      }
+      ++row;
+      from = 0;
     }
-    const int t = p.indices ? __ldg(p.indices + (int64_t)row * p.indices_stride + col) : col;
-    const int slot = latent_slot(p.cache, req, t);
-    if (slot < 0) continue;
-    float v[kChunks][4];
-    float s = __ldg(p.cache.scales + slot);
-    s = s != s ? s : fminf(fmaxf(s, kLatentLeastScale), kLatentMostScale);
-    const uint32_t kr = __ldg(reinterpret_cast<const uint32_t*>(p.cache.rope + (int64_t)slot * kLatentRope) + lane);
-    float sum = q0 * __uint_as_float(kr << 16) + q1 * __uint_as_float(kr & 0xffff0000u);
+    return false;
+  }
+  __device__ __forceinline__ void advance() { from = to; }
+};
+
+// What a node sees of its row's nodes: bit j % 32 of word j / 32.
+__device__ __forceinline__ uint32_t ld_seen_word(const LatentDecodeParams& p, int row, int node, int word) {
+  if (word < 0) return 0xffffffffu;  // the tokens before them
+  if (word >= (p.nodes + 31) / 32) return 0u;
+  if (p.tree) return (uint32_t)__ldg(p.tree + ((int64_t)row * p.nodes + node) * p.tree_words + word);
+  const int n = node + 1 - 32 * word;
+  return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u;
+}
+
+__device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) { return __vmaxu2(a, b); }
+
+// kChunks: 128-byte pieces of a token's codes.
+template <int kChunks>
+__global__ void __launch_bounds__(kLdThreads, 1) qsa_latent_decode_kernel(const __grid_constant__ LatentDecodeParams p) {
+  constexpr int kRank = 128 * kChunks;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw_s = smem_u32(smem_raw);
+  const uint32_t base_s = (raw_s + 1023u) & ~1023u;
+  uint8_t* smem = smem_raw + (base_s - raw_s);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kLdBars);
+  uint64_t* full = bars;                       // [slots] loaders -> products
+  uint64_t* empty = full + kLdSlots;           // [slots] products -> loaders
+  uint64_t* meta_full = empty + kLdSlots;      // [kLdMeta] loaders -> softmax
+  uint64_t* meta_empty = meta_full + kLdMeta;  // [kLdMeta] softmax -> loaders
+  uint64_t* q_full = meta_empty + kLdMeta;     // softmax -> products, each segment
+  uint64_t* s_full = q_full + 1;               // products -> softmax
+  uint64_t* s_empty = s_full + 1;              // softmax -> products
+  uint64_t* p_full = s_empty + 1;              // softmax -> products
+  uint64_t* o_full = p_full + 1;               // products -> softmax
+  uint64_t* o_empty = o_full + 1;              // results taken -> products, each segment
+  uint64_t* drain = o_empty + 1;
+  uint32_t* tmem_at = reinterpret_cast<uint32_t*>(smem + kLdMisc);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + kLdMisc + 8);
+  int* begin = reinterpret_cast<int*>(smem + kLdMisc + 16);                 // row, tile
+  int64_t* share = reinterpret_cast<int64_t*>(smem + kLdMisc + 24);         // first unit, units
+  LdMeta* metas = reinterpret_cast<LdMeta*>(smem + kLdMetaAt);
+  float* head_f = reinterpret_cast<float*>(smem + kLdRow);
+
+  const int rt = (int)(blockIdx.x % p.row_tiles), group = (int)(blockIdx.x / p.row_tiles);
+  const int pairs = p.nodes * p.heads;
+  const int mine = min(kLdPairs, pairs - rt * kLdPairs);  // pairs of this CTA
+
+  if (tid == 0) {
+    for (int i = 0; i < kLdSlots; ++i) mbar_init(full + i, 4), mbar_init(empty + i, 1);
+    for (int i = 0; i < kLdMeta; ++i) mbar_init(meta_full + i, 4), mbar_init(meta_empty + i, 4);
+    mbar_init(q_full, 128);
+    mbar_init(s_full, 1);
+    mbar_init(s_empty, 128);
+    mbar_init(p_full, 128);
+    mbar_init(o_full, 1);
+    mbar_init(o_empty, 128);
+    mbar_init(drain, 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == kLdMmaWarp) {
+    tmem_alloc(tmem_at, 512);
+    tmem_relinquish();
+    tc_fence_before();
+  }
+  if (tid < 64) {  // the rotated part has no second terms: every other row stays zero
 #pragma unroll
-    for (int i = 0; i < kChunks; ++i) {
-      const uint32_t c = __ldg(reinterpret_cast<const uint32_t*>(p.cache.codes + (int64_t)slot * kRank + 128 * i) + lane);
-      const float2 lo = e4m3x2_to_f32x2((uint16_t)c), hi = e4m3x2_to_f32x2((uint16_t)(c >> 16));
-      v[i][0] = lo.x, v[i][1] = lo.y, v[i][2] = hi.x, v[i][3] = hi.y;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) sum = fmaf(x[i][j], v[i][j], sum);
+    for (int i = 0; i < 8; ++i) *reinterpret_cast<uint4*>(smem + kLdQr + (2 * tid + 1) * 128 + i * 16) = make_uint4(0u, 0u, 0u, 0u);
+    fence_proxy_async_smem();
+  }
+
+  // the group's share of the tiles
+  if (!p.planned) {
+    if (tid == 0) {
+      begin[0] = group, begin[1] = 0;
+      share[1] = ld_tiles(p, group);
     }
+  } else {
+    // each thread counts the tiles of a run of rows
+    __shared__ int64_t warp_sum[kLdThreads / 32];
+    const int run = (p.rows + kLdThreads - 1) / kLdThreads;
+    const int r0 = min(tid * run, p.rows), r1 = min(r0 + run, p.rows);
+    int64_t sum = 0;
+#pragma unroll 8
+    for (int r = r0; r < r1; ++r) sum += ld_tiles(p, r);
+    int64_t upto = sum;
 #pragma unroll
-    for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-    const float score = sum * s * p.score_scale_log2;
-    const float next = fmaxf(m, score);
-    const float back = exp2f(m - next), w = exp2f(score - next);
-    m = next;
-    l = l * back + w;
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t v = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += v;
+    }
+    if (lane == 31) warp_sum[warp] = upto;
+    if (tid == 0) begin[0] = p.rows, begin[1] = 0, share[1] = 0;
+    __syncthreads();
+    int64_t total = 0;
 #pragma unroll
-    for (int i = 0; i < kChunks; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) o[i][j] = o[i][j] * back + w * s * v[i][j];
+    for (int w = 0; w < kLdThreads / 32; ++w) {
+      if (w < warp) upto += warp_sum[w];
+      total += warp_sum[w];
+    }
+    const int64_t groups = min((int64_t)p.groups, total);  // each has a tile at least
+    if (group < groups) {
+      const int64_t u0 = total * group / groups, u1 = total * (group + 1) / groups;
+      int64_t before = upto - sum;
+      if (before <= u0 && u0 < upto) {
+        int r = r0;
+        for (;; ++r) {
+          const int t = ld_tiles(p, r);
+          if (u0 < before + t) break;
+          before += t;
+        }
+        begin[0] = r, begin[1] = (int)(u0 - before);
+        share[1] = u1 - u0;
+        if (rt == 0) p.begins[group] = make_int2(r, (int)(u0 - before));
+      }
+    } else if (rt == 0 && tid == 0) {
+      p.begins[group] = make_int2(p.rows, 0);
+    }
   }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  __nv_bfloat16* out = p.out + at * kRank + 4 * lane;
+  __syncwarp();
+  __syncthreads();
+  launch_dependents();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_at;
+  LdWalk walk;
+  walk.row = begin[0], walk.from = begin[1], walk.left = share[1];
+  bool failed = false;
+
+  if (warp >= kLdLoader0 && warp < kLdMmaWarp) {
+    // =============================== loaders ================================
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 128;\n");
+    // Warp w has tokens 32w .. 32w + 31 of every tile: a lane looks up its own
+    // token, and 8 lanes fetch a token's 128 bytes.
+    const int w = warp - kLdLoader0;
+    const int piece = lane & 7, sub = lane >> 3;
+    const int tok = 32 * w + lane;  // the lane's own token
+    const int first_node = rt * kLdPairs / p.heads, last_node = (rt * kLdPairs + mine - 1) / p.heads;
+    int issued = 0, told = 0;  // slots filled by this warp, and announced
+    int tile_n = 0;
+    auto announce = [&](int upto) {  // slots up to `upto` have landed
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0)
+        for (int i = told; i < upto; ++i) mbar_arrive(full + i % kLdSlots);
+      told = upto;
+    };
+    auto wait_free = [&](uint64_t* bar, uint32_t parity) -> bool {
+      if (!__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) {
+        cp_async_wait<0>();  // what is under way must not wait for what is not
+        if (told < issued) announce(issued);
+        if (!__all_sync(0xffffffffu, wait_or_abort(bar, parity, abort_flag, p.wait_limit_ns))) return false;
+      }
+      return true;
+    };
+    while (!failed && walk.next(p)) {
+      int count;
+      const int columns = ld_columns(p, walk.row, count);
+      const int64_t req = p.t2r ? (int64_t)__ldg(p.t2r + walk.row) : (int64_t)walk.row;
+      const int own = p.nodes > 1 ? count - p.nodes : 0x7fffffff;
+      auto lookup = [&](int tile) -> int {
+        const int col = tile * kLdTile + tok;
+        if (tile >= walk.to || col >= columns) return -1;
+        if (col >= own) {  // seen by a node of this CTA?
+          const int d = col - own;
+          uint32_t any = 0;
+          if (p.tree) {
+#pragma unroll 4
+            for (int i = first_node; i <= last_node; ++i) any |= ld_seen_word(p, walk.row, i, d / 32);
+          } else {
+            any = ld_seen_word(p, walk.row, last_node, d / 32);
+          }
+          if (!((any >> (d % 32)) & 1u)) return -1;
+        }
+        const int t = p.indices ? __ldg(p.indices + (int64_t)walk.row * p.indices_stride + col) : col;
+        return latent_slot(p.cache, req, t);
+      };
+      int slot = lookup(walk.from);
+      float scale = slot >= 0 ? __ldg(p.cache.scales + slot) : 0.f;
+#pragma unroll 1
+      for (int tile = walk.from; tile < walk.to && !failed; ++tile, ++tile_n) {
+        const int next = lookup(tile + 1);
+        const int m = tile_n % kLdMeta;
+        if (tile_n >= kLdMeta && !wait_free(meta_empty + m, (uint32_t)((tile_n / kLdMeta - 1) & 1))) {
+          failed = true;
+          break;
+        }
+        {
+          const int at = (tok >> 6) * kLdHalf + (tok & 63);
+          const float s = slot < 0 ? 0.f : scale != scale ? scale : fminf(fmaxf(scale, kLatentLeastScale), kLatentMostScale);
+          metas[m].s[at] = s;
+          metas[m].lg[at] = slot < 0 ? -INFINITY : log2f(s);
+          // a NaN token is a NaN in the weights of those that see it, and nothing in the others'
+          metas[m].inv[at] = slot < 0 || s != s ? 0.f : 1.0f / s;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(meta_full + m);
+        }
+        int from[8];
 #pragma unroll
-  for (int i = 0; i < kChunks; ++i) {
-    const __nv_bfloat162 a = __floats2bfloat162_rn(o[i][0] * inv, o[i][1] * inv);
-    const __nv_bfloat162 b = __floats2bfloat162_rn(o[i][2] * inv, o[i][3] * inv);
-    *reinterpret_cast<__nv_bfloat162*>(out + 128 * i) = a;
-    *reinterpret_cast<__nv_bfloat162*>(out + 128 * i + 2) = b;
+        for (int k = 0; k < 8; ++k) from[k] = __shfl_sync(0xffffffffu, slot, 4 * k + sub);
+        // row of pass k: 32 w + 4 k + sub, so its swizzle is (4 (k & 1) + sub)'s
+        const uint32_t dst0 = base_s + kLdRing + (32 * w + sub) * 128;
+        const uint32_t even = (uint32_t)(piece ^ sub) << 4, odd = (uint32_t)(piece ^ (4 + sub)) << 4;
+#pragma unroll 1
+        for (int c = 0; c <= kChunks; ++c) {
+          const int s = issued % kLdSlots;
+          if (issued >= kLdSlots && !wait_free(empty + s, (uint32_t)((issued / kLdSlots - 1) & 1))) {
+            failed = true;
+            break;
+          }
+          const uint8_t* src = c < kChunks ? p.cache.codes + c * 128 : reinterpret_cast<const uint8_t*>(p.cache.rope);
+          const int64_t stride = c < kChunks ? kRank : 2 * kLatentRope;
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            cp_async_16(dst0 + s * kLdSlot + k * 512 + (k & 1 ? odd : even), src + (int64_t)max(from[k], 0) * stride + piece * 16,
+                        from[k] < 0 ? 0u : 16u);
+          cp_async_commit();
+          ++issued;
+          if (issued - told > kLdLag) {
+            cp_async_wait<kLdLag>();
+            announce(issued - kLdLag);
+          }
+        }
+        slot = next;
+        scale = slot >= 0 ? __ldg(p.cache.scales + slot) : 0.f;
+      }
+      walk.advance();
+    }
+    cp_async_wait_all();
+    announce(issued);
+    // rows without a column: zeros, by this CTA's warps in turn
+    for (int64_t r = p.planned ? (int64_t)group + (int64_t)p.groups * w : (w == 0 ? (int64_t)group : (int64_t)p.rows); r < p.rows;
+         r += (int64_t)p.groups * 4) {
+      if (ld_tiles(p, (int)r) > 0) continue;
+      uint4* out = reinterpret_cast<uint4*>(p.out + (r * pairs + rt * kLdPairs) * kRank);
+      for (int i = lane; i < mine * kRank / 8; i += 32) out[i] = make_uint4(0u, 0u, 0u, 0u);
+    }
+  } else if (warp >= kLdMmaWarp) {
+    // =============================== products ===============================
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 128;\n");
+    if (warp == kLdMmaWarp && lane == 0) {
+      constexpr uint32_t kIdescS = idesc_e4m3(128, kLdTile, false, false);
+      constexpr uint32_t kIdescR = idesc_f16(128, kLdTile, true, false);
+      const uint32_t idesc_o = idesc_e4m3(128, (mine + 15) / 16 * 16, true, false);
+      int pos = 0, n = 0, seg = 0;  // ring position, tile, segment
+      auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
+        if (!wait_or_abort(bar, parity, abort_flag, p.wait_limit_ns)) return false;
+        tc_fence_after();
+        return true;
+      };
+      auto weigh = [&](int at, int tile, bool first) -> bool {  // O^T (+)= V^T P^T of a tile whose slots begin at `at`
+        if (!wait(p_full, (uint32_t)(tile & 1))) return false;
+        if (first && seg > 0 && !wait(o_empty, (uint32_t)((seg - 1) & 1))) return false;
+#pragma unroll 1
+        for (int c = 0; c < kChunks; ++c) {
+          const int s = (at + c) % kLdSlots;
+          const uint32_t a0 = base_s + kLdRing + s * kLdSlot, b0 = base_s + kLdP;
+#pragma unroll
+          for (int kk = 0; kk < kLdTile / 32; ++kk) {
+            const uint64_t ad = smem_desc_sw128(a0 + kk * 32 * 128, kLdSlot, 1024);
+            mma_f8(tmem + kLdTmemO + c * kLdPairs, ad, smem_desc_sw128(b0 + kk * 32, 16, 1024), idesc_o, !first || kk > 0);
+            mma_f8(tmem + kLdTmemO + c * kLdPairs, ad, smem_desc_sw128(b0 + 8192 + kk * 32, 16, 1024), idesc_o, 1u);
+          }
+          mma_commit(empty + s);
+        }
+        mma_commit(o_full);
+        return true;
+      };
+      while (!failed && walk.next(p)) {
+        if (!wait(q_full, (uint32_t)(seg & 1))) {
+          failed = true;
+          break;
+        }
+        int at = 0;
+#pragma unroll 1
+        for (int tile = walk.from; tile < walk.to; ++tile, ++n) {
+          const int before = at;
+          at = pos;
+          if (n > 0 && !wait(s_empty, (uint32_t)((n - 1) & 1))) {
+            failed = true;
+            break;
+          }
+#pragma unroll 1
+          for (int c = 0; c <= kChunks; ++c, ++pos) {
+            const int s = pos % kLdSlots;
+            if (!wait(full + s, (uint32_t)((pos / kLdSlots) & 1))) {
+              failed = true;
+              break;
+            }
+            const uint32_t b0 = base_s + kLdRing + s * kLdSlot;
+            if (c < kChunks) {
+#pragma unroll
+              for (int kk = 0; kk < 4; ++kk)
+                mma_f8_ts(tmem + kLdTmemS, tmem + c * 32 + kk * 8, smem_desc_sw128(b0 + kk * 32, 16, 1024), kIdescS,
+                          c > 0 || kk > 0);
+            } else {
+#pragma unroll
+              for (int kk = 0; kk < 4; ++kk)
+                mma_f16_ss(tmem + kLdTmemS, smem_desc_sw128(base_s + kLdQr + kk * 32, 16, 1024),
+                           smem_desc_sw128(b0 + kk * 32, 16, 1024), kIdescR, 1u);
+              mma_commit(empty + s);
+            }
+          }
+          if (failed) break;
+          mma_commit(s_full);
+          if (tile > walk.from && !weigh(before, n - 1, tile - 1 == walk.from)) {
+            failed = true;
+            break;
+          }
+        }
+        if (!failed && !weigh(at, n - 1, walk.to - walk.from == 1)) failed = true;
+        ++seg;
+        walk.advance();
+      }
+      mma_commit(drain);
+      if (!mbar_wait_bounded(drain, 0u, kLdDrainNs)) failed = true;
+    }
+    __syncwarp();
+  } else {
+    // ========================== softmax, results ===========================
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 240;\n");
+    const bool odd = (lane & 1) != 0;
+    const int pair = 16 * warp + (lane >> 1);           // this lane pair's (node, head) in the CTA
+    const bool live = 16 * warp < mine;                 // the warp has one
+    const int rho = rt * kLdPairs + pair;
+    const int node = min(rho / p.heads, p.nodes - 1);
+    const uint32_t lane_base = (uint32_t)(warp * 32) << 16;
+    uint8_t* prow = smem + kLdP;
+    int n = 0, seg = 0;
+    while (walk.next(p)) {
+      int count;
+      ld_columns(p, walk.row, count);
+      const int own = p.nodes > 1 ? count - p.nodes : 0x7fffffff;
+      // ---- the queries: each lane of a pair converts one half of the row
+      float qs = 0.f;
+      if (live) {
+        uint4 raw[8 * kChunks], rr[4];
+        const uint4* q = reinterpret_cast<const uint4*>(p.q + ((int64_t)walk.row * pairs + rho) * (kRank + kLatentRope));
+#pragma unroll
+        for (int i = 0; i < 8 * kChunks; ++i) raw[i] = pair < mine ? __ldg(q + (odd ? 8 * kChunks : 0) + i) : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) rr[i] = pair < mine ? __ldg(q + 16 * kChunks + (odd ? 4 : 0) + i) : make_uint4(0u, 0u, 0u, 0u);
+        uint32_t top = 0, rtop = 0;  // largest |q| as bits, two at a time
+#pragma unroll
+        for (int i = 0; i < 8 * kChunks; ++i)
+          top = max_u16x2(max_u16x2(top, max_u16x2(raw[i].x & 0x7fff7fffu, raw[i].y & 0x7fff7fffu)),
+                          max_u16x2(raw[i].z & 0x7fff7fffu, raw[i].w & 0x7fff7fffu));
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          rtop = max_u16x2(max_u16x2(rtop, max_u16x2(rr[i].x & 0x7fff7fffu, rr[i].y & 0x7fff7fffu)),
+                           max_u16x2(rr[i].z & 0x7fff7fffu, rr[i].w & 0x7fff7fffu));
+        top = max_u16x2(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        rtop = max_u16x2(rtop, __shfl_xor_sync(0xffffffffu, rtop, 1));
+        const int t = (int)max(top & 0xffffu, top >> 16), u = (int)max(rtop & 0xffffu, rtop >> 16);
+        // 2^a takes the largest latent query into [128, 256), as far as the rotated
+        // ones stay far from bf16's end
+        int a = t == 0 ? 0 : 7 - (max(t >> 7, 1) - 127);
+        if (u != 0) a = min(a, 40 - (max(u >> 7, 1) - 127));
+        a = min(max(a, -120), 120);
+        const float up = __uint_as_float((uint32_t)(127 + a) << 23);
+        qs = __uint_as_float((uint32_t)(127 - a) << 23) * p.score_scale_log2;
+        if (t >= 0x7f80 || u >= 0x7f80) qs = __int_as_float(0x7fffffff);  // an infinity or NaN
+        // terms in place: hi of dims 0-3, 4-7, lo of 0-3, 4-7
+#pragma unroll
+        for (int i = 0; i < 8 * kChunks; ++i) {
+          const uint32_t w4[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+          uint32_t hi[4], lo[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float x = __uint_as_float(w4[j] << 16) * up, y = __uint_as_float(w4[j] & 0xffff0000u) * up;
+            hi[j] = __nv_cvt_float2_to_fp8x2(make_float2(x, y), __NV_SATFINITE, __NV_E4M3);
+            const float2 back = e4m3x2_to_f32x2((uint16_t)hi[j]);
+            lo[j] = __nv_cvt_float2_to_fp8x2(make_float2((x - back.x) * 16.f, (y - back.y) * 16.f), __NV_SATFINITE, __NV_E4M3);
+          }
+          raw[i] = make_uint4(hi[0] | hi[1] << 16, hi[2] | hi[3] << 16, lo[0] | lo[1] << 16, lo[2] | lo[3] << 16);
+        }
+        // the even lane's row is the first terms, the odd one's the second
+#pragma unroll
+        for (int b = 0; b < kChunks; ++b) {
+          uint32_t first[16], second[16];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const uint4 v = raw[8 * b + i];
+            const uint32_t r0 = __shfl_xor_sync(0xffffffffu, odd ? v.x : v.z, 1), r1 = __shfl_xor_sync(0xffffffffu, odd ? v.y : v.w, 1);
+            first[2 * i] = odd ? r0 : v.x, first[2 * i + 1] = odd ? r1 : v.y;
+            second[2 * i] = odd ? v.z : r0, second[2 * i + 1] = odd ? v.w : r1;
+          }
+          tmem_st(tmem + lane_base + b * 16, first);
+          tmem_st(tmem + lane_base + 16 * kChunks + b * 16, second);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t w4[4] = {rr[i].x, rr[i].y, rr[i].z, rr[i].w};
+          uint32_t o4[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const __nv_bfloat162 v = __floats2bfloat162_rn(__uint_as_float(w4[j] << 16) * up, __uint_as_float(w4[j] & 0xffff0000u) * up);
+            o4[j] = *reinterpret_cast<const uint32_t*>(&v);
+          }
+          *reinterpret_cast<uint4*>(smem + kLdQr + sw128_offset(32 * warp + (lane & ~1), (odd ? 64 : 0) + 16 * i)) =
+              make_uint4(o4[0], o4[1], o4[2], o4[3]);
+        }
+        tmem_wait_st();
+        fence_proxy_async_smem();
+      }
+      tc_fence_before();
+      mbar_arrive(q_full);
+
+      float r = kLowest, l = 0.f;
+      const float km = odd ? qs * 0.0625f : qs, kr = odd ? qs : qs * 0.0625f;  // own and the other lane's term
+#pragma unroll 1
+      for (int tile = walk.from; tile < walk.to; ++tile, ++n) {
+        const int m = n % kLdMeta;
+        if (!failed)
+          failed = !(wait_or_abort(meta_full + m, (uint32_t)((n / kLdMeta) & 1), abort_flag, p.wait_limit_ns) &&
+                     wait_or_abort(s_full, (uint32_t)(n & 1), abort_flag, p.wait_limit_ns));
+        failed = __any_sync(0xffffffffu, failed);
+        tc_fence_after();
+        float u[64];
+        float top = -INFINITY;
+        if (live && !failed) {
+          const float* ms = metas[m].s + (odd ? kLdHalf : 0);
+          const float* ml = metas[m].lg + (odd ? kLdHalf : 0);
+#pragma unroll
+          for (int b = 0; b < 2; ++b) {
+            float x[32], y[32];
+            tmem_ld_wait<32>(tmem + lane_base + kLdTmemS + 32 * b, x);
+            tmem_ld_wait<32>(tmem + lane_base + kLdTmemS + 64 + 32 * b, y);
+            if (b == 1) {
+              tc_fence_before();
+              mbar_arrive(s_empty);
+            }
+#pragma unroll
+            for (int j = 0; j < 32; j += 4) {
+              const float4 s4 = *reinterpret_cast<const float4*>(ms + 32 * b + j);
+              const float4 l4 = *reinterpret_cast<const float4*>(ml + 32 * b + j);
+              const float ss[4] = {s4.x, s4.y, s4.z, s4.w}, ll[4] = {l4.x, l4.y, l4.z, l4.w};
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const float other = __shfl_xor_sync(0xffffffffu, odd ? x[j + i] : y[j + i], 1);
+                const float v = fmaf(odd ? y[j + i] : x[j + i], km, other * kr);
+                u[32 * b + j + i] = fmaf(v, ss[i], ll[i]);
+              }
+            }
+          }
+          const int d0 = tile * kLdTile + (odd ? 64 : 0) - own;
+          if (p.nodes > 1 && tile * kLdTile + kLdTile > own) {
+            const int word = d0 >> 5;
+            const uint32_t w0 = ld_seen_word(p, walk.row, node, word), w1 = ld_seen_word(p, walk.row, node, word + 1),
+                           w2 = ld_seen_word(p, walk.row, node, word + 2);
+            const uint32_t b0 = __funnelshift_r(w0, w1, d0 & 31), b1 = __funnelshift_r(w1, w2, d0 & 31);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) {
+              if (!((b0 >> j) & 1u)) u[j] = -INFINITY;
+              if (!((b1 >> j) & 1u)) u[32 + j] = -INFINITY;
+            }
+          }
+#pragma unroll
+          for (int j = 0; j < 64; ++j) top = fmaxf(top, u[j]);
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        } else {
+          mbar_arrive(s_empty);
+        }
+        // a reference that a weight passes by too much moves, and O and l with it
+        const bool begun = tile > walk.from;
+        if (bar_vote(1, 128, top > r + kLdLazy || failed)) {
+          const float next = fmaxf(r, top);
+          const float f = ex2(r - next);  // 0 before the first weight
+          l *= f;
+          r = next;
+          if (begun) {
+            if (live && !odd) head_f[pair] = f;
+            if (!failed) failed = !wait_or_abort(o_full, (uint32_t)((n - 1) & 1), abort_flag, p.wait_limit_ns);
+          }
+          failed = __any_sync(0xffffffffu, failed);
+          if (bar_vote(1, 128, failed)) {
+            failed = true;
+            break;
+          }
+          if (begun) {
+            tc_fence_after();
+#pragma unroll 1
+            for (int c = 0; c < kChunks; ++c)
+#pragma unroll 1
+              for (int b = 0; b < mine; b += 32) {
+                const uint32_t at = tmem + lane_base + kLdTmemO + c * kLdPairs + b;
+                float x[32];
+                uint32_t y[32];
+                tmem_ld_wait<32>(at, x);
+#pragma unroll
+                for (int j = 0; j < 32; ++j) y[j] = __float_as_uint(x[j] * head_f[b + j]);
+                tmem_st(at, y);
+              }
+            tmem_wait_st();
+            tc_fence_before();
+          }
+        }
+        // ---- weights
+        uint32_t hi[16], lo[16];
+        if (live) {
+          const float* mi = metas[m].inv + (odd ? kLdHalf : 0);
+          const float rb = r - kLdOne;
+#pragma unroll
+          for (int j = 0; j < 64; j += 4) {
+            const float4 i4 = *reinterpret_cast<const float4*>(mi + j);
+            const float ii[4] = {i4.x, i4.y, i4.z, i4.w};
+            uint32_t h2[2], l2[2];
+#pragma unroll
+            for (int i = 0; i < 4; i += 2) {
+              const __nv_bfloat162 w2 = __floats2bfloat162_rn(ex2(u[j + i] - rb), ex2(u[j + i + 1] - rb));
+              const float2 w = __bfloat1622float2(w2);
+              l = fmaf(w.x, ii[i], l);
+              l = fmaf(w.y, ii[i + 1], l);
+              h2[i / 2] = __nv_cvt_float2_to_fp8x2(w, __NV_SATFINITE, __NV_E4M3);
+              const __half2 back(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)h2[i / 2], __NV_E4M3));
+              const __half2 left = __hsub2(__floats2half2_rn(w.x, w.y), back);
+              l2[i / 2] = __nv_cvt_halfraw2_to_fp8x2(static_cast<__half2_raw>(left), __NV_SATFINITE, __NV_E4M3);
+            }
+            hi[j / 4] = h2[0] | h2[1] << 16;
+            lo[j / 4] = l2[0] | l2[1] << 16;
+          }
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(meta_empty + m);
+        // the product of the tile before has read its weights
+        if (n > 0 && !failed) failed = !wait_or_abort(o_full, (uint32_t)((n - 1) & 1), abort_flag, p.wait_limit_ns);
+        failed = __any_sync(0xffffffffu, failed);
+        if (live) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const uint32_t at = sw128_offset(pair, (odd ? 64 : 0) + 16 * k);
+            *reinterpret_cast<uint4*>(prow + at) = make_uint4(hi[4 * k], hi[4 * k + 1], hi[4 * k + 2], hi[4 * k + 3]);
+            *reinterpret_cast<uint4*>(prow + 8192 + at) = make_uint4(lo[4 * k], lo[4 * k + 1], lo[4 * k + 2], lo[4 * k + 3]);
+          }
+          fence_proxy_async_smem();
+        }
+        mbar_arrive(p_full);
+      }
+      // ---- the segment's results
+      if (!failed) failed = !wait_or_abort(o_full, (uint32_t)((n - 1) & 1), abort_flag, p.wait_limit_ns);
+      failed = __any_sync(0xffffffffu, failed);
+      l += __shfl_xor_sync(0xffffffffu, l, 1);
+      if (live && !odd) head_f[pair] = l == 0.f ? 0.f : 1.0f / l;
+      const int piece = 2 * group + (walk.from > 0 ? 0 : 1);
+      if (!walk.whole && !odd && pair < mine)
+        p.part_lse[((int64_t)piece * p.row_tiles + rt) * kLdPairs + pair] = l == 0.f ? -INFINITY : log2f(l) + (r - kLdOne);
+      if (bar_vote(1, 128, failed)) {
+        failed = true;
+        break;
+      }
+      tc_fence_after();
+      const int64_t at = walk.whole ? ((int64_t)walk.row * pairs + rt * kLdPairs) * kRank
+                                    : ((int64_t)piece * p.row_tiles + rt) * kLdPairs * kRank;
+#pragma unroll 1
+      for (int c = 0; c < kChunks; ++c)
+#pragma unroll 1
+        for (int b = 0; b < mine; b += 32) {
+          float x[32];
+          tmem_ld_wait<32>(tmem + lane_base + kLdTmemO + c * kLdPairs + b, x);
+          const int64_t to = at + (int64_t)b * kRank + c * 128 + 32 * warp + lane;
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            if (b + j >= mine) break;
+            const float v = x[j] * head_f[b + j];
+            if (walk.whole)
+              p.out[to + j * kRank] = __float2bfloat16_rn(v);
+            else
+              p.part_o[to + j * kRank] = v;
+          }
+        }
+      tc_fence_before();
+      mbar_arrive(o_empty);
+      bar_sync(1, 128);  // the factors are read before the next segment's
+      ++seg;
+      walk.advance();
+    }
   }
+
+  if (failed) {
+    *abort_flag = 1;
+    if (p.err) atomicOr(p.err, 1);
+  }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kLdMmaWarp) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// Joins the pieces of a row that several groups share: one block for each group
+// that ends a row's first piece, 64-pair part and pair.
+__global__ void __launch_bounds__(128) qsa_latent_join_kernel(const __grid_constant__ LatentDecodeParams p) {
+  const int pair = blockIdx.x, rt = blockIdx.y, g = blockIdx.z + 1;
+  const int pairs = p.nodes * p.heads;
+  if (rt * kLdPairs + pair >= pairs) return;
+  wait_for_prerequisites();
+  const int2 b = p.begins[g];
+  if (b.x >= p.rows || b.y == 0) return;
+  const int2 before = p.begins[g - 1];
+  if (before.x == b.x && before.y > 0) return;  // the row's second piece lies further back
+  int last = g;
+  while (last + 1 < p.groups) {
+    const int2 e = p.begins[last + 1];
+    if (e.x != b.x || e.y == 0) break;
+    ++last;
+  }
+  // pieces: the second of group g - 1, the first of groups g .. last
+  auto place = [&](int i) { return ((int64_t)(i == 0 ? 2 * g - 1 : 2 * (g + i - 1)) * p.row_tiles + rt) * kLdPairs + pair; };
+  const int pieces = last - g + 2;
+  float top = -INFINITY;
+  bool nan = false;
+  for (int i = 0; i < pieces; ++i) {
+    const float v = p.part_lse[place(i)];
+    top = fmaxf(top, v);
+    nan = nan || v != v;
+  }
+  const int rank = p.cache.rank;
+  const int d = 4 * threadIdx.x;
+  if (d >= rank) return;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  float sum = 0.f;
+  if (top > -INFINITY || nan) {
+#pragma unroll 4
+    for (int i = 0; i < pieces; ++i) {
+      const int64_t at = place(i);
+      const float v = p.part_lse[at];
+      if (v == -INFINITY) continue;
+      const float w = exp2f(v - top);
+      const float4 x = *reinterpret_cast<const float4*>(p.part_o + at * rank + d);
+      sum += w;
+      o.x = fmaf(w, x.x, o.x), o.y = fmaf(w, x.y, o.y), o.z = fmaf(w, x.z, o.z), o.w = fmaf(w, x.w, o.w);
+    }
+    const float inv = 1.0f / sum;
+    o.x *= inv, o.y *= inv, o.z *= inv, o.w *= inv;
+  }
+  const __nv_bfloat162 lo = __floats2bfloat162_rn(o.x, o.y), hi = __floats2bfloat162_rn(o.z, o.w);
+  *reinterpret_cast<uint2*>(p.out + ((int64_t)b.x * pairs + rt * kLdPairs + pair) * rank + d) =
+      make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+}
+
+int sm_count() {
+  static std::atomic<int> known[64] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 148;
+  int n = known[dev & 63].load(std::memory_order_relaxed);
+  if (n == 0) {
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n < 1) n = 148;
+    known[dev & 63].store(n, std::memory_order_relaxed);
+  }
+  return n;
+}
+
+int64_t align256(int64_t x) { return (x + 255) / 256 * 256; }
+
+template <int kChunks>
+cudaError_t launch(const LatentDecodeParams& p, cudaStream_t stream) {
+  // the shared memory beyond the default limit, once per device
+  static std::atomic<uint64_t> ready{0};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const uint64_t bit = 1ull << (dev & 63);
+  if (!(ready.load(std::memory_order_acquire) & bit)) {
+    e = cudaFuncSetAttribute(qsa_latent_decode_kernel<kChunks>, cudaFuncAttributeMaxDynamicSharedMemorySize, kLdSmem);
+    if (e != cudaSuccess) return e;
+    ready.fetch_or(bit, std::memory_order_acq_rel);
+  }
+  const int64_t grid = (int64_t)p.groups * p.row_tiles;
+  if (grid > 0x7fffffffll) return cudaErrorInvalidValue;
+  qsa_latent_decode_kernel<kChunks><<<(unsigned)grid, kLdThreads, kLdSmem, stream>>>(p);
+  return cudaGetLastError();
 }
 
 }  // namespace
 
+int64_t latent_decode_plan(LatentDecodeParams& p) {
+  p.row_tiles = (p.nodes * p.heads + kLdPairs - 1) / kLdPairs;
+  const int64_t columns = p.indices ? p.topk : (int64_t)p.cache.pages_per_req * p.cache.page_size;
+  const int sms = sm_count();
+  p.planned = (columns + kLdTile - 1) / kLdTile > kLdDirectTiles || (int64_t)p.rows * p.row_tiles > sms;
+  p.groups = p.planned ? (sms / p.row_tiles > 1 ? sms / p.row_tiles : 1) : p.rows;
+  if (!p.planned) return 0;
+  const int64_t pieces = 2ll * p.groups * p.row_tiles * kLdPairs;
+  return align256(pieces * p.cache.rank * 4) + align256(pieces * 4) + align256(8ll * p.groups);
+}
+
+void latent_decode_place(LatentDecodeParams& p, void* workspace) {
+  char* at = static_cast<char*>(workspace);
+  const int64_t pieces = 2ll * p.groups * p.row_tiles * kLdPairs;
+  p.part_o = reinterpret_cast<float*>(at);
+  at += align256(pieces * p.cache.rank * 4);
+  p.part_lse = reinterpret_cast<float*>(at);
+  at += align256(pieces * 4);
+  p.begins = reinterpret_cast<int2*>(at);
+}
+
 cudaError_t launch_latent_decode(const LatentDecodeParams& p, cudaStream_t stream) {
-  const int64_t grid = ((int64_t)p.rows * p.nodes * p.heads + kLdWarps - 1) / kLdWarps;
-  if (grid > 0x7fffffffll) return cudaErrorInvalidValue;
+  cudaError_t e;
   switch (p.cache.rank / 128) {
-    case 1: qsa_latent_decode_kernel<1><<<(unsigned)grid, 32 * kLdWarps, 0, stream>>>(p); break;
-    case 2: qsa_latent_decode_kernel<2><<<(unsigned)grid, 32 * kLdWarps, 0, stream>>>(p); break;
-    case 3: qsa_latent_decode_kernel<3><<<(unsigned)grid, 32 * kLdWarps, 0, stream>>>(p); break;
-    default: qsa_latent_decode_kernel<4><<<(unsigned)grid, 32 * kLdWarps, 0, stream>>>(p); break;
+    case 1: e = launch<1>(p, stream); break;
+    case 2: e = launch<2>(p, stream); break;
+    case 3: e = launch<3>(p, stream); break;
+    default: e = launch<4>(p, stream); break;
   }
-  return cudaGetLastError();
+  if (e != cudaSuccess || !p.planned || p.groups < 2) return e;
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3(kLdPairs, (unsigned)p.row_tiles, (unsigned)(p.groups - 1));
+  config.blockDim = dim3(128);
+  config.stream = stream;
+  cudaLaunchAttribute attr = {};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = &attr;
+  config.numAttrs = 1;
+  return cudaLaunchKernelEx(&config, qsa_latent_join_kernel, p);
 }
 
 }  // namespace qsa
