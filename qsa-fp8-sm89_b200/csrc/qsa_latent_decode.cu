@@ -10,7 +10,7 @@
 //                   lanes: a product of codes with codes needs no conversion of
 //                   the cache, and a warp's lane pair has both terms' scores of
 //                   one head: a shuffle joins them, and each lane goes on with
-//                   64 of the 128 tokens. The rotated part is a bf16 product
+//                   half of the warp's tokens. The rotated part is a bf16 product
 //                   into the same accumulator (q 2^a exact in bf16, zeros in the
 //                   lanes of the second terms).
 //   O^T = V^T P^T   128 values of the latent x 64 pairs, four times for a rank of
@@ -32,9 +32,10 @@
 //
 // Warps: four loaders bring 128-token tiles, 128 bytes of each token at a
 // time, into a ring of 16 KiB slots by cp.async (gathered rows in the 128-byte
-// swizzle that the matrix unit reads); one issues the products; four do the
-// softmax and the results. The product of scores of tile i + 1 runs while tile i's
-// softmax does, and P V of tile i after it.
+// swizzle that the matrix unit reads); one issues the products; eight do the
+// softmax and the results, two for each quarter of the lanes, with half of the
+// tokens each. The product of scores of tile i + 1 runs while tile i's softmax
+// does, and P V of tile i after it.
 //
 // Work: group g of CTAs (one CTA for each 64 pairs of a row, so that the CTAs that
 // read the same tokens run side by side) has an even share of all rows' tiles: at
@@ -56,31 +57,33 @@ constexpr int kLdTile = 128;     // tokens of a tile
 constexpr int kLdSlot = kLdTile * 128;
 constexpr int kLdSlots = 11;
 constexpr int kLdMeta = 4;       // tiles whose scales are held
-constexpr int kLdLag = 6;        // slots under way before a loader looks back
-constexpr int kLdLoader0 = 4, kLdMmaWarp = 8;
-// Three warpgroups: softmax, loaders, and the warp of the products with three idle
-// ones. The softmax takes registers that the others hand back: 240 + 2 x 128 of
-// the 3 x 168 that the block is launched with.
-constexpr int kLdThreads = 384;
+constexpr int kLdLag = 7;        // slots under way before a loader looks back
+constexpr int kLdSoft = 256;     // threads of the softmax
+constexpr int kLdLoader0 = 8, kLdMmaWarp = 12;
+// Four warpgroups: two of softmax, loaders, and the warp of the products with three
+// idle ones. The softmax takes registers that the others hand back: 2 x 168 + 104 +
+// 72 of the 4 x 128 that the block is launched with.
+constexpr int kLdThreads = 512;
 constexpr int64_t kLdDirectTiles = 4;  // tiles of a row that is not split
 constexpr float kLdOne = 6.f;    // log2 of the weight at the reference
 constexpr float kLdLazy = 2.8f;  // log2 by which a weight may pass it
 constexpr float kLowest = -3.402823466e38f;
 constexpr uint64_t kLdDrainNs = 1000000000ull;
 
-// Scales of a tile: s, log2 s, 1 / s, each in two halves of 64 tokens that a lane
-// pair reads at once, apart by a bank group.
-constexpr int kLdHalf = 68;
+// Scales of a tile: s, log2 s, 1 / s, each in four quarters of 32 tokens. A lane
+// pair reads two of them at once, apart by a bank group.
+constexpr int kLdQuarter = 36;
 struct LdMeta {
-  float s[2 * kLdHalf], lg[2 * kLdHalf], inv[2 * kLdHalf];
+  float s[4 * kLdQuarter], lg[4 * kLdQuarter], inv[4 * kLdQuarter];
 };
 
 constexpr int kLdQr = 0;                           // rotated queries: 128 rows of 64 bf16
 constexpr int kLdP = kLdQr + 16384;                // weights: two terms of 64 rows of 128 tokens
 constexpr int kLdRing = kLdP + 16384;
 constexpr int kLdMetaAt = kLdRing + kLdSlots * kLdSlot;
-constexpr int kLdRow = kLdMetaAt + kLdMeta * (int)sizeof(LdMeta);  // float [64]: factors of heads
-constexpr int kLdBars = kLdRow + kLdPairs * 4;
+constexpr int kLdRow = kLdMetaAt + kLdMeta * (int)sizeof(LdMeta);  // float [64]: factors of pairs
+constexpr int kLdShare = kLdRow + kLdPairs * 4;                    // float [2][64]: what the two sets of warps tell
+constexpr int kLdBars = kLdShare + 2 * kLdPairs * 4;
 constexpr int kLdNumBars = 2 * kLdSlots + 2 * kLdMeta + 7;
 constexpr int kLdMisc = kLdBars + kLdNumBars * 8;  // tensor memory address, abort flag, group's range
 constexpr int kLdSmem = kLdMisc + 64 + 1024;
@@ -132,8 +135,6 @@ __device__ __forceinline__ uint32_t ld_seen_word(const LatentDecodeParams& p, in
   return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u;
 }
 
-__device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) { return __vmaxu2(a, b); }
-
 // kChunks: 128-byte pieces of a token's codes.
 template <int kChunks>
 __global__ void __launch_bounds__(kLdThreads, 1) qsa_latent_decode_kernel(const __grid_constant__ LatentDecodeParams p) {
@@ -162,6 +163,7 @@ __global__ void __launch_bounds__(kLdThreads, 1) qsa_latent_decode_kernel(const 
   int64_t* share = reinterpret_cast<int64_t*>(smem + kLdMisc + 24);         // first unit, units
   LdMeta* metas = reinterpret_cast<LdMeta*>(smem + kLdMetaAt);
   float* head_f = reinterpret_cast<float*>(smem + kLdRow);
+  float* told_f = reinterpret_cast<float*>(smem + kLdShare);
 
   const int rt = (int)(blockIdx.x % p.row_tiles), group = (int)(blockIdx.x / p.row_tiles);
   const int pairs = p.nodes * p.heads;
@@ -169,13 +171,13 @@ __global__ void __launch_bounds__(kLdThreads, 1) qsa_latent_decode_kernel(const 
 
   if (tid == 0) {
     for (int i = 0; i < kLdSlots; ++i) mbar_init(full + i, 4), mbar_init(empty + i, 1);
-    for (int i = 0; i < kLdMeta; ++i) mbar_init(meta_full + i, 4), mbar_init(meta_empty + i, 4);
-    mbar_init(q_full, 128);
+    for (int i = 0; i < kLdMeta; ++i) mbar_init(meta_full + i, 4), mbar_init(meta_empty + i, kLdSoft / 32);
+    mbar_init(q_full, kLdSoft);
     mbar_init(s_full, 1);
-    mbar_init(s_empty, 128);
-    mbar_init(p_full, 128);
+    mbar_init(s_empty, kLdSoft);
+    mbar_init(p_full, kLdSoft);
     mbar_init(o_full, 1);
-    mbar_init(o_empty, 128);
+    mbar_init(o_empty, kLdSoft);
     mbar_init(drain, 1);
     *abort_flag = 0;
     fence_mbar_init();
@@ -250,7 +252,7 @@ __global__ void __launch_bounds__(kLdThreads, 1) qsa_latent_decode_kernel(const 
 
   if (warp >= kLdLoader0 && warp < kLdMmaWarp) {
     // =============================== loaders ================================
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 128;\n");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 104;\n");
     // Warp w has tokens 32w .. 32w + 31 of every tile: a lane looks up its own
     // token, and 8 lanes fetch a token's 128 bytes.
     const int w = warp - kLdLoader0;
@@ -267,10 +269,11 @@ __global__ void __launch_bounds__(kLdThreads, 1) qsa_latent_decode_kernel(const 
       told = upto;
     };
     auto wait_free = [&](uint64_t* bar, uint32_t parity) -> bool {
-      if (!__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) {
-        cp_async_wait<0>();  // what is under way must not wait for what is not
-        if (told < issued) announce(issued);
-        if (!__all_sync(0xffffffffu, wait_or_abort(bar, parity, abort_flag, p.wait_limit_ns))) return false;
+      while (!__all_sync(0xffffffffu, mbar_test_wait(bar, parity))) {
+        // what is under way must not wait for what is not
+        if (told == issued) return __all_sync(0xffffffffu, wait_or_abort(bar, parity, abort_flag, p.wait_limit_ns));
+        cp_async_wait_dyn(issued - told - 1);
+        announce(told + 1);
       }
       return true;
     };
@@ -307,7 +310,7 @@ __global__ void __launch_bounds__(kLdThreads, 1) qsa_latent_decode_kernel(const 
           break;
         }
         {
-          const int at = (tok >> 6) * kLdHalf + (tok & 63);
+          const int at = (tok >> 5) * kLdQuarter + (tok & 31);
           const float s = slot < 0 ? 0.f : scale != scale ? scale : fminf(fmaxf(scale, kLatentLeastScale), kLatentMostScale);
           metas[m].s[at] = s;
           metas[m].lg[at] = slot < 0 ? -INFINITY : log2f(s);
@@ -358,56 +361,65 @@ __global__ void __launch_bounds__(kLdThreads, 1) qsa_latent_decode_kernel(const 
     }
   } else if (warp >= kLdMmaWarp) {
     // =============================== products ===============================
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 128;\n");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;\n");
     if (warp == kLdMmaWarp && lane == 0) {
       constexpr uint32_t kIdescS = idesc_e4m3(128, kLdTile, false, false);
       constexpr uint32_t kIdescR = idesc_f16(128, kLdTile, true, false);
       const uint32_t idesc_o = idesc_e4m3(128, (mine + 15) / 16 * 16, true, false);
       int pos = 0, n = 0, seg = 0;  // ring position, tile, segment
-      auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
-        if (!wait_or_abort(bar, parity, abort_flag, p.wait_limit_ns)) return false;
+      int due = -1, due_at = 0, due_seg = 0;  // a tile whose P V is still to come, its first slot and segment
+      bool due_first = false;                 // it is its segment's first
+      auto weigh = [&]() {  // O^T (+)= V^T P^T
         tc_fence_after();
-        return true;
-      };
-      auto weigh = [&](int at, int tile, bool first) -> bool {  // O^T (+)= V^T P^T of a tile whose slots begin at `at`
-        if (!wait(p_full, (uint32_t)(tile & 1))) return false;
-        if (first && seg > 0 && !wait(o_empty, (uint32_t)((seg - 1) & 1))) return false;
 #pragma unroll 1
         for (int c = 0; c < kChunks; ++c) {
-          const int s = (at + c) % kLdSlots;
+          const int s = (due_at + c) % kLdSlots;
           const uint32_t a0 = base_s + kLdRing + s * kLdSlot, b0 = base_s + kLdP;
 #pragma unroll
           for (int kk = 0; kk < kLdTile / 32; ++kk) {
             const uint64_t ad = smem_desc_sw128(a0 + kk * 32 * 128, kLdSlot, 1024);
-            mma_f8(tmem + kLdTmemO + c * kLdPairs, ad, smem_desc_sw128(b0 + kk * 32, 16, 1024), idesc_o, !first || kk > 0);
+            mma_f8(tmem + kLdTmemO + c * kLdPairs, ad, smem_desc_sw128(b0 + kk * 32, 16, 1024), idesc_o, !due_first || kk > 0);
             mma_f8(tmem + kLdTmemO + c * kLdPairs, ad, smem_desc_sw128(b0 + 8192 + kk * 32, 16, 1024), idesc_o, 1u);
           }
           mma_commit(empty + s);
         }
         mma_commit(o_full);
-        return true;
+        due = -1;
+      };
+      // The products of a tile's scores wait for its tokens, and those of the tile
+      // before for its weights: whichever is there goes first, so that slots come
+      // free while tokens are under way. weights: wait for those alone.
+      auto wait = [&](uint64_t* bar, uint32_t parity, bool weights) -> bool {
+        uint64_t t0 = 0;
+        while (true) {
+          if (due >= 0 && mbar_test_wait(p_full, (uint32_t)(due & 1)) &&
+              (!due_first || due_seg == 0 || mbar_test_wait(o_empty, (uint32_t)((due_seg - 1) & 1))))
+            weigh();
+          if (weights ? due < 0 : mbar_test_wait(bar, parity)) {
+            tc_fence_after();
+            return true;
+          }
+          if (*abort_flag) return false;
+          uint64_t t1;
+          asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t1));
+          if (t0 == 0) t0 = t1;
+          if (t1 - t0 > p.wait_limit_ns) {
+            *abort_flag = 1;
+            return false;
+          }
+        }
       };
       while (!failed && walk.next(p)) {
-        if (!wait(q_full, (uint32_t)(seg & 1))) {
-          failed = true;
-          break;
-        }
-        int at = 0;
+        failed = !wait(q_full, (uint32_t)(seg & 1), false);
 #pragma unroll 1
-        for (int tile = walk.from; tile < walk.to; ++tile, ++n) {
-          const int before = at;
-          at = pos;
-          if (n > 0 && !wait(s_empty, (uint32_t)((n - 1) & 1))) {
-            failed = true;
-            break;
-          }
+        for (int tile = walk.from; tile < walk.to && !failed; ++tile, ++n) {
+          const int at = pos;
+          if (n > 0) failed = !wait(s_empty, (uint32_t)((n - 1) & 1), false);
 #pragma unroll 1
-          for (int c = 0; c <= kChunks; ++c, ++pos) {
+          for (int c = 0; c <= kChunks && !failed; ++c, ++pos) {
             const int s = pos % kLdSlots;
-            if (!wait(full + s, (uint32_t)((pos / kLdSlots) & 1))) {
-              failed = true;
-              break;
-            }
+            failed = !wait(full + s, (uint32_t)((pos / kLdSlots) & 1), false);
+            if (failed) break;
             const uint32_t b0 = base_s + kLdRing + s * kLdSlot;
             if (c < kChunks) {
 #pragma unroll
@@ -424,55 +436,69 @@ __global__ void __launch_bounds__(kLdThreads, 1) qsa_latent_decode_kernel(const 
           }
           if (failed) break;
           mma_commit(s_full);
-          if (tile > walk.from && !weigh(before, n - 1, tile - 1 == walk.from)) {
-            failed = true;
-            break;
-          }
+          if (due >= 0) failed = !wait(nullptr, 0u, true);
+          due = n, due_at = at, due_seg = seg, due_first = tile == walk.from;
         }
-        if (!failed && !weigh(at, n - 1, walk.to - walk.from == 1)) failed = true;
         ++seg;
         walk.advance();
       }
+      if (due >= 0 && !failed) failed = !wait(nullptr, 0u, true);
       mma_commit(drain);
       if (!mbar_wait_bounded(drain, 0u, kLdDrainNs)) failed = true;
     }
     __syncwarp();
   } else {
     // ========================== softmax, results ===========================
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 240;\n");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 168;\n");
     const bool odd = (lane & 1) != 0;
-    const int pair = 16 * warp + (lane >> 1);           // this lane pair's (node, head) in the CTA
-    const bool live = 16 * warp < mine;                 // the warp has one
+    const int set = warp >> 2, q4 = warp & 3;
+    const int pair = 16 * q4 + (lane >> 1);             // this lane pair's (node, head) in the CTA
+    const bool live = 16 * q4 < mine;                   // the warp has one
     const int rho = rt * kLdPairs + pair;
     const int node = min(rho / p.heads, p.nodes - 1);
-    const uint32_t lane_base = (uint32_t)(warp * 32) << 16;
-    uint8_t* prow = smem + kLdP;
-    int n = 0, seg = 0;
-    while (walk.next(p)) {
+    const int quarter = 2 * set + (odd ? 1 : 0);        // this lane's 32 tokens of a tile
+    const uint32_t lane_base = (uint32_t)(q4 * 32) << 16;
+    int n = 0;
+    // a segment's queries are loaded before the results of the one before it are
+    // stored: each lane of a pair, in each set, has a quarter of the row
+    constexpr int kWords = 4 * kChunks;  // 16-byte words of a quarter
+    uint4 raw[kWords], rr[2];
+    auto load_q = [&](int row) {
+      const uint4* q = reinterpret_cast<const uint4*>(p.q + ((int64_t)row * pairs + rho) * (kRank + kLatentRope));
+      const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+      for (int i = 0; i < kWords; ++i) raw[i] = pair < mine ? __ldg(q + quarter * kWords + i) : zero;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) rr[i] = pair < mine ? __ldg(q + 16 * kChunks + quarter * 2 + i) : zero;
+    };
+    bool more = walk.next(p);
+    if (more) load_q(walk.row);
+    while (more) {
+      const LdWalk now = walk;
       int count;
-      ld_columns(p, walk.row, count);
+      ld_columns(p, now.row, count);
       const int own = p.nodes > 1 ? count - p.nodes : 0x7fffffff;
-      // ---- the queries: each lane of a pair converts one half of the row
+      walk.advance();
+      more = walk.next(p);
+      // ---- the queries
       float qs = 0.f;
       if (live) {
-        uint4 raw[8 * kChunks], rr[4];
-        const uint4* q = reinterpret_cast<const uint4*>(p.q + ((int64_t)walk.row * pairs + rho) * (kRank + kLatentRope));
-#pragma unroll
-        for (int i = 0; i < 8 * kChunks; ++i) raw[i] = pair < mine ? __ldg(q + (odd ? 8 * kChunks : 0) + i) : make_uint4(0u, 0u, 0u, 0u);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) rr[i] = pair < mine ? __ldg(q + 16 * kChunks + (odd ? 4 : 0) + i) : make_uint4(0u, 0u, 0u, 0u);
         uint32_t top = 0, rtop = 0;  // largest |q| as bits, two at a time
 #pragma unroll
-        for (int i = 0; i < 8 * kChunks; ++i)
-          top = max_u16x2(max_u16x2(top, max_u16x2(raw[i].x & 0x7fff7fffu, raw[i].y & 0x7fff7fffu)),
-                          max_u16x2(raw[i].z & 0x7fff7fffu, raw[i].w & 0x7fff7fffu));
+        for (int i = 0; i < kWords; ++i)
+          top = __vmaxu2(__vmaxu2(top, __vmaxu2(raw[i].x & 0x7fff7fffu, raw[i].y & 0x7fff7fffu)),
+                         __vmaxu2(raw[i].z & 0x7fff7fffu, raw[i].w & 0x7fff7fffu));
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          rtop = max_u16x2(max_u16x2(rtop, max_u16x2(rr[i].x & 0x7fff7fffu, rr[i].y & 0x7fff7fffu)),
-                           max_u16x2(rr[i].z & 0x7fff7fffu, rr[i].w & 0x7fff7fffu));
-        top = max_u16x2(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        rtop = max_u16x2(rtop, __shfl_xor_sync(0xffffffffu, rtop, 1));
-        const int t = (int)max(top & 0xffffu, top >> 16), u = (int)max(rtop & 0xffffu, rtop >> 16);
+        for (int i = 0; i < 2; ++i)
+          rtop = __vmaxu2(__vmaxu2(rtop, __vmaxu2(rr[i].x & 0x7fff7fffu, rr[i].y & 0x7fff7fffu)),
+                          __vmaxu2(rr[i].z & 0x7fff7fffu, rr[i].w & 0x7fff7fffu));
+        // both maxima of this lane, then of the row's four
+        uint32_t both = max(top & 0xffffu, top >> 16) | max(rtop & 0xffffu, rtop >> 16) << 16;
+        both = __vmaxu2(both, __shfl_xor_sync(0xffffffffu, both, 1));
+        if (!odd) told_f[set * kLdPairs + pair] = __uint_as_float(both);
+        bar_sync(2 + q4, 64);
+        both = __vmaxu2(both, __float_as_uint(told_f[(set ^ 1) * kLdPairs + pair]));
+        const int t = (int)(both & 0xffffu), u = (int)(both >> 16);
         // 2^a takes the largest latent query into [128, 256), as far as the rotated
         // ones stay far from bf16's end
         int a = t == 0 ? 0 : 7 - (max(t >> 7, 1) - 127);
@@ -481,36 +507,33 @@ __global__ void __launch_bounds__(kLdThreads, 1) qsa_latent_decode_kernel(const 
         const float up = __uint_as_float((uint32_t)(127 + a) << 23);
         qs = __uint_as_float((uint32_t)(127 - a) << 23) * p.score_scale_log2;
         if (t >= 0x7f80 || u >= 0x7f80) qs = __int_as_float(0x7fffffff);  // an infinity or NaN
-        // terms in place: hi of dims 0-3, 4-7, lo of 0-3, 4-7
-#pragma unroll
-        for (int i = 0; i < 8 * kChunks; ++i) {
-          const uint32_t w4[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
-          uint32_t hi[4], lo[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float x = __uint_as_float(w4[j] << 16) * up, y = __uint_as_float(w4[j] & 0xffff0000u) * up;
-            hi[j] = __nv_cvt_float2_to_fp8x2(make_float2(x, y), __NV_SATFINITE, __NV_E4M3);
-            const float2 back = e4m3x2_to_f32x2((uint16_t)hi[j]);
-            lo[j] = __nv_cvt_float2_to_fp8x2(make_float2((x - back.x) * 16.f, (y - back.y) * 16.f), __NV_SATFINITE, __NV_E4M3);
-          }
-          raw[i] = make_uint4(hi[0] | hi[1] << 16, hi[2] | hi[3] << 16, lo[0] | lo[1] << 16, lo[2] | lo[3] << 16);
-        }
-        // the even lane's row is the first terms, the odd one's the second
+        // the even lane's row is the first terms, the odd one's the second: this
+        // lane's quarter of both, the other lane's from it
 #pragma unroll
         for (int b = 0; b < kChunks; ++b) {
-          uint32_t first[16], second[16];
+          uint32_t first[8], second[8];  // of the even lane's quarter, of the odd one's
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const uint4 v = raw[8 * b + i];
-            const uint32_t r0 = __shfl_xor_sync(0xffffffffu, odd ? v.x : v.z, 1), r1 = __shfl_xor_sync(0xffffffffu, odd ? v.y : v.w, 1);
-            first[2 * i] = odd ? r0 : v.x, first[2 * i + 1] = odd ? r1 : v.y;
-            second[2 * i] = odd ? v.z : r0, second[2 * i + 1] = odd ? v.w : r1;
+          for (int i = 0; i < 4; ++i) {
+            const uint4 v = raw[4 * b + i];
+            const uint32_t w4[4] = {v.x, v.y, v.z, v.w};
+            uint32_t hi[4], lo[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const float x = __uint_as_float(w4[j] << 16) * up, y = __uint_as_float(w4[j] & 0xffff0000u) * up;
+              hi[j] = __nv_cvt_float2_to_fp8x2(make_float2(x, y), __NV_SATFINITE, __NV_E4M3);
+              const float2 back = e4m3x2_to_f32x2((uint16_t)hi[j]);
+              lo[j] = __nv_cvt_float2_to_fp8x2(make_float2((x - back.x) * 16.f, (y - back.y) * 16.f), __NV_SATFINITE, __NV_E4M3);
+            }
+            const uint32_t h0 = hi[0] | hi[1] << 16, h1 = hi[2] | hi[3] << 16, l0 = lo[0] | lo[1] << 16, l1 = lo[2] | lo[3] << 16;
+            const uint32_t r0 = __shfl_xor_sync(0xffffffffu, odd ? h0 : l0, 1), r1 = __shfl_xor_sync(0xffffffffu, odd ? h1 : l1, 1);
+            first[2 * i] = odd ? r0 : h0, first[2 * i + 1] = odd ? r1 : h1;
+            second[2 * i] = odd ? l0 : r0, second[2 * i + 1] = odd ? l1 : r1;
           }
-          tmem_st(tmem + lane_base + b * 16, first);
-          tmem_st(tmem + lane_base + 16 * kChunks + b * 16, second);
+          tmem_st(tmem + lane_base + 2 * set * 8 * kChunks + b * 8, first);
+          tmem_st(tmem + lane_base + (2 * set + 1) * 8 * kChunks + b * 8, second);
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < 2; ++i) {
           const uint32_t w4[4] = {rr[i].x, rr[i].y, rr[i].z, rr[i].w};
           uint32_t o4[4];
 #pragma unroll
@@ -518,7 +541,7 @@ __global__ void __launch_bounds__(kLdThreads, 1) qsa_latent_decode_kernel(const 
             const __nv_bfloat162 v = __floats2bfloat162_rn(__uint_as_float(w4[j] << 16) * up, __uint_as_float(w4[j] & 0xffff0000u) * up);
             o4[j] = *reinterpret_cast<const uint32_t*>(&v);
           }
-          *reinterpret_cast<uint4*>(smem + kLdQr + sw128_offset(32 * warp + (lane & ~1), (odd ? 64 : 0) + 16 * i)) =
+          *reinterpret_cast<uint4*>(smem + kLdQr + sw128_offset(32 * q4 + (lane & ~1), 32 * quarter + 16 * i)) =
               make_uint4(o4[0], o4[1], o4[2], o4[3]);
         }
         tmem_wait_st();
@@ -530,99 +553,94 @@ __global__ void __launch_bounds__(kLdThreads, 1) qsa_latent_decode_kernel(const 
       float r = kLowest, l = 0.f;
       const float km = odd ? qs * 0.0625f : qs, kr = odd ? qs : qs * 0.0625f;  // own and the other lane's term
 #pragma unroll 1
-      for (int tile = walk.from; tile < walk.to; ++tile, ++n) {
+      for (int tile = now.from; tile < now.to; ++tile, ++n) {
         const int m = n % kLdMeta;
         if (!failed)
           failed = !(wait_or_abort(meta_full + m, (uint32_t)((n / kLdMeta) & 1), abort_flag, p.wait_limit_ns) &&
                      wait_or_abort(s_full, (uint32_t)(n & 1), abort_flag, p.wait_limit_ns));
         failed = __any_sync(0xffffffffu, failed);
         tc_fence_after();
-        float u[64];
+        float u[32];
         float top = -INFINITY;
         if (live && !failed) {
-          const float* ms = metas[m].s + (odd ? kLdHalf : 0);
-          const float* ml = metas[m].lg + (odd ? kLdHalf : 0);
+          const float* ms = metas[m].s + quarter * kLdQuarter;
+          const float* ml = metas[m].lg + quarter * kLdQuarter;
+          float x[32], y[32];
+          tmem_ld_wait<32>(tmem + lane_base + kLdTmemS + 64 * set, x);
+          tmem_ld_wait<32>(tmem + lane_base + kLdTmemS + 64 * set + 32, y);
+          tc_fence_before();
+          mbar_arrive(s_empty);
 #pragma unroll
-          for (int b = 0; b < 2; ++b) {
-            float x[32], y[32];
-            tmem_ld_wait<32>(tmem + lane_base + kLdTmemS + 32 * b, x);
-            tmem_ld_wait<32>(tmem + lane_base + kLdTmemS + 64 + 32 * b, y);
-            if (b == 1) {
-              tc_fence_before();
-              mbar_arrive(s_empty);
-            }
+          for (int j = 0; j < 32; j += 4) {
+            const float4 s4 = *reinterpret_cast<const float4*>(ms + j);
+            const float4 l4 = *reinterpret_cast<const float4*>(ml + j);
+            const float ss[4] = {s4.x, s4.y, s4.z, s4.w}, ll[4] = {l4.x, l4.y, l4.z, l4.w};
 #pragma unroll
-            for (int j = 0; j < 32; j += 4) {
-              const float4 s4 = *reinterpret_cast<const float4*>(ms + 32 * b + j);
-              const float4 l4 = *reinterpret_cast<const float4*>(ml + 32 * b + j);
-              const float ss[4] = {s4.x, s4.y, s4.z, s4.w}, ll[4] = {l4.x, l4.y, l4.z, l4.w};
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const float other = __shfl_xor_sync(0xffffffffu, odd ? x[j + i] : y[j + i], 1);
-                const float v = fmaf(odd ? y[j + i] : x[j + i], km, other * kr);
-                u[32 * b + j + i] = fmaf(v, ss[i], ll[i]);
-              }
+            for (int i = 0; i < 4; ++i) {
+              const float other = __shfl_xor_sync(0xffffffffu, odd ? x[j + i] : y[j + i], 1);
+              const float v = fmaf(odd ? y[j + i] : x[j + i], km, other * kr);
+              u[j + i] = fmaf(v, ss[i], ll[i]);
             }
           }
-          const int d0 = tile * kLdTile + (odd ? 64 : 0) - own;
           if (p.nodes > 1 && tile * kLdTile + kLdTile > own) {
+            const int d0 = tile * kLdTile + 32 * quarter - own;
             const int word = d0 >> 5;
-            const uint32_t w0 = ld_seen_word(p, walk.row, node, word), w1 = ld_seen_word(p, walk.row, node, word + 1),
-                           w2 = ld_seen_word(p, walk.row, node, word + 2);
-            const uint32_t b0 = __funnelshift_r(w0, w1, d0 & 31), b1 = __funnelshift_r(w1, w2, d0 & 31);
+            const uint32_t bits = __funnelshift_r(ld_seen_word(p, now.row, node, word), ld_seen_word(p, now.row, node, word + 1), d0 & 31);
 #pragma unroll
-            for (int j = 0; j < 32; ++j) {
-              if (!((b0 >> j) & 1u)) u[j] = -INFINITY;
-              if (!((b1 >> j) & 1u)) u[32 + j] = -INFINITY;
-            }
+            for (int j = 0; j < 32; ++j)
+              if (!((bits >> j) & 1u)) u[j] = -INFINITY;
           }
 #pragma unroll
-          for (int j = 0; j < 64; ++j) top = fmaxf(top, u[j]);
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+          for (int j = 0; j < 32; ++j) top = fmaxf(top, u[j]);
         } else {
           mbar_arrive(s_empty);
         }
         // a reference that a weight passes by too much moves, and O and l with it
-        const bool begun = tile > walk.from;
-        if (bar_vote(1, 128, top > r + kLdLazy || failed)) {
+        const bool begun = tile > now.from;
+        if (bar_vote(1, kLdSoft, top > r + kLdLazy || failed)) {
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+          if (live && !odd) told_f[set * kLdPairs + pair] = top;
+          if (begun && !failed) failed = !wait_or_abort(o_full, (uint32_t)((n - 1) & 1), abort_flag, p.wait_limit_ns);
+          failed = __any_sync(0xffffffffu, failed);
+          if (bar_vote(1, kLdSoft, failed)) {
+            failed = true;
+            break;
+          }
+          if (live) top = fmaxf(top, told_f[(set ^ 1) * kLdPairs + pair]);
           const float next = fmaxf(r, top);
           const float f = ex2(r - next);  // 0 before the first weight
           l *= f;
           r = next;
-          if (begun) {
-            if (live && !odd) head_f[pair] = f;
-            if (!failed) failed = !wait_or_abort(o_full, (uint32_t)((n - 1) & 1), abort_flag, p.wait_limit_ns);
-          }
-          failed = __any_sync(0xffffffffu, failed);
-          if (bar_vote(1, 128, failed)) {
-            failed = true;
-            break;
-          }
+          if (live && !odd && set == 0) head_f[pair] = f;
+          bar_sync(1, kLdSoft);  // the factors are there, and what the sets told is read
           if (begun) {
             tc_fence_after();
 #pragma unroll 1
-            for (int c = 0; c < kChunks; ++c)
-#pragma unroll 1
-              for (int b = 0; b < mine; b += 32) {
-                const uint32_t at = tmem + lane_base + kLdTmemO + c * kLdPairs + b;
-                float x[32];
-                uint32_t y[32];
-                tmem_ld_wait<32>(at, x);
+            for (int c = set; c < 4 * kChunks; c += 2) {
+              // 16 pairs at a time, where one has moved
+              const int b = c % 4 * 16;
+              if (b >= mine) continue;
+              const float own_f = head_f[b + (lane & 15)];
+              if (__all_sync(0xffffffffu, own_f == 1.f)) continue;
+              const uint32_t at = tmem + lane_base + kLdTmemO + c / 4 * kLdPairs + b;
+              float x[16];
+              uint32_t y[16];
+              tmem_ld_wait<16>(at, x);
 #pragma unroll
-                for (int j = 0; j < 32; ++j) y[j] = __float_as_uint(x[j] * head_f[b + j]);
-                tmem_st(at, y);
-              }
+              for (int j = 0; j < 16; ++j) y[j] = __float_as_uint(x[j] * head_f[b + j]);
+              tmem_st(at, y);
+            }
             tmem_wait_st();
             tc_fence_before();
           }
         }
         // ---- weights
-        uint32_t hi[16], lo[16];
+        uint32_t hi[8], lo[8];
         if (live) {
-          const float* mi = metas[m].inv + (odd ? kLdHalf : 0);
+          const float* mi = metas[m].inv + quarter * kLdQuarter;
           const float rb = r - kLdOne;
 #pragma unroll
-          for (int j = 0; j < 64; j += 4) {
+          for (int j = 0; j < 32; j += 4) {
             const float4 i4 = *reinterpret_cast<const float4*>(mi + j);
             const float ii[4] = {i4.x, i4.y, i4.z, i4.w};
             uint32_t h2[2], l2[2];
@@ -648,52 +666,56 @@ __global__ void __launch_bounds__(kLdThreads, 1) qsa_latent_decode_kernel(const 
         failed = __any_sync(0xffffffffu, failed);
         if (live) {
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const uint32_t at = sw128_offset(pair, (odd ? 64 : 0) + 16 * k);
-            *reinterpret_cast<uint4*>(prow + at) = make_uint4(hi[4 * k], hi[4 * k + 1], hi[4 * k + 2], hi[4 * k + 3]);
-            *reinterpret_cast<uint4*>(prow + 8192 + at) = make_uint4(lo[4 * k], lo[4 * k + 1], lo[4 * k + 2], lo[4 * k + 3]);
+          for (int k = 0; k < 2; ++k) {
+            uint8_t* at = smem + kLdP + sw128_offset(pair, 32 * quarter + 16 * k);
+            *reinterpret_cast<uint4*>(at) = make_uint4(hi[4 * k], hi[4 * k + 1], hi[4 * k + 2], hi[4 * k + 3]);
+            *reinterpret_cast<uint4*>(at + 8192) = make_uint4(lo[4 * k], lo[4 * k + 1], lo[4 * k + 2], lo[4 * k + 3]);
           }
           fence_proxy_async_smem();
         }
         mbar_arrive(p_full);
       }
       // ---- the segment's results
+      if (more) load_q(walk.row);
       if (!failed) failed = !wait_or_abort(o_full, (uint32_t)((n - 1) & 1), abort_flag, p.wait_limit_ns);
       failed = __any_sync(0xffffffffu, failed);
       l += __shfl_xor_sync(0xffffffffu, l, 1);
-      if (live && !odd) head_f[pair] = l == 0.f ? 0.f : 1.0f / l;
-      const int piece = 2 * group + (walk.from > 0 ? 0 : 1);
-      if (!walk.whole && !odd && pair < mine)
-        p.part_lse[((int64_t)piece * p.row_tiles + rt) * kLdPairs + pair] = l == 0.f ? -INFINITY : log2f(l) + (r - kLdOne);
-      if (bar_vote(1, 128, failed)) {
+      if (live && !odd) told_f[set * kLdPairs + pair] = l;
+      if (bar_vote(1, kLdSoft, failed)) {
         failed = true;
         break;
       }
+      const int piece = 2 * group + (now.from > 0 ? 0 : 1);
+      if (live && !odd && set == 0) {
+        l += told_f[kLdPairs + pair];
+        head_f[pair] = l == 0.f ? 0.f : 1.0f / l;
+        if (!now.whole && pair < mine)
+          p.part_lse[((int64_t)piece * p.row_tiles + rt) * kLdPairs + pair] = l == 0.f ? -INFINITY : log2f(l) + (r - kLdOne);
+      }
+      bar_sync(1, kLdSoft);
       tc_fence_after();
-      const int64_t at = walk.whole ? ((int64_t)walk.row * pairs + rt * kLdPairs) * kRank
+      const int64_t at = now.whole ? ((int64_t)now.row * pairs + rt * kLdPairs) * kRank
                                     : ((int64_t)piece * p.row_tiles + rt) * kLdPairs * kRank;
 #pragma unroll 1
-      for (int c = 0; c < kChunks; ++c)
-#pragma unroll 1
-        for (int b = 0; b < mine; b += 32) {
-          float x[32];
-          tmem_ld_wait<32>(tmem + lane_base + kLdTmemO + c * kLdPairs + b, x);
-          const int64_t to = at + (int64_t)b * kRank + c * 128 + 32 * warp + lane;
+      for (int c = set; c < 4 * kChunks; c += 2) {
+        const int b = c % 4 * 16;
+        if (b >= mine) continue;
+        float x[16];
+        tmem_ld_wait<16>(tmem + lane_base + kLdTmemO + c / 4 * kLdPairs + b, x);
+        const int64_t to = at + (int64_t)b * kRank + c / 4 * 128 + 32 * q4 + lane;
 #pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            if (b + j >= mine) break;
-            const float v = x[j] * head_f[b + j];
-            if (walk.whole)
-              p.out[to + j * kRank] = __float2bfloat16_rn(v);
-            else
-              p.part_o[to + j * kRank] = v;
-          }
+        for (int j = 0; j < 16; ++j) {
+          if (b + j >= mine) break;
+          const float v = x[j] * head_f[b + j];
+          if (now.whole)
+            p.out[to + j * kRank] = __float2bfloat16_rn(v);
+          else
+            p.part_o[to + j * kRank] = v;
         }
+      }
       tc_fence_before();
       mbar_arrive(o_empty);
-      bar_sync(1, 128);  // the factors are read before the next segment's
-      ++seg;
-      walk.advance();
+      bar_sync(1, kLdSoft);  // the factors are read before the next segment's
     }
   }
 
