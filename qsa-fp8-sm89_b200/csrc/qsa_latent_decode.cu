@@ -32,7 +32,7 @@
 //
 // Warps: four loaders bring 128-token tiles, 128 bytes of each token at a
 // time, into a ring of 16 KiB slots by cp.async (gathered rows in the 128-byte
-// swizzle that the matrix unit reads); one issues the products; eight do the
+// swizzle that the matrix unit reads); two issue the products; eight do the
 // softmax and the results, two for each quarter of the lanes, with half of the
 // tokens each. The product of scores of tile i + 1 runs while tile i's softmax
 // does, and P V of tile i after it.
@@ -57,12 +57,11 @@ constexpr int kLdTile = 128;     // tokens of a tile
 constexpr int kLdSlot = kLdTile * 128;
 constexpr int kLdSlots = 11;
 constexpr int kLdMeta = 4;       // tiles whose scales are held
-constexpr int kLdLag = 7;        // slots under way before a loader looks back
 constexpr int kLdSoft = 256;     // threads of the softmax
-constexpr int kLdLoader0 = 8, kLdMmaWarp = 12;
-// Four warpgroups: two of softmax, loaders, and the warp of the products with three
-// idle ones. The softmax takes registers that the others hand back: 2 x 168 + 104 +
-// 72 of the 4 x 128 that the block is launched with.
+constexpr int kLdLoader0 = 8, kLdMmaWarp = 12, kLdFenceWarp = 13, kLdWeighWarp = 14;
+// Four warpgroups: two of softmax, loaders, and the warps of the two products and of
+// the fence with an idle one. The softmax takes registers that the others hand back: 2 x 160 + 96 +
+// 96 of the 4 x 128 that the block is launched with.
 constexpr int kLdThreads = 512;
 constexpr int64_t kLdDirectTiles = 4;  // tiles of a row that is not split
 constexpr float kLdOne = 6.f;    // log2 of the weight at the reference
@@ -82,9 +81,10 @@ constexpr int kLdP = kLdQr + 16384;                // weights: two terms of 64 r
 constexpr int kLdRing = kLdP + 16384;
 constexpr int kLdMetaAt = kLdRing + kLdSlots * kLdSlot;
 constexpr int kLdRow = kLdMetaAt + kLdMeta * (int)sizeof(LdMeta);  // float [64]: factors of pairs
-constexpr int kLdShare = kLdRow + kLdPairs * 4;                    // float [2][64]: what the two sets of warps tell
-constexpr int kLdBars = kLdShare + 2 * kLdPairs * 4;
-constexpr int kLdNumBars = 2 * kLdSlots + 2 * kLdMeta + 7;
+constexpr int kLdShare = kLdRow + kLdPairs * 4;                    // float [2][64] x 2: what the two sets of warps tell, of scores and of queries
+constexpr int kLdBars = kLdShare + 4 * kLdPairs * 4;
+constexpr int kLdReady = 4;      // tiles that may be ready at once
+constexpr int kLdNumBars = 2 * kLdSlots + kLdReady + 2 * kLdMeta + 8;
 constexpr int kLdMisc = kLdBars + kLdNumBars * 8;  // tensor memory address, abort flag, group's range
 constexpr int kLdSmem = kLdMisc + 64 + 1024;
 static_assert(kLdSmem <= 232448 && kLdBars % 8 == 0 && kLdMisc % 8 == 0 && kLdMetaAt % 16 == 0, "shared memory");
@@ -146,7 +146,7 @@ __global__ void __launch_bounds__(kLdThreads, 1) qsa_latent_decode_kernel(const 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kLdBars);
-  uint64_t* full = bars;                       // [slots] loaders -> products
+  uint64_t* full = bars;                       // [slots] loaders -> fence
   uint64_t* empty = full + kLdSlots;           // [slots] products -> loaders
   uint64_t* meta_full = empty + kLdSlots;      // [kLdMeta] loaders -> softmax
   uint64_t* meta_empty = meta_full + kLdMeta;  // [kLdMeta] softmax -> loaders
@@ -156,7 +156,8 @@ __global__ void __launch_bounds__(kLdThreads, 1) qsa_latent_decode_kernel(const 
   uint64_t* p_full = s_empty + 1;              // softmax -> products
   uint64_t* o_full = p_full + 1;               // products -> softmax
   uint64_t* o_empty = o_full + 1;              // results taken -> products, each segment
-  uint64_t* drain = o_empty + 1;
+  uint64_t* ready = o_empty + 1;               // [kLdReady] fence -> products, each tile
+  uint64_t* drain = ready + kLdReady;          // [2]
   uint32_t* tmem_at = reinterpret_cast<uint32_t*>(smem + kLdMisc);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + kLdMisc + 8);
   int* begin = reinterpret_cast<int*>(smem + kLdMisc + 16);                 // row, tile
@@ -170,7 +171,7 @@ __global__ void __launch_bounds__(kLdThreads, 1) qsa_latent_decode_kernel(const 
   const int mine = min(kLdPairs, pairs - rt * kLdPairs);  // pairs of this CTA
 
   if (tid == 0) {
-    for (int i = 0; i < kLdSlots; ++i) mbar_init(full + i, 4), mbar_init(empty + i, 1);
+    for (int i = 0; i < kLdSlots; ++i) mbar_init(full + i, 128), mbar_init(empty + i, 1);
     for (int i = 0; i < kLdMeta; ++i) mbar_init(meta_full + i, 4), mbar_init(meta_empty + i, kLdSoft / 32);
     mbar_init(q_full, kLdSoft);
     mbar_init(s_full, 1);
@@ -178,7 +179,8 @@ __global__ void __launch_bounds__(kLdThreads, 1) qsa_latent_decode_kernel(const 
     mbar_init(p_full, kLdSoft);
     mbar_init(o_full, 1);
     mbar_init(o_empty, kLdSoft);
-    mbar_init(drain, 1);
+    for (int i = 0; i < kLdReady; ++i) mbar_init(ready + i, 1);
+    for (int i = 0; i < 2; ++i) mbar_init(drain + i, 1);
     *abort_flag = 0;
     fence_mbar_init();
   }
@@ -252,37 +254,31 @@ __global__ void __launch_bounds__(kLdThreads, 1) qsa_latent_decode_kernel(const 
 
   if (warp >= kLdLoader0 && warp < kLdMmaWarp) {
     // =============================== loaders ================================
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 104;\n");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 96;\n");
     // Warp w has tokens 32w .. 32w + 31 of every tile: a lane looks up its own
     // token, and 8 lanes fetch a token's 128 bytes.
     const int w = warp - kLdLoader0;
     const int piece = lane & 7, sub = lane >> 3;
     const int tok = 32 * w + lane;  // the lane's own token
     const int first_node = rt * kLdPairs / p.heads, last_node = (rt * kLdPairs + mine - 1) / p.heads;
-    int issued = 0, told = 0;  // slots filled by this warp, and announced
-    int tile_n = 0;
-    auto announce = [&](int upto) {  // slots up to `upto` have landed
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0)
-        for (int i = told; i < upto; ++i) mbar_arrive(full + i % kLdSlots);
-      told = upto;
-    };
+    int issued = 0, tile_n = 0;
     auto wait_free = [&](uint64_t* bar, uint32_t parity) -> bool {
-      while (!__all_sync(0xffffffffu, mbar_test_wait(bar, parity))) {
-        // what is under way must not wait for what is not
-        if (told == issued) return __all_sync(0xffffffffu, wait_or_abort(bar, parity, abort_flag, p.wait_limit_ns));
-        cp_async_wait_dyn(issued - told - 1);
-        announce(told + 1);
-      }
-      return true;
+      return __all_sync(0xffffffffu, wait_or_abort(bar, parity, abort_flag, p.wait_limit_ns));
     };
     while (!failed && walk.next(p)) {
       int count;
-      const int columns = ld_columns(p, walk.row, count);
-      const int64_t req = p.t2r ? (int64_t)__ldg(p.t2r + walk.row) : (int64_t)walk.row;
+      const int row = walk.row;
+      const int columns = ld_columns(p, row, count);
+      const int64_t req = p.t2r ? (int64_t)__ldg(p.t2r + row) : (int64_t)row;
       const int own = p.nodes > 1 ? count - p.nodes : 0x7fffffff;
-      auto lookup = [&](int tile) -> int {
+      {  // the queries, which the softmax will load, into L2
+        const char* q = reinterpret_cast<const char*>(p.q + ((int64_t)row * pairs + rt * kLdPairs) * (kRank + kLatentRope));
+        for (int i = tok; i < mine * (kRank + kLatentRope) * 2 / 128; i += 128)
+          asm volatile("prefetch.global.L2 [%0];\n" ::"l"(q + i * 128));
+      }
+      // A token's lookup is three loads in a row (its index, its page, its scale):
+      // each is made a tile before the next one needs it.
+      auto token = [&](int tile) -> int {  // -1: masked
         const int col = tile * kLdTile + tok;
         if (tile >= walk.to || col >= columns) return -1;
         if (col >= own) {  // seen by a node of this CTA?
@@ -290,35 +286,38 @@ __global__ void __launch_bounds__(kLdThreads, 1) qsa_latent_decode_kernel(const 
           uint32_t any = 0;
           if (p.tree) {
 #pragma unroll 4
-            for (int i = first_node; i <= last_node; ++i) any |= ld_seen_word(p, walk.row, i, d / 32);
+            for (int i = first_node; i <= last_node; ++i) any |= ld_seen_word(p, row, i, d / 32);
           } else {
-            any = ld_seen_word(p, walk.row, last_node, d / 32);
+            any = ld_seen_word(p, row, last_node, d / 32);
           }
           if (!((any >> (d % 32)) & 1u)) return -1;
         }
-        const int t = p.indices ? __ldg(p.indices + (int64_t)walk.row * p.indices_stride + col) : col;
-        return latent_slot(p.cache, req, t);
+        return p.indices ? __ldg(p.indices + (int64_t)row * p.indices_stride + col) : col;
       };
-      int slot = lookup(walk.from);
-      float scale = slot >= 0 ? __ldg(p.cache.scales + slot) : 0.f;
+      struct Page {
+        int page, off;
+      };
+      auto find = [&](int t) -> Page {
+        const uint32_t lp = __umulhi(2u * (uint32_t)max(t, 0), p.cache.page_mul) >> p.cache.page_shift;
+        const bool in = t >= 0 && (int)lp < p.cache.pages_per_req;
+        return {in ? __ldg(p.cache.btable + req * p.cache.btable_stride + lp) : -1, t - (int)lp * p.cache.page_size};
+      };
+      auto slot_of = [&](Page x) -> int {
+        return x.page >= 0 && x.page < p.cache.num_pages ? x.page * p.cache.page_size + x.off : -1;
+      };
+      auto scale_of = [&](int slot) -> float { return slot >= 0 ? __ldg(p.cache.scales + slot) : 0.f; };
+      const int t0 = token(walk.from), t1 = token(walk.from + 1);
+      int ahead = token(walk.from + 2);
+      const Page p0 = find(t0);
+      Page page = find(t1);
+      int slot = slot_of(p0);
+      float scale = scale_of(slot);
 #pragma unroll 1
-      for (int tile = walk.from; tile < walk.to && !failed; ++tile, ++tile_n) {
-        const int next = lookup(tile + 1);
-        const int m = tile_n % kLdMeta;
-        if (tile_n >= kLdMeta && !wait_free(meta_empty + m, (uint32_t)((tile_n / kLdMeta - 1) & 1))) {
-          failed = true;
-          break;
-        }
-        {
-          const int at = (tok >> 5) * kLdQuarter + (tok & 31);
-          const float s = slot < 0 ? 0.f : scale != scale ? scale : fminf(fmaxf(scale, kLatentLeastScale), kLatentMostScale);
-          metas[m].s[at] = s;
-          metas[m].lg[at] = slot < 0 ? -INFINITY : log2f(s);
-          // a NaN token is a NaN in the weights of those that see it, and nothing in the others'
-          metas[m].inv[at] = slot < 0 || s != s ? 0.f : 1.0f / s;
-          __syncwarp();
-          if (lane == 0) mbar_arrive(meta_full + m);
-        }
+      for (int tile = walk.from; tile < walk.to; ++tile, ++tile_n) {
+        const int next_slot = slot_of(page);
+        const float next_scale = scale_of(next_slot);
+        page = find(ahead);
+        ahead = token(tile + 3);
         int from[8];
 #pragma unroll
         for (int k = 0; k < 8; ++k) from[k] = __shfl_sync(0xffffffffu, slot, 4 * k + sub);
@@ -332,26 +331,36 @@ __global__ void __launch_bounds__(kLdThreads, 1) qsa_latent_decode_kernel(const 
             failed = true;
             break;
           }
-          const uint8_t* src = c < kChunks ? p.cache.codes + c * 128 : reinterpret_cast<const uint8_t*>(p.cache.rope);
+          const uint8_t* src = (c < kChunks ? p.cache.codes + c * 128 : reinterpret_cast<const uint8_t*>(p.cache.rope)) + piece * 16;
           const int64_t stride = c < kChunks ? kRank : 2 * kLatentRope;
 #pragma unroll
           for (int k = 0; k < 8; ++k)
-            cp_async_16(dst0 + s * kLdSlot + k * 512 + (k & 1 ? odd : even), src + (int64_t)max(from[k], 0) * stride + piece * 16,
+            cp_async_16(dst0 + s * kLdSlot + k * 512 + (k & 1 ? odd : even), src + (int64_t)max(from[k], 0) * stride,
                         from[k] < 0 ? 0u : 16u);
-          cp_async_commit();
+          cp_async_mbar_arrive_noinc(smem_u32(full + s));
           ++issued;
-          if (issued - told > kLdLag) {
-            cp_async_wait<kLdLag>();
-            announce(issued - kLdLag);
-          }
         }
-        slot = next;
-        scale = slot >= 0 ? __ldg(p.cache.scales + slot) : 0.f;
+        const int m = tile_n % kLdMeta;
+        if (failed || (tile_n >= kLdMeta && !wait_free(meta_empty + m, (uint32_t)((tile_n / kLdMeta - 1) & 1)))) {
+          failed = true;
+          break;
+        }
+        {
+          const int at = (tok >> 5) * kLdQuarter + (tok & 31);
+          const float s = slot < 0 ? 0.f : scale != scale ? scale : fminf(fmaxf(scale, kLatentLeastScale), kLatentMostScale);
+          metas[m].s[at] = s;
+          metas[m].lg[at] = slot < 0 ? -INFINITY : log2f(s);
+          // a NaN token is a NaN in the weights of those that see it, and nothing in the others'
+          metas[m].inv[at] = slot < 0 || s != s ? 0.f : 1.0f / s;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(meta_full + m);
+        }
+        slot = next_slot;
+        scale = next_scale;
       }
       walk.advance();
     }
     cp_async_wait_all();
-    announce(issued);
     // rows without a column: zeros, by this CTA's warps in turn
     for (int64_t r = p.planned ? (int64_t)group + (int64_t)p.groups * w : (w == 0 ? (int64_t)group : (int64_t)p.rows); r < p.rows;
          r += (int64_t)p.groups * 4) {
@@ -361,95 +370,104 @@ __global__ void __launch_bounds__(kLdThreads, 1) qsa_latent_decode_kernel(const 
     }
   } else if (warp >= kLdMmaWarp) {
     // =============================== products ===============================
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;\n");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 96;\n");
+    const uint32_t ring = desc_low(base_s + kLdRing);  // K: tokens by bytes (V^T: the same, MN-major)
+    auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
+      if (!wait_or_abort(bar, parity, abort_flag, p.wait_limit_ns)) return false;
+      tc_fence_after();
+      return true;
+    };
+    // Scores and weighted sums are issued by a thread each: a wait costs a thread
+    // some 200 cycles even where there is nothing to wait for, in which the other's
+    // products go on.
     if (warp == kLdMmaWarp && lane == 0) {
+      // S = Q K^T
       constexpr uint32_t kIdescS = idesc_e4m3(128, kLdTile, false, false);
       constexpr uint32_t kIdescR = idesc_f16(128, kLdTile, true, false);
-      const uint32_t idesc_o = idesc_e4m3(128, (mine + 15) / 16 * 16, true, false);
-      int pos = 0, n = 0, seg = 0;  // ring position, tile, segment
-      int due = -1, due_at = 0, due_seg = 0;  // a tile whose P V is still to come, its first slot and segment
-      bool due_first = false;                 // it is its segment's first
-      auto weigh = [&]() {  // O^T (+)= V^T P^T
-        tc_fence_after();
-#pragma unroll 1
-        for (int c = 0; c < kChunks; ++c) {
-          const int s = (due_at + c) % kLdSlots;
-          const uint32_t a0 = base_s + kLdRing + s * kLdSlot, b0 = base_s + kLdP;
-#pragma unroll
-          for (int kk = 0; kk < kLdTile / 32; ++kk) {
-            const uint64_t ad = smem_desc_sw128(a0 + kk * 32 * 128, kLdSlot, 1024);
-            mma_f8(tmem + kLdTmemO + c * kLdPairs, ad, smem_desc_sw128(b0 + kk * 32, 16, 1024), idesc_o, !due_first || kk > 0);
-            mma_f8(tmem + kLdTmemO + c * kLdPairs, ad, smem_desc_sw128(b0 + 8192 + kk * 32, 16, 1024), idesc_o, 1u);
-          }
-          mma_commit(empty + s);
-        }
-        mma_commit(o_full);
-        due = -1;
-      };
-      // The products of a tile's scores wait for its tokens, and those of the tile
-      // before for its weights: whichever is there goes first, so that slots come
-      // free while tokens are under way. weights: wait for those alone.
-      auto wait = [&](uint64_t* bar, uint32_t parity, bool weights) -> bool {
-        uint64_t t0 = 0;
-        while (true) {
-          if (due >= 0 && mbar_test_wait(p_full, (uint32_t)(due & 1)) &&
-              (!due_first || due_seg == 0 || mbar_test_wait(o_empty, (uint32_t)((due_seg - 1) & 1))))
-            weigh();
-          if (weights ? due < 0 : mbar_test_wait(bar, parity)) {
-            tc_fence_after();
-            return true;
-          }
-          if (*abort_flag) return false;
-          uint64_t t1;
-          asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t1));
-          if (t0 == 0) t0 = t1;
-          if (t1 - t0 > p.wait_limit_ns) {
-            *abort_flag = 1;
-            return false;
-          }
-        }
-      };
+      const uint32_t rotated = desc_low(base_s + kLdQr);
+      int s = 0, n = 0, seg = 0;  // ring slot, tile, segment
       while (!failed && walk.next(p)) {
-        failed = !wait(q_full, (uint32_t)(seg & 1), false);
+        failed = !wait(q_full, (uint32_t)(seg & 1));
 #pragma unroll 1
         for (int tile = walk.from; tile < walk.to && !failed; ++tile, ++n) {
-          const int at = pos;
-          if (n > 0) failed = !wait(s_empty, (uint32_t)((n - 1) & 1), false);
-#pragma unroll 1
-          for (int c = 0; c <= kChunks && !failed; ++c, ++pos) {
-            const int s = pos % kLdSlots;
-            failed = !wait(full + s, (uint32_t)((pos / kLdSlots) & 1), false);
-            if (failed) break;
-            const uint32_t b0 = base_s + kLdRing + s * kLdSlot;
+          failed = !wait(ready + n % kLdReady, (uint32_t)((n / kLdReady) & 1)) ||
+                   (n > 0 && !wait(s_empty, (uint32_t)((n - 1) & 1)));
+          if (failed) break;
+#pragma unroll
+          for (int c = 0; c <= kChunks; ++c) {
+            const uint32_t bd = ring + s * (kLdSlot / 16);
             if (c < kChunks) {
 #pragma unroll
               for (int kk = 0; kk < 4; ++kk)
-                mma_f8_ts(tmem + kLdTmemS, tmem + c * 32 + kk * 8, smem_desc_sw128(b0 + kk * 32, 16, 1024), kIdescS,
-                          c > 0 || kk > 0);
+                mma_f8_ts(tmem + kLdTmemS, tmem + c * 32 + kk * 8, bd + kk * 2, kIdescS, c > 0 || kk > 0);
             } else {
 #pragma unroll
-              for (int kk = 0; kk < 4; ++kk)
-                mma_f16_ss(tmem + kLdTmemS, smem_desc_sw128(base_s + kLdQr + kk * 32, 16, 1024),
-                           smem_desc_sw128(b0 + kk * 32, 16, 1024), kIdescR, 1u);
+              for (int kk = 0; kk < 4; ++kk) mma_f16_ss(tmem + kLdTmemS, rotated + kk * 2, bd + kk * 2, kIdescR, 1u);
+              mma_commit(s_full);
               mma_commit(empty + s);
             }
+            s = s + 1 == kLdSlots ? 0 : s + 1;
           }
-          if (failed) break;
-          mma_commit(s_full);
-          if (due >= 0) failed = !wait(nullptr, 0u, true);
-          due = n, due_at = at, due_seg = seg, due_first = tile == walk.from;
         }
         ++seg;
         walk.advance();
       }
-      if (due >= 0 && !failed) failed = !wait(nullptr, 0u, true);
       mma_commit(drain);
       if (!mbar_wait_bounded(drain, 0u, kLdDrainNs)) failed = true;
+    } else if (warp == kLdWeighWarp && lane == 0) {
+      // O^T (+)= V^T P^T
+      const uint32_t idesc_o = idesc_e4m3(128, (mine + 15) / 16 * 16, true, false);
+      const uint32_t weights = desc_low(base_s + kLdP);
+      int s = 0, n = 0, seg = 0;
+      while (!failed && walk.next(p)) {
+#pragma unroll 1
+        for (int tile = walk.from; tile < walk.to && !failed; ++tile, ++n) {
+          const bool first = tile == walk.from;
+          failed = !wait(p_full, (uint32_t)(n & 1)) || (first && seg > 0 && !wait(o_empty, (uint32_t)((seg - 1) & 1)));
+          if (failed) break;
+#pragma unroll
+          for (int c = 0; c < kChunks; ++c) {
+            const uint32_t ad = ring + s * (kLdSlot / 16);
+#pragma unroll
+            for (int kk = 0; kk < kLdTile / 32; ++kk) {
+              mma_f8_ss(tmem + kLdTmemO + c * kLdPairs, ad + kk * 256, weights + kk * 2, idesc_o, kk > 0 ? 1u : !first);
+              mma_f8_ss(tmem + kLdTmemO + c * kLdPairs, ad + kk * 256, weights + 512 + kk * 2, idesc_o, 1u);
+            }
+            mma_commit(empty + s);
+            s = s + 1 == kLdSlots ? 0 : s + 1;
+          }
+          mma_commit(o_full);
+          s = s + 1 == kLdSlots ? 0 : s + 1;  // the rotated part's
+        }
+        ++seg;
+        walk.advance();
+      }
+      mma_commit(drain + 1);
+      if (!mbar_wait_bounded(drain + 1, 0u, kLdDrainNs)) failed = true;
+    } else if (warp == kLdFenceWarp && lane == 0) {
+      // The copies wrote by one path to shared memory and the products read by
+      // another: the fence between them waits for what its own thread has under
+      // way, 1 us in a thread that copies or multiplies, and nothing in this one.
+      int s = 0, n = 0;
+      uint32_t turn = 0;
+      while (!failed && walk.next(p)) {
+#pragma unroll 1
+        for (int tile = walk.from; tile < walk.to && !failed; ++tile, ++n) {
+#pragma unroll 1
+          for (int c = 0; c <= kChunks && !failed; ++c) {
+            failed = !wait_or_abort(full + s, turn, abort_flag, p.wait_limit_ns);
+            if (++s == kLdSlots) s = 0, turn ^= 1u;
+          }
+          fence_proxy_async_smem();
+          mbar_arrive(ready + n % kLdReady);
+        }
+        walk.advance();
+      }
     }
     __syncwarp();
   } else {
     // ========================== softmax, results ===========================
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 168;\n");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 160;\n");
     const bool odd = (lane & 1) != 0;
     const int set = warp >> 2, q4 = warp & 3;
     const int pair = 16 * q4 + (lane >> 1);             // this lane pair's (node, head) in the CTA
@@ -459,8 +477,8 @@ __global__ void __launch_bounds__(kLdThreads, 1) qsa_latent_decode_kernel(const 
     const int quarter = 2 * set + (odd ? 1 : 0);        // this lane's 32 tokens of a tile
     const uint32_t lane_base = (uint32_t)(q4 * 32) << 16;
     int n = 0;
-    // a segment's queries are loaded before the results of the one before it are
-    // stored: each lane of a pair, in each set, has a quarter of the row
+    // a segment's queries are placed while the last product of the one before it is
+    // under way: each lane of a pair, in each set, has a quarter of the row
     constexpr int kWords = 4 * kChunks;  // 16-byte words of a quarter
     uint4 raw[kWords], rr[2];
     auto load_q = [&](int row) {
@@ -471,16 +489,9 @@ __global__ void __launch_bounds__(kLdThreads, 1) qsa_latent_decode_kernel(const 
 #pragma unroll
       for (int i = 0; i < 2; ++i) rr[i] = pair < mine ? __ldg(q + 16 * kChunks + quarter * 2 + i) : zero;
     };
-    bool more = walk.next(p);
-    if (more) load_q(walk.row);
-    while (more) {
-      const LdWalk now = walk;
-      int count;
-      ld_columns(p, now.row, count);
-      const int own = p.nodes > 1 ? count - p.nodes : 0x7fffffff;
-      walk.advance();
-      more = walk.next(p);
-      // ---- the queries
+    // The queries as two terms into tensor memory, and their rotated part into shared
+    // memory; returns what a product of them is to be multiplied by.
+    auto place_q = [&]() -> float {
       float qs = 0.f;
       if (live) {
         uint32_t top = 0, rtop = 0;  // largest |q| as bits, two at a time
@@ -495,9 +506,9 @@ __global__ void __launch_bounds__(kLdThreads, 1) qsa_latent_decode_kernel(const 
         // both maxima of this lane, then of the row's four
         uint32_t both = max(top & 0xffffu, top >> 16) | max(rtop & 0xffffu, rtop >> 16) << 16;
         both = __vmaxu2(both, __shfl_xor_sync(0xffffffffu, both, 1));
-        if (!odd) told_f[set * kLdPairs + pair] = __uint_as_float(both);
+        if (!odd) told_f[(2 + set) * kLdPairs + pair] = __uint_as_float(both);
         bar_sync(2 + q4, 64);
-        both = __vmaxu2(both, __float_as_uint(told_f[(set ^ 1) * kLdPairs + pair]));
+        both = __vmaxu2(both, __float_as_uint(told_f[(2 + (set ^ 1)) * kLdPairs + pair]));
         const int t = (int)(both & 0xffffu), u = (int)(both >> 16);
         // 2^a takes the largest latent query into [128, 256), as far as the rotated
         // ones stay far from bf16's end
@@ -549,7 +560,22 @@ __global__ void __launch_bounds__(kLdThreads, 1) qsa_latent_decode_kernel(const 
       }
       tc_fence_before();
       mbar_arrive(q_full);
-
+      return qs;
+    };
+    bool more = walk.next(p);
+    float next_qs = 0.f;
+    if (more) {
+      load_q(walk.row);
+      next_qs = place_q();
+    }
+    while (more) {
+      const LdWalk now = walk;
+      int count;
+      ld_columns(p, now.row, count);
+      const int own = p.nodes > 1 ? count - p.nodes : 0x7fffffff;
+      walk.advance();
+      more = walk.next(p);
+      const float qs = next_qs;
       float r = kLowest, l = 0.f;
       const float km = odd ? qs * 0.0625f : qs, kr = odd ? qs : qs * 0.0625f;  // own and the other lane's term
 #pragma unroll 1
@@ -676,7 +702,10 @@ __global__ void __launch_bounds__(kLdThreads, 1) qsa_latent_decode_kernel(const 
         mbar_arrive(p_full);
       }
       // ---- the segment's results
-      if (more) load_q(walk.row);
+      if (more && !failed) {
+        load_q(walk.row);
+        next_qs = place_q();
+      }
       if (!failed) failed = !wait_or_abort(o_full, (uint32_t)((n - 1) & 1), abort_flag, p.wait_limit_ns);
       failed = __any_sync(0xffffffffu, failed);
       l += __shfl_xor_sync(0xffffffffu, l, 1);
@@ -696,23 +725,34 @@ __global__ void __launch_bounds__(kLdThreads, 1) qsa_latent_decode_kernel(const 
       tc_fence_after();
       const int64_t at = now.whole ? ((int64_t)now.row * pairs + rt * kLdPairs) * kRank
                                     : ((int64_t)piece * p.row_tiles + rt) * kLdPairs * kRank;
+      auto store = [&](auto* to, auto round) {
 #pragma unroll 1
-      for (int c = set; c < 4 * kChunks; c += 2) {
-        const int b = c % 4 * 16;
-        if (b >= mine) continue;
-        float x[16];
-        tmem_ld_wait<16>(tmem + lane_base + kLdTmemO + c / 4 * kLdPairs + b, x);
-        const int64_t to = at + (int64_t)b * kRank + c / 4 * 128 + 32 * q4 + lane;
+        for (int c = set; c < 4 * kChunks; c += 2) {
+          const int b = c % 4 * 16;
+          if (b >= mine) continue;
+          float x[16];
+          tmem_ld_wait<16>(tmem + lane_base + kLdTmemO + c / 4 * kLdPairs + b, x);
+          auto* out = to + (int64_t)b * kRank + c / 4 * 128;
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          if (b + j >= mine) break;
-          const float v = x[j] * head_f[b + j];
-          if (now.whole)
-            p.out[to + j * kRank] = __float2bfloat16_rn(v);
-          else
-            p.part_o[to + j * kRank] = v;
+          for (int j = 0; j < 16; j += 4) {
+            const float4 f = *reinterpret_cast<const float4*>(head_f + b + j);
+            x[j] *= f.x, x[j + 1] *= f.y, x[j + 2] *= f.z, x[j + 3] *= f.w;
+          }
+          const int some = mine - b;
+          if (some >= 16) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) out[j * kRank] = round(x[j]);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+              if (j < some) out[j * kRank] = round(x[j]);
+          }
         }
-      }
+      };
+      if (now.whole)
+        store(p.out + at + 32 * q4 + lane, [](float v) { return __float2bfloat16_rn(v); });
+      else
+        store(p.part_o + at + 32 * q4 + lane, [](float v) { return v; });
       tc_fence_before();
       mbar_arrive(o_empty);
       bar_sync(1, kLdSoft);  // the factors are read before the next segment's

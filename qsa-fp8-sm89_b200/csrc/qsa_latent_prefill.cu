@@ -262,11 +262,11 @@ __global__ void __launch_bounds__(kLpThreads, 1)
         for (int c = 0; c < 3; ++c) {
           const int pos = 5 * j + c;
           if (!wait_slot(pos)) return false;
-          const uint32_t a0 = base_s + kLpQ + (3 * t + c) * kLpChunk, b0 = base_s + kLpRing + pos % kLpSlots * kLpChunk;
+          const uint32_t a0 = desc_low(base_s + kLpQ) + (3 * t + c) * (kLpChunk / 16);
+          const uint32_t b0 = desc_low(base_s + kLpRing) + pos % kLpSlots * (kLpChunk / 16);
 #pragma unroll
           for (int kk = 0; kk < 4; ++kk)
-            mma_f16_ss(tmem + kLpTmemS + t * 128, smem_desc_sw128(a0 + kk * 32, 16, 1024), smem_desc_sw128(b0 + kk * 32, 16, 1024),
-                       kIdescS, c > 0 || kk > 0);
+            mma_f16_ss(tmem + kLpTmemS + t * 128, a0 + kk * 2, b0 + kk * 2, kIdescS, kk > 0 ? 1u : c > 0);
           if (last) mma_commit(empty + pos % kLpSlots);
         }
         mma_commit(s_full + t);
@@ -280,11 +280,11 @@ __global__ void __launch_bounds__(kLpThreads, 1)
         for (int c = 0; c < 2; ++c) {
           const int pos = 5 * j + 3 + c;
           if (!wait_slot(pos)) return false;
-          const uint32_t b0 = base_s + kLpRing + pos % kLpSlots * kLpChunk;
+          const uint32_t b0 = desc_low(base_s + kLpRing) + pos % kLpSlots * (kLpChunk / 16);
 #pragma unroll
           for (int kk = 0; kk < 8; ++kk)
-            mma_f16_ts(tmem + kLpTmemO + t * 128 + c * 64, tmem + kLpTmemS + t * 128 + kk * 8,
-                       smem_desc_sw128(b0 + kk * 2048, kLpChunk, 1024), kIdescO, j > 0 || kk > 0);
+            mma_f16_ts(tmem + kLpTmemO + t * 128 + c * 64, tmem + kLpTmemS + t * 128 + kk * 8, b0 + kk * 128, kIdescO,
+                       kk > 0 ? 1u : j > 0);
           if (last) mma_commit(empty + pos % kLpSlots);
         }
         mma_commit(o_full + t);

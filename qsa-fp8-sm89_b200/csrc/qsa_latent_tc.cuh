@@ -52,26 +52,41 @@ __device__ __forceinline__ bool wait_or_abort(uint64_t* bar, uint32_t parity, vo
   }
 }
 
+// Descriptors of 128-byte swizzled operands whose 8-row groups lie 1024 bytes
+// apart: the high words are all the same, the low word is the address in 16-byte
+// steps (and the step between 128-byte columns where an operand has several).
+constexpr uint32_t kDescHigh = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t desc_low(uint32_t saddr, uint32_t column_step = 16) {
+  return ((saddr >> 4) & 0x3FFF) | (column_step >> 4) << 16;
+}
+
 // D[tmem] (+)= A B with A in tensor memory (ts) or shared memory (ss), B in shared memory.
-__device__ __forceinline__ void mma_f8_ts(uint32_t d, uint32_t a, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+__device__ __forceinline__ void mma_f8_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
-      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d), "r"(a), "l"(b_desc), "r"(idesc),
-      "r"(accumulate)
+      "{\n.reg .pred p;\n.reg .b64 bd;\nsetp.ne.b32 p, %4, 0;\nmov.b64 bd, {%2, %5};\n"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], [%1], bd, %3, p;\n}\n" ::"r"(d), "r"(a), "r"(b), "r"(idesc),
+      "r"(accumulate), "n"(kDescHigh)
       : "memory");
 }
-__device__ __forceinline__ void mma_f16_ts(uint32_t d, uint32_t a, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+__device__ __forceinline__ void mma_f8_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d), "r"(a), "l"(b_desc), "r"(idesc),
-      "r"(accumulate)
+      "{\n.reg .pred p;\n.reg .b64 ad, bd;\nsetp.ne.b32 p, %4, 0;\nmov.b64 ad, {%1, %5};\nmov.b64 bd, {%2, %5};\n"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], ad, bd, %3, p;\n}\n" ::"r"(d), "r"(a), "r"(b), "r"(idesc),
+      "r"(accumulate), "n"(kDescHigh)
       : "memory");
 }
-__device__ __forceinline__ void mma_f16_ss(uint32_t d, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+__device__ __forceinline__ void mma_f16_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d), "l"(a_desc), "l"(b_desc), "r"(idesc),
-      "r"(accumulate)
+      "{\n.reg .pred p;\n.reg .b64 bd;\nsetp.ne.b32 p, %4, 0;\nmov.b64 bd, {%2, %5};\n"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], bd, %3, p;\n}\n" ::"r"(d), "r"(a), "r"(b), "r"(idesc),
+      "r"(accumulate), "n"(kDescHigh)
+      : "memory");
+}
+__device__ __forceinline__ void mma_f16_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n.reg .pred p;\n.reg .b64 ad, bd;\nsetp.ne.b32 p, %4, 0;\nmov.b64 ad, {%1, %5};\nmov.b64 bd, {%2, %5};\n"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], ad, bd, %3, p;\n}\n" ::"r"(d), "r"(a), "r"(b), "r"(idesc),
+      "r"(accumulate), "n"(kDescHigh)
       : "memory");
 }
 
