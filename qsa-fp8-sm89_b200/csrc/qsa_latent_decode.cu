@@ -19,16 +19,17 @@
 //                   columns of tensor memory for 64 pairs (O itself would need
 //                   all 512 for its 128 lanes).
 // q: the terms are exact for a bf16 value within 2^13 of the head's largest and
-// off by 2^-21 of the largest at most below. P: a weight is rounded to bf16's 8
-// bits, which two terms hold down to 2^-8 of the reference's, to steps of 2^-15 of
-// that below; the sum of weights takes the bf16 value, so that most of this
-// rounding cancels in the quotient.
-//
-// Softmax. With s_t a weight on the codes is w_t = 2^(score_t + log2 s_t - r): one
-// running reference r of score + log2 s bounds all that goes into E4M3, and the
-// softmax's own sum is l = sum w_t / s_t. Scales within 2^-60 .. 2^60 keep both in
-// fp32's range. r moves only when a tile passes it by 2.8 (2^6 2^2.8 < 448), and
-// then O is rescaled in tensor memory; the usual tile needs one vote.
+// off by 2^-21 of the largest at most below.
+// P: with s_t a weight on the codes is w_t = 2^(score_t + log2 s_t - r). Each 32
+// tokens of a pair have a power of two of their own, which the product applies
+// (block scales), with their largest weight brought to 2^7 .. 2^8: a weight is
+// rounded to bf16's 8 bits, which two terms hold down to 2^-10 of the 32's largest,
+// and to steps of 2^-17 of it below. One scale for all tokens would lose what many
+// small weights add up to beside a few large ones (E4M3 ends at 2^-9). The sum of
+// weights takes the bf16 value, so that most of this rounding cancels in the
+// quotient: l = sum w_t / s_t, in fp32; scales within 2^-60 .. 2^60 keep it in range.
+// r is the largest score + log2 s of the first tile that has one. It moves, and O
+// with it, only when a tile passes it by 2^60.
 //
 // Warps: four loaders bring 128-token tiles, 128 bytes of each token at a
 // time, into a ring of 16 KiB slots by cp.async (gathered rows in the 128-byte
@@ -64,8 +65,9 @@ constexpr int kLdLoader0 = 8, kLdMmaWarp = 12, kLdFenceWarp = 13, kLdWeighWarp =
 // 96 of the 4 x 128 that the block is launched with.
 constexpr int kLdThreads = 512;
 constexpr int64_t kLdDirectTiles = 4;  // tiles of a row that is not split
-constexpr float kLdOne = 6.f;    // log2 of the weight at the reference
-constexpr float kLdLazy = 2.8f;  // log2 by which a weight may pass it
+constexpr float kLdOne = 8.f;    // log2 that bounds the largest weight of 32
+constexpr float kLdFar = 60.f;   // log2 by which a weight may pass the reference
+constexpr float kLdNear = -110.f;  // log2 below it under which 32 weights get no smaller scale
 constexpr float kLowest = -3.402823466e38f;
 constexpr uint64_t kLdDrainNs = 1000000000ull;
 
@@ -81,15 +83,19 @@ constexpr int kLdP = kLdQr + 16384;                // weights: two terms of 64 r
 constexpr int kLdRing = kLdP + 16384;
 constexpr int kLdMetaAt = kLdRing + kLdSlots * kLdSlot;
 constexpr int kLdRow = kLdMetaAt + kLdMeta * (int)sizeof(LdMeta);  // float [64]: factors of pairs
-constexpr int kLdShare = kLdRow + kLdPairs * 4;                    // float [2][64] x 2: what the two sets of warps tell, of scores and of queries
-constexpr int kLdBars = kLdShare + 4 * kLdPairs * 4;
+constexpr int kLdShare = kLdRow + kLdPairs * 4;                    // what the two sets of warps tell: float2 [2 tiles][2][64], float [2][64] of queries
+constexpr int kLdScales = kLdShare + 4 * kLdPairs * 8 + 2 * kLdPairs * 4;  // bytes [2 tiles][64][4 x 32 tokens]
+constexpr int kLdQx = kLdScales + 2 * kLdPairs * 4;                        // a rank of 512: the last 32 values of Q
+constexpr int kLdBars = kLdQx + 4096;
 constexpr int kLdReady = 4;      // tiles that may be ready at once
 constexpr int kLdNumBars = 2 * kLdSlots + kLdReady + 2 * kLdMeta + 8;
 constexpr int kLdMisc = kLdBars + kLdNumBars * 8;  // tensor memory address, abort flag, group's range
 constexpr int kLdSmem = kLdMisc + 64 + 1024;
 static_assert(kLdSmem <= 232448 && kLdBars % 8 == 0 && kLdMisc % 8 == 0 && kLdMetaAt % 16 == 0, "shared memory");
 
-constexpr uint32_t kLdTmemS = 128, kLdTmemO = 256;  // columns; Q from 0
+// Columns of tensor memory: Q from 0, up to 120 (of a rank of 512 the last 32 values,
+// which would take 8 more, lie in shared memory), the scales of V^T (ones) and P.
+constexpr uint32_t kLdTmemOnes = 120, kLdTmemScales = 124, kLdTmemS = 128, kLdTmemO = 256;
 
 // Columns of a row that may hold a token.
 __device__ __forceinline__ int ld_columns(const LatentDecodeParams& p, int row, int& count) {
@@ -164,11 +170,19 @@ __global__ void __launch_bounds__(kLdThreads, 1) qsa_latent_decode_kernel(const 
   int64_t* share = reinterpret_cast<int64_t*>(smem + kLdMisc + 24);         // first unit, units
   LdMeta* metas = reinterpret_cast<LdMeta*>(smem + kLdMetaAt);
   float* head_f = reinterpret_cast<float*>(smem + kLdRow);
-  float* told_f = reinterpret_cast<float*>(smem + kLdShare);
+  float2* told_f = reinterpret_cast<float2*>(smem + kLdShare);
+  uint8_t* told_scales = smem + kLdScales;
+  float* told_q = reinterpret_cast<float*>(smem + kLdShare + 4 * kLdPairs * 8);
 
   const int rt = (int)(blockIdx.x % p.row_tiles), group = (int)(blockIdx.x / p.row_tiles);
   const int pairs = p.nodes * p.heads;
   const int mine = min(kLdPairs, pairs - rt * kLdPairs);  // pairs of this CTA
+  // Up to 32 pairs have both terms of the weights side by side as columns of one
+  // product, which is half the products (their number, not their width, is what
+  // they cost: 62 cycles each from 16 to 64 columns), and two columns of O each.
+  const bool few = mine <= kLdPairs / 2;
+  const int cols = (mine + 15) / 16 * 16;            // columns of the first terms
+  const int lo_row = few ? cols : kLdPairs;          // where the second terms' rows of P begin
 
   if (tid == 0) {
     for (int i = 0; i < kLdSlots; ++i) mbar_init(full + i, 128), mbar_init(empty + i, 1);
@@ -384,7 +398,7 @@ __global__ void __launch_bounds__(kLdThreads, 1) qsa_latent_decode_kernel(const 
       // S = Q K^T
       constexpr uint32_t kIdescS = idesc_e4m3(128, kLdTile, false, false);
       constexpr uint32_t kIdescR = idesc_f16(128, kLdTile, true, false);
-      const uint32_t rotated = desc_low(base_s + kLdQr);
+      const uint32_t rotated = desc_low(base_s + kLdQr), last = desc_low(base_s + kLdQx, 2048);
       int s = 0, n = 0, seg = 0;  // ring slot, tile, segment
       while (!failed && walk.next(p)) {
         failed = !wait(q_full, (uint32_t)(seg & 1));
@@ -398,8 +412,12 @@ __global__ void __launch_bounds__(kLdThreads, 1) qsa_latent_decode_kernel(const 
             const uint32_t bd = ring + s * (kLdSlot / 16);
             if (c < kChunks) {
 #pragma unroll
-              for (int kk = 0; kk < 4; ++kk)
-                mma_f8_ts(tmem + kLdTmemS, tmem + c * 32 + kk * 8, bd + kk * 2, kIdescS, c > 0 || kk > 0);
+              for (int kk = 0; kk < 4; ++kk) {
+                if (c * 4 + kk < 15)
+                  mma_f8_ts(tmem + kLdTmemS, tmem + c * 32 + kk * 8, bd + kk * 2, kIdescS, c > 0 || kk > 0);
+                else
+                  mma_f8_ss_plain_a(tmem + kLdTmemS, last, bd + kk * 2, kIdescS, 1u);
+              }
             } else {
 #pragma unroll
               for (int kk = 0; kk < 4; ++kk) mma_f16_ss(tmem + kLdTmemS, rotated + kk * 2, bd + kk * 2, kIdescR, 1u);
@@ -416,8 +434,9 @@ __global__ void __launch_bounds__(kLdThreads, 1) qsa_latent_decode_kernel(const 
       if (!mbar_wait_bounded(drain, 0u, kLdDrainNs)) failed = true;
     } else if (warp == kLdWeighWarp && lane == 0) {
       // O^T (+)= V^T P^T
-      const uint32_t idesc_o = idesc_e4m3(128, (mine + 15) / 16 * 16, true, false);
-      const uint32_t weights = desc_low(base_s + kLdP);
+      const uint32_t idesc_o = idesc_mxf8(128, few ? 2 * cols : cols, true, false);
+      const uint32_t ones = tmem + kLdTmemOnes, scales = tmem + kLdTmemScales;
+      const uint32_t weights = desc_low(base_s + kLdP), second = kLdPairs * 128 / 16;
       int s = 0, n = 0, seg = 0;
       while (!failed && walk.next(p)) {
 #pragma unroll 1
@@ -430,8 +449,10 @@ __global__ void __launch_bounds__(kLdThreads, 1) qsa_latent_decode_kernel(const 
             const uint32_t ad = ring + s * (kLdSlot / 16);
 #pragma unroll
             for (int kk = 0; kk < kLdTile / 32; ++kk) {
-              mma_f8_ss(tmem + kLdTmemO + c * kLdPairs, ad + kk * 256, weights + kk * 2, idesc_o, kk > 0 ? 1u : !first);
-              mma_f8_ss(tmem + kLdTmemO + c * kLdPairs, ad + kk * 256, weights + 512 + kk * 2, idesc_o, 1u);
+              const uint32_t idesc = idesc_o | kk << 4;  // the kk-th 32 tokens' scales
+              mma_mxf8_ss(tmem + kLdTmemO + c * kLdPairs, ad + kk * 256, weights + kk * 2, idesc, ones, scales, kk > 0 ? 1u : !first);
+              if (!few)
+                mma_mxf8_ss(tmem + kLdTmemO + c * kLdPairs, ad + kk * 256, weights + second + kk * 2, idesc, ones, scales, 1u);
             }
             mma_commit(empty + s);
             s = s + 1 == kLdSlots ? 0 : s + 1;
@@ -506,9 +527,9 @@ __global__ void __launch_bounds__(kLdThreads, 1) qsa_latent_decode_kernel(const 
         // both maxima of this lane, then of the row's four
         uint32_t both = max(top & 0xffffu, top >> 16) | max(rtop & 0xffffu, rtop >> 16) << 16;
         both = __vmaxu2(both, __shfl_xor_sync(0xffffffffu, both, 1));
-        if (!odd) told_f[(2 + set) * kLdPairs + pair] = __uint_as_float(both);
+        if (!odd) told_q[set * kLdPairs + pair] = __uint_as_float(both);
         bar_sync(2 + q4, 64);
-        both = __vmaxu2(both, __float_as_uint(told_f[(2 + (set ^ 1)) * kLdPairs + pair]));
+        both = __vmaxu2(both, __float_as_uint(told_q[(set ^ 1) * kLdPairs + pair]));
         const int t = (int)(both & 0xffffu), u = (int)(both >> 16);
         // 2^a takes the largest latent query into [128, 256), as far as the rotated
         // ones stay far from bf16's end
@@ -541,7 +562,13 @@ __global__ void __launch_bounds__(kLdThreads, 1) qsa_latent_decode_kernel(const 
             second[2 * i] = odd ? l0 : r0, second[2 * i + 1] = odd ? l1 : r1;
           }
           tmem_st(tmem + lane_base + 2 * set * 8 * kChunks + b * 8, first);
-          tmem_st(tmem + lane_base + (2 * set + 1) * 8 * kChunks + b * 8, second);
+          if (kChunks == 4 && b == 3 && set == 1) {
+            uint8_t* at = smem + kLdQx + (4 * q4 + (lane >> 3)) * 128 + (lane & 7) * 16;
+            *reinterpret_cast<uint4*>(at) = make_uint4(second[0], second[1], second[2], second[3]);
+            *reinterpret_cast<uint4*>(at + 2048) = make_uint4(second[4], second[5], second[6], second[7]);
+          } else {
+            tmem_st(tmem + lane_base + (2 * set + 1) * 8 * kChunks + b * 8, second);
+          }
         }
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
@@ -562,6 +589,13 @@ __global__ void __launch_bounds__(kLdThreads, 1) qsa_latent_decode_kernel(const 
       mbar_arrive(q_full);
       return qs;
     };
+    if (set == 0) {
+      const uint32_t ones[4] = {0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu};
+      tmem_st(tmem + lane_base + kLdTmemOnes, ones);
+      tmem_wait_st();
+    }
+    // the rows of P whose scales this lane's two words hold
+    const int scale0 = few && lane >= cols ? lane - cols : lane, scale1 = few ? lane : lane + 32;
     bool more = walk.next(p);
     float next_qs = 0.f;
     if (more) {
@@ -621,50 +655,62 @@ __global__ void __launch_bounds__(kLdThreads, 1) qsa_latent_decode_kernel(const 
         } else {
           mbar_arrive(s_empty);
         }
+        // the scale of this lane's 32 weights
+        uint8_t* scales = told_scales + (n & 1) * 4 * kLdPairs;
+        auto scale32 = [&]() -> float {
+          const float e = fminf(fmaxf(ceilf(top - r), kLdNear), kLdFar);
+          if (live) scales[4 * pair + quarter] = (uint8_t)(127 - (int)kLdOne + (int)e);
+          return e;
+        };
+        float e = scale32();
         // a reference that a weight passes by too much moves, and O and l with it
         const bool begun = tile > now.from;
-        if (bar_vote(1, kLdSoft, top > r + kLdLazy || failed)) {
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-          if (live && !odd) told_f[set * kLdPairs + pair] = top;
+        const float pair_top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        float2* told = told_f + (n & 1) * 2 * kLdPairs;  // of this tile, from each set: the pair's maximum and reference
+        if (live && !odd) told[set * kLdPairs + pair] = make_float2(pair_top, r);
+        if (bar_vote(1, kLdSoft, top > r + kLdFar || failed)) {
           if (begun && !failed) failed = !wait_or_abort(o_full, (uint32_t)((n - 1) & 1), abort_flag, p.wait_limit_ns);
           failed = __any_sync(0xffffffffu, failed);
           if (bar_vote(1, kLdSoft, failed)) {
             failed = true;
             break;
           }
-          if (live) top = fmaxf(top, told_f[(set ^ 1) * kLdPairs + pair]);
-          const float next = fmaxf(r, top);
-          const float f = ex2(r - next);  // 0 before the first weight
-          l *= f;
-          r = next;
-          if (live && !odd && set == 0) head_f[pair] = f;
-          bar_sync(1, kLdSoft);  // the factors are there, and what the sets told is read
+          if (live) {
+            const float next = fmaxf(r, fmaxf(pair_top, told[(set ^ 1) * kLdPairs + pair].x));
+            l *= ex2(r - next);  // 0 before the first weight
+            r = next;
+          }
           if (begun) {
             tc_fence_after();
+            // 16 pairs at a time, where one has moved; a lane works out the factor of one
 #pragma unroll 1
-            for (int c = set; c < 4 * kChunks; c += 2) {
-              // 16 pairs at a time, where one has moved
-              const int b = c % 4 * 16;
-              if (b >= mine) continue;
-              const float own_f = head_f[b + (lane & 15)];
-              if (__all_sync(0xffffffffu, own_f == 1.f)) continue;
-              const uint32_t at = tmem + lane_base + kLdTmemO + c / 4 * kLdPairs + b;
-              float x[16];
-              uint32_t y[16];
-              tmem_ld_wait<16>(at, x);
+            for (int b = 0; b < cols; b += 16) {
+              const float2 t0 = told[b + (lane & 15)], t1 = told[kLdPairs + b + (lane & 15)];
+              const float f = ex2(t0.y - fmaxf(t0.y, fmaxf(t0.x, t1.x)));
+              if (__all_sync(0xffffffffu, f == 1.f)) continue;
+#pragma unroll 1
+              for (int c = set; c < kChunks * (few ? 2 : 1); c += 2) {
+                const uint32_t at = tmem + lane_base + kLdTmemO + (few ? c / 2 : c) * kLdPairs + b + (few ? c % 2 * cols : 0);
+                float x[16];
+                uint32_t y[16];
+                tmem_ld_wait<16>(at, x);
 #pragma unroll
-              for (int j = 0; j < 16; ++j) y[j] = __float_as_uint(x[j] * head_f[b + j]);
-              tmem_st(at, y);
+                for (int j = 0; j < 16; ++j) y[j] = __float_as_uint(x[j] * __shfl_sync(0xffffffffu, f, j));
+                tmem_st(at, y);
+              }
             }
             tmem_wait_st();
             tc_fence_before();
           }
+          e = scale32();
+          bar_sync(1, kLdSoft);
         }
         // ---- weights
         uint32_t hi[8], lo[8];
         if (live) {
           const float* mi = metas[m].inv + quarter * kLdQuarter;
-          const float rb = r - kLdOne;
+          const float rb = r + (e - kLdOne);
+          float sum = 0.f;
 #pragma unroll
           for (int j = 0; j < 32; j += 4) {
             const float4 i4 = *reinterpret_cast<const float4*>(mi + j);
@@ -674,8 +720,8 @@ __global__ void __launch_bounds__(kLdThreads, 1) qsa_latent_decode_kernel(const 
             for (int i = 0; i < 4; i += 2) {
               const __nv_bfloat162 w2 = __floats2bfloat162_rn(ex2(u[j + i] - rb), ex2(u[j + i + 1] - rb));
               const float2 w = __bfloat1622float2(w2);
-              l = fmaf(w.x, ii[i], l);
-              l = fmaf(w.y, ii[i + 1], l);
+              sum = fmaf(w.x, ii[i], sum);
+              sum = fmaf(w.y, ii[i + 1], sum);
               h2[i / 2] = __nv_cvt_float2_to_fp8x2(w, __NV_SATFINITE, __NV_E4M3);
               const __half2 back(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)h2[i / 2], __NV_E4M3));
               const __half2 left = __hsub2(__floats2half2_rn(w.x, w.y), back);
@@ -684,6 +730,7 @@ __global__ void __launch_bounds__(kLdThreads, 1) qsa_latent_decode_kernel(const 
             hi[j / 4] = h2[0] | h2[1] << 16;
             lo[j / 4] = l2[0] | l2[1] << 16;
           }
+          l = fmaf(sum, ex2(e - kLdOne), l);
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(meta_empty + m);
@@ -695,9 +742,16 @@ __global__ void __launch_bounds__(kLdThreads, 1) qsa_latent_decode_kernel(const 
           for (int k = 0; k < 2; ++k) {
             uint8_t* at = smem + kLdP + sw128_offset(pair, 32 * quarter + 16 * k);
             *reinterpret_cast<uint4*>(at) = make_uint4(hi[4 * k], hi[4 * k + 1], hi[4 * k + 2], hi[4 * k + 3]);
-            *reinterpret_cast<uint4*>(at + 8192) = make_uint4(lo[4 * k], lo[4 * k + 1], lo[4 * k + 2], lo[4 * k + 3]);
+            *reinterpret_cast<uint4*>(at + lo_row * 128) = make_uint4(lo[4 * k], lo[4 * k + 1], lo[4 * k + 2], lo[4 * k + 3]);
           }
           fence_proxy_async_smem();
+        }
+        if (set == 0) {
+          const uint32_t* words = reinterpret_cast<const uint32_t*>(scales);
+          const uint32_t both[2] = {words[scale0], words[scale1]};
+          tmem_st(tmem + lane_base + kLdTmemScales, both);
+          tmem_wait_st();
+          tc_fence_before();
         }
         mbar_arrive(p_full);
       }
@@ -709,17 +763,17 @@ __global__ void __launch_bounds__(kLdThreads, 1) qsa_latent_decode_kernel(const 
       if (!failed) failed = !wait_or_abort(o_full, (uint32_t)((n - 1) & 1), abort_flag, p.wait_limit_ns);
       failed = __any_sync(0xffffffffu, failed);
       l += __shfl_xor_sync(0xffffffffu, l, 1);
-      if (live && !odd) told_f[set * kLdPairs + pair] = l;
+      if (live && !odd && set == 1) head_f[pair] = l;
       if (bar_vote(1, kLdSoft, failed)) {
         failed = true;
         break;
       }
       const int piece = 2 * group + (now.from > 0 ? 0 : 1);
       if (live && !odd && set == 0) {
-        l += told_f[kLdPairs + pair];
+        l += head_f[pair];
         head_f[pair] = l == 0.f ? 0.f : 1.0f / l;
         if (!now.whole && pair < mine)
-          p.part_lse[((int64_t)piece * p.row_tiles + rt) * kLdPairs + pair] = l == 0.f ? -INFINITY : log2f(l) + (r - kLdOne);
+          p.part_lse[((int64_t)piece * p.row_tiles + rt) * kLdPairs + pair] = l == 0.f ? -INFINITY : log2f(l) + r;
       }
       bar_sync(1, kLdSoft);
       tc_fence_after();
@@ -732,6 +786,12 @@ __global__ void __launch_bounds__(kLdThreads, 1) qsa_latent_decode_kernel(const 
           if (b >= mine) continue;
           float x[16];
           tmem_ld_wait<16>(tmem + lane_base + kLdTmemO + c / 4 * kLdPairs + b, x);
+          if (few) {
+            float y[16];
+            tmem_ld_wait<16>(tmem + lane_base + kLdTmemO + c / 4 * kLdPairs + cols + b, y);
+#pragma unroll
+            for (int j = 0; j < 16; ++j) x[j] += y[j];
+          }
           auto* out = to + (int64_t)b * kRank + c / 4 * 128;
 #pragma unroll
           for (int j = 0; j < 16; j += 4) {

@@ -60,6 +60,10 @@ __device__ __forceinline__ uint32_t desc_low(uint32_t saddr, uint32_t column_ste
   return ((saddr >> 4) & 0x3FFF) | (column_step >> 4) << 16;
 }
 
+// The same for an operand without swizzle: 8 rows of 16 bytes side by side, the
+// next 8 rows 128 bytes on, the next 16 bytes of the rows `column_step` on.
+constexpr uint32_t kDescHighPlain = (128u >> 4) | (1u << 14);
+
 // D[tmem] (+)= A B with A in tensor memory (ts) or shared memory (ss), B in shared memory.
 __device__ __forceinline__ void mma_f8_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
@@ -73,6 +77,24 @@ __device__ __forceinline__ void mma_f8_ss(uint32_t d, uint32_t a, uint32_t b, ui
       "{\n.reg .pred p;\n.reg .b64 ad, bd;\nsetp.ne.b32 p, %4, 0;\nmov.b64 ad, {%1, %5};\nmov.b64 bd, {%2, %5};\n"
       "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], ad, bd, %3, p;\n}\n" ::"r"(d), "r"(a), "r"(b), "r"(idesc),
       "r"(accumulate), "n"(kDescHigh)
+      : "memory");
+}
+__device__ __forceinline__ void mma_f8_ss_plain_a(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n.reg .pred p;\n.reg .b64 ad, bd;\nsetp.ne.b32 p, %4, 0;\nmov.b64 ad, {%1, %6};\nmov.b64 bd, {%2, %5};\n"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], ad, bd, %3, p;\n}\n" ::"r"(d), "r"(a), "r"(b), "r"(idesc),
+      "r"(accumulate), "n"(kDescHigh), "n"(kDescHighPlain)
+      : "memory");
+}
+// With a power of two for each row of A and of B (exponent + 127, a byte for each 32
+// values of K, four to a word): rows 32 c + l of an operand have theirs in lane l of
+// column c, the same in every quarter of the lanes. The byte is named by idesc.
+__device__ __forceinline__ void mma_mxf8_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t a_scales,
+                                            uint32_t b_scales, uint32_t accumulate) {
+  asm volatile(
+      "{\n.reg .pred p;\n.reg .b64 ad, bd;\nsetp.ne.b32 p, %4, 0;\nmov.b64 ad, {%1, %5};\nmov.b64 bd, {%2, %5};\n"
+      "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], ad, bd, %3, [%6], [%7], p;\n}\n" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "n"(kDescHigh), "r"(a_scales), "r"(b_scales)
       : "memory");
 }
 __device__ __forceinline__ void mma_f16_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
@@ -96,6 +118,13 @@ __host__ __device__ constexpr uint32_t idesc_f16(int m, int n, bool bf16, bool b
          ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
 
+// Instruction descriptor of kind::mxf8f6f4, E4M3 A and B, scales of 8 exponent bits;
+// B's byte of a scale word is added as byte << 4.
+__host__ __device__ constexpr uint32_t idesc_mxf8(int m, int n, bool a_mn_major, bool b_mn_major) {
+  return ((a_mn_major ? 1u : 0u) << 15) | ((b_mn_major ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | (1u << 23) |
+         ((uint32_t)(m >> 4) << 24);
+}
+
 // Consecutive 32-bit columns of a thread's lane.
 __device__ __forceinline__ void tmem_st(uint32_t taddr, const uint32_t (&v)[8]) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};\n" ::"r"(taddr), "r"(v[0]), "r"(v[1]),
@@ -108,6 +137,14 @@ __device__ __forceinline__ void tmem_st(uint32_t taddr, const uint32_t (&v)[16])
 }
 __device__ __forceinline__ void tmem_st(uint32_t taddr, const uint32_t (&v)[32]) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};\n" ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
+               : "memory");
+}
+__device__ __forceinline__ void tmem_st(uint32_t taddr, const uint32_t (&v)[2]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x2.b32 [%0], {%1,%2};\n" ::"r"(taddr), "r"(v[0]), "r"(v[1]) : "memory");
+}
+__device__ __forceinline__ void tmem_st(uint32_t taddr, const uint32_t (&v)[4]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1,%2,%3,%4};\n" ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]),
+               "r"(v[3])
                : "memory");
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory"); }
