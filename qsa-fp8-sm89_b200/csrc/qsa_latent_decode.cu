@@ -261,7 +261,7 @@ __global__ void __launch_bounds__(kLdThreads, 1) qsa_latent_decode_kernel(const 
   __syncthreads();
   launch_dependents();
   tc_fence_after();
-  const uint32_t tmem = *tmem_at;
+  constexpr uint32_t tmem = 0;  // all of it is this block's
   LdWalk walk;
   walk.row = begin[0], walk.from = begin[1], walk.left = share[1];
   bool failed = false;
@@ -387,14 +387,13 @@ __global__ void __launch_bounds__(kLdThreads, 1) qsa_latent_decode_kernel(const 
     asm volatile("setmaxnreg.dec.sync.aligned.u32 96;\n");
     const uint32_t ring = desc_low(base_s + kLdRing);  // K: tokens by bytes (V^T: the same, MN-major)
     auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
-      if (!wait_or_abort(bar, parity, abort_flag, p.wait_limit_ns)) return false;
+      if (!__all_sync(0xffffffffu, wait_or_abort(bar, parity, abort_flag, p.wait_limit_ns))) return false;
       tc_fence_after();
       return true;
     };
-    // Scores and weighted sums are issued by a thread each: a wait costs a thread
-    // some 200 cycles even where there is nothing to wait for, in which the other's
+    // Scores and weighted sums are issued by a warp each: a wait costs some 200 cycles even where there is nothing to wait for, in which the other's
     // products go on.
-    if (warp == kLdMmaWarp && lane == 0) {
+    if (warp == kLdMmaWarp) {
       // S = Q K^T
       constexpr uint32_t kIdescS = idesc_e4m3(128, kLdTile, false, false);
       constexpr uint32_t kIdescR = idesc_f16(128, kLdTile, true, false);
@@ -421,8 +420,8 @@ __global__ void __launch_bounds__(kLdThreads, 1) qsa_latent_decode_kernel(const 
             } else {
 #pragma unroll
               for (int kk = 0; kk < 4; ++kk) mma_f16_ss(tmem + kLdTmemS, rotated + kk * 2, bd + kk * 2, kIdescR, 1u);
-              mma_commit(s_full);
-              mma_commit(empty + s);
+              warp_commit(s_full);
+              warp_commit(empty + s);
             }
             s = s + 1 == kLdSlots ? 0 : s + 1;
           }
@@ -430,9 +429,9 @@ __global__ void __launch_bounds__(kLdThreads, 1) qsa_latent_decode_kernel(const 
         ++seg;
         walk.advance();
       }
-      mma_commit(drain);
+      warp_commit(drain);
       if (!mbar_wait_bounded(drain, 0u, kLdDrainNs)) failed = true;
-    } else if (warp == kLdWeighWarp && lane == 0) {
+    } else if (warp == kLdWeighWarp) {
       // O^T (+)= V^T P^T
       const uint32_t idesc_o = idesc_mxf8(128, few ? 2 * cols : cols, true, false);
       const uint32_t ones = tmem + kLdTmemOnes, scales = tmem + kLdTmemScales;
@@ -454,16 +453,16 @@ __global__ void __launch_bounds__(kLdThreads, 1) qsa_latent_decode_kernel(const 
               if (!few)
                 mma_mxf8_ss(tmem + kLdTmemO + c * kLdPairs, ad + kk * 256, weights + second + kk * 2, idesc, ones, scales, 1u);
             }
-            mma_commit(empty + s);
+            warp_commit(empty + s);
             s = s + 1 == kLdSlots ? 0 : s + 1;
           }
-          mma_commit(o_full);
+          warp_commit(o_full);
           s = s + 1 == kLdSlots ? 0 : s + 1;  // the rotated part's
         }
         ++seg;
         walk.advance();
       }
-      mma_commit(drain + 1);
+      warp_commit(drain + 1);
       if (!mbar_wait_bounded(drain + 1, 0u, kLdDrainNs)) failed = true;
     } else if (warp == kLdFenceWarp && lane == 0) {
       // The copies wrote by one path to shared memory and the products read by

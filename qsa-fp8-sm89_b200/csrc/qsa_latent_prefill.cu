@@ -187,7 +187,7 @@ __global__ void __launch_bounds__(kLpThreads, 1)
   __syncwarp();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_at;
+  constexpr uint32_t tmem = 0;  // all of it is this block's
   const LpBlock b = *found;
   bool failed = false;
   // keys that tile t's last query sees, in tiles of 128
@@ -246,12 +246,12 @@ __global__ void __launch_bounds__(kLpThreads, 1)
       }
       for (int f = max(fix_tiles - 2, 0); f < fix_tiles; ++f)
         if (!mbar_wait_bounded(v_full + f % 2, (uint32_t)((f / 2) & 1), kLpDrainNs)) failed = true;
-    } else if (warp == kLpMmaWarp && lane == 0 && nk > 0) {
+    } else if (warp == kLpMmaWarp && nk > 0) {
       // ============================== products ==============================
       constexpr uint32_t kIdescS = idesc_f16(128, kLpTile, kBf16, false);
       constexpr uint32_t kIdescO = idesc_f16(128, 64, kBf16, true);
       auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
-        if (!wait_or_abort(bar, parity, abort_flag, p.wait_limit_ns)) return false;
+        if (!__all_sync(0xffffffffu, wait_or_abort(bar, parity, abort_flag, p.wait_limit_ns))) return false;
         tc_fence_after();
         return true;
       };
@@ -267,9 +267,9 @@ __global__ void __launch_bounds__(kLpThreads, 1)
 #pragma unroll
           for (int kk = 0; kk < 4; ++kk)
             mma_f16_ss(tmem + kLpTmemS + t * 128, a0 + kk * 2, b0 + kk * 2, kIdescS, kk > 0 ? 1u : c > 0);
-          if (last) mma_commit(empty + pos % kLpSlots);
+          if (last) warp_commit(empty + pos % kLpSlots);
         }
-        mma_commit(s_full + t);
+        warp_commit(s_full + t);
         return true;
       };
       auto weigh = [&](int t, int j) -> bool {  // O_t += P_t V(j)
@@ -285,9 +285,9 @@ __global__ void __launch_bounds__(kLpThreads, 1)
           for (int kk = 0; kk < 8; ++kk)
             mma_f16_ts(tmem + kLpTmemO + t * 128 + c * 64, tmem + kLpTmemS + t * 128 + kk * 8, b0 + kk * 128, kIdescO,
                        kk > 0 ? 1u : j > 0);
-          if (last) mma_commit(empty + pos % kLpSlots);
+          if (last) warp_commit(empty + pos % kLpSlots);
         }
-        mma_commit(o_full + t);
+        warp_commit(o_full + t);
         return true;
       };
       for (int t = 0; t < 2 && !failed; ++t)
@@ -299,7 +299,7 @@ __global__ void __launch_bounds__(kLpThreads, 1)
           const int tiles = t == 0 ? nk0 : nk1;
           if (j < tiles) failed = !weigh(t, j) || (j + 1 < tiles && !scores(t, j + 1));
         }
-      mma_commit(drain);
+      warp_commit(drain);
       if (!mbar_wait_bounded(drain, 0u, kLpDrainNs)) failed = true;
     } else if (warp >= kLpFixWarp) {
       // ====================== values that must not count ====================

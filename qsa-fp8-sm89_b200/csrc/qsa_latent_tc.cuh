@@ -64,51 +64,59 @@ __device__ __forceinline__ uint32_t desc_low(uint32_t saddr, uint32_t column_ste
 // next 8 rows 128 bytes on, the next 16 bytes of the rows `column_step` on.
 constexpr uint32_t kDescHighPlain = (128u >> 4) | (1u << 14);
 
-// D[tmem] (+)= A B with A in tensor memory (ts) or shared memory (ss), B in shared memory.
+// D[tmem] (+)= A B with A in tensor memory (ts) or shared memory (ss), B in shared
+// memory. A whole warp calls these, with the same arguments, and one lane issues: the
+// operands then stay in uniform registers, and a product takes 40 cycles to issue
+// instead of 50 (64 rows of B at most; with 128 the product itself takes 64).
 __device__ __forceinline__ void mma_f8_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n.reg .pred p;\n.reg .b64 bd;\nsetp.ne.b32 p, %4, 0;\nmov.b64 bd, {%2, %5};\n"
-      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], [%1], bd, %3, p;\n}\n" ::"r"(d), "r"(a), "r"(b), "r"(idesc),
-      "r"(accumulate), "n"(kDescHigh)
-      : "memory");
-}
-__device__ __forceinline__ void mma_f8_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n.reg .pred p;\n.reg .b64 ad, bd;\nsetp.ne.b32 p, %4, 0;\nmov.b64 ad, {%1, %5};\nmov.b64 bd, {%2, %5};\n"
-      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], ad, bd, %3, p;\n}\n" ::"r"(d), "r"(a), "r"(b), "r"(idesc),
+      "{\n.reg .pred p, e;\nelect.sync _|e, 0xffffffff;\nsetp.ne.b32 p, %4, 0;\n"
+      ".reg .b64 bd;\nmov.b64 bd, {%2, %5};\n"
+      "@e tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], [%1], bd, %3, p;\n}\n" ::"r"(d), "r"(a), "r"(b), "r"(idesc),
       "r"(accumulate), "n"(kDescHigh)
       : "memory");
 }
 __device__ __forceinline__ void mma_f8_ss_plain_a(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n.reg .pred p;\n.reg .b64 ad, bd;\nsetp.ne.b32 p, %4, 0;\nmov.b64 ad, {%1, %6};\nmov.b64 bd, {%2, %5};\n"
-      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], ad, bd, %3, p;\n}\n" ::"r"(d), "r"(a), "r"(b), "r"(idesc),
+      "{\n.reg .pred p, e;\nelect.sync _|e, 0xffffffff;\nsetp.ne.b32 p, %4, 0;\n"
+      ".reg .b64 ad, bd;\nmov.b64 ad, {%1, %6};\nmov.b64 bd, {%2, %5};\n"
+      "@e tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], ad, bd, %3, p;\n}\n" ::"r"(d), "r"(a), "r"(b), "r"(idesc),
       "r"(accumulate), "n"(kDescHigh), "n"(kDescHighPlain)
-      : "memory");
-}
-// With a power of two for each row of A and of B (exponent + 127, a byte for each 32
-// values of K, four to a word): rows 32 c + l of an operand have theirs in lane l of
-// column c, the same in every quarter of the lanes. The byte is named by idesc.
-__device__ __forceinline__ void mma_mxf8_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t a_scales,
-                                            uint32_t b_scales, uint32_t accumulate) {
-  asm volatile(
-      "{\n.reg .pred p;\n.reg .b64 ad, bd;\nsetp.ne.b32 p, %4, 0;\nmov.b64 ad, {%1, %5};\nmov.b64 bd, {%2, %5};\n"
-      "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], ad, bd, %3, [%6], [%7], p;\n}\n" ::"r"(d),
-      "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "n"(kDescHigh), "r"(a_scales), "r"(b_scales)
       : "memory");
 }
 __device__ __forceinline__ void mma_f16_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n.reg .pred p;\n.reg .b64 bd;\nsetp.ne.b32 p, %4, 0;\nmov.b64 bd, {%2, %5};\n"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], bd, %3, p;\n}\n" ::"r"(d), "r"(a), "r"(b), "r"(idesc),
+      "{\n.reg .pred p, e;\nelect.sync _|e, 0xffffffff;\nsetp.ne.b32 p, %4, 0;\n"
+      ".reg .b64 bd;\nmov.b64 bd, {%2, %5};\n"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], bd, %3, p;\n}\n" ::"r"(d), "r"(a), "r"(b), "r"(idesc),
       "r"(accumulate), "n"(kDescHigh)
       : "memory");
 }
 __device__ __forceinline__ void mma_f16_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n.reg .pred p;\n.reg .b64 ad, bd;\nsetp.ne.b32 p, %4, 0;\nmov.b64 ad, {%1, %5};\nmov.b64 bd, {%2, %5};\n"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], ad, bd, %3, p;\n}\n" ::"r"(d), "r"(a), "r"(b), "r"(idesc),
+      "{\n.reg .pred p, e;\nelect.sync _|e, 0xffffffff;\nsetp.ne.b32 p, %4, 0;\n"
+      ".reg .b64 ad, bd;\nmov.b64 ad, {%1, %5};\nmov.b64 bd, {%2, %5};\n"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], ad, bd, %3, p;\n}\n" ::"r"(d), "r"(a), "r"(b), "r"(idesc),
       "r"(accumulate), "n"(kDescHigh)
+      : "memory");
+}
+// With a power of two for each row of A and of B (exponent + 127, a byte for each 32
+// values of K, four to a word): rows 32 c + l of an operand have theirs in lane l of
+// column c, the same in every quarter of the lanes. The byte is named by idesc.
+__device__ __forceinline__ void mma_mxf8_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t a_scales, uint32_t b_scales,
+                                            uint32_t accumulate) {
+  asm volatile(
+      "{\n.reg .pred p, e;\nelect.sync _|e, 0xffffffff;\nsetp.ne.b32 p, %4, 0;\n"
+      ".reg .b64 ad, bd;\nmov.b64 ad, {%1, %5};\nmov.b64 bd, {%2, %5};\n"
+      "@e tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], ad, bd, %3, [%6], [%7], p;\n}\n" ::"r"(d), "r"(a), "r"(b), "r"(idesc),
+      "r"(accumulate), "n"(kDescHigh), "r"(a_scales), "r"(b_scales)
+      : "memory");
+}
+// Arrives once on `bar` when every product that the warp issued so far is done.
+__device__ __forceinline__ void warp_commit(uint64_t* bar) {
+  asm volatile(
+      "{\n.reg .pred e;\nelect.sync _|e, 0xffffffff;\n"
+      "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(smem_u32(bar))
       : "memory");
 }
 
