@@ -5,12 +5,12 @@
 //
 // A row's (node, head) pairs share every token, 64 of them a CTA, so that the
 // tokens are an operand of large tensor-core products and are fetched once:
-//   S   = Q K^T     128 lanes x 128 tokens. Q lies in tensor memory as two
+//   S   = Q K^T     128 lanes x 64 tokens. Q lies in tensor memory as two
 //                   E4M3 terms a value, q 2^a = t0 + t1 / 16, in neighbouring
 //                   lanes: a product of codes with codes needs no conversion of
 //                   the cache, and a warp's lane pair has both terms' scores of
 //                   one head: a shuffle joins them, and each lane goes on with
-//                   half of the warp's tokens. The rotated part is a bf16 product
+//                   32 of the tokens. The rotated part is a bf16 product
 //                   into the same accumulator (q 2^a exact in bf16, zeros in the
 //                   lanes of the second terms).
 //   O^T = V^T P^T   128 values of the latent x 64 pairs, four times for a rank of
@@ -28,15 +28,18 @@
 // small weights add up to beside a few large ones (E4M3 ends at 2^-9). The sum of
 // weights takes the bf16 value, so that most of this rounding cancels in the
 // quotient: l = sum w_t / s_t, in fp32; scales within 2^-60 .. 2^60 keep it in range.
+// (The conversions to E4M3 share a unit with 2^x that they kept 94 % busy: the terms
+// are cut out of the fp32 weights by integer operations instead.)
 // r is the largest score + log2 s of the first tile that has one. It moves, and O
-// with it, only when a tile passes it by 2^60.
+// with it, only when a tile passes it by 2^60; each set tells the other its r, tile
+// by tile.
 //
-// Warps: four loaders bring 128-token tiles, 128 bytes of each token at a
-// time, into a ring of 16 KiB slots by cp.async (gathered rows in the 128-byte
-// swizzle that the matrix unit reads); two issue the products; eight do the
-// softmax and the results, two for each quarter of the lanes, with half of the
-// tokens each. The product of scores of tile i + 1 runs while tile i's softmax
-// does, and P V of tile i after it.
+// Tiles of 64 tokens go in turn to two sets of warps, each with a ring, scores and
+// weights of its own, so that one set's softmax runs beside the other's and beside
+// the products. A set is two loaders, which bring a tile 128 bytes of each token at a
+// time into 8 KiB slots by cp.async (gathered rows, in the 128-byte swizzle that the
+// matrix unit reads), and four softmax warps. One warp issues the products of scores
+// and one those of weights, of both sets, in the tiles' order.
 //
 // Work: group g of CTAs (one CTA for each 64 pairs of a row, so that the CTAs that
 // read the same tokens run side by side) has an even share of all rows' tiles: at
@@ -54,44 +57,49 @@ namespace qsa {
 namespace {
 
 constexpr int kLdPairs = 64;     // (node, head) pairs of a CTA
-constexpr int kLdTile = 128;     // tokens of a tile
+constexpr int kLdTile = 64;      // tokens of a tile
 constexpr int kLdSlot = kLdTile * 128;
-constexpr int kLdSlots = 11;
+constexpr int kLdSlots = 11;     // of a set's ring
 constexpr int kLdMeta = 4;       // tiles whose scales are held
-constexpr int kLdSoft = 256;     // threads of the softmax
+constexpr int kLdReady = 16;     // tiles that may be ready at once: a ring holds 5 of two pieces each
+constexpr int kLdSoft = 256;     // threads of the softmax, half of them in each set
 constexpr int kLdLoader0 = 8, kLdMmaWarp = 12, kLdFenceWarp = 13, kLdWeighWarp = 14;
-// Four warpgroups: two of softmax, loaders, and the warps of the two products and of
-// the fence with an idle one. The softmax takes registers that the others hand back: 2 x 160 + 96 +
-// 96 of the 4 x 128 that the block is launched with.
+// Four warpgroups: a set's softmax each, loaders, and the warps of the two products and
+// of the fence with an idle one. The softmax takes registers that the others hand back:
+// 2 x 160 + 96 + 96 of the 4 x 128 that the block is launched with.
 constexpr int kLdThreads = 512;
-constexpr int64_t kLdDirectTiles = 4;  // tiles of a row that is not split
+constexpr int64_t kLdDirectTiles = 8;  // tiles of a row that is not split
 constexpr float kLdOne = 8.f;    // log2 that bounds the largest weight of 32
 constexpr float kLdFar = 60.f;   // log2 by which a weight may pass the reference
 constexpr float kLdNear = -110.f;  // log2 below it under which 32 weights get no smaller scale
 constexpr float kLowest = -3.402823466e38f;
 constexpr uint64_t kLdDrainNs = 1000000000ull;
 
-// Scales of a tile: s, log2 s, 1 / s, each in four quarters of 32 tokens. A lane
-// pair reads two of them at once, apart by a bank group.
-constexpr int kLdQuarter = 36;
+// Scales of a tile: s, log2 s, 1 / s, in two halves of 32 tokens that a lane pair
+// reads at once, apart by a bank group.
+constexpr int kLdHalf = 36;
 struct LdMeta {
-  float s[4 * kLdQuarter], lg[4 * kLdQuarter], inv[4 * kLdQuarter];
+  float s[2 * kLdHalf], lg[2 * kLdHalf], inv[2 * kLdHalf];
 };
 
-constexpr int kLdQr = 0;                           // rotated queries: 128 rows of 64 bf16
-constexpr int kLdP = kLdQr + 16384;                // weights: two terms of 64 rows of 128 tokens
-constexpr int kLdRing = kLdP + 16384;
-constexpr int kLdMetaAt = kLdRing + kLdSlots * kLdSlot;
-constexpr int kLdRow = kLdMetaAt + kLdMeta * (int)sizeof(LdMeta);  // float [64]: factors of pairs
-constexpr int kLdShare = kLdRow + kLdPairs * 4;                    // what the two sets of warps tell: float2 [2 tiles][2][64], float [2][64] of queries
-constexpr int kLdScales = kLdShare + 4 * kLdPairs * 8 + 2 * kLdPairs * 4;  // bytes [2 tiles][64][4 x 32 tokens]
-constexpr int kLdQx = kLdScales + 2 * kLdPairs * 4;                        // a rank of 512: the last 32 values of Q
-constexpr int kLdBars = kLdQx + 4096;
-constexpr int kLdReady = 4;      // tiles that may be ready at once
-constexpr int kLdNumBars = 2 * kLdSlots + kLdReady + 2 * kLdMeta + 8;
+// Named barriers: of a set, of both, and of a quarter of the lanes' two warps.
+constexpr int kLdBarSet = 1, kLdBarAll = 3, kLdBarQuarter = 4;
+
+constexpr int kLdQr = 0;                // rotated queries: 128 rows of 64 bf16
+constexpr int kLdP = kLdQr + 16384;     // weights: two terms of 64 rows of 64 tokens of either set
+constexpr int kLdRing = kLdP + 16384;   // [2 sets][kLdSlots]
+constexpr int kLdQx = kLdRing + 2 * kLdSlots * kLdSlot;            // a rank of 512: the last 32 values of Q
+constexpr int kLdMetaAt = kLdQx + 4096;
+constexpr int kLdRow = kLdMetaAt + kLdMeta * (int)sizeof(LdMeta);  // float [64]: factors of pairs at a segment's end
+constexpr int kLdRef = kLdRow + kLdPairs * 4;                      // float [64]: r
+constexpr int kLdMove = kLdRef + kLdPairs * 4;                     // float [2 sets][64]: factors of a moving r
+constexpr int kLdTold = kLdMove + 2 * kLdPairs * 4;                // uint32 [2 sets][64]: maxima of queries
+constexpr int kLdScales = kLdTold + 2 * kLdPairs * 4;              // bytes [2 sets][2 tiles][64][4], of 32 tokens each
+constexpr int kLdBars = kLdScales + 4 * kLdPairs * 4;
+constexpr int kLdNumBars = 4 * kLdSlots + 2 * kLdMeta + kLdReady + 16;
 constexpr int kLdMisc = kLdBars + kLdNumBars * 8;  // tensor memory address, abort flag, group's range
 constexpr int kLdSmem = kLdMisc + 64 + 1024;
-static_assert(kLdSmem <= 232448 && kLdBars % 8 == 0 && kLdMisc % 8 == 0 && kLdMetaAt % 16 == 0, "shared memory");
+static_assert(kLdSmem + 256 <= 232448 && kLdBars % 8 == 0 && kLdMisc % 8 == 0 && kLdMetaAt % 16 == 0, "shared memory");
 
 // Columns of tensor memory: Q from 0, up to 120 (of a rank of 512 the last 32 values,
 // which would take 8 more, lie in shared memory), the scales of V^T (ones) and P.
@@ -141,6 +149,19 @@ __device__ __forceinline__ uint32_t ld_seen_word(const LatentDecodeParams& p, in
   return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u;
 }
 
+// The maximum, NaN where there is one.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;\n" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+// Bits 20 to 27 of four words as the bytes of one.
+__device__ __forceinline__ uint32_t pack_codes(const uint32_t (&x)[4]) {
+  const uint32_t even = __byte_perm(x[0], x[2], 0x7632), odd = __byte_perm(x[1], x[3], 0x7632);
+  return ((even >> 4) & 0x00ff00ffu) | ((odd << 4) & 0xff00ff00u);
+}
+
 // kChunks: 128-byte pieces of a token's codes.
 template <int kChunks>
 __global__ void __launch_bounds__(kLdThreads, 1) qsa_latent_decode_kernel(const __grid_constant__ LatentDecodeParams p) {
@@ -152,27 +173,27 @@ __global__ void __launch_bounds__(kLdThreads, 1) qsa_latent_decode_kernel(const 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kLdBars);
-  uint64_t* full = bars;                       // [slots] loaders -> fence
-  uint64_t* empty = full + kLdSlots;           // [slots] products -> loaders
-  uint64_t* meta_full = empty + kLdSlots;      // [kLdMeta] loaders -> softmax
+  uint64_t* full = bars;                       // [2 sets][slots] loaders -> fence
+  uint64_t* empty = full + 2 * kLdSlots;       // [2 sets][slots] products -> loaders
+  uint64_t* meta_full = empty + 2 * kLdSlots;  // [kLdMeta] loaders -> softmax
   uint64_t* meta_empty = meta_full + kLdMeta;  // [kLdMeta] softmax -> loaders
-  uint64_t* q_full = meta_empty + kLdMeta;     // softmax -> products, each segment
-  uint64_t* s_full = q_full + 1;               // products -> softmax
-  uint64_t* s_empty = s_full + 1;              // softmax -> products
-  uint64_t* p_full = s_empty + 1;              // softmax -> products
-  uint64_t* o_full = p_full + 1;               // products -> softmax
-  uint64_t* o_empty = o_full + 1;              // results taken -> products, each segment
-  uint64_t* ready = o_empty + 1;               // [kLdReady] fence -> products, each tile
-  uint64_t* drain = ready + kLdReady;          // [2]
+  uint64_t* ready = meta_empty + kLdMeta;      // [kLdReady] fence -> products, each tile
+  uint64_t* s_full = ready + kLdReady;         // [2 sets] products -> softmax
+  uint64_t* s_empty = s_full + 2;              // [2 sets] softmax -> products
+  uint64_t* p_full = s_empty + 2;              // [2 sets] softmax -> products
+  uint64_t* o_full = p_full + 2;               // [2 sets] products -> softmax
+  uint64_t* r_done = o_full + 2;               // [2 sets] softmax -> the other set's
+  uint64_t* q_full = r_done + 2;               // softmax -> products, each segment
+  uint64_t* o_done = q_full + 1;               // products -> softmax, each segment
+  uint64_t* o_empty = o_done + 1;              // results taken -> products, each segment
+  uint64_t* drain = o_empty + 1;               // [2]
   uint32_t* tmem_at = reinterpret_cast<uint32_t*>(smem + kLdMisc);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + kLdMisc + 8);
-  int* begin = reinterpret_cast<int*>(smem + kLdMisc + 16);                 // row, tile
-  int64_t* share = reinterpret_cast<int64_t*>(smem + kLdMisc + 24);         // first unit, units
+  int* begin = reinterpret_cast<int*>(smem + kLdMisc + 16);          // row, tile
+  int64_t* share = reinterpret_cast<int64_t*>(smem + kLdMisc + 24);  // first unit, units
   LdMeta* metas = reinterpret_cast<LdMeta*>(smem + kLdMetaAt);
   float* head_f = reinterpret_cast<float*>(smem + kLdRow);
-  float2* told_f = reinterpret_cast<float2*>(smem + kLdShare);
-  uint8_t* told_scales = smem + kLdScales;
-  float* told_q = reinterpret_cast<float*>(smem + kLdShare + 4 * kLdPairs * 8);
+  float* pair_r = reinterpret_cast<float*>(smem + kLdRef);
 
   const int rt = (int)(blockIdx.x % p.row_tiles), group = (int)(blockIdx.x / p.row_tiles);
   const int pairs = p.nodes * p.heads;
@@ -185,16 +206,20 @@ __global__ void __launch_bounds__(kLdThreads, 1) qsa_latent_decode_kernel(const 
   const int lo_row = few ? cols : kLdPairs;          // where the second terms' rows of P begin
 
   if (tid == 0) {
-    for (int i = 0; i < kLdSlots; ++i) mbar_init(full + i, 128), mbar_init(empty + i, 1);
-    for (int i = 0; i < kLdMeta; ++i) mbar_init(meta_full + i, 4), mbar_init(meta_empty + i, kLdSoft / 32);
-    mbar_init(q_full, kLdSoft);
-    mbar_init(s_full, 1);
-    mbar_init(s_empty, kLdSoft);
-    mbar_init(p_full, kLdSoft);
-    mbar_init(o_full, 1);
-    mbar_init(o_empty, kLdSoft);
+    for (int i = 0; i < 2 * kLdSlots; ++i) mbar_init(full + i, 64), mbar_init(empty + i, 1);
+    for (int i = 0; i < kLdMeta; ++i) mbar_init(meta_full + i, 2), mbar_init(meta_empty + i, 4);
     for (int i = 0; i < kLdReady; ++i) mbar_init(ready + i, 1);
-    for (int i = 0; i < 2; ++i) mbar_init(drain + i, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(s_full + i, 1);
+      mbar_init(s_empty + i, kLdSoft / 2);
+      mbar_init(p_full + i, kLdSoft / 2);
+      mbar_init(o_full + i, 1);
+      mbar_init(r_done + i, 4);
+      mbar_init(drain + i, 1);
+    }
+    mbar_init(q_full, kLdSoft);
+    mbar_init(o_done, 1);
+    mbar_init(o_empty, kLdSoft);
     *abort_flag = 0;
     fence_mbar_init();
   }
@@ -269,12 +294,14 @@ __global__ void __launch_bounds__(kLdThreads, 1) qsa_latent_decode_kernel(const 
   if (warp >= kLdLoader0 && warp < kLdMmaWarp) {
     // =============================== loaders ================================
     asm volatile("setmaxnreg.dec.sync.aligned.u32 96;\n");
-    // Warp w has tokens 32w .. 32w + 31 of every tile: a lane looks up its own
+    // Two warps a set, 32 tokens of each of its tiles each: a lane looks up its own
     // token, and 8 lanes fetch a token's 128 bytes.
-    const int w = warp - kLdLoader0;
+    const int w = warp - kLdLoader0, set = w >> 1;
     const int piece = lane & 7, sub = lane >> 3;
-    const int tok = 32 * w + lane;  // the lane's own token
+    const int tok = 32 * (w & 1) + lane;  // the lane's own token
     const int first_node = rt * kLdPairs / p.heads, last_node = (rt * kLdPairs + mine - 1) / p.heads;
+    uint64_t* const my_full = full + set * kLdSlots;
+    uint64_t* const my_empty = empty + set * kLdSlots;
     int issued = 0, tile_n = 0;
     auto wait_free = [&](uint64_t* bar, uint32_t parity) -> bool {
       return __all_sync(0xffffffffu, wait_or_abort(bar, parity, abort_flag, p.wait_limit_ns));
@@ -287,7 +314,7 @@ __global__ void __launch_bounds__(kLdThreads, 1) qsa_latent_decode_kernel(const 
       const int own = p.nodes > 1 ? count - p.nodes : 0x7fffffff;
       {  // the queries, which the softmax will load, into L2
         const char* q = reinterpret_cast<const char*>(p.q + ((int64_t)row * pairs + rt * kLdPairs) * (kRank + kLatentRope));
-        for (int i = tok; i < mine * (kRank + kLatentRope) * 2 / 128; i += 128)
+        for (int i = 32 * w + lane; i < mine * (kRank + kLatentRope) * 2 / 128; i += 128)
           asm volatile("prefetch.global.L2 [%0];\n" ::"l"(q + i * 128));
       }
       // A token's lookup is three loads in a row (its index, its page, its scale):
@@ -320,28 +347,31 @@ __global__ void __launch_bounds__(kLdThreads, 1) qsa_latent_decode_kernel(const 
         return x.page >= 0 && x.page < p.cache.num_pages ? x.page * p.cache.page_size + x.off : -1;
       };
       auto scale_of = [&](int slot) -> float { return slot >= 0 ? __ldg(p.cache.scales + slot) : 0.f; };
-      const int t0 = token(walk.from), t1 = token(walk.from + 1);
-      int ahead = token(walk.from + 2);
+      // this set's tiles: every other one
+      const int begin_at = walk.from + ((set ^ tile_n) & 1);
+      const int t0 = token(begin_at), t1 = token(begin_at + 2);
+      int ahead = token(begin_at + 4);
       const Page p0 = find(t0);
       Page page = find(t1);
       int slot = slot_of(p0);
       float scale = scale_of(slot);
 #pragma unroll 1
-      for (int tile = walk.from; tile < walk.to; ++tile, ++tile_n) {
+      for (int tile = begin_at; tile < walk.to; tile += 2) {
+        const int n = tile_n + tile - walk.from;
         const int next_slot = slot_of(page);
         const float next_scale = scale_of(next_slot);
         page = find(ahead);
-        ahead = token(tile + 3);
+        ahead = token(tile + 6);
         int from[8];
 #pragma unroll
         for (int k = 0; k < 8; ++k) from[k] = __shfl_sync(0xffffffffu, slot, 4 * k + sub);
-        // row of pass k: 32 w + 4 k + sub, so its swizzle is (4 (k & 1) + sub)'s
-        const uint32_t dst0 = base_s + kLdRing + (32 * w + sub) * 128;
+        // row of pass k: 32 (w & 1) + 4 k + sub, so its swizzle is (4 (k & 1) + sub)'s
+        const uint32_t dst0 = base_s + kLdRing + set * kLdSlots * kLdSlot + (32 * (w & 1) + sub) * 128;
         const uint32_t even = (uint32_t)(piece ^ sub) << 4, odd = (uint32_t)(piece ^ (4 + sub)) << 4;
 #pragma unroll 1
         for (int c = 0; c <= kChunks; ++c) {
           const int s = issued % kLdSlots;
-          if (issued >= kLdSlots && !wait_free(empty + s, (uint32_t)((issued / kLdSlots - 1) & 1))) {
+          if (issued >= kLdSlots && !wait_free(my_empty + s, (uint32_t)((issued / kLdSlots - 1) & 1))) {
             failed = true;
             break;
           }
@@ -351,16 +381,16 @@ __global__ void __launch_bounds__(kLdThreads, 1) qsa_latent_decode_kernel(const 
           for (int k = 0; k < 8; ++k)
             cp_async_16(dst0 + s * kLdSlot + k * 512 + (k & 1 ? odd : even), src + (int64_t)max(from[k], 0) * stride,
                         from[k] < 0 ? 0u : 16u);
-          cp_async_mbar_arrive_noinc(smem_u32(full + s));
+          cp_async_mbar_arrive_noinc(smem_u32(my_full + s));
           ++issued;
         }
-        const int m = tile_n % kLdMeta;
-        if (failed || (tile_n >= kLdMeta && !wait_free(meta_empty + m, (uint32_t)((tile_n / kLdMeta - 1) & 1)))) {
+        const int m = n % kLdMeta;
+        if (failed || (n >= kLdMeta && !wait_free(meta_empty + m, (uint32_t)((n / kLdMeta - 1) & 1)))) {
           failed = true;
           break;
         }
         {
-          const int at = (tok >> 5) * kLdQuarter + (tok & 31);
+          const int at = (w & 1) * kLdHalf + lane;
           const float s = slot < 0 ? 0.f : scale != scale ? scale : fminf(fmaxf(scale, kLatentLeastScale), kLatentMostScale);
           metas[m].s[at] = s;
           metas[m].lg[at] = slot < 0 ? -INFINITY : log2f(s);
@@ -372,6 +402,7 @@ __global__ void __launch_bounds__(kLdThreads, 1) qsa_latent_decode_kernel(const 
         slot = next_slot;
         scale = next_scale;
       }
+      tile_n += walk.to - walk.from;
       walk.advance();
     }
     cp_async_wait_all();
@@ -398,33 +429,37 @@ __global__ void __launch_bounds__(kLdThreads, 1) qsa_latent_decode_kernel(const 
       constexpr uint32_t kIdescS = idesc_e4m3(128, kLdTile, false, false);
       constexpr uint32_t kIdescR = idesc_f16(128, kLdTile, true, false);
       const uint32_t rotated = desc_low(base_s + kLdQr), last = desc_low(base_s + kLdQx, 2048);
-      int s = 0, n = 0, seg = 0;  // ring slot, tile, segment
+      int slot[2] = {0, 0}, n = 0, seg = 0;  // ring slots, tile, segment
       while (!failed && walk.next(p)) {
         failed = !wait(q_full, (uint32_t)(seg & 1));
 #pragma unroll 1
         for (int tile = walk.from; tile < walk.to && !failed; ++tile, ++n) {
+          const int set = n & 1;
           failed = !wait(ready + n % kLdReady, (uint32_t)((n / kLdReady) & 1)) ||
-                   (n > 0 && !wait(s_empty, (uint32_t)((n - 1) & 1)));
+                   (n >= 2 && !wait(s_empty + set, (uint32_t)(((n >> 1) - 1) & 1)));
           if (failed) break;
+          const uint32_t d = tmem + kLdTmemS + set * kLdTile;
+          int s = set ? slot[1] : slot[0];
 #pragma unroll
           for (int c = 0; c <= kChunks; ++c) {
-            const uint32_t bd = ring + s * (kLdSlot / 16);
+            const uint32_t bd = ring + (set * kLdSlots + s) * (kLdSlot / 16);
             if (c < kChunks) {
 #pragma unroll
               for (int kk = 0; kk < 4; ++kk) {
                 if (c * 4 + kk < 15)
-                  mma_f8_ts(tmem + kLdTmemS, tmem + c * 32 + kk * 8, bd + kk * 2, kIdescS, c > 0 || kk > 0);
+                  mma_f8_ts(d, tmem + c * 32 + kk * 8, bd + kk * 2, kIdescS, c > 0 || kk > 0);
                 else
-                  mma_f8_ss_plain_a(tmem + kLdTmemS, last, bd + kk * 2, kIdescS, 1u);
+                  mma_f8_ss_plain_a(d, last, bd + kk * 2, kIdescS, 1u);
               }
             } else {
 #pragma unroll
-              for (int kk = 0; kk < 4; ++kk) mma_f16_ss(tmem + kLdTmemS, rotated + kk * 2, bd + kk * 2, kIdescR, 1u);
-              warp_commit(s_full);
-              warp_commit(empty + s);
+              for (int kk = 0; kk < 4; ++kk) mma_f16_ss(d, rotated + kk * 2, bd + kk * 2, kIdescR, 1u);
+              warp_commit(s_full + set);
+              warp_commit(empty + set * kLdSlots + s);
             }
             s = s + 1 == kLdSlots ? 0 : s + 1;
           }
+          if (set) slot[1] = s; else slot[0] = s;
         }
         ++seg;
         walk.advance();
@@ -434,31 +469,37 @@ __global__ void __launch_bounds__(kLdThreads, 1) qsa_latent_decode_kernel(const 
     } else if (warp == kLdWeighWarp) {
       // O^T (+)= V^T P^T
       const uint32_t idesc_o = idesc_mxf8(128, few ? 2 * cols : cols, true, false);
-      const uint32_t ones = tmem + kLdTmemOnes, scales = tmem + kLdTmemScales;
       const uint32_t weights = desc_low(base_s + kLdP), second = kLdPairs * 128 / 16;
-      int s = 0, n = 0, seg = 0;
+      int slot[2] = {0, 0}, n = 0, seg = 0;
       while (!failed && walk.next(p)) {
 #pragma unroll 1
         for (int tile = walk.from; tile < walk.to && !failed; ++tile, ++n) {
+          const int set = n & 1;
           const bool first = tile == walk.from;
-          failed = !wait(p_full, (uint32_t)(n & 1)) || (first && seg > 0 && !wait(o_empty, (uint32_t)((seg - 1) & 1)));
+          failed = !wait(p_full + set, (uint32_t)((n >> 1) & 1)) ||
+                   (first && seg > 0 && !wait(o_empty, (uint32_t)((seg - 1) & 1)));
           if (failed) break;
+          const uint32_t ones = tmem + kLdTmemOnes, scales = tmem + kLdTmemScales + 2 * set;
+          const uint32_t pd = weights + set * 4;
+          int s = set ? slot[1] : slot[0];
 #pragma unroll
           for (int c = 0; c < kChunks; ++c) {
-            const uint32_t ad = ring + s * (kLdSlot / 16);
+            const uint32_t ad = ring + (set * kLdSlots + s) * (kLdSlot / 16);
 #pragma unroll
             for (int kk = 0; kk < kLdTile / 32; ++kk) {
               const uint32_t idesc = idesc_o | kk << 4;  // the kk-th 32 tokens' scales
-              mma_mxf8_ss(tmem + kLdTmemO + c * kLdPairs, ad + kk * 256, weights + kk * 2, idesc, ones, scales, kk > 0 ? 1u : !first);
+              mma_mxf8_ss(tmem + kLdTmemO + c * kLdPairs, ad + kk * 256, pd + kk * 2, idesc, ones, scales, kk > 0 ? 1u : !first);
               if (!few)
-                mma_mxf8_ss(tmem + kLdTmemO + c * kLdPairs, ad + kk * 256, weights + second + kk * 2, idesc, ones, scales, 1u);
+                mma_mxf8_ss(tmem + kLdTmemO + c * kLdPairs, ad + kk * 256, pd + second + kk * 2, idesc, ones, scales, 1u);
             }
-            warp_commit(empty + s);
+            warp_commit(empty + set * kLdSlots + s);
             s = s + 1 == kLdSlots ? 0 : s + 1;
           }
-          warp_commit(o_full);
+          warp_commit(o_full + set);
           s = s + 1 == kLdSlots ? 0 : s + 1;  // the rotated part's
+          if (set) slot[1] = s; else slot[0] = s;
         }
+        warp_commit(o_done);
         ++seg;
         walk.advance();
       }
@@ -468,16 +509,20 @@ __global__ void __launch_bounds__(kLdThreads, 1) qsa_latent_decode_kernel(const 
       // The copies wrote by one path to shared memory and the products read by
       // another: the fence between them waits for what its own thread has under
       // way, 1 us in a thread that copies or multiplies, and nothing in this one.
-      int s = 0, n = 0;
-      uint32_t turn = 0;
+      int slot[2] = {0, 0}, n = 0;
+      uint32_t turn[2] = {0, 0};
       while (!failed && walk.next(p)) {
 #pragma unroll 1
         for (int tile = walk.from; tile < walk.to && !failed; ++tile, ++n) {
+          const int set = n & 1;
+          int s = set ? slot[1] : slot[0];
+          uint32_t t = set ? turn[1] : turn[0];
 #pragma unroll 1
           for (int c = 0; c <= kChunks && !failed; ++c) {
-            failed = !wait_or_abort(full + s, turn, abort_flag, p.wait_limit_ns);
-            if (++s == kLdSlots) s = 0, turn ^= 1u;
+            failed = !wait_or_abort(full + set * kLdSlots + s, t, abort_flag, p.wait_limit_ns);
+            if (++s == kLdSlots) s = 0, t ^= 1u;
           }
+          if (set) slot[1] = s, turn[1] = t; else slot[0] = s, turn[0] = t;
           fence_proxy_async_smem();
           mbar_arrive(ready + n % kLdReady);
         }
@@ -494,9 +539,10 @@ __global__ void __launch_bounds__(kLdThreads, 1) qsa_latent_decode_kernel(const 
     const bool live = 16 * q4 < mine;                   // the warp has one
     const int rho = rt * kLdPairs + pair;
     const int node = min(rho / p.heads, p.nodes - 1);
-    const int quarter = 2 * set + (odd ? 1 : 0);        // this lane's 32 tokens of a tile
+    const int half = odd ? 1 : 0;                       // this lane's 32 tokens of a tile
+    const int quarter = 2 * set + half;                 // and its quarter of a row of queries
     const uint32_t lane_base = (uint32_t)(q4 * 32) << 16;
-    int n = 0;
+    int first_n = 0, seg = 0;  // tiles before the segment, segments
     // a segment's queries are placed while the last product of the one before it is
     // under way: each lane of a pair, in each set, has a quarter of the row
     constexpr int kWords = 4 * kChunks;  // 16-byte words of a quarter
@@ -526,9 +572,10 @@ __global__ void __launch_bounds__(kLdThreads, 1) qsa_latent_decode_kernel(const 
         // both maxima of this lane, then of the row's four
         uint32_t both = max(top & 0xffffu, top >> 16) | max(rtop & 0xffffu, rtop >> 16) << 16;
         both = __vmaxu2(both, __shfl_xor_sync(0xffffffffu, both, 1));
-        if (!odd) told_q[set * kLdPairs + pair] = __uint_as_float(both);
-        bar_sync(2 + q4, 64);
-        both = __vmaxu2(both, __float_as_uint(told_q[(set ^ 1) * kLdPairs + pair]));
+        uint32_t* told = reinterpret_cast<uint32_t*>(smem + kLdTold);
+        if (!odd) told[set * kLdPairs + pair] = both;
+        bar_sync(kLdBarQuarter + q4, 64);
+        both = __vmaxu2(both, told[(set ^ 1) * kLdPairs + pair]);
         const int t = (int)(both & 0xffffu), u = (int)(both >> 16);
         // 2^a takes the largest latent query into [128, 256), as far as the rotated
         // ones stay far from bf16's end
@@ -612,23 +659,25 @@ __global__ void __launch_bounds__(kLdThreads, 1) qsa_latent_decode_kernel(const 
       float r = kLowest, l = 0.f;
       const float km = odd ? qs * 0.0625f : qs, kr = odd ? qs : qs * 0.0625f;  // own and the other lane's term
 #pragma unroll 1
-      for (int tile = now.from; tile < now.to; ++tile, ++n) {
+      for (int tile = now.from + ((set ^ first_n) & 1); tile < now.to; tile += 2) {
+        const int n = first_n + tile - now.from;
         const int m = n % kLdMeta;
+        const uint32_t turn = (uint32_t)((n >> 1) & 1);
         if (!failed)
           failed = !(wait_or_abort(meta_full + m, (uint32_t)((n / kLdMeta) & 1), abort_flag, p.wait_limit_ns) &&
-                     wait_or_abort(s_full, (uint32_t)(n & 1), abort_flag, p.wait_limit_ns));
+                     wait_or_abort(s_full + set, turn, abort_flag, p.wait_limit_ns));
         failed = __any_sync(0xffffffffu, failed);
         tc_fence_after();
         float u[32];
         float top = -INFINITY;
         if (live && !failed) {
-          const float* ms = metas[m].s + quarter * kLdQuarter;
-          const float* ml = metas[m].lg + quarter * kLdQuarter;
+          const float* ms = metas[m].s + half * kLdHalf;
+          const float* ml = metas[m].lg + half * kLdHalf;
           float x[32], y[32];
-          tmem_ld_wait<32>(tmem + lane_base + kLdTmemS + 64 * set, x);
-          tmem_ld_wait<32>(tmem + lane_base + kLdTmemS + 64 * set + 32, y);
+          tmem_ld_wait<32>(tmem + lane_base + kLdTmemS + kLdTile * set, x);
+          tmem_ld_wait<32>(tmem + lane_base + kLdTmemS + kLdTile * set + 32, y);
           tc_fence_before();
-          mbar_arrive(s_empty);
+          mbar_arrive(s_empty + set);
 #pragma unroll
           for (int j = 0; j < 32; j += 4) {
             const float4 s4 = *reinterpret_cast<const float4*>(ms + j);
@@ -642,7 +691,7 @@ __global__ void __launch_bounds__(kLdThreads, 1) qsa_latent_decode_kernel(const 
             }
           }
           if (p.nodes > 1 && tile * kLdTile + kLdTile > own) {
-            const int d0 = tile * kLdTile + 32 * quarter - own;
+            const int d0 = tile * kLdTile + 32 * half - own;
             const int word = d0 >> 5;
             const uint32_t bits = __funnelshift_r(ld_seen_word(p, now.row, node, word), ld_seen_word(p, now.row, node, word + 1), d0 & 31);
 #pragma unroll
@@ -650,45 +699,57 @@ __global__ void __launch_bounds__(kLdThreads, 1) qsa_latent_decode_kernel(const 
               if (!((bits >> j) & 1u)) u[j] = -INFINITY;
           }
 #pragma unroll
-          for (int j = 0; j < 32; ++j) top = fmaxf(top, u[j]);
+          for (int j = 0; j < 32; ++j) top = max_nan(top, u[j]);
         } else {
-          mbar_arrive(s_empty);
+          mbar_arrive(s_empty + set);
+        }
+        // the reference, as the tile before left it
+        const bool begun = tile > now.from;
+        if (begun) {
+          if (!failed) failed = !wait_or_abort(r_done + (set ^ 1), (uint32_t)(((n - 1) >> 1) & 1), abort_flag, p.wait_limit_ns);
+          failed = __any_sync(0xffffffffu, failed);
+          if (live) {
+            const float next = pair_r[pair];
+            l *= ex2(r - next);
+            r = next;
+          }
         }
         // the scale of this lane's 32 weights
-        uint8_t* scales = told_scales + (n & 1) * 4 * kLdPairs;
+        uint8_t* scales = smem + kLdScales + (2 * set + (int)turn) * 4 * kLdPairs;
         auto scale32 = [&]() -> float {
           const float e = fminf(fmaxf(ceilf(top - r), kLdNear), kLdFar);
-          if (live) scales[4 * pair + quarter] = (uint8_t)(127 - (int)kLdOne + (int)e);
+          if (live) scales[4 * pair + half] = (uint8_t)(127 - (int)kLdOne + (int)e);
           return e;
         };
         float e = scale32();
         // a reference that a weight passes by too much moves, and O and l with it
-        const bool begun = tile > now.from;
-        const float pair_top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        float2* told = told_f + (n & 1) * 2 * kLdPairs;  // of this tile, from each set: the pair's maximum and reference
-        if (live && !odd) told[set * kLdPairs + pair] = make_float2(pair_top, r);
-        if (bar_vote(1, kLdSoft, top > r + kLdFar || failed)) {
-          if (begun && !failed) failed = !wait_or_abort(o_full, (uint32_t)((n - 1) & 1), abort_flag, p.wait_limit_ns);
+        if (bar_vote(kLdBarSet + set, kLdSoft / 2, top > r + kLdFar || failed)) {
+          float* move = reinterpret_cast<float*>(smem + kLdMove) + set * kLdPairs;
+          if (live) {
+            const float next = fmaxf(r, fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1)));
+            const float f = ex2(r - next);  // 0 before the first weight
+            l *= f;
+            r = next;
+            if (!odd) move[pair] = f;
+          }
+          // all products before this tile's
+          if (begun && !failed)
+            failed = !((n < 2 || wait_or_abort(o_full + set, turn ^ 1u, abort_flag, p.wait_limit_ns)) &&
+                       wait_or_abort(o_full + (set ^ 1), (uint32_t)(((n - 1) >> 1) & 1), abort_flag, p.wait_limit_ns));
           failed = __any_sync(0xffffffffu, failed);
-          if (bar_vote(1, kLdSoft, failed)) {
+          if (bar_vote(kLdBarSet + set, kLdSoft / 2, failed)) {
             failed = true;
             break;
           }
-          if (live) {
-            const float next = fmaxf(r, fmaxf(pair_top, told[(set ^ 1) * kLdPairs + pair].x));
-            l *= ex2(r - next);  // 0 before the first weight
-            r = next;
-          }
           if (begun) {
             tc_fence_after();
-            // 16 pairs at a time, where one has moved; a lane works out the factor of one
+            // 16 pairs at a time, where one has moved
 #pragma unroll 1
             for (int b = 0; b < cols; b += 16) {
-              const float2 t0 = told[b + (lane & 15)], t1 = told[kLdPairs + b + (lane & 15)];
-              const float f = ex2(t0.y - fmaxf(t0.y, fmaxf(t0.x, t1.x)));
+              const float f = move[b + (lane & 15)];
               if (__all_sync(0xffffffffu, f == 1.f)) continue;
 #pragma unroll 1
-              for (int c = set; c < kChunks * (few ? 2 : 1); c += 2) {
+              for (int c = 0; c < kChunks * (few ? 2 : 1); ++c) {
                 const uint32_t at = tmem + lane_base + kLdTmemO + (few ? c / 2 : c) * kLdPairs + b + (few ? c % 2 * cols : 0);
                 float x[16];
                 uint32_t y[16];
@@ -702,68 +763,86 @@ __global__ void __launch_bounds__(kLdThreads, 1) qsa_latent_decode_kernel(const 
             tc_fence_before();
           }
           e = scale32();
-          bar_sync(1, kLdSoft);
+          bar_sync(kLdBarSet + set, kLdSoft / 2);
         }
+        if (live && !odd) pair_r[pair] = r;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(r_done + set);
         // ---- weights
         uint32_t hi[8], lo[8];
         if (live) {
-          const float* mi = metas[m].inv + quarter * kLdQuarter;
+          const float* mi = metas[m].inv + half * kLdHalf;
           const float rb = r + (e - kLdOne);
           float sum = 0.f;
 #pragma unroll
           for (int j = 0; j < 32; j += 4) {
             const float4 i4 = *reinterpret_cast<const float4*>(mi + j);
             const float ii[4] = {i4.x, i4.y, i4.z, i4.w};
-            uint32_t h2[2], l2[2];
+            uint32_t first[4], second[4];  // codes in bits 20 to 26
 #pragma unroll
-            for (int i = 0; i < 4; i += 2) {
-              const __nv_bfloat162 w2 = __floats2bfloat162_rn(ex2(u[j + i] - rb), ex2(u[j + i + 1] - rb));
-              const float2 w = __bfloat1622float2(w2);
-              sum = fmaf(w.x, ii[i], sum);
-              sum = fmaf(w.y, ii[i + 1], sum);
-              h2[i / 2] = __nv_cvt_float2_to_fp8x2(w, __NV_SATFINITE, __NV_E4M3);
-              const __half2 back(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)h2[i / 2], __NV_E4M3));
-              const __half2 left = __hsub2(__floats2half2_rn(w.x, w.y), back);
-              l2[i / 2] = __nv_cvt_halfraw2_to_fp8x2(static_cast<__half2_raw>(left), __NV_SATFINITE, __NV_E4M3);
+            for (int i = 0; i < 4; ++i) {
+              // rounded to 8 bits
+              const float w = __uint_as_float((__float_as_uint(ex2(u[j + i] - rb)) + 0x8000u) & 0xffff0000u);
+              sum = fmaf(w, ii[i], sum);
+              // times 2^-120 an E4M3 value is an fp32 one whose bits 20 to 26 are its code,
+              // subnormal values too; half of the last step goes in before it is cut off
+              const float t = fmaf(w, 0x1p-120f, 0x1p-130f);
+              first[i] = __float_as_uint(t) & 0xfff00000u;
+              second[i] = __float_as_uint(t - __uint_as_float(first[i]));
             }
-            hi[j / 4] = h2[0] | h2[1] << 16;
-            lo[j / 4] = l2[0] | l2[1] << 16;
+            hi[j / 4] = pack_codes(first);
+            lo[j / 4] = pack_codes(second);
           }
           l = fmaf(sum, ex2(e - kLdOne), l);
+          if (!(top <= 3.402823466e38f)) l = __int_as_float(0x7fffffff);  // a NaN, or a score past fp32
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(meta_empty + m);
-        // the product of the tile before has read its weights
-        if (n > 0 && !failed) failed = !wait_or_abort(o_full, (uint32_t)((n - 1) & 1), abort_flag, p.wait_limit_ns);
+        // the product of the set's tile before has read its weights and their scales
+        if (n >= 2 && !failed) failed = !wait_or_abort(o_full + set, turn ^ 1u, abort_flag, p.wait_limit_ns);
         failed = __any_sync(0xffffffffu, failed);
         if (live) {
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
-            uint8_t* at = smem + kLdP + sw128_offset(pair, 32 * quarter + 16 * k);
+            uint8_t* at = smem + kLdP + sw128_offset(pair, 64 * set + 32 * half + 16 * k);
             *reinterpret_cast<uint4*>(at) = make_uint4(hi[4 * k], hi[4 * k + 1], hi[4 * k + 2], hi[4 * k + 3]);
             *reinterpret_cast<uint4*>(at + lo_row * 128) = make_uint4(lo[4 * k], lo[4 * k + 1], lo[4 * k + 2], lo[4 * k + 3]);
           }
           fence_proxy_async_smem();
         }
-        if (set == 0) {
+        {
           const uint32_t* words = reinterpret_cast<const uint32_t*>(scales);
           const uint32_t both[2] = {words[scale0], words[scale1]};
-          tmem_st(tmem + lane_base + kLdTmemScales, both);
+          tmem_st(tmem + lane_base + kLdTmemScales + 2 * set, both);
           tmem_wait_st();
           tc_fence_before();
         }
-        mbar_arrive(p_full);
+        mbar_arrive(p_full + set);
       }
       // ---- the segment's results
-      if (more && !failed) {
+      const int last = first_n + (now.to - now.from) - 1;
+      if ((last & 1) != set && !failed)  // the other set's last tile
+        failed = !wait_or_abort(r_done + (set ^ 1), (uint32_t)((last >> 1) & 1), abort_flag, p.wait_limit_ns);
+      failed = __any_sync(0xffffffffu, failed);
+      if (bar_vote(kLdBarAll, kLdSoft, failed)) {
+        failed = true;
+        break;
+      }
+      // all scores are done, and the queries free
+      if (more) {
         load_q(walk.row);
         next_qs = place_q();
       }
-      if (!failed) failed = !wait_or_abort(o_full, (uint32_t)((n - 1) & 1), abort_flag, p.wait_limit_ns);
+      failed = !wait_or_abort(o_done, (uint32_t)(seg & 1), abort_flag, p.wait_limit_ns);
       failed = __any_sync(0xffffffffu, failed);
+      if (live) {
+        const float end_r = pair_r[pair];
+        l *= ex2(r - end_r);
+        r = end_r;
+      }
       l += __shfl_xor_sync(0xffffffffu, l, 1);
       if (live && !odd && set == 1) head_f[pair] = l;
-      if (bar_vote(1, kLdSoft, failed)) {
+      if (bar_vote(kLdBarAll, kLdSoft, failed)) {
         failed = true;
         break;
       }
@@ -774,7 +853,7 @@ __global__ void __launch_bounds__(kLdThreads, 1) qsa_latent_decode_kernel(const 
         if (!now.whole && pair < mine)
           p.part_lse[((int64_t)piece * p.row_tiles + rt) * kLdPairs + pair] = l == 0.f ? -INFINITY : log2f(l) + r;
       }
-      bar_sync(1, kLdSoft);
+      bar_sync(kLdBarAll, kLdSoft);
       tc_fence_after();
       const int64_t at = now.whole ? ((int64_t)now.row * pairs + rt * kLdPairs) * kRank
                                     : ((int64_t)piece * p.row_tiles + rt) * kLdPairs * kRank;
@@ -814,7 +893,9 @@ __global__ void __launch_bounds__(kLdThreads, 1) qsa_latent_decode_kernel(const 
         store(p.part_o + at + 32 * q4 + lane, [](float v) { return v; });
       tc_fence_before();
       mbar_arrive(o_empty);
-      bar_sync(1, kLdSoft);  // the factors are read before the next segment's
+      bar_sync(kLdBarAll, kLdSoft);  // the factors are read before the next segment's
+      first_n = last + 1;
+      ++seg;
     }
   }
 

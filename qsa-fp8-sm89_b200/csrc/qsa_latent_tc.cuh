@@ -24,24 +24,23 @@ __device__ __forceinline__ bool bar_vote(int id, int count, bool pred) {
   return r != 0u;
 }
 
-// One look at a barrier, without waiting (try_wait may wait for some microseconds).
-__device__ __forceinline__ bool mbar_test_wait(uint64_t* bar, uint32_t parity) {
+// Bounded wait that also gives up once another role raised the abort flag; it
+// raises the flag when its own limit runs out. The thread sleeps at the barrier for
+// up to 20 us at a time: a reading of the timer takes the unit that 2^x takes.
+__device__ __forceinline__ bool mbar_sleep_wait(uint64_t* bar, uint32_t parity) {
   uint32_t ok;
-  asm volatile("{\n.reg .pred p;\nmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}\n"
+  asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 20000;\nselp.u32 %0, 1, 0, p;\n}\n"
                : "=r"(ok)
                : "r"(smem_u32(bar)), "r"(parity)
                : "memory");
   return ok != 0;
 }
-
-// Bounded wait that also gives up once another role raised the abort flag; it
-// raises the flag when its own limit runs out.
 __device__ __forceinline__ bool wait_or_abort(uint64_t* bar, uint32_t parity, volatile int* abort_flag, uint64_t limit_ns) {
-  if (mbar_try_wait(bar, parity)) return true;
+  if (mbar_sleep_wait(bar, parity)) return true;
   uint64_t t0;
   asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t0));
   while (true) {
-    if (mbar_try_wait(bar, parity)) return true;
+    if (mbar_sleep_wait(bar, parity)) return true;
     if (*abort_flag) return false;
     uint64_t t1;
     asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t1));
