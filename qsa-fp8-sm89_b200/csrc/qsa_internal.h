@@ -275,10 +275,13 @@ struct LatentDecodeParams {
   // The split: a CTA takes one of the row_tiles 64-row parts of a row's (node,
   // head) pairs, over the columns that its group (of `groups`) has.
   int row_tiles, groups;
-  int planned;    // groups share all rows' tiles evenly (workspace); else group g has row g
-  int2* begins;   // [groups] row and tile that each group begins with
-  float* part_o;  // [2 groups, row_tiles, 64, rank] results of pieces of rows
-  float* part_lse;  // [2 groups, row_tiles, 64] their log2-sum-exp2, -inf for none
+  int planned;  // groups share all rows' tiles evenly; else group g has row g
+  // workspace
+  uint8_t* queries;   // [rows, ceil(pairs / 16)] blocks: 16 pairs' queries as the products take them
+  int64_t* total;     // tiles of all rows
+  int2* begins;       // [groups] row and tile that each group begins with
+  float* part_o;      // [2 groups, row_tiles, 64, rank] results of pieces of rows
+  float* part_lse;    // [2 groups, row_tiles, 64] their log2-sum-exp2, -inf for none
   int* err;
   uint64_t wait_limit_ns;
 };

@@ -41,10 +41,14 @@
 // matrix unit reads), and four softmax warps. One warp issues the products of scores
 // and one those of weights, of both sets, in the tiles' order.
 //
+// A first kernel turns the queries into what the products take and shares out the
+// work: done in this one, at the start of each segment, it held up everything for 10
+// us. The second starts while the first still runs, and the joins likewise.
+//
 // Work: group g of CTAs (one CTA for each 64 pairs of a row, so that the CTAs that
 // read the same tokens run side by side) has an even share of all rows' tiles: at
 // most two pieces of rows and any whole rows between. Pieces are joined by their
-// log-sums in a second kernel. Few short rows are a CTA each.
+// log-sums in a last kernel. Few short rows are a CTA each.
 //
 // Every wait is bounded; a CTA that gives up records it in the device error word,
 // waits for its own copies and products, frees its tensor memory and returns.
@@ -82,8 +86,13 @@ struct LdMeta {
   float s[2 * kLdHalf], lg[2 * kLdHalf], inv[2 * kLdHalf];
 };
 
-// Named barriers: of a set, of both, and of a quarter of the lanes' two warps.
-constexpr int kLdBarSet = 1, kLdBarAll = 3, kLdBarQuarter = 4;
+constexpr int kLdBarSet = 1, kLdBarAll = 3;  // named barriers: of a set (1, 2), of both
+
+// A block of 16 pairs' queries: words [rank / 16][32 lanes][4] for tensor memory (a
+// pair's first terms in lane 2 i, its second ones in 2 i + 1), bf16 [16][64] rotated
+// ones, float [16] what a product is to be multiplied by.
+constexpr int kLdBlockPairs = 16;
+__host__ __device__ constexpr int ld_block_bytes(int rank) { return 32 * rank + 16 * 128 + 256; }
 
 constexpr int kLdQr = 0;                // rotated queries: 128 rows of 64 bf16
 constexpr int kLdP = kLdQr + 16384;     // weights: two terms of 64 rows of 64 tokens of either set
@@ -93,8 +102,7 @@ constexpr int kLdMetaAt = kLdQx + 4096;
 constexpr int kLdRow = kLdMetaAt + kLdMeta * (int)sizeof(LdMeta);  // float [64]: factors of pairs at a segment's end
 constexpr int kLdRef = kLdRow + kLdPairs * 4;                      // float [64]: r
 constexpr int kLdMove = kLdRef + kLdPairs * 4;                     // float [2 sets][64]: factors of a moving r
-constexpr int kLdTold = kLdMove + 2 * kLdPairs * 4;                // uint32 [2 sets][64]: maxima of queries
-constexpr int kLdScales = kLdTold + 2 * kLdPairs * 4;              // bytes [2 sets][2 tiles][64][4], of 32 tokens each
+constexpr int kLdScales = kLdMove + 2 * kLdPairs * 4;              // bytes [2 sets][2 tiles][64][4], of 32 tokens each
 constexpr int kLdBars = kLdScales + 4 * kLdPairs * 4;
 constexpr int kLdNumBars = 4 * kLdSlots + 2 * kLdMeta + kLdReady + 16;
 constexpr int kLdMisc = kLdBars + kLdNumBars * 8;  // tensor memory address, abort flag, group's range
@@ -234,57 +242,22 @@ __global__ void __launch_bounds__(kLdThreads, 1) qsa_latent_decode_kernel(const 
     fence_proxy_async_smem();
   }
 
-  // the group's share of the tiles
-  if (!p.planned) {
-    if (tid == 0) {
-      begin[0] = group, begin[1] = 0;
+  wait_for_prerequisites();
+  launch_dependents();
+  if (tid == 0) {
+    // the group's share of the tiles
+    begin[0] = group, begin[1] = 0;
+    if (p.planned) {
+      const int2 b = p.begins[group];
+      const int64_t total = *p.total, groups = min((int64_t)p.groups, total);
+      begin[0] = b.x, begin[1] = b.y;
+      share[1] = group < groups ? total * (group + 1) / groups - total * group / groups : 0;
+    } else {
       share[1] = ld_tiles(p, group);
-    }
-  } else {
-    // each thread counts the tiles of a run of rows
-    __shared__ int64_t warp_sum[kLdThreads / 32];
-    const int run = (p.rows + kLdThreads - 1) / kLdThreads;
-    const int r0 = min(tid * run, p.rows), r1 = min(r0 + run, p.rows);
-    int64_t sum = 0;
-#pragma unroll 8
-    for (int r = r0; r < r1; ++r) sum += ld_tiles(p, r);
-    int64_t upto = sum;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int64_t v = __shfl_up_sync(0xffffffffu, upto, o);
-      if (lane >= o) upto += v;
-    }
-    if (lane == 31) warp_sum[warp] = upto;
-    if (tid == 0) begin[0] = p.rows, begin[1] = 0, share[1] = 0;
-    __syncthreads();
-    int64_t total = 0;
-#pragma unroll
-    for (int w = 0; w < kLdThreads / 32; ++w) {
-      if (w < warp) upto += warp_sum[w];
-      total += warp_sum[w];
-    }
-    const int64_t groups = min((int64_t)p.groups, total);  // each has a tile at least
-    if (group < groups) {
-      const int64_t u0 = total * group / groups, u1 = total * (group + 1) / groups;
-      int64_t before = upto - sum;
-      if (before <= u0 && u0 < upto) {
-        int r = r0;
-        for (;; ++r) {
-          const int t = ld_tiles(p, r);
-          if (u0 < before + t) break;
-          before += t;
-        }
-        begin[0] = r, begin[1] = (int)(u0 - before);
-        share[1] = u1 - u0;
-        if (rt == 0) p.begins[group] = make_int2(r, (int)(u0 - before));
-      }
-    } else if (rt == 0 && tid == 0) {
-      p.begins[group] = make_int2(p.rows, 0);
     }
   }
   __syncwarp();
   __syncthreads();
-  launch_dependents();
   tc_fence_after();
   constexpr uint32_t tmem = 0;  // all of it is this block's
   LdWalk walk;
@@ -312,11 +285,6 @@ __global__ void __launch_bounds__(kLdThreads, 1) qsa_latent_decode_kernel(const 
       const int columns = ld_columns(p, row, count);
       const int64_t req = p.t2r ? (int64_t)__ldg(p.t2r + row) : (int64_t)row;
       const int own = p.nodes > 1 ? count - p.nodes : 0x7fffffff;
-      {  // the queries, which the softmax will load, into L2
-        const char* q = reinterpret_cast<const char*>(p.q + ((int64_t)row * pairs + rt * kLdPairs) * (kRank + kLatentRope));
-        for (int i = 32 * w + lane; i < mine * (kRank + kLatentRope) * 2 / 128; i += 128)
-          asm volatile("prefetch.global.L2 [%0];\n" ::"l"(q + i * 128));
-      }
       // A token's lookup is three loads in a row (its index, its page, its scale):
       // each is made a tile before the next one needs it.
       auto token = [&](int tile) -> int {  // -1: masked
@@ -540,93 +508,39 @@ __global__ void __launch_bounds__(kLdThreads, 1) qsa_latent_decode_kernel(const 
     const int rho = rt * kLdPairs + pair;
     const int node = min(rho / p.heads, p.nodes - 1);
     const int half = odd ? 1 : 0;                       // this lane's 32 tokens of a tile
-    const int quarter = 2 * set + half;                 // and its quarter of a row of queries
     const uint32_t lane_base = (uint32_t)(q4 * 32) << 16;
     int first_n = 0, seg = 0;  // tiles before the segment, segments
-    // a segment's queries are placed while the last product of the one before it is
-    // under way: each lane of a pair, in each set, has a quarter of the row
-    constexpr int kWords = 4 * kChunks;  // 16-byte words of a quarter
-    uint4 raw[kWords], rr[2];
-    auto load_q = [&](int row) {
-      const uint4* q = reinterpret_cast<const uint4*>(p.q + ((int64_t)row * pairs + rho) * (kRank + kLatentRope));
-      const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
-#pragma unroll
-      for (int i = 0; i < kWords; ++i) raw[i] = pair < mine ? __ldg(q + quarter * kWords + i) : zero;
-#pragma unroll
-      for (int i = 0; i < 2; ++i) rr[i] = pair < mine ? __ldg(q + 16 * kChunks + quarter * 2 + i) : zero;
-    };
-    // The queries as two terms into tensor memory, and their rotated part into shared
-    // memory; returns what a product of them is to be multiplied by.
-    auto place_q = [&]() -> float {
+    // A segment's queries go to their places once the scores of the one before it are
+    // done, while its last product is under way; returns what a product of them is to
+    // be multiplied by.
+    const int row_blocks = (pairs + kLdBlockPairs - 1) / kLdBlockPairs;
+    auto place_q = [&](int row) -> float {
       float qs = 0.f;
       if (live) {
-        uint32_t top = 0, rtop = 0;  // largest |q| as bits, two at a time
+        const uint8_t* block = p.queries + ((int64_t)row * row_blocks + rt * 4 + q4) * ld_block_bytes(kRank);
+        const uint4* words = reinterpret_cast<const uint4*>(block) + set * 4 * kChunks * 32 + lane;
+        const uint4* rotated = reinterpret_cast<const uint4*>(block + 32 * kRank) + set * 64 + lane;
+        uint4 w[4 * kChunks], t[2];
 #pragma unroll
-        for (int i = 0; i < kWords; ++i)
-          top = __vmaxu2(__vmaxu2(top, __vmaxu2(raw[i].x & 0x7fff7fffu, raw[i].y & 0x7fff7fffu)),
-                         __vmaxu2(raw[i].z & 0x7fff7fffu, raw[i].w & 0x7fff7fffu));
+        for (int i = 0; i < 4 * kChunks; ++i) w[i] = __ldg(words + i * 32);
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
-          rtop = __vmaxu2(__vmaxu2(rtop, __vmaxu2(rr[i].x & 0x7fff7fffu, rr[i].y & 0x7fff7fffu)),
-                          __vmaxu2(rr[i].z & 0x7fff7fffu, rr[i].w & 0x7fff7fffu));
-        // both maxima of this lane, then of the row's four
-        uint32_t both = max(top & 0xffffu, top >> 16) | max(rtop & 0xffffu, rtop >> 16) << 16;
-        both = __vmaxu2(both, __shfl_xor_sync(0xffffffffu, both, 1));
-        uint32_t* told = reinterpret_cast<uint32_t*>(smem + kLdTold);
-        if (!odd) told[set * kLdPairs + pair] = both;
-        bar_sync(kLdBarQuarter + q4, 64);
-        both = __vmaxu2(both, told[(set ^ 1) * kLdPairs + pair]);
-        const int t = (int)(both & 0xffffu), u = (int)(both >> 16);
-        // 2^a takes the largest latent query into [128, 256), as far as the rotated
-        // ones stay far from bf16's end
-        int a = t == 0 ? 0 : 7 - (max(t >> 7, 1) - 127);
-        if (u != 0) a = min(a, 40 - (max(u >> 7, 1) - 127));
-        a = min(max(a, -120), 120);
-        const float up = __uint_as_float((uint32_t)(127 + a) << 23);
-        qs = __uint_as_float((uint32_t)(127 - a) << 23) * p.score_scale_log2;
-        if (t >= 0x7f80 || u >= 0x7f80) qs = __int_as_float(0x7fffffff);  // an infinity or NaN
-        // the even lane's row is the first terms, the odd one's the second: this
-        // lane's quarter of both, the other lane's from it
+        for (int i = 0; i < 2; ++i) t[i] = __ldg(rotated + i * 32);
+        qs = __ldg(reinterpret_cast<const float*>(block + 32 * kRank + 16 * 128) + (lane >> 1));
 #pragma unroll
-        for (int b = 0; b < kChunks; ++b) {
-          uint32_t first[8], second[8];  // of the even lane's quarter, of the odd one's
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint4 v = raw[4 * b + i];
-            const uint32_t w4[4] = {v.x, v.y, v.z, v.w};
-            uint32_t hi[4], lo[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const float x = __uint_as_float(w4[j] << 16) * up, y = __uint_as_float(w4[j] & 0xffff0000u) * up;
-              hi[j] = __nv_cvt_float2_to_fp8x2(make_float2(x, y), __NV_SATFINITE, __NV_E4M3);
-              const float2 back = e4m3x2_to_f32x2((uint16_t)hi[j]);
-              lo[j] = __nv_cvt_float2_to_fp8x2(make_float2((x - back.x) * 16.f, (y - back.y) * 16.f), __NV_SATFINITE, __NV_E4M3);
-            }
-            const uint32_t h0 = hi[0] | hi[1] << 16, h1 = hi[2] | hi[3] << 16, l0 = lo[0] | lo[1] << 16, l1 = lo[2] | lo[3] << 16;
-            const uint32_t r0 = __shfl_xor_sync(0xffffffffu, odd ? h0 : l0, 1), r1 = __shfl_xor_sync(0xffffffffu, odd ? h1 : l1, 1);
-            first[2 * i] = odd ? r0 : h0, first[2 * i + 1] = odd ? r1 : h1;
-            second[2 * i] = odd ? l0 : r0, second[2 * i + 1] = odd ? l1 : r1;
-          }
-          tmem_st(tmem + lane_base + 2 * set * 8 * kChunks + b * 8, first);
-          if (kChunks == 4 && b == 3 && set == 1) {
+        for (int i = 0; i < 4 * kChunks; i += 2) {
+          const uint32_t v[8] = {w[i].x, w[i].y, w[i].z, w[i].w, w[i + 1].x, w[i + 1].y, w[i + 1].z, w[i + 1].w};
+          if (kChunks == 4 && set == 1 && i == 14) {
             uint8_t* at = smem + kLdQx + (4 * q4 + (lane >> 3)) * 128 + (lane & 7) * 16;
-            *reinterpret_cast<uint4*>(at) = make_uint4(second[0], second[1], second[2], second[3]);
-            *reinterpret_cast<uint4*>(at + 2048) = make_uint4(second[4], second[5], second[6], second[7]);
+            *reinterpret_cast<uint4*>(at) = w[i];
+            *reinterpret_cast<uint4*>(at + 2048) = w[i + 1];
           } else {
-            tmem_st(tmem + lane_base + (2 * set + 1) * 8 * kChunks + b * 8, second);
+            tmem_st(tmem + lane_base + (set * 4 * kChunks + i) * 4, v);
           }
         }
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const uint32_t w4[4] = {rr[i].x, rr[i].y, rr[i].z, rr[i].w};
-          uint32_t o4[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const __nv_bfloat162 v = __floats2bfloat162_rn(__uint_as_float(w4[j] << 16) * up, __uint_as_float(w4[j] & 0xffff0000u) * up);
-            o4[j] = *reinterpret_cast<const uint32_t*>(&v);
-          }
-          *reinterpret_cast<uint4*>(smem + kLdQr + sw128_offset(32 * q4 + (lane & ~1), 32 * quarter + 16 * i)) =
-              make_uint4(o4[0], o4[1], o4[2], o4[3]);
+          const int piece = set * 64 + i * 32 + lane;  // 16 bytes of row piece / 8
+          *reinterpret_cast<uint4*>(smem + kLdQr + sw128_offset(32 * q4 + 2 * (piece >> 3), 16 * (piece & 7))) = t[i];
         }
         tmem_wait_st();
         fence_proxy_async_smem();
@@ -644,10 +558,7 @@ __global__ void __launch_bounds__(kLdThreads, 1) qsa_latent_decode_kernel(const 
     const int scale0 = few && lane >= cols ? lane - cols : lane, scale1 = few ? lane : lane + 32;
     bool more = walk.next(p);
     float next_qs = 0.f;
-    if (more) {
-      load_q(walk.row);
-      next_qs = place_q();
-    }
+    if (more) next_qs = place_q(walk.row);
     while (more) {
       const LdWalk now = walk;
       int count;
@@ -829,10 +740,7 @@ __global__ void __launch_bounds__(kLdThreads, 1) qsa_latent_decode_kernel(const 
         break;
       }
       // all scores are done, and the queries free
-      if (more) {
-        load_q(walk.row);
-        next_qs = place_q();
-      }
+      if (more) next_qs = place_q(walk.row);
       failed = !wait_or_abort(o_done, (uint32_t)(seg & 1), abort_flag, p.wait_limit_ns);
       failed = __any_sync(0xffffffffu, failed);
       if (live) {
@@ -912,6 +820,116 @@ __global__ void __launch_bounds__(kLdThreads, 1) qsa_latent_decode_kernel(const 
   }
 }
 
+// The queries as the products take them, 16 pairs a block and a pair a warp: q 2^a =
+// t0 + t1 / 16 in E4M3, with 2^a taking the largest latent query into [128, 256) as
+// far as the rotated ones stay far from bf16's end. The block past those shares out
+// the tiles.
+constexpr int kLpreThreads = 32 * kLdBlockPairs;
+template <int kChunks>
+__global__ void __launch_bounds__(kLpreThreads) qsa_latent_prepare_kernel(const __grid_constant__ LatentDecodeParams p) {
+  constexpr int kRank = 128 * kChunks;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int pairs = p.nodes * p.heads, row_blocks = (pairs + kLdBlockPairs - 1) / kLdBlockPairs;
+  launch_dependents();
+  // the first block shares out the tiles: it takes longest
+  const int64_t at = (int64_t)blockIdx.x - p.planned;
+  if (at >= 0) {
+    const int row = (int)(at / row_blocks), pair = (int)(at - (int64_t)row * row_blocks) * kLdBlockPairs + warp;
+    uint8_t* block = p.queries + at * ld_block_bytes(kRank);
+    uint32_t* words = reinterpret_cast<uint32_t*>(block);
+    uint2 raw[kChunks];  // 4 values of each of this lane's words
+    uint32_t rot = 0;
+#pragma unroll
+    for (int i = 0; i < kChunks; ++i) raw[i] = make_uint2(0u, 0u);
+    if (pair < pairs) {
+      const __nv_bfloat16* q = p.q + ((int64_t)row * pairs + pair) * (kRank + kLatentRope);
+#pragma unroll
+      for (int i = 0; i < kChunks; ++i) raw[i] = __ldg(reinterpret_cast<const uint2*>(q) + 32 * i + lane);
+      rot = __ldg(reinterpret_cast<const uint32_t*>(q + kRank) + lane);
+    }
+    uint32_t top = 0;  // largest |q| as bits, two at a time
+#pragma unroll
+    for (int i = 0; i < kChunks; ++i) top = __vmaxu2(top, __vmaxu2(raw[i].x & 0x7fff7fffu, raw[i].y & 0x7fff7fffu));
+    const uint32_t rtop = rot & 0x7fff7fffu;
+    uint32_t both = max(top & 0xffffu, top >> 16) | max(rtop & 0xffffu, rtop >> 16) << 16;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) both = __vmaxu2(both, __shfl_xor_sync(0xffffffffu, both, o));
+    const int t = (int)(both & 0xffffu), u = (int)(both >> 16);
+    int a = t == 0 ? 0 : 7 - (max(t >> 7, 1) - 127);
+    if (u != 0) a = min(a, 40 - (max(u >> 7, 1) - 127));
+    a = min(max(a, -120), 120);
+    const float up = __uint_as_float((uint32_t)(127 + a) << 23);
+    float qs = pair < pairs ? __uint_as_float((uint32_t)(127 - a) << 23) * p.score_scale_log2 : 0.f;
+    if (t >= 0x7f80 || u >= 0x7f80) qs = __int_as_float(0x7fffffff);  // an infinity or NaN
+#pragma unroll
+    for (int i = 0; i < kChunks; ++i) {
+      const uint32_t v[2] = {raw[i].x, raw[i].y};
+      uint32_t hi[2], lo[2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const float x = __uint_as_float(v[j] << 16) * up, y = __uint_as_float(v[j] & 0xffff0000u) * up;
+        hi[j] = __nv_cvt_float2_to_fp8x2(make_float2(x, y), __NV_SATFINITE, __NV_E4M3);
+        const float2 back = e4m3x2_to_f32x2((uint16_t)hi[j]);
+        lo[j] = __nv_cvt_float2_to_fp8x2(make_float2((x - back.x) * 16.f, (y - back.y) * 16.f), __NV_SATFINITE, __NV_E4M3);
+      }
+      const int col = 32 * i + lane;
+      uint32_t* to = words + ((col >> 2) * 32 + 2 * warp) * 4 + (col & 3);
+      to[0] = hi[0] | hi[1] << 16;
+      to[4] = lo[0] | lo[1] << 16;
+    }
+    const __nv_bfloat162 r2 = __floats2bfloat162_rn(__uint_as_float(rot << 16) * up, __uint_as_float(rot & 0xffff0000u) * up);
+    reinterpret_cast<__nv_bfloat162*>(block + 32 * kRank)[warp * 32 + lane] = r2;
+    if (lane == 0) reinterpret_cast<float*>(block + 32 * kRank + 16 * 128)[warp] = qs;
+    return;
+  }
+  // each thread counts the tiles of a run of rows
+  __shared__ int64_t before[kLpreThreads + 1];
+  __shared__ int64_t warp_sum[kLpreThreads / 32];
+  const int run = (p.rows + kLpreThreads - 1) / kLpreThreads;
+  const int r0 = min(tid * run, p.rows), r1 = min(r0 + run, p.rows);
+  int64_t sum = 0;
+#pragma unroll 8
+  for (int r = r0; r < r1; ++r) sum += ld_tiles(p, r);
+  int64_t upto = sum;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t v = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += v;
+  }
+  if (lane == 31) warp_sum[warp] = upto;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kLpreThreads / 32; ++w)
+    if (w < warp) upto += warp_sum[w];
+  before[tid + 1] = upto;
+  if (tid == 0) before[0] = 0;
+  __syncthreads();
+  const int64_t total = before[kLpreThreads];
+  const int64_t groups = min((int64_t)p.groups, total);  // each has a tile at least
+  if (tid == 0) *p.total = total;
+  for (int g = tid; g < p.groups; g += kLpreThreads) {
+    if (g >= groups) {
+      p.begins[g] = make_int2(p.rows, 0);
+      continue;
+    }
+    const int64_t u = total * g / groups;
+    int lo = 0, hi = kLpreThreads;  // the last run that begins at or before the group's first tile
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) / 2;
+      if (before[mid] <= u) lo = mid; else hi = mid;
+    }
+    int64_t first = before[lo];
+    for (int r = lo * run;; ++r) {
+      const int t = ld_tiles(p, r);
+      if (u < first + t) {
+        p.begins[g] = make_int2(r, (int)(u - first));
+        break;
+      }
+      first += t;
+    }
+  }
+}
+
 // Joins the pieces of a row that several groups share: one block for each group
 // that ends a row's first piece, 64-pair part and pair.
 __global__ void __launch_bounds__(128) qsa_latent_join_kernel(const __grid_constant__ LatentDecodeParams p) {
@@ -977,6 +995,23 @@ int sm_count() {
 
 int64_t align256(int64_t x) { return (x + 255) / 256 * 256; }
 
+// Launches a kernel that waits for its prerequisites itself (early: it may start
+// before the stream's last kernel has ended).
+template <typename Kernel>
+cudaError_t start(Kernel kernel, dim3 grid, int threads, int smem, bool early, cudaStream_t stream, const LatentDecodeParams& p) {
+  cudaLaunchConfig_t config = {};
+  config.gridDim = grid;
+  config.blockDim = dim3(threads);
+  config.dynamicSmemBytes = smem;
+  config.stream = stream;
+  cudaLaunchAttribute attr = {};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = &attr;
+  config.numAttrs = early ? 1 : 0;
+  return cudaLaunchKernelEx(&config, kernel, p);
+}
+
 template <int kChunks>
 cudaError_t launch(const LatentDecodeParams& p, cudaStream_t stream) {
   // the shared memory beyond the default limit, once per device
@@ -991,9 +1026,17 @@ cudaError_t launch(const LatentDecodeParams& p, cudaStream_t stream) {
     ready.fetch_or(bit, std::memory_order_acq_rel);
   }
   const int64_t grid = (int64_t)p.groups * p.row_tiles;
-  if (grid > 0x7fffffffll) return cudaErrorInvalidValue;
-  qsa_latent_decode_kernel<kChunks><<<(unsigned)grid, kLdThreads, kLdSmem, stream>>>(p);
-  return cudaGetLastError();
+  const int64_t blocks = (int64_t)p.rows * ((p.nodes * p.heads + kLdBlockPairs - 1) / kLdBlockPairs) + p.planned;
+  if (grid > 0x7fffffffll || blocks > 0x7fffffffll) return cudaErrorInvalidValue;
+  e = start(qsa_latent_prepare_kernel<kChunks>, dim3((unsigned)blocks), kLpreThreads, 0, false, stream, p);
+  if (e == cudaSuccess) e = start(qsa_latent_decode_kernel<kChunks>, dim3((unsigned)grid), kLdThreads, kLdSmem, true, stream, p);
+  if (e == cudaSuccess && p.planned && p.groups > 1)
+    e = start(qsa_latent_join_kernel, dim3(kLdPairs, (unsigned)p.row_tiles, (unsigned)(p.groups - 1)), 128, 0, true, stream, p);
+  return e;
+}
+
+int64_t query_bytes(const LatentDecodeParams& p) {
+  return align256((int64_t)p.rows * ((p.nodes * p.heads + kLdBlockPairs - 1) / kLdBlockPairs) * ld_block_bytes(p.cache.rank));
 }
 
 }  // namespace
@@ -1004,40 +1047,37 @@ int64_t latent_decode_plan(LatentDecodeParams& p) {
   const int sms = sm_count();
   p.planned = (columns + kLdTile - 1) / kLdTile > kLdDirectTiles || (int64_t)p.rows * p.row_tiles > sms;
   p.groups = p.planned ? (sms / p.row_tiles > 1 ? sms / p.row_tiles : 1) : p.rows;
-  if (!p.planned) return 0;
-  const int64_t pieces = 2ll * p.groups * p.row_tiles * kLdPairs;
-  return align256(pieces * p.cache.rank * 4) + align256(pieces * 4) + align256(8ll * p.groups);
+  int64_t need = query_bytes(p);
+  if (p.planned) {
+    const int64_t pieces = 2ll * p.groups * p.row_tiles * kLdPairs;
+    need += align256(pieces * p.cache.rank * 4) + align256(pieces * 4) + align256(8ll * p.groups) + 256;
+  }
+  return need;
 }
 
 void latent_decode_place(LatentDecodeParams& p, void* workspace) {
   char* at = static_cast<char*>(workspace);
+  auto take = [&](int64_t bytes) {
+    char* here = at;
+    at += align256(bytes);
+    return here;
+  };
+  p.queries = reinterpret_cast<uint8_t*>(take(query_bytes(p)));
+  if (!p.planned) return;
   const int64_t pieces = 2ll * p.groups * p.row_tiles * kLdPairs;
-  p.part_o = reinterpret_cast<float*>(at);
-  at += align256(pieces * p.cache.rank * 4);
-  p.part_lse = reinterpret_cast<float*>(at);
-  at += align256(pieces * 4);
-  p.begins = reinterpret_cast<int2*>(at);
+  p.part_o = reinterpret_cast<float*>(take(pieces * p.cache.rank * 4));
+  p.part_lse = reinterpret_cast<float*>(take(pieces * 4));
+  p.begins = reinterpret_cast<int2*>(take(8ll * p.groups));
+  p.total = reinterpret_cast<int64_t*>(take(8));
 }
 
 cudaError_t launch_latent_decode(const LatentDecodeParams& p, cudaStream_t stream) {
-  cudaError_t e;
   switch (p.cache.rank / 128) {
-    case 1: e = launch<1>(p, stream); break;
-    case 2: e = launch<2>(p, stream); break;
-    case 3: e = launch<3>(p, stream); break;
-    default: e = launch<4>(p, stream); break;
+    case 1: return launch<1>(p, stream);
+    case 2: return launch<2>(p, stream);
+    case 3: return launch<3>(p, stream);
+    default: return launch<4>(p, stream);
   }
-  if (e != cudaSuccess || !p.planned || p.groups < 2) return e;
-  cudaLaunchConfig_t config = {};
-  config.gridDim = dim3(kLdPairs, (unsigned)p.row_tiles, (unsigned)(p.groups - 1));
-  config.blockDim = dim3(128);
-  config.stream = stream;
-  cudaLaunchAttribute attr = {};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  config.attrs = &attr;
-  config.numAttrs = 1;
-  return cudaLaunchKernelEx(&config, qsa_latent_join_kernel, p);
 }
 
 }  // namespace qsa
