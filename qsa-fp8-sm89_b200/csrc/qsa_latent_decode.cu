@@ -157,13 +157,6 @@ __device__ __forceinline__ uint32_t ld_seen_word(const LatentDecodeParams& p, in
   return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u;
 }
 
-// The maximum, NaN where there is one.
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;\n" : "=f"(r) : "f"(a), "f"(b));
-  return r;
-}
-
 // Bits 20 to 27 of four words as the bytes of one.
 __device__ __forceinline__ uint32_t pack_codes(const uint32_t (&x)[4]) {
   const uint32_t even = __byte_perm(x[0], x[2], 0x7632), odd = __byte_perm(x[1], x[3], 0x7632);
@@ -408,25 +401,26 @@ __global__ void __launch_bounds__(kLdThreads, 1) qsa_latent_decode_kernel(const 
           if (failed) break;
           const uint32_t d = tmem + kLdTmemS + set * kLdTile;
           int s = set ? slot[1] : slot[0];
-#pragma unroll
-          for (int c = 0; c <= kChunks; ++c) {
+          // rolled: the roles' code together is more than the instruction caches hold
+#pragma unroll 1
+          for (int c = 0; c < kChunks; ++c) {
             const uint32_t bd = ring + (set * kLdSlots + s) * (kLdSlot / 16);
-            if (c < kChunks) {
-#pragma unroll
-              for (int kk = 0; kk < 4; ++kk) {
-                if (c * 4 + kk < 15)
-                  mma_f8_ts(d, tmem + c * 32 + kk * 8, bd + kk * 2, kIdescS, c > 0 || kk > 0);
-                else
-                  mma_f8_ss_plain_a(d, last, bd + kk * 2, kIdescS, 1u);
-              }
-            } else {
-#pragma unroll
-              for (int kk = 0; kk < 4; ++kk) mma_f16_ss(d, rotated + kk * 2, bd + kk * 2, kIdescR, 1u);
-              warp_commit(s_full + set);
-              warp_commit(empty + set * kLdSlots + s);
-            }
+            const uint32_t a = tmem + c * 32;
+            mma_f8_ts(d, a, bd, kIdescS, c > 0);
+            mma_f8_ts(d, a + 8, bd + 2, kIdescS, 1u);
+            mma_f8_ts(d, a + 16, bd + 4, kIdescS, 1u);
+            if (kChunks == 4 && c == 3)
+              mma_f8_ss_plain_a(d, last, bd + 6, kIdescS, 1u);
+            else
+              mma_f8_ts(d, a + 24, bd + 6, kIdescS, 1u);
             s = s + 1 == kLdSlots ? 0 : s + 1;
           }
+          const uint32_t bd = ring + (set * kLdSlots + s) * (kLdSlot / 16);
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk) mma_f16_ss(d, rotated + kk * 2, bd + kk * 2, kIdescR, 1u);
+          warp_commit(s_full + set);
+          warp_commit(empty + set * kLdSlots + s);
+          s = s + 1 == kLdSlots ? 0 : s + 1;
           if (set) slot[1] = s; else slot[0] = s;
         }
         ++seg;
@@ -450,15 +444,14 @@ __global__ void __launch_bounds__(kLdThreads, 1) qsa_latent_decode_kernel(const 
           const uint32_t ones = tmem + kLdTmemOnes, scales = tmem + kLdTmemScales + 2 * set;
           const uint32_t pd = weights + set * 4;
           int s = set ? slot[1] : slot[0];
-#pragma unroll
+#pragma unroll 1
           for (int c = 0; c < kChunks; ++c) {
-            const uint32_t ad = ring + (set * kLdSlots + s) * (kLdSlot / 16);
+            const uint32_t ad = ring + (set * kLdSlots + s) * (kLdSlot / 16), d = tmem + kLdTmemO + c * kLdPairs;
 #pragma unroll
             for (int kk = 0; kk < kLdTile / 32; ++kk) {
               const uint32_t idesc = idesc_o | kk << 4;  // the kk-th 32 tokens' scales
-              mma_mxf8_ss(tmem + kLdTmemO + c * kLdPairs, ad + kk * 256, pd + kk * 2, idesc, ones, scales, kk > 0 ? 1u : !first);
-              if (!few)
-                mma_mxf8_ss(tmem + kLdTmemO + c * kLdPairs, ad + kk * 256, pd + second + kk * 2, idesc, ones, scales, 1u);
+              mma_mxf8_ss(d, ad + kk * 256, pd + kk * 2, idesc, ones, scales, kk > 0 ? 1u : !first);
+              if (!few) mma_mxf8_ss(d, ad + kk * 256, pd + second + kk * 2, idesc, ones, scales, 1u);
             }
             warp_commit(empty + set * kLdSlots + s);
             s = s + 1 == kLdSlots ? 0 : s + 1;
@@ -595,13 +588,15 @@ __global__ void __launch_bounds__(kLdThreads, 1) qsa_latent_decode_kernel(const 
             const float4 l4 = *reinterpret_cast<const float4*>(ml + j);
             const float ss[4] = {s4.x, s4.y, s4.z, s4.w}, ll[4] = {l4.x, l4.y, l4.z, l4.w};
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const float other = __shfl_xor_sync(0xffffffffu, odd ? x[j + i] : y[j + i], 1);
-              const float v = fmaf(odd ? y[j + i] : x[j + i], km, other * kr);
-              u[j + i] = fmaf(v, ss[i], ll[i]);
+            for (int i = 0; i < 4; i += 2) {
+              const float a = __shfl_xor_sync(0xffffffffu, odd ? x[j + i] : y[j + i], 1);
+              const float b = __shfl_xor_sync(0xffffffffu, odd ? x[j + i + 1] : y[j + i + 1], 1);
+              const uint64_t own_term = pair2(odd ? y[j + i] : x[j + i], odd ? y[j + i + 1] : x[j + i + 1]);
+              const uint64_t v = fma2(own_term, pair2(km, km), mul2(pair2(a, b), pair2(kr, kr)));
+              unpair2(fma2(v, pair2(ss[i], ss[i + 1]), pair2(ll[i], ll[i + 1])), u[j + i], u[j + i + 1]);
             }
           }
-          if (p.nodes > 1 && tile * kLdTile + kLdTile > own) {
+          if (__builtin_expect(p.nodes > 1 && tile * kLdTile + kLdTile > own, 0)) {
             const int d0 = tile * kLdTile + 32 * half - own;
             const int word = d0 >> 5;
             const uint32_t bits = __funnelshift_r(ld_seen_word(p, now.row, node, word), ld_seen_word(p, now.row, node, word + 1), d0 & 31);
@@ -610,7 +605,7 @@ __global__ void __launch_bounds__(kLdThreads, 1) qsa_latent_decode_kernel(const 
               if (!((bits >> j) & 1u)) u[j] = -INFINITY;
           }
 #pragma unroll
-          for (int j = 0; j < 32; ++j) top = max_nan(top, u[j]);
+          for (int j = 0; j < 32; j += 2) top = max3_nan(top, u[j], u[j + 1]);
         } else {
           mbar_arrive(s_empty + set);
         }
@@ -634,7 +629,7 @@ __global__ void __launch_bounds__(kLdThreads, 1) qsa_latent_decode_kernel(const 
         };
         float e = scale32();
         // a reference that a weight passes by too much moves, and O and l with it
-        if (bar_vote(kLdBarSet + set, kLdSoft / 2, top > r + kLdFar || failed)) {
+        if (__builtin_expect(bar_vote(kLdBarSet + set, kLdSoft / 2, top > r + kLdFar || failed), 0)) {
           float* move = reinterpret_cast<float*>(smem + kLdMove) + set * kLdPairs;
           if (live) {
             const float next = fmaxf(r, fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1)));
@@ -684,26 +679,34 @@ __global__ void __launch_bounds__(kLdThreads, 1) qsa_latent_decode_kernel(const 
         if (live) {
           const float* mi = metas[m].inv + half * kLdHalf;
           const float rb = r + (e - kLdOne);
-          float sum = 0.f;
+          uint64_t sum2 = 0;
 #pragma unroll
           for (int j = 0; j < 32; j += 4) {
             const float4 i4 = *reinterpret_cast<const float4*>(mi + j);
             const float ii[4] = {i4.x, i4.y, i4.z, i4.w};
             uint32_t first[4], second[4];  // codes in bits 20 to 26
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
+            for (int i = 0; i < 4; i += 2) {
+              float a, b, c, d;
+              unpair2(add2(pair2(u[j + i], u[j + i + 1]), pair2(-rb, -rb)), a, b);
               // rounded to 8 bits
-              const float w = __uint_as_float((__float_as_uint(ex2(u[j + i] - rb)) + 0x8000u) & 0xffff0000u);
-              sum = fmaf(w, ii[i], sum);
+              const uint64_t w = pair2(__uint_as_float((__float_as_uint(ex2(a)) + 0x8000u) & 0xffff0000u),
+                                       __uint_as_float((__float_as_uint(ex2(b)) + 0x8000u) & 0xffff0000u));
+              sum2 = fma2(w, pair2(ii[i], ii[i + 1]), sum2);
               // times 2^-120 an E4M3 value is an fp32 one whose bits 20 to 26 are its code,
               // subnormal values too; half of the last step goes in before it is cut off
-              const float t = fmaf(w, 0x1p-120f, 0x1p-130f);
-              first[i] = __float_as_uint(t) & 0xfff00000u;
-              second[i] = __float_as_uint(t - __uint_as_float(first[i]));
+              const uint64_t t = fma2(w, pair2(0x1p-120f, 0x1p-120f), pair2(0x1p-130f, 0x1p-130f));
+              unpair2(t, a, b);
+              first[i] = __float_as_uint(a) & 0xfff00000u, first[i + 1] = __float_as_uint(b) & 0xfff00000u;
+              unpair2(add2(t, pair2(-__uint_as_float(first[i]), -__uint_as_float(first[i + 1]))), c, d);
+              second[i] = __float_as_uint(c), second[i + 1] = __float_as_uint(d);
             }
             hi[j / 4] = pack_codes(first);
             lo[j / 4] = pack_codes(second);
           }
+          float sum, sum_b;
+          unpair2(sum2, sum, sum_b);
+          sum += sum_b;
           l = fmaf(sum, ex2(e - kLdOne), l);
           if (!(top <= 3.402823466e38f)) l = __int_as_float(0x7fffffff);  // a NaN, or a score past fp32
         }
@@ -785,14 +788,9 @@ __global__ void __launch_bounds__(kLdThreads, 1) qsa_latent_decode_kernel(const 
             x[j] *= f.x, x[j + 1] *= f.y, x[j + 2] *= f.z, x[j + 3] *= f.w;
           }
           const int some = mine - b;
-          if (some >= 16) {
 #pragma unroll
-            for (int j = 0; j < 16; ++j) out[j * kRank] = round(x[j]);
-          } else {
-#pragma unroll
-            for (int j = 0; j < 16; ++j)
-              if (j < some) out[j * kRank] = round(x[j]);
-          }
+          for (int j = 0; j < 16; ++j)
+            if (j < some) out[j * kRank] = round(x[j]);
         }
       };
       if (now.whole)
