@@ -67,7 +67,7 @@ constexpr int kLdSlots = 11;     // of a set's ring
 constexpr int kLdMeta = 4;       // tiles whose scales are held
 constexpr int kLdReady = 16;     // tiles that may be ready at once: a ring holds 5 of two pieces each
 constexpr int kLdSoft = 256;     // threads of the softmax, half of them in each set
-constexpr int kLdLoader0 = 8, kLdMmaWarp = 12, kLdFenceWarp = 13, kLdWeighWarp = 14;
+constexpr int kLdLoader0 = 8, kLdFenceWarp = 13, kLdWeighWarp = 14, kLdMmaWarp = 15;
 // Four warpgroups: a set's softmax each, loaders, and the warps of the two products and
 // of the fence with an idle one. The softmax takes registers that the others hand back:
 // 2 x 160 + 96 + 96 of the 4 x 128 that the block is launched with.
@@ -257,7 +257,7 @@ __global__ void __launch_bounds__(kLdThreads, 1) qsa_latent_decode_kernel(const 
   walk.row = begin[0], walk.from = begin[1], walk.left = share[1];
   bool failed = false;
 
-  if (warp >= kLdLoader0 && warp < kLdMmaWarp) {
+  if (warp >= kLdLoader0 && warp < kLdLoader0 + 4) {
     // =============================== loaders ================================
     asm volatile("setmaxnreg.dec.sync.aligned.u32 96;\n");
     // Two warps a set, 32 tokens of each of its tiles each: a lane looks up its own
@@ -374,7 +374,7 @@ __global__ void __launch_bounds__(kLdThreads, 1) qsa_latent_decode_kernel(const 
       uint4* out = reinterpret_cast<uint4*>(p.out + (r * pairs + rt * kLdPairs) * kRank);
       for (int i = lane; i < mine * kRank / 8; i += 32) out[i] = make_uint4(0u, 0u, 0u, 0u);
     }
-  } else if (warp >= kLdMmaWarp) {
+  } else if (warp >= kLdLoader0 + 4) {
     // =============================== products ===============================
     asm volatile("setmaxnreg.dec.sync.aligned.u32 96;\n");
     const uint32_t ring = desc_low(base_s + kLdRing);  // K: tokens by bytes (V^T: the same, MN-major)
@@ -496,8 +496,14 @@ __global__ void __launch_bounds__(kLdThreads, 1) qsa_latent_decode_kernel(const 
     asm volatile("setmaxnreg.inc.sync.aligned.u32 160;\n");
     const bool odd = (lane & 1) != 0;
     const int set = warp >> 2, q4 = warp & 3;
-    const int pair = 16 * q4 + (lane >> 1);             // this lane pair's (node, head) in the CTA
-    const bool live = 16 * q4 < mine;                   // the warp has one
+    // Quarter q of the lanes has the pairs 16 q .. 16 q + 15. Up to 32 pairs stand
+    // there twice, in a quarter or two for each set, so that the sets' warps run on
+    // different quarters of the SM too.
+    const int blocks = cols / 16;                       // of 16 pairs
+    const int block0 = few ? q4 % blocks : q4;          // the quarter's
+    const bool placed = few ? q4 < 2 * blocks : q4 < blocks;
+    const int pair = 16 * block0 + (lane >> 1);         // this lane pair's (node, head) in the CTA
+    const bool live = placed && (!few || q4 / blocks == set);  // the warp has scores to look at
     const int rho = rt * kLdPairs + pair;
     const int node = min(rho / p.heads, p.nodes - 1);
     const int half = odd ? 1 : 0;                       // this lane's 32 tokens of a tile
@@ -509,8 +515,8 @@ __global__ void __launch_bounds__(kLdThreads, 1) qsa_latent_decode_kernel(const 
     const int row_blocks = (pairs + kLdBlockPairs - 1) / kLdBlockPairs;
     auto place_q = [&](int row) -> float {
       float qs = 0.f;
-      if (live) {
-        const uint8_t* block = p.queries + ((int64_t)row * row_blocks + rt * 4 + q4) * ld_block_bytes(kRank);
+      if (placed) {
+        const uint8_t* block = p.queries + ((int64_t)row * row_blocks + rt * 4 + block0) * ld_block_bytes(kRank);
         const uint4* words = reinterpret_cast<const uint4*>(block) + set * 4 * kChunks * 32 + lane;
         const uint4* rotated = reinterpret_cast<const uint4*>(block + 32 * kRank) + set * 64 + lane;
         uint4 w[4 * kChunks], t[2];
@@ -578,8 +584,8 @@ __global__ void __launch_bounds__(kLdThreads, 1) qsa_latent_decode_kernel(const 
           const float* ms = metas[m].s + half * kLdHalf;
           const float* ml = metas[m].lg + half * kLdHalf;
           float x[32], y[32];
-          tmem_ld_wait<32>(tmem + lane_base + kLdTmemS + kLdTile * set, x);
-          tmem_ld_wait<32>(tmem + lane_base + kLdTmemS + kLdTile * set + 32, y);
+          const uint32_t at = tmem + lane_base + kLdTmemS + kLdTile * set;
+          tmem_ld_2x32_wait(at, at + 32, x, y);
           tc_fence_before();
           mbar_arrive(s_empty + set);
 #pragma unroll
@@ -616,8 +622,7 @@ __global__ void __launch_bounds__(kLdThreads, 1) qsa_latent_decode_kernel(const 
           failed = __any_sync(0xffffffffu, failed);
           if (live) {
             const float next = pair_r[pair];
-            l *= ex2(r - next);
-            r = next;
+            if (next != r) l *= ex2(r - next), r = next;
           }
         }
         // the scale of this lane's 32 weights
