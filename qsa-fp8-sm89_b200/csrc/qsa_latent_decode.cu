@@ -105,7 +105,7 @@ constexpr int kLdMove = kLdRef + kLdPairs * 4;                     // float [2 s
 constexpr int kLdScales = kLdMove + 2 * kLdPairs * 4;              // bytes [2 sets][2 tiles][64][4], of 32 tokens each
 constexpr int kLdBars = kLdScales + 4 * kLdPairs * 4;
 constexpr int kLdNumBars = 4 * kLdSlots + 2 * kLdMeta + kLdReady + 16;
-constexpr int kLdMisc = kLdBars + kLdNumBars * 8;  // tensor memory address, abort flag, group's range
+constexpr int kLdMisc = kLdBars + kLdNumBars * 8;  // tensor memory address, group's range
 constexpr int kLdSmem = kLdMisc + 64 + 1024;
 static_assert(kLdSmem + 256 <= 232448 && kLdBars % 8 == 0 && kLdMisc % 8 == 0 && kLdMetaAt % 16 == 0, "shared memory");
 
@@ -189,7 +189,7 @@ __global__ void __launch_bounds__(kLdThreads, 1) qsa_latent_decode_kernel(const 
   uint64_t* o_empty = o_done + 1;              // results taken -> products, each segment
   uint64_t* drain = o_empty + 1;               // [2]
   uint32_t* tmem_at = reinterpret_cast<uint32_t*>(smem + kLdMisc);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + kLdMisc + 8);
+  const uint32_t tries = tries_of(p.wait_limit_ns);
   int* begin = reinterpret_cast<int*>(smem + kLdMisc + 16);          // row, tile
   int64_t* share = reinterpret_cast<int64_t*>(smem + kLdMisc + 24);  // first unit, units
   LdMeta* metas = reinterpret_cast<LdMeta*>(smem + kLdMetaAt);
@@ -205,23 +205,23 @@ __global__ void __launch_bounds__(kLdThreads, 1) qsa_latent_decode_kernel(const 
   const bool few = mine <= kLdPairs / 2;
   const int cols = (mine + 15) / 16 * 16;            // columns of the first terms
   const int lo_row = few ? cols : kLdPairs;          // where the second terms' rows of P begin
+  const int blocks = cols / 16;                      // of 16 pairs: a softmax warp of each set has one
 
   if (tid == 0) {
     for (int i = 0; i < 2 * kLdSlots; ++i) mbar_init(full + i, 64), mbar_init(empty + i, 1);
-    for (int i = 0; i < kLdMeta; ++i) mbar_init(meta_full + i, 2), mbar_init(meta_empty + i, 4);
+    for (int i = 0; i < kLdMeta; ++i) mbar_init(meta_full + i, 2), mbar_init(meta_empty + i, blocks);
     for (int i = 0; i < kLdReady; ++i) mbar_init(ready + i, 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(s_full + i, 1);
-      mbar_init(s_empty + i, kLdSoft / 2);
+      mbar_init(s_empty + i, 32 * blocks);
       mbar_init(p_full + i, kLdSoft / 2);
       mbar_init(o_full + i, 1);
-      mbar_init(r_done + i, 4);
+      mbar_init(r_done + i, blocks);
       mbar_init(drain + i, 1);
     }
     mbar_init(q_full, kLdSoft);
     mbar_init(o_done, 1);
     mbar_init(o_empty, kLdSoft);
-    *abort_flag = 0;
     fence_mbar_init();
   }
   if (warp == kLdMmaWarp) {
@@ -270,7 +270,7 @@ __global__ void __launch_bounds__(kLdThreads, 1) qsa_latent_decode_kernel(const 
     uint64_t* const my_empty = empty + set * kLdSlots;
     int issued = 0, tile_n = 0;
     auto wait_free = [&](uint64_t* bar, uint32_t parity) -> bool {
-      return __all_sync(0xffffffffu, wait_or_abort(bar, parity, abort_flag, p.wait_limit_ns));
+      return __all_sync(0xffffffffu, wait_tries(bar, parity, tries));
     };
     while (!failed && walk.next(p)) {
       int count;
@@ -379,7 +379,7 @@ __global__ void __launch_bounds__(kLdThreads, 1) qsa_latent_decode_kernel(const 
     asm volatile("setmaxnreg.dec.sync.aligned.u32 96;\n");
     const uint32_t ring = desc_low(base_s + kLdRing);  // K: tokens by bytes (V^T: the same, MN-major)
     auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
-      if (!__all_sync(0xffffffffu, wait_or_abort(bar, parity, abort_flag, p.wait_limit_ns))) return false;
+      if (!__all_sync(0xffffffffu, wait_tries(bar, parity, tries))) return false;
       tc_fence_after();
       return true;
     };
@@ -480,7 +480,7 @@ __global__ void __launch_bounds__(kLdThreads, 1) qsa_latent_decode_kernel(const 
           uint32_t t = set ? turn[1] : turn[0];
 #pragma unroll 1
           for (int c = 0; c <= kChunks && !failed; ++c) {
-            failed = !wait_or_abort(full + set * kLdSlots + s, t, abort_flag, p.wait_limit_ns);
+            failed = !wait_tries(full + set * kLdSlots + s, t, tries);
             if (++s == kLdSlots) s = 0, t ^= 1u;
           }
           if (set) slot[1] = s, turn[1] = t; else slot[0] = s, turn[0] = t;
@@ -499,7 +499,6 @@ __global__ void __launch_bounds__(kLdThreads, 1) qsa_latent_decode_kernel(const 
     // Quarter q of the lanes has the pairs 16 q .. 16 q + 15. Up to 32 pairs stand
     // there twice, in a quarter or two for each set, so that the sets' warps run on
     // different quarters of the SM too.
-    const int blocks = cols / 16;                       // of 16 pairs
     const int block0 = few ? q4 % blocks : q4;          // the quarter's
     const bool placed = few ? q4 < 2 * blocks : q4 < blocks;
     const int pair = 16 * block0 + (lane >> 1);         // this lane pair's (node, head) in the CTA
@@ -573,14 +572,14 @@ __global__ void __launch_bounds__(kLdThreads, 1) qsa_latent_decode_kernel(const 
         const int n = first_n + tile - now.from;
         const int m = n % kLdMeta;
         const uint32_t turn = (uint32_t)((n >> 1) & 1);
-        if (!failed)
-          failed = !(wait_or_abort(meta_full + m, (uint32_t)((n / kLdMeta) & 1), abort_flag, p.wait_limit_ns) &&
-                     wait_or_abort(s_full + set, turn, abort_flag, p.wait_limit_ns));
-        failed = __any_sync(0xffffffffu, failed);
-        tc_fence_after();
+        const bool begun = tile > now.from;
         float u[32];
         float top = -INFINITY;
-        if (live && !failed) {
+        if (live) {
+          if (!failed)
+            failed = !(wait_tries(meta_full + m, (uint32_t)((n / kLdMeta) & 1), tries) && wait_tries(s_full + set, turn, tries));
+          failed = __any_sync(0xffffffffu, failed);
+          tc_fence_after();
           const float* ms = metas[m].s + half * kLdHalf;
           const float* ml = metas[m].lg + half * kLdHalf;
           float x[32], y[32];
@@ -612,15 +611,10 @@ __global__ void __launch_bounds__(kLdThreads, 1) qsa_latent_decode_kernel(const 
           }
 #pragma unroll
           for (int j = 0; j < 32; j += 2) top = max3_nan(top, u[j], u[j + 1]);
-        } else {
-          mbar_arrive(s_empty + set);
-        }
-        // the reference, as the tile before left it
-        const bool begun = tile > now.from;
-        if (begun) {
-          if (!failed) failed = !wait_or_abort(r_done + (set ^ 1), (uint32_t)(((n - 1) >> 1) & 1), abort_flag, p.wait_limit_ns);
-          failed = __any_sync(0xffffffffu, failed);
-          if (live) {
+          // the reference, as the tile before left it
+          if (begun) {
+            if (!failed) failed = !wait_tries(r_done + (set ^ 1), (uint32_t)(((n - 1) >> 1) & 1), tries);
+            failed = __any_sync(0xffffffffu, failed);
             const float next = pair_r[pair];
             if (next != r) l *= ex2(r - next), r = next;
           }
@@ -645,8 +639,8 @@ __global__ void __launch_bounds__(kLdThreads, 1) qsa_latent_decode_kernel(const 
           }
           // all products before this tile's
           if (begun && !failed)
-            failed = !((n < 2 || wait_or_abort(o_full + set, turn ^ 1u, abort_flag, p.wait_limit_ns)) &&
-                       wait_or_abort(o_full + (set ^ 1), (uint32_t)(((n - 1) >> 1) & 1), abort_flag, p.wait_limit_ns));
+            failed = !((n < 2 || wait_tries(o_full + set, turn ^ 1u, tries)) &&
+                       wait_tries(o_full + (set ^ 1), (uint32_t)(((n - 1) >> 1) & 1), tries));
           failed = __any_sync(0xffffffffu, failed);
           if (bar_vote(kLdBarSet + set, kLdSoft / 2, failed)) {
             failed = true;
@@ -676,9 +670,11 @@ __global__ void __launch_bounds__(kLdThreads, 1) qsa_latent_decode_kernel(const 
           e = scale32();
           bar_sync(kLdBarSet + set, kLdSoft / 2);
         }
-        if (live && !odd) pair_r[pair] = r;
-        __syncwarp();
-        if (lane == 0) mbar_arrive(r_done + set);
+        if (live) {
+          if (!odd) pair_r[pair] = r;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(r_done + set);
+        }
         // ---- weights
         uint32_t hi[8], lo[8];
         if (live) {
@@ -715,10 +711,12 @@ __global__ void __launch_bounds__(kLdThreads, 1) qsa_latent_decode_kernel(const 
           l = fmaf(sum, ex2(e - kLdOne), l);
           if (!(top <= 3.402823466e38f)) l = __int_as_float(0x7fffffff);  // a NaN, or a score past fp32
         }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(meta_empty + m);
+        if (live) {
+          __syncwarp();
+          if (lane == 0) mbar_arrive(meta_empty + m);
+        }
         // the product of the set's tile before has read its weights and their scales
-        if (n >= 2 && !failed) failed = !wait_or_abort(o_full + set, turn ^ 1u, abort_flag, p.wait_limit_ns);
+        if (n >= 2 && !failed) failed = !wait_tries(o_full + set, turn ^ 1u, tries);
         failed = __any_sync(0xffffffffu, failed);
         if (live) {
 #pragma unroll
@@ -741,7 +739,7 @@ __global__ void __launch_bounds__(kLdThreads, 1) qsa_latent_decode_kernel(const 
       // ---- the segment's results
       const int last = first_n + (now.to - now.from) - 1;
       if ((last & 1) != set && !failed)  // the other set's last tile
-        failed = !wait_or_abort(r_done + (set ^ 1), (uint32_t)((last >> 1) & 1), abort_flag, p.wait_limit_ns);
+        failed = !wait_tries(r_done + (set ^ 1), (uint32_t)((last >> 1) & 1), tries);
       failed = __any_sync(0xffffffffu, failed);
       if (bar_vote(kLdBarAll, kLdSoft, failed)) {
         failed = true;
@@ -749,7 +747,7 @@ __global__ void __launch_bounds__(kLdThreads, 1) qsa_latent_decode_kernel(const 
       }
       // all scores are done, and the queries free
       if (more) next_qs = place_q(walk.row);
-      failed = !wait_or_abort(o_done, (uint32_t)(seg & 1), abort_flag, p.wait_limit_ns);
+      failed = !wait_tries(o_done, (uint32_t)(seg & 1), tries);
       failed = __any_sync(0xffffffffu, failed);
       if (live) {
         const float end_r = pair_r[pair];
@@ -811,7 +809,6 @@ __global__ void __launch_bounds__(kLdThreads, 1) qsa_latent_decode_kernel(const 
   }
 
   if (failed) {
-    *abort_flag = 1;
     if (p.err) atomicOr(p.err, 1);
   }
   __syncwarp();

@@ -115,7 +115,7 @@ __global__ void __launch_bounds__(kLpThreads, 1)
   uint64_t* fixed = v_full + 2;        // fixers -> products, softmax
   uint64_t* drain = fixed + 1;
   uint32_t* tmem_at = reinterpret_cast<uint32_t*>(smem + kLpMisc);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + kLpMisc + 8);
+  const uint32_t tries = tries_of(p.wait_limit_ns);
   volatile int* odd_values = reinterpret_cast<volatile int*>(smem + kLpMisc + 12);  // values that were cleared
   LpBlock* found = reinterpret_cast<LpBlock*>(smem + kLpMisc + 16);
 
@@ -131,7 +131,6 @@ __global__ void __launch_bounds__(kLpThreads, 1)
     }
     mbar_init(fixed, 64);
     mbar_init(drain, 1);
-    *abort_flag = 0;
     *odd_values = 0;
     *found = LpBlock{0, 0, 0, 0, -1};  // a block past the last one
     fence_mbar_init();
@@ -220,7 +219,7 @@ __global__ void __launch_bounds__(kLpThreads, 1)
           // a tile's values are brought both or not at all
           for (int at = pos; at <= (c == 3 ? pos + 1 : pos) && !failed; ++at)
             failed = at >= kLpSlots &&
-                     !wait_or_abort(empty + at % kLpSlots, (uint32_t)((at / kLpSlots - 1) & 1), abort_flag, p.wait_limit_ns);
+                     !wait_tries(empty + at % kLpSlots, (uint32_t)((at / kLpSlots - 1) & 1), tries);
           if (failed) break;
           // values for the fixers land on a barrier of their own, each phase of which
           // they wait for; the products wait for the fixers then
@@ -251,7 +250,7 @@ __global__ void __launch_bounds__(kLpThreads, 1)
       constexpr uint32_t kIdescS = idesc_f16(128, kLpTile, kBf16, false);
       constexpr uint32_t kIdescO = idesc_f16(128, 64, kBf16, true);
       auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
-        if (!__all_sync(0xffffffffu, wait_or_abort(bar, parity, abort_flag, p.wait_limit_ns))) return false;
+        if (!__all_sync(0xffffffffu, wait_tries(bar, parity, tries))) return false;
         tc_fence_after();
         return true;
       };
@@ -308,7 +307,7 @@ __global__ void __launch_bounds__(kLpThreads, 1)
       for (int j = whole; j < nk; ++j) {
         bool any = false;
         const int f = j - whole;
-        failed = !__all_sync(0xffffffffu, wait_or_abort(v_full + f % 2, (uint32_t)((f / 2) & 1), abort_flag, p.wait_limit_ns));
+        failed = !__all_sync(0xffffffffu, wait_tries(v_full + f % 2, (uint32_t)((f / 2) & 1), tries));
         if (failed) break;
 #pragma unroll 1
         for (int c = 0; c < 2; ++c) {
@@ -350,7 +349,7 @@ __global__ void __launch_bounds__(kLpThreads, 1)
     float r = kLowest, l = 0.f;
 #pragma unroll 1
     for (int j = 0; j < tiles; ++j) {
-      if (!failed) failed = !wait_or_abort(s_full + t, (uint32_t)(j & 1), abort_flag, p.wait_limit_ns);
+      if (!failed) failed = !wait_tries(s_full + t, (uint32_t)(j & 1), tries);
       failed = __any_sync(0xffffffffu, failed);
       if (failed) break;
       tc_fence_after();
@@ -381,7 +380,7 @@ __global__ void __launch_bounds__(kLpThreads, 1)
         r = next;
         l *= f;
         if (j > 0) {
-          failed = !wait_or_abort(o_full + t, (uint32_t)((j - 1) & 1), abort_flag, p.wait_limit_ns);
+          failed = !wait_tries(o_full + t, (uint32_t)((j - 1) & 1), tries);
           failed = __any_sync(0xffffffffu, failed);
           if (failed) break;
           tc_fence_after();
@@ -415,8 +414,8 @@ __global__ void __launch_bounds__(kLpThreads, 1)
       tc_fence_before();
       mbar_arrive(p_full + t);
     }
-    if (tiles > 0 && !failed) failed = !wait_or_abort(o_full + t, (uint32_t)((tiles - 1) & 1), abort_flag, p.wait_limit_ns);
-    if (nk > whole && !failed) failed = !wait_or_abort(fixed, (uint32_t)((nk - whole - 1) & 1), abort_flag, p.wait_limit_ns);
+    if (tiles > 0 && !failed) failed = !wait_tries(o_full + t, (uint32_t)((tiles - 1) & 1), tries);
+    if (nk > whole && !failed) failed = !wait_tries(fixed, (uint32_t)((nk - whole - 1) & 1), tries);
     failed = __any_sync(0xffffffffu, failed);
     if (!failed && b.first >= 0) {
       tc_fence_after();
@@ -450,7 +449,6 @@ __global__ void __launch_bounds__(kLpThreads, 1)
   }
 
   if (failed) {
-    *abort_flag = 1;
     if (p.err) atomicOr(p.err, 1);
   }
   __syncwarp();

@@ -24,32 +24,18 @@ __device__ __forceinline__ bool bar_vote(int id, int count, bool pred) {
   return r != 0u;
 }
 
-// Bounded wait that also gives up once another role raised the abort flag; it
-// raises the flag when its own limit runs out. The thread sleeps at the barrier for
-// up to 20 us at a time: a reading of the timer takes the unit that 2^x takes.
-__device__ __forceinline__ bool mbar_sleep_wait(uint64_t* bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 20000;\nselp.u32 %0, 1, 0, p;\n}\n"
-               : "=r"(ok)
-               : "r"(smem_u32(bar)), "r"(parity)
-               : "memory");
-  return ok != 0;
+// Bounded wait: false once `tries` looks at the barrier, of 20 ns or more each, have
+// not seen the phase end. It is this short because it stands in so many places: the
+// roles' code together is more than the instruction caches hold. (A try with a time to
+// sleep wakes up to 2 us after its barrier.)
+__device__ __forceinline__ bool wait_tries(uint64_t* bar, uint32_t parity, uint32_t tries) {
+#pragma unroll 1
+  for (uint32_t i = 0; !mbar_try_wait(bar, parity); ++i)
+    if (i >= tries) return false;
+  return true;
 }
-__device__ __forceinline__ bool wait_or_abort(uint64_t* bar, uint32_t parity, volatile int* abort_flag, uint64_t limit_ns) {
-  if (mbar_sleep_wait(bar, parity)) return true;
-  uint64_t t0;
-  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t0));
-  while (true) {
-    if (mbar_sleep_wait(bar, parity)) return true;
-    if (*abort_flag) return false;
-    uint64_t t1;
-    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t1));
-    if (t1 - t0 > limit_ns) {
-      *abort_flag = 1;
-      return false;
-    }
-  }
-}
+// Tries that a limit in ns allows.
+__device__ __forceinline__ uint32_t tries_of(uint64_t limit_ns) { return (uint32_t)(limit_ns / 1024 < 0x7fffffffu ? limit_ns / 1024 : 0x7fffffffu); }
 
 // Descriptors of 128-byte swizzled operands whose 8-row groups lie 1024 bytes
 // apart: the high words are all the same, the low word is the address in 16-byte
