@@ -298,7 +298,8 @@ struct LatentPrefillParams {
   void* out;
   const int32_t* cu_q;
   const int32_t* cu_k;
-  float score_scale_log2;
+  float score_scale_log2;  // |softmax_scale| * log2(e), above zero
+  int negative;            // softmax_scale is
   int entries, q_tokens, k_tokens, heads, causal, dtype;
   int64_t q_stride, q_head_stride, k_stride, k_head_stride, v_stride, v_head_stride, k_rope_stride;
   int* err;

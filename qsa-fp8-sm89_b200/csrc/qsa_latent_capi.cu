@@ -214,7 +214,9 @@ int qsa_b200_latent_prefill(const qsa_b200_latent_prefill_args* a, qsa_b200_stre
   p.out = a->out;
   p.cu_q = a->cu_q;
   p.cu_k = a->cu_k;
-  p.score_scale_log2 = a->softmax_scale * 1.4426950408889634f;
+  const float scale = std::fabs(a->softmax_scale) * 1.4426950408889634f;
+  p.score_scale_log2 = scale == 0.f ? 0x1p-149f : scale;  // what is masked stays below all else
+  p.negative = a->softmax_scale < 0.f ? 1 : 0;
   p.entries = a->entries;
   p.q_tokens = a->q_tokens;
   p.k_tokens = a->k_tokens;

@@ -248,7 +248,7 @@ __global__ void __launch_bounds__(kLpThreads, 1)
     } else if (warp == kLpMmaWarp && nk > 0) {
       // ============================== products ==============================
       constexpr uint32_t kIdescS = idesc_f16(128, kLpTile, kBf16, false);
-      constexpr uint32_t kIdescO = idesc_f16(128, 64, kBf16, true);
+      constexpr uint32_t kIdescO = idesc_f16(128, 128, kBf16, true), kIdescHalf = idesc_f16(128, 64, kBf16, true);
       auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
         if (!__all_sync(0xffffffffu, wait_tries(bar, parity, tries))) return false;
         tc_fence_after();
@@ -275,16 +275,24 @@ __global__ void __launch_bounds__(kLpThreads, 1)
         const bool last = t == 1 || j >= nk1;
         if (!wait(p_full + t, (uint32_t)(j & 1))) return false;
         if (j >= whole && !wait(fixed, (uint32_t)((j - whole) & 1))) return false;
-#pragma unroll 1
-        for (int c = 0; c < 2; ++c) {
-          const int pos = 5 * j + 3 + c;
-          if (!wait_slot(pos)) return false;
-          const uint32_t b0 = desc_low(base_s + kLpRing) + pos % kLpSlots * (kLpChunk / 16);
+        const int pos = 5 * j + 3, s0 = pos % kLpSlots;
+        if (!wait_slot(pos) || !wait_slot(pos + 1)) return false;
+        const uint32_t d = tmem + kLpTmemO + t * 128, a = tmem + kLpTmemS + t * 128;
+        if (s0 + 1 < kLpSlots) {  // both halves of the values in one product
+          const uint32_t b0 = desc_low(base_s + kLpRing, kLpChunk) + s0 * (kLpChunk / 16);
 #pragma unroll
-          for (int kk = 0; kk < 8; ++kk)
-            mma_f16_ts(tmem + kLpTmemO + t * 128 + c * 64, tmem + kLpTmemS + t * 128 + kk * 8, b0 + kk * 128, kIdescO,
-                       kk > 0 ? 1u : j > 0);
-          if (last) warp_commit(empty + pos % kLpSlots);
+          for (int kk = 0; kk < 8; ++kk) mma_f16_ts(d, a + kk * 8, b0 + kk * 128, kIdescO, kk > 0 ? 1u : j > 0);
+        } else {
+#pragma unroll 1
+          for (int c = 0; c < 2; ++c) {
+            const uint32_t b0 = desc_low(base_s + kLpRing) + (pos + c) % kLpSlots * (kLpChunk / 16);
+#pragma unroll
+            for (int kk = 0; kk < 8; ++kk) mma_f16_ts(d + c * 64, a + kk * 8, b0 + kk * 128, kIdescHalf, kk > 0 ? 1u : j > 0);
+          }
+        }
+        if (last) {
+          warp_commit(empty + s0);
+          warp_commit(empty + (pos + 1) % kLpSlots);
         }
         warp_commit(o_full + t);
         return true;
@@ -354,25 +362,31 @@ __global__ void __launch_bounds__(kLpThreads, 1)
       if (failed) break;
       tc_fence_after();
       float s[4][32];
-#pragma unroll
-      for (int c = 0; c < 4; ++c) tmem_ld_wait<32>(s_at + 32 * c, s[c]);
-      float top = -INFINITY;
+      tmem_ld_2x32_wait(s_at, s_at + 32, s[0], s[1]);
+      tmem_ld_2x32_wait(s_at + 64, s_at + 96, s[2], s[3]);
       const int left = (int)min((int64_t)kLpTile, seen - (int64_t)j * kLpTile);  // visible columns of the tile
-      const bool cut = __any_sync(0xffffffffu, left < kLpTile);
+      if (p.negative) {
 #pragma unroll
-      for (int c = 0; c < 4; ++c)
+        for (int c = 0; c < 4; ++c)
 #pragma unroll
-        for (int k = 0; k < 32; ++k) s[c][k] *= p.score_scale_log2;
-      if (cut) {
+          for (int k = 0; k < 32; ++k) s[c][k] = -s[c][k];
+      }
+      if (__any_sync(0xffffffffu, left < kLpTile)) {
 #pragma unroll
         for (int c = 0; c < 4; ++c)
 #pragma unroll
           for (int k = 0; k < 32; ++k) s[c][k] = 32 * c + k < left ? s[c][k] : -INFINITY;
       }
+      float tops[4];
 #pragma unroll
-      for (int c = 0; c < 4; ++c)
+      for (int c = 0; c < 4; ++c) tops[c] = max3(s[c][0], s[c][1], s[c][2]);
 #pragma unroll
-        for (int k = 0; k < 32; ++k) top = fmaxf(top, s[c][k]);
+      for (int k = 3; k < 31; k += 2)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tops[c] = max3(tops[c], s[c][k], s[c][k + 1]);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) tops[c] = fmaxf(tops[c], s[c][31]);
+      const float top = fmaxf(max3(tops[0], tops[1], tops[2]), tops[3]) * p.score_scale_log2;
       const bool moves = top > r + kLpLazy;
       if (__any_sync(0xffffffffu, moves)) {
         const float next = moves ? top : r;
@@ -395,7 +409,8 @@ __global__ void __launch_bounds__(kLpThreads, 1)
           }
         }
       }
-      float sum0 = 0.f, sum1 = 0.f;
+      uint64_t sum[2] = {0, 0};
+      const uint64_t scale2 = pair2(p.score_scale_log2, p.score_scale_log2), back2 = pair2(-r, -r);
 #pragma unroll
       for (int c = 0; c < 4; c += 2) {
         uint32_t w[32];
@@ -403,13 +418,19 @@ __global__ void __launch_bounds__(kLpThreads, 1)
         for (int h = 0; h < 2; ++h)
 #pragma unroll
           for (int k = 0; k < 32; k += 2) {
-            const float a = ex2(s[c + h][k] - r), d = ex2(s[c + h][k + 1] - r);
-            sum0 += a, sum1 += d;
+            float a, d;
+            unpair2(fma2(pair2(s[c + h][k], s[c + h][k + 1]), scale2, back2), a, d);
+            a = ex2(a), d = ex2(d);
+            sum[h] = add2(sum[h], pair2(a, d));
             w[16 * h + k / 2] = pack2<T>(a, d);
           }
         tmem_st(s_at + 16 * c, w);
       }
-      l += sum0 + sum1;
+      {
+        float a, d;
+        unpair2(add2(sum[0], sum[1]), a, d);
+        l += a + d;
+      }
       tmem_wait_st();
       tc_fence_before();
       mbar_arrive(p_full + t);
