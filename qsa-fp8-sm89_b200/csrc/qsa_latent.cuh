@@ -1,6 +1,7 @@
 // Device helpers of the latent cache's kernels: the tokens that a call's entries
 // name, and their places in the cache.
 #pragma once
+#include <atomic>
 
 #include "qsa_common.cuh"
 #include "qsa_internal.h"
@@ -65,5 +66,18 @@ __device__ __forceinline__ void latent_load4(const __half* at, float (&x)[4]) {
 __device__ __forceinline__ float latent_to_float(float x) { return x; }
 __device__ __forceinline__ float latent_to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
 __device__ __forceinline__ float latent_to_float(__half x) { return __half2float(x); }
+
+// SMs of the current device.
+inline int latent_sm_count() {
+  static std::atomic<int> known[64] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 148;
+  int n = known[dev & 63].load(std::memory_order_relaxed);
+  if (n == 0) {
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n < 1) n = 148;
+    known[dev & 63].store(n, std::memory_order_relaxed);
+  }
+  return n;
+}
 
 }  // namespace qsa

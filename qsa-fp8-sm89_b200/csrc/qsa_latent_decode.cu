@@ -981,18 +981,6 @@ __global__ void __launch_bounds__(128) qsa_latent_join_kernel(const __grid_const
       make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
 }
 
-int sm_count() {
-  static std::atomic<int> known[64] = {};
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) return 148;
-  int n = known[dev & 63].load(std::memory_order_relaxed);
-  if (n == 0) {
-    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n < 1) n = 148;
-    known[dev & 63].store(n, std::memory_order_relaxed);
-  }
-  return n;
-}
-
 int64_t align256(int64_t x) { return (x + 255) / 256 * 256; }
 
 // Launches a kernel that waits for its prerequisites itself (early: it may start
@@ -1044,7 +1032,7 @@ int64_t query_bytes(const LatentDecodeParams& p) {
 int64_t latent_decode_plan(LatentDecodeParams& p) {
   p.row_tiles = (p.nodes * p.heads + kLdPairs - 1) / kLdPairs;
   const int64_t columns = p.indices ? p.topk : (int64_t)p.cache.pages_per_req * p.cache.page_size;
-  const int sms = sm_count();
+  const int sms = latent_sm_count();
   p.planned = (columns + kLdTile - 1) / kLdTile > kLdDirectTiles || (int64_t)p.rows * p.row_tiles > sms;
   p.groups = p.planned ? (sms / p.row_tiles > 1 ? sms / p.row_tiles : 1) : p.rows;
   int64_t need = query_bytes(p);

@@ -105,6 +105,76 @@ __device__ __forceinline__ void warp_commit(uint64_t* bar) {
       : "memory");
 }
 
+// The same for a pair of CTAs (a cluster of two): the even one issues. Each holds its
+// 128 of the 256 rows of A and D, and half of B's columns (its N is the instruction's
+// over two), all at the same addresses.
+__device__ __forceinline__ void pair_mma_f16_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n.reg .pred p, e;\nelect.sync _|e, 0xffffffff;\nsetp.ne.b32 p, %4, 0;\n"
+      ".reg .b64 bd;\nmov.b64 bd, {%2, %5};\n"
+      "@e tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], bd, %3, p;\n}\n" ::"r"(d), "r"(a), "r"(b), "r"(idesc),
+      "r"(accumulate), "n"(kDescHigh)
+      : "memory");
+}
+__device__ __forceinline__ void pair_mma_f16_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n.reg .pred p, e;\nelect.sync _|e, 0xffffffff;\nsetp.ne.b32 p, %4, 0;\n"
+      ".reg .b64 ad, bd;\nmov.b64 ad, {%1, %5};\nmov.b64 bd, {%2, %5};\n"
+      "@e tcgen05.mma.cta_group::2.kind::f16 [%0], ad, bd, %3, p;\n}\n" ::"r"(d), "r"(a), "r"(b), "r"(idesc),
+      "r"(accumulate), "n"(kDescHigh)
+      : "memory");
+}
+// Arrives on the barrier at this address in both CTAs.
+__device__ __forceinline__ void pair_commit(uint64_t* bar) {
+  asm volatile(
+      "{\n.reg .pred e;\nelect.sync _|e, 0xffffffff;\n"
+      "@e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n}\n" ::"r"(smem_u32(bar)),
+      "h"((uint16_t)3)
+      : "memory");
+}
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_ctarank;\n" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t smem_of(const void* at, uint32_t rank) {  // the address in another CTA of the cluster
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(r) : "r"(smem_u32(at)), "r"(rank));
+  return r;
+}
+// Arrivals and waits between the CTAs of a cluster.
+__device__ __forceinline__ void cluster_arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];\n" ::"r"(bar) : "memory");
+}
+// Orders nothing but what tcgen05 fences do, as tensor memory needs: the release above
+// takes 500 cycles and more.
+__device__ __forceinline__ void cluster_arrive_relaxed(uint32_t bar) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];\n" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ bool cluster_wait_tries(uint64_t* bar, uint32_t parity, uint32_t tries) {
+#pragma unroll 1
+  for (uint32_t i = 0;; ++i) {
+    uint32_t ok;
+    asm volatile(
+        "{\n.reg .pred p;\nmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}\n"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    if (ok) return true;
+    if (i >= tries) return false;
+  }
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+}
+__device__ __forceinline__ void pair_tmem_alloc(uint32_t* at, uint32_t columns) {  // a warp of each CTA
+  asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(at)), "r"(columns) : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;\n" ::: "memory");
+}
+__device__ __forceinline__ void pair_tmem_free(uint32_t taddr, uint32_t columns) {
+  asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;\n" ::"r"(taddr), "r"(columns) : "memory");
+}
+
 // Instruction descriptor of kind::f16, A and B both bf16 or both f16, FP32 accumulator.
 __host__ __device__ constexpr uint32_t idesc_f16(int m, int n, bool bf16, bool b_mn_major) {
   return (1u << 4) | ((bf16 ? 1u : 0u) << 7) | ((bf16 ? 1u : 0u) << 10) | ((b_mn_major ? 1u : 0u) << 16) |
