@@ -169,25 +169,54 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kLpThreads, 1)
     *found = LpBlock{0, 0, 0, 0, -1, 0};  // a block past the last one
     fence_mbar_init();
   }
-  // The entry that the block belongs to. An entry's blocks run over some heads at a
-  // time, so that their keys and values are still in the L2 when the next block reads
-  // them, and for those from its end, the longest first.
-  {
+  // The entry that the block belongs to: those with the most keys first where there are
+  // no more than a warp has lanes, in their order otherwise. An entry's blocks run over
+  // some heads at a time, so that their keys and values are still in the L2 when the next
+  // block reads them, and for those from its end, the longest first.
+  auto bounds = [&](int e, LpBlock& b) -> int {  // of an entry, and its blocks
+    b.q_at = b.n = b.k_at = b.m = 0;
+    if (e < p.entries) {
+      b.q_at = max(__ldg(p.cu_q + e), 0);
+      b.n = max(min(__ldg(p.cu_q + e + 1), p.q_tokens) - b.q_at, 0);
+      b.k_at = min(max(__ldg(p.cu_k + e), 0), p.k_tokens);
+      b.m = max(min(__ldg(p.cu_k + e + 1), p.k_tokens) - b.k_at, 0);
+    }
+    return (b.n + L::kBlock - 1) / L::kBlock;
+  };
+  auto place = [&](int local, int blocks, LpBlock& b) {  // the entry's block `local`
+    const int first_head = local / (blocks * kLpHeads) * kLpHeads;
+    const int of_them = local - first_head * blocks, some = min(p.heads - first_head, kLpHeads);
+    b.first = (blocks - 1 - of_them / some) * L::kBlock;
+    b.head = first_head + of_them % some;
+  };
+  LpBlock b;
+  __syncwarp();
+  if (p.entries <= 32) {
+    int blocks = bounds(lane, b), before = 0;
+#pragma unroll 1
+    for (int e = 0; e < p.entries; ++e) {
+      const int keys = __shfl_sync(0xffffffffu, b.m, e), others = __shfl_sync(0xffffffffu, blocks, e);
+      before += keys > b.m || (keys == b.m && e < lane) ? others : 0;
+    }
+    const uint32_t mine =
+        __ballot_sync(0xffffffffu, at_block >= before * p.heads && at_block < (before + blocks) * p.heads);
+    const int from = mine ? __ffs(mine) - 1 : 0;
+    b.q_at = __shfl_sync(0xffffffffu, b.q_at, from);
+    b.n = __shfl_sync(0xffffffffu, b.n, from);
+    b.k_at = __shfl_sync(0xffffffffu, b.k_at, from);
+    b.m = __shfl_sync(0xffffffffu, b.m, from);
+    blocks = __shfl_sync(0xffffffffu, blocks, from);
+    before = __shfl_sync(0xffffffffu, before, from);
+    if (mine) place(at_block - before * p.heads, blocks, b);
+    else b.first = -1;
+    __syncthreads();  // the barriers are ready
+  } else {
     __shared__ int warp_sum[kLpThreads / 32];
     int before = 0;  // blocks of the entries before this round's
-    __syncwarp();
     __syncthreads();
     for (int e0 = 0; e0 < p.entries; e0 += kLpThreads) {
-      const int e = e0 + tid;
-      int q0 = 0, n = 0, k0 = 0, m = 0;
-      if (e < p.entries) {
-        q0 = max(__ldg(p.cu_q + e), 0);
-        n = max(min(__ldg(p.cu_q + e + 1), p.q_tokens) - q0, 0);
-        k0 = min(max(__ldg(p.cu_k + e), 0), p.k_tokens);
-        m = max(min(__ldg(p.cu_k + e + 1), p.k_tokens) - k0, 0);
-      }
-      const int mine = (n + L::kBlock - 1) / L::kBlock;
-      int upto = mine;
+      const int blocks = bounds(e0 + tid, b);
+      int upto = blocks;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const int v = __shfl_up_sync(0xffffffffu, upto, o);
@@ -202,22 +231,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kLpThreads, 1)
         total += warp_sum[w];
       }
       upto += before;
-      if (at_block >= (upto - mine) * p.heads && at_block < upto * p.heads) {
-        const int local = at_block - (upto - mine) * p.heads, first_head = local / (mine * kLpHeads) * kLpHeads;
-        const int of_them = local - first_head * mine, some = min(p.heads - first_head, kLpHeads);
-        LpBlock b;
-        b.q_at = q0, b.n = n, b.k_at = k0, b.m = m;
-        b.first = (mine - 1 - of_them / some) * L::kBlock;
-        b.head = first_head + of_them % some;
+      if (at_block >= (upto - blocks) * p.heads && at_block < upto * p.heads) {
+        place(at_block - (upto - blocks) * p.heads, blocks, b);
         *found = b;
       }
       before += total;
       __syncthreads();
       if (at_block < before * p.heads) break;
     }
+    b = *found;
   }
-  const LpBlock b = *found;
-  if (b.first < 0) return;  // both CTAs
+  if (b.first < 0) return;  // a block past the last one, for both CTAs
   const int head = b.head;
   bool failed = false;
   // tiles of keys that the last query of t sees
