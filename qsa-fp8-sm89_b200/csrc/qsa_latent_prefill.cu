@@ -19,8 +19,9 @@
 // even and odd tiles of keys, joined at the end.
 //
 // Softmax: a thread has a row, its scores in registers; references are lazy (a row
-// passes its own by 2^15, all that f16 weights hold, before O is rescaled), sums in
-// fp32. The first 64 weights are taken against the reference as it stands while the
+// passes its own by 2^15, all that f16 weights hold, before O is rescaled; theirs sits
+// 2^7 below the row's largest score, so that they are whole down to 2^-21 of the
+// largest), sums in fp32. The first 64 weights are taken against the reference as it stands while the
 // tile's largest score is looked for, and handed to the products while the others are
 // taken.
 //
@@ -59,7 +60,7 @@ constexpr int kLpChunk = kLpTile * 128;      // bytes of 128 tokens of 64 values
 constexpr int kLpThreads = 384;
 constexpr int kLpLoadWarp = 8, kLpMmaWarp = 9, kLpFixWarp = 10;
 constexpr int kLpHeads = 8;                   // heads whose blocks of an entry follow one another
-constexpr float kLpLazy = 15.f;              // log2 by which a score may pass its row's reference
+constexpr float kLpMost = 15.f;              // log2 of the largest weight
 constexpr float kLowest = -3.402823466e38f;
 constexpr uint64_t kLpDrainNs = 20000000ull;
 
@@ -124,6 +125,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kLpThreads, 1)
   using L = Lp<kSplit>;
   constexpr int kStages = L::kStages, kAhead = L::kAhead;
   constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
+  constexpr float kSits = kBf16 ? 0.f : 7.f;  // log2 of the largest weight where the reference has just moved
   constexpr uint32_t kExp = kBf16 ? 0x7f80u : 0x7c00u;  // exponent bits of an infinity or NaN
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_s = smem_u32(smem_raw);
@@ -183,7 +185,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kLpThreads, 1)
     }
     return (b.n + L::kBlock - 1) / L::kBlock;
   };
-  auto place = [&](int local, int blocks, LpBlock& b) {  // the entry's block `local`
+  auto place = [&](int64_t before, int blocks, LpBlock& b) {  // the block of an entry that follows so many
+    const int local = (int)(at_block - before * p.heads);
     const int first_head = local / (blocks * kLpHeads) * kLpHeads;
     const int of_them = local - first_head * blocks, some = min(p.heads - first_head, kLpHeads);
     b.first = (blocks - 1 - of_them / some) * L::kBlock;
@@ -192,14 +195,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kLpThreads, 1)
   LpBlock b;
   __syncwarp();
   if (p.entries <= 32) {
-    int blocks = bounds(lane, b), before = 0;
+    int blocks = bounds(lane, b);
+    int64_t before = 0;
 #pragma unroll 1
     for (int e = 0; e < p.entries; ++e) {
       const int keys = __shfl_sync(0xffffffffu, b.m, e), others = __shfl_sync(0xffffffffu, blocks, e);
       before += keys > b.m || (keys == b.m && e < lane) ? others : 0;
     }
-    const uint32_t mine =
-        __ballot_sync(0xffffffffu, at_block >= before * p.heads && at_block < (before + blocks) * p.heads);
+    const uint32_t mine = __ballot_sync(0xffffffffu, at_block >= before * p.heads && at_block < (before + blocks) * p.heads);
     const int from = mine ? __ffs(mine) - 1 : 0;
     b.q_at = __shfl_sync(0xffffffffu, b.q_at, from);
     b.n = __shfl_sync(0xffffffffu, b.n, from);
@@ -207,7 +210,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kLpThreads, 1)
     b.m = __shfl_sync(0xffffffffu, b.m, from);
     blocks = __shfl_sync(0xffffffffu, blocks, from);
     before = __shfl_sync(0xffffffffu, before, from);
-    if (mine) place(at_block - before * p.heads, blocks, b);
+    if (mine) place(before, blocks, b);
     else b.first = -1;
     __syncthreads();  // the barriers are ready
   } else {
@@ -231,13 +234,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kLpThreads, 1)
         total += warp_sum[w];
       }
       upto += before;
-      if (at_block >= (upto - blocks) * p.heads && at_block < upto * p.heads) {
-        place(at_block - (upto - blocks) * p.heads, blocks, b);
+      const int64_t others = upto - blocks;
+      if (at_block >= others * p.heads && at_block < (int64_t)upto * p.heads) {
+        place(others, blocks, b);
         *found = b;
       }
       before += total;
       __syncthreads();
-      if (at_block < before * p.heads) break;
+      if (at_block < (int64_t)before * p.heads) break;
     }
     b = *found;
   }
@@ -272,8 +276,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kLpThreads, 1)
     // values for the fixers land on a barrier of their own, each phase of which
     // they wait for; the products wait for the fixers then
     const bool fix = n >= fix_from;
-    mbar_expect(full + st, (n == 0 ? 3 * kLpChunk : 0) + (n < nk ? 3 * (kLpChunk / 2) : 0) + (j >= 0 && !fix ? kLpChunk : 0));
-    if (n == 0) load_queries(0, full);
+    mbar_expect(full + st, (n == 0 && nk0 > 0 ? 3 * kLpChunk : 0) + (n < nk ? 3 * (kLpChunk / 2) : 0) + (j >= 0 && !fix ? kLpChunk : 0));
+    if (n == 0 && nk0 > 0) load_queries(0, full);  // else the results' zeros are written there
     if (n < nk) {
       const int at = b.k_at + n * kLpTile + (int)rank * (kLpTile / 2);
       for (int c = 0; c < 2; ++c) tma_3d(dst + c * (kLpChunk / 2), &maps.k, full + st, 64 * c, head, at);
@@ -490,9 +494,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kLpThreads, 1)
         const float top = fmaxf(max3(tops[0], tops[1], tops[2]), tops[3]) * p.score_scale_log2;
         sum[0] = sum[1] = 0;
         weights(0);
-        const bool moves = top > r + kLpLazy;
+        const bool moves = top > r + kLpMost;
         if (!__any_sync(0xffffffffu, moves)) break;
-        const float next = moves ? top : r;
+        const float next = moves ? top - kSits : r;
         const float f = ex2(r - next);
         r = next;
         l *= f;

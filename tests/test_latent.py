@@ -911,3 +911,255 @@ def test_latent_c_abi_with_a_callers_workspace(rows):
         _check_decode(out, q, cache, btable)
     assert torch.equal(ws[need:], tail)
     assert torch.equal(out, qsa.qsa_latent_decode(q, *cache, btable, softmax_scale=0.07))
+
+
+# ------------------------------------------------------------ more of each ----
+@pytest.mark.gpu
+def test_latent_append_and_read_where_entries_end_inside_a_warps_tokens():
+    """Entries of 0 to 3 tokens, many of them, some without any, and tokens before and behind them."""
+    import qsa_b200 as qsa
+
+    gen = _gen(40)
+    counts = torch.randint(0, 4, (700,), generator=gen, device="cuda")
+    counts[:5], counts[100:140] = torch.tensor([0, 0, 1, 0, 3], device="cuda"), 0
+    cu = torch.cat([torch.full((1,), 3, device="cuda"), 3 + counts.cumsum(0)]).to(torch.int32)
+    tokens = int(cu[-1]) + 2
+    reqs = torch.randperm(700, generator=gen, device="cuda").to(torch.int32)
+    starts = torch.randint(0, 9, (700,), generator=gen, device="cuda", dtype=torch.int32)
+    btable, pool = _pages(gen, 700, 4)
+    codes, rope, scales = _filled(gen, pool, 3, 128)
+    before = codes.clone(), rope.clone(), scales.clone()
+    x = torch.randn((tokens, 192), generator=gen, device="cuda", dtype=torch.float32)
+    qsa.qsa_latent_append(x[:, :128].contiguous(), x[:, 128:].contiguous(), codes, rope, scales, btable, starts, reqs=reqs, cu_tokens=cu)
+    named, pos, slot = place = L.places(btable.cpu().numpy(), starts.cpu().numpy(), reqs.cpu().numpy(), cu.cpu().numpy(), tokens, 3, pool)
+    _check_append(before, (codes, rope, scales), np64(x[:, :128]), np64(x[:, 128:]), None, 1e-6, None, None, False, place)
+    c = torch.full((tokens, 128), 7.0, device="cuda")
+    r = torch.full((tokens, 64), 7.0, device="cuda")
+    qsa.qsa_latent_read(codes, rope, scales, btable, starts, cu, tokens, reqs=reqs, out=(c, r))
+    lat, rot = L.values(u8(codes), np64(rope), np64(scales))
+    assert named[3:-2].all() and not named[:3].any() and not named[-2:].any() and (slot[named] >= 0).all()
+    assert np.array_equal(np64(c)[named], lat.reshape(-1, 128)[slot[named]]) and np.array_equal(np64(r)[named], rot.reshape(-1, 64)[slot[named]])
+    assert (c[~torch.from_numpy(named).cuda()] == 7).all() and (r[~torch.from_numpy(named).cuda()] == 7).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads", [16, 40])
+def test_latent_decode_many_small_weights_beside_a_large_one(heads):
+    """20000 tokens of one value, each 2^-17 of one token's weight: together they are
+    13 % of the result. Weights may be rounded to 8 bits, and those that share 32
+    places with the large one to steps of 2^-15 of it; none of the others is lost."""
+    import qsa_b200 as qsa
+
+    rank, n, sink = 256, 20001, 7777
+    gen = _gen(41)
+    btable, pool = _pages(gen, 1, -(-n // 64))
+    latent = torch.zeros((n, rank), device="cuda")
+    latent[:, 0], latent[:, 5] = 0.0, 1.0
+    latent[sink, 0], latent[sink, 5] = 1.0, 0.0
+    codes, rope, scales = qsa.latent_cache(pool, 64, rank)
+    qsa.qsa_latent_append(latent, torch.zeros((n, 64), device="cuda"), codes, rope, scales, btable, i32([0]), cu_tokens=i32([0, n]))
+    q = torch.zeros((1, heads, rank + 64), device="cuda")
+    q[:, :, 0] = 17.0  # log2 of how far the sink's weight is above the others'
+    scale = float(np.log(2.0))
+    out = np64(qsa.qsa_latent_decode(q.bfloat16(), codes, rope, scales, btable, counts=i32([n]), softmax_scale=scale))
+    others = (n - 1) * 2.0 ** -17
+    want = others / (1 + others)
+    # 2^-7 for the weights in both sums, 2^-8 for the output, 31 tokens that lose all, of 20000
+    assert (np.abs(out[0, :, 5] / want - 1) <= 2.0 ** -7 + 2.0 ** -8 + 31 / 20000 + 2.0 ** -12).all(), out[0, :, 5] / want
+    assert (np.abs(out[0, :, 0] * (1 + others) - 1) <= 2.0 ** -7 + 2.0 ** -8 + 2.0 ** -12).all()
+    assert not out[0, :, 1:5].any() and not out[0, :, 6:].any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rank", RANKS)
+@pytest.mark.parametrize("order", ["rising", "falling", "steps"])
+def test_latent_decode_scores_that_move_far_from_tile_to_tile(rank, order):
+    """References pass by more than 2^60 and more than fp32's exponent range between
+    the tiles of a row, which two sets of a kernel take in turn."""
+    import qsa_b200 as qsa
+
+    gen = _gen(42)
+    n = 64 * 9 + 20
+    btable, pool = _pages(gen, 2, -(-n // 16))
+    cache = _filled(gen, pool, 16, rank, 0.5)
+    codes = cache[0].view(torch.uint8)
+    level = torch.arange(n, device="cuda") // 64 if order != "steps" else (torch.arange(n, device="cuda") // 64) % 3 * 3
+    if order == "falling":
+        level = 9 - level
+    for r in range(2):
+        at = L.slots(btable.cpu().numpy(), r, np.arange(n), 16, pool)
+        at = torch.from_numpy(np.asarray(at)).cuda()
+        codes.view(-1, rank)[at, 0] = torch.tensor([0x30 + 2 * i for i in range(10)], device="cuda", dtype=torch.uint8)[level]  # 0.5 to 2.25
+        cache[2].view(-1)[at] = 1.0
+    q = _queries(gen, 2, 1, 33, rank, 0.2)
+    q[..., 0] = 900.0
+    out = qsa.qsa_latent_decode(q, *cache, btable, counts=i32([n, n - 64]), softmax_scale=0.3)
+    _check_decode(out, q, cache, btable, counts=i32([n, n - 64]), scale=0.3)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["tree", "padded"])
+def test_latent_decode_reads_no_drafted_token_that_no_node_sees(kind):
+    import qsa_b200 as qsa
+
+    gen = _gen(43)
+    rows, nodes, heads, rank = 3, 40, 5, 384
+    counts = [100, 40, 260]
+    btable, pool = _pages(gen, rows, 20)
+    cache = _filled(gen, pool, 16, rank)
+    tree = np.zeros((rows, nodes, 2), np.int64)
+    for i in range(nodes):
+        for j in range(i + 1):
+            if j not in (3, 17, 33) and (kind == "tree" or i < 30 and j < 30):
+                tree[:, i, j // 32] |= 1 << (j % 32)
+    unseen = [3, 17, 33] if kind == "tree" else [3, 17] + list(range(30, 40))
+    for r, c in enumerate(counts):
+        at = torch.from_numpy(np.asarray(L.slots(btable.cpu().numpy(), r, np.array([c - nodes + j for j in unseen]), 16, pool))).cuda()
+        cache[0].view(torch.uint8).view(-1, rank)[at] = 0x7F
+        cache[1].view(-1, 64)[at] = float("nan")
+        cache[2].view(-1)[at] = float("inf")
+    words = torch.from_numpy(tree.astype(np.uint32).view(np.int32)).cuda()
+    q = _queries(gen, rows, nodes, heads, rank, 0.3)
+    out = qsa.qsa_latent_decode(q, *cache, btable, counts=i32(counts), tree=words, softmax_scale=0.07)
+    assert not torch.isnan(out).any()
+    _check_decode(out, q, cache, btable, counts=i32(counts), tree=words)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,heads", [(600, 3), (1100, 17), (530, 128)])
+def test_latent_decode_more_rows_than_threads_plan(rows, heads):
+    """Uneven rows, empty ones among them, shared out over all SMs; the requests' pages
+    are few, so rows share them."""
+    import qsa_b200 as qsa
+
+    gen = _gen(44)
+    btable, pool = _pages(gen, 5, 60)
+    cache = _filled(gen, pool, 16, 128)
+    counts = torch.randint(0, 70, (rows,), generator=gen, device="cuda", dtype=torch.int32)
+    counts[::7] = 0
+    counts[rows // 2] = 900  # one long row among short ones
+    counts[-1] = 640
+    t2r = torch.randint(0, 5, (rows,), generator=gen, device="cuda", dtype=torch.int32)
+    t2r[rows - 3] = 5  # past the block table
+    q = _queries(gen, rows, 1, heads, 128, 0.4)
+    out = qsa.qsa_latent_decode(q, *cache, btable, t2r, counts=counts, softmax_scale=0.07)
+    # the oracle takes a sample and the special ones
+    at = sorted(set(range(0, rows, 37)) | {rows // 2, rows - 1, rows - 3, 7, 8})
+    pick = torch.tensor(at, device="cuda")
+    _check_decode(out[pick], q[pick], cache, btable, t2r[pick], counts=counts[pick])
+    assert not out[::7][counts[::7] == 0].any()
+    again = qsa.qsa_latent_decode(q, *cache, btable, t2r, counts=counts, softmax_scale=0.07)
+    assert torch.equal(out, again)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("entries", [32, 33, 390, 1000])
+def test_latent_prefill_many_entries(entries):
+    """Around the numbers of entries that a warp and a block look through at once."""
+    import qsa_b200 as qsa
+
+    gen = _gen(45)
+    lens = torch.randint(0, 5, (entries,), generator=gen, device="cuda").tolist()
+    lens[entries // 2], lens[-1], lens[0] = 300, 70, 0
+    more = torch.randint(0, 40, (entries,), generator=gen, device="cuda").tolist()
+    cu_q = np.concatenate([[0], np.cumsum(lens)])
+    cu_k = np.concatenate([[0], np.cumsum(np.array(lens) + more)])
+    q, k, k_rope, v = _prompt(gen, int(cu_q[-1]), int(cu_k[-1]), 2, torch.bfloat16)
+    for causal in (True, False):
+        out = qsa.qsa_latent_prefill(q, k, k_rope, v, i32(cu_q), i32(cu_k), causal=causal)
+        _check_prefill(out, q, k, k_rope, v, cu_q, cu_k, causal, 192 ** -0.5)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("heads,lens,cached", [(1, [700, 30], [400, 0]), (17, [513, 255, 1], [0, 100, 700]), (90, [600], [0]),
+                                               (90, [600, 1100], [-400, -600]), (3, [600], [-400])])
+def test_latent_prefill_blocks_of_both_sizes(heads, lens, cached, dtype):
+    """Few blocks have 256 queries and share out their tiles of keys, many have 512;
+    17 and 90 heads are no multiple of those that follow one another; with fewer keys
+    than queries the first queries of a block, or half of it, see none."""
+    import qsa_b200 as qsa
+
+    gen = _gen(46)
+    cu_q = np.concatenate([[0], np.cumsum(lens)])
+    cu_k = np.concatenate([[0], np.cumsum(np.array(lens) + cached)])
+    q, k, k_rope, v = _prompt(gen, int(cu_q[-1]), int(cu_k[-1]), heads, dtype)
+    out = qsa.qsa_latent_prefill(q, k, k_rope, v, i32(cu_q), i32(cu_k), causal=True)
+    _check_prefill(out, q, k, k_rope, v, cu_q, cu_k, True, 192 ** -0.5)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("heads", [2, 90])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_latent_prefill_references_that_move(sign, heads, dtype):
+    """Scores that rise and fall by more than 2^15, and more than fp32's exponents, from
+    tile to tile; a negative scale turns them round."""
+    import qsa_b200 as qsa
+
+    gen = _gen(47)
+    n = 128 * 7 + 5
+    q, k, k_rope, v = _prompt(gen, n, n, heads, dtype)
+    q[..., 0] = 40.0
+    level = torch.tensor([0.0, 1.0, 6.0, 2.0, 2.5, 20.0, 3.0, 21.0], device="cuda")[torch.arange(n, device="cuda") // 128]
+    k = k.clone()
+    k[..., 0] = level[:, None].to(dtype)
+    out = qsa.qsa_latent_prefill(q, k, k_rope, v, i32([0, n]), i32([0, n]), causal=True, softmax_scale=sign * 0.3)
+    _check_prefill(out, q, k, k_rope, v, [0, n], [0, n], True, sign * 0.3)
+
+
+@pytest.mark.gpu
+def test_latent_prefill_two_streams_at_once():
+    import qsa_b200 as qsa
+
+    gen = _gen(48)
+    q, k, k_rope, v = _prompt(gen, 1500, 1500, 20, torch.bfloat16)
+    cu = i32([0, 400, 1500])
+    call = lambda: qsa.qsa_latent_prefill(q, k, k_rope, v, cu, cu)
+    eager = call()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        a = [call() for _ in range(4)]
+    b = [call() for _ in range(4)]
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, eager) for x in a + b)
+
+
+@pytest.fixture
+def _wait_limit():
+    from qsa_b200 import capi
+
+    capi.device_error(clear=True)
+    yield capi
+    capi.testing_set_wait_limit_ns(0)
+    capi.device_error(clear=True)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("which", ["decode", "decode shared out", "prefill", "prefill of few blocks"])
+def test_a_latent_wait_that_runs_out_is_reported_and_the_next_call_is_right(which, _wait_limit):
+    import qsa_b200 as qsa
+
+    gen = _gen(49)
+    if "decode" in which:
+        n = 5000 if "shared" in which else 300
+        btable, pool = _pages(gen, 2, -(-n // 16))
+        cache = _filled(gen, pool, 16, 512)
+        q = _queries(gen, 2, 1, 64, 512, 0.3)
+        call = lambda: qsa.qsa_latent_decode(q, *cache, btable, counts=i32([n, n - 1]), softmax_scale=0.07)
+    else:
+        n, heads = 900, 3 if "few" in which else 90
+        q, k, k_rope, v = _prompt(gen, n, n, heads, torch.bfloat16)
+        call = lambda: qsa.qsa_latent_prefill(q, k, k_rope, v, i32([0, n]), i32([0, n]))
+    want = call()
+    _wait_limit.testing_set_wait_limit_ns(1)
+    call()
+    torch.cuda.synchronize()  # the kernel returned: no hang, no fault
+    assert _wait_limit.testing_set_wait_limit_ns(0) == 1
+    assert _wait_limit.device_error() == 1
+    with pytest.raises(RuntimeError, match="device-side failure"):
+        _wait_limit.check_device_error(clear=True)
+    assert torch.equal(call(), want)
+    torch.cuda.synchronize()
+    _wait_limit.check_device_error()
