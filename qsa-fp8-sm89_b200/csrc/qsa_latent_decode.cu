@@ -937,41 +937,67 @@ __global__ void __launch_bounds__(128) qsa_latent_join_kernel(const __grid_const
   const int pairs = p.nodes * p.heads;
   if (rt * kLdPairs + pair >= pairs) return;
   wait_for_prerequisites();
-  const int2 b = p.begins[g];
+  // A load for all lanes at a time: one after the other, the pieces' loads took most of
+  // 20 us.
+  const int lane = threadIdx.x & 31;
+  auto begin_of = [&](int at) { return at < p.groups ? p.begins[at] : make_int2(-1, 0); };
+  int2 e = begin_of(g - 1 + lane);
+  const int2 b = make_int2(__shfl_sync(0xffffffffu, e.x, 1), __shfl_sync(0xffffffffu, e.y, 1));
   if (b.x >= p.rows || b.y == 0) return;
-  const int2 before = p.begins[g - 1];
+  const int2 before = make_int2(__shfl_sync(0xffffffffu, e.x, 0), __shfl_sync(0xffffffffu, e.y, 0));
   if (before.x == b.x && before.y > 0) return;  // the row's second piece lies further back
-  int last = g;
-  while (last + 1 < p.groups) {
-    const int2 e = p.begins[last + 1];
-    if (e.x != b.x || e.y == 0) break;
-    ++last;
+  if (lane == 0) e = b;  // looked at, as group g's is
+  int last = g - 1;      // of the row's groups
+  for (;;) {
+    const uint32_t others = __ballot_sync(0xffffffffu, e.x != b.x || e.y == 0);
+    if (others) {
+      last += __ffs(others) - 2;
+      break;
+    }
+    last += 32;
+    e = begin_of(last + lane);
   }
   // pieces: the second of group g - 1, the first of groups g .. last
   auto place = [&](int i) { return ((int64_t)(i == 0 ? 2 * g - 1 : 2 * (g + i - 1)) * p.row_tiles + rt) * kLdPairs + pair; };
   const int pieces = last - g + 2;
   float top = -INFINITY;
   bool nan = false;
-  for (int i = 0; i < pieces; ++i) {
+  float first_v = -INFINITY;
+  for (int i = lane; i < pieces; i += 32) {
     const float v = p.part_lse[place(i)];
+    if (i == lane) first_v = v;
     top = fmaxf(top, v);
     nan = nan || v != v;
   }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  nan = __any_sync(0xffffffffu, nan);
   const int rank = p.cache.rank;
   const int d = 4 * threadIdx.x;
-  if (d >= rank) return;
+  if (d >= rank) return;  // whole warps
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
   float sum = 0.f;
   if (top > -INFINITY || nan) {
-#pragma unroll 4
-    for (int i = 0; i < pieces; ++i) {
-      const int64_t at = place(i);
-      const float v = p.part_lse[at];
-      if (v == -INFINITY) continue;
-      const float w = exp2f(v - top);
-      const float4 x = *reinterpret_cast<const float4*>(p.part_o + at * rank + d);
-      sum += w;
-      o.x = fmaf(w, x.x, o.x), o.y = fmaf(w, x.y, o.y), o.z = fmaf(w, x.z, o.z), o.w = fmaf(w, x.w, o.w);
+    for (int first = 0; first < pieces; first += 32) {
+      // a piece without a visible token has written no results
+      const float v = first == 0 ? first_v : first + lane < pieces ? p.part_lse[place(first + lane)] : -INFINITY;
+      const float mine = v == -INFINITY ? 0.f : exp2f(v - top);
+#pragma unroll 1
+      for (int k = 0; k < min(32, pieces - first); k += 4) {
+        float w[4];
+        float4 x[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          w[j] = __shfl_sync(0xffffffffu, mine, k + j);
+          x[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (w[j] != 0.f) x[j] = *reinterpret_cast<const float4*>(p.part_o + place(first + k + j) * rank + d);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          sum += w[j];
+          o.x = fmaf(w[j], x[j].x, o.x), o.y = fmaf(w[j], x[j].y, o.y), o.z = fmaf(w[j], x[j].z, o.z), o.w = fmaf(w[j], x[j].w, o.w);
+        }
+      }
     }
     const float inv = 1.0f / sum;
     o.x *= inv, o.y *= inv, o.z *= inv, o.w *= inv;
@@ -1019,7 +1045,7 @@ cudaError_t launch(const LatentDecodeParams& p, cudaStream_t stream) {
   e = start(qsa_latent_prepare_kernel<kChunks>, dim3((unsigned)blocks), kLpreThreads, 0, false, stream, p);
   if (e == cudaSuccess) e = start(qsa_latent_decode_kernel<kChunks>, dim3((unsigned)grid), kLdThreads, kLdSmem, true, stream, p);
   if (e == cudaSuccess && p.planned && p.groups > 1)
-    e = start(qsa_latent_join_kernel, dim3(kLdPairs, (unsigned)p.row_tiles, (unsigned)(p.groups - 1)), 128, 0, true, stream, p);
+    e = start(qsa_latent_join_kernel, dim3((unsigned)(p.nodes * p.heads < kLdPairs ? p.nodes * p.heads : kLdPairs), (unsigned)p.row_tiles, (unsigned)(p.groups - 1)), 128, 0, true, stream, p);
   return e;
 }
 
