@@ -21,10 +21,10 @@ extern "C" {
 #endif
 
 /* Sets the limit, in nanoseconds, of every pipeline wait of the tensor-core
- * decode kernel launched from now on in this process (0 restores the
- * default of 1 s); returns the previous limit. A CTA whose wait runs out
+ * decode, latent decode and latent prefill kernels launched from now on in this
+ * process (0 restores the default of 1 s); returns the previous limit. A CTA whose wait runs out
  * records code 1 in the device error word (qsa_b200_device_error), waits
- * (with the 1 s limit) for its own copies and MMAs in flight, frees its
+ * (with a limit of its own) for its copies and MMAs in flight, frees its
  * tensor memory and returns; its outputs are then undefined. Process-wide;
  * meant for tests only. */
 QSA_B200_TESTING_API uint64_t qsa_b200_testing_set_wait_limit_ns(uint64_t ns);

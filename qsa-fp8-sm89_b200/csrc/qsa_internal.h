@@ -72,7 +72,7 @@ struct DecodeParams {
 
   int* err;  // device error word of the current device
   // Limit of each pipeline wait of the tensor-core kernel, in ns of
-  // globaltimer: 1 s, unless the test hook qsa_b200_testing_set_wait_limit_ns
+  // globaltimer (the latent kernels count tries of a wait by it): 1 s, unless the test hook qsa_b200_testing_set_wait_limit_ns
   // shortened it. A CTA whose wait runs out sets err and returns.
   uint64_t wait_limit_ns;
 };

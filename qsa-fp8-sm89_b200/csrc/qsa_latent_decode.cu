@@ -18,8 +18,10 @@
 //                   way; P is two E4M3 terms a weight. A transposed O takes 256
 //                   columns of tensor memory for 64 pairs (O itself would need
 //                   all 512 for its 128 lanes).
+//
 // q: the terms are exact for a bf16 value within 2^13 of the head's largest and
 // off by 2^-21 of the largest at most below.
+//
 // P: with s_t a weight on the codes is w_t = 2^(score_t + log2 s_t - r). Each 32
 // tokens of a pair have a power of two of their own, which the product applies
 // (block scales), with their largest weight brought to 2^7 .. 2^8: a weight is
@@ -49,6 +51,13 @@
 // read the same tokens run side by side) has an even share of all rows' tiles: at
 // most two pieces of rows and any whole rows between. Pieces are joined by their
 // log-sums in a last kernel. Few short rows are a CTA each.
+//
+// Measured at a rank of 512: 8 contexts of 90001 to 131072 tokens, 16 heads, 164 us (3.5
+// TB/s; the main kernel 141); 32 of 4096 to 8192, 128 heads, 102 us (540 TFLOP/s); 16
+// trees of 24 nodes and 16 heads 108 us; 256 rows of 512 selected tokens, 32 heads, 59
+// us; 4 rows of 64 tokens 12.3 us. A tile takes a set some 3300 cycles of softmax, more
+// than twice what the same steps take in a loop by themselves: the roles' code is more
+// than the instruction caches hold.
 //
 // Every wait is bounded; a CTA that gives up records it in the device error word,
 // waits for its own copies and products, frees its tensor memory and returns.

@@ -215,7 +215,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kLpThreads, 1)
     __syncthreads();  // the barriers are ready
   } else {
     __shared__ int warp_sum[kLpThreads / 32];
-    int before = 0;  // blocks of the entries before this round's
+    int before = 0;  // blocks of the entries looked through
     __syncthreads();
     for (int e0 = 0; e0 < p.entries; e0 += kLpThreads) {
       const int blocks = bounds(e0 + tid, b);
@@ -667,7 +667,7 @@ cudaError_t launch(const LatentPrefillParams& p, int64_t blocks, cudaStream_t st
 cudaError_t launch_latent_prefill(const LatentPrefillParams& p, cudaStream_t stream) {
   // An entry's blocks are its length over theirs, rounded up. Large blocks bring keys
   // and values for twice the queries, but a pair of SMs each has to have some: 8192
-  // tokens take 136 us in large and 83 in small blocks of 4 heads (64 large ones), 138
+  // tokens take 136 us in large and 82 in small blocks of 4 heads (64 large ones), 138
   // and 130 of 6, 140 and 159 of 8, 276 and 305 of 16; five chunks of up to 700 over up
   // to 2700 keys, 16 heads, 76 and 61.
   const int64_t most = p.entries < p.q_tokens ? p.entries : p.q_tokens;
