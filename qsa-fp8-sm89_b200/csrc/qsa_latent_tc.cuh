@@ -69,14 +69,6 @@ __device__ __forceinline__ void mma_f8_ss_plain_a(uint32_t d, uint32_t a, uint32
       "r"(accumulate), "n"(kDescHigh), "n"(kDescHighPlain)
       : "memory");
 }
-__device__ __forceinline__ void mma_f16_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n.reg .pred p, e;\nelect.sync _|e, 0xffffffff;\nsetp.ne.b32 p, %4, 0;\n"
-      ".reg .b64 bd;\nmov.b64 bd, {%2, %5};\n"
-      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], bd, %3, p;\n}\n" ::"r"(d), "r"(a), "r"(b), "r"(idesc),
-      "r"(accumulate), "n"(kDescHigh)
-      : "memory");
-}
 __device__ __forceinline__ void mma_f16_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
       "{\n.reg .pred p, e;\nelect.sync _|e, 0xffffffff;\nsetp.ne.b32 p, %4, 0;\n"
