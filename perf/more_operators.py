@@ -36,21 +36,13 @@ E_LOW, E_HIGH = -60, 60
 DTYPES = {"bf16": torch.bfloat16, "f16": torch.float16, "f32": torch.float32}
 
 
-_loaded = None
-
-
 def _package():
-    """The framework, looked for once as a program's import does: the search of its folder takes 28 us."""
-    global _loaded
-    if _loaded is not None:
-        return _loaded
     root = str(Path(__file__).resolve().parents[1] / "qsa-fp8-sm89_b200")
     if root not in sys.path:
         sys.path.insert(0, root)
     import qsa_b200
 
-    _loaded = qsa_b200
-    return _loaded
+    return qsa_b200
 
 
 # ------------------------------------------------------------------ cases ----
