@@ -29,11 +29,12 @@
 // and to steps of 2^-17 of it below. One scale for all tokens would lose what many
 // small weights add up to beside a few large ones (E4M3 ends at 2^-9). The sum of
 // weights takes the bf16 value, so that most of this rounding cancels in the
-// quotient: l = sum w_t / s_t, in fp32; scales within 2^-60 .. 2^60 keep it in range.
+// quotient: l = sum w_t / s_t, in fp32. With scales within 2^-60 .. 2^60, weights up to
+// 2^32 (below) and 2^31 tokens at most it stays under 2^(32 + 60 + 31) = 2^123.
 // (The conversions to E4M3 share a unit with 2^x that they kept 94 % busy: the terms
 // are cut out of the fp32 weights by integer operations instead.)
 // r is the largest score + log2 s of the first tile that has one. It moves, and O
-// with it, only when a tile passes it by 2^60; each set tells the other its r, tile
+// with it, only when a tile passes it by 2^32; each set tells the other its r, tile
 // by tile.
 //
 // Tiles of 64 tokens go in turn to two sets of warps, each with a ring, scores and
@@ -83,7 +84,7 @@ constexpr int kLdLoader0 = 8, kLdFenceWarp = 13, kLdWeighWarp = 14, kLdMmaWarp =
 constexpr int kLdThreads = 512;
 constexpr int64_t kLdDirectTiles = 8;  // tiles of a row that is not split
 constexpr float kLdOne = 8.f;    // log2 that bounds the largest weight of 32
-constexpr float kLdFar = 60.f;   // log2 by which a weight may pass the reference
+constexpr float kLdFar = 32.f;   // log2 by which a weight may pass the reference: the sum of weights has to stay in fp32
 constexpr float kLdNear = -110.f;  // log2 below it under which 32 weights get no smaller scale
 constexpr float kLowest = -3.402823466e38f;
 constexpr uint64_t kLdDrainNs = 1000000000ull;

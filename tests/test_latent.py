@@ -1163,3 +1163,35 @@ def test_a_latent_wait_that_runs_out_is_reported_and_the_next_call_is_right(whic
     assert torch.equal(call(), want)
     torch.cuda.synchronize()
     _wait_limit.check_device_error()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rank", [128, 512])
+@pytest.mark.parametrize("rows,n", [(2, 512), (2, 6000), (400, 1500)])
+def test_latent_decode_tokens_of_the_least_scale_whose_scores_rise(rows, n, rank):
+    """All scales are 2^-60, and from the second tile on scores lie 2^59.5 above the
+    first tile's: a sum of weights over scales, taken against the first tile's largest,
+    would pass 2^128. Rows that one block has to itself, rows in pieces, and many rows
+    shared out. The first tile's weights are 2^-59.5 of the others: below every bound."""
+    import qsa_b200 as qsa
+
+    gen = _gen(60)
+    reqs, heads = min(rows, 3), 4
+    btable, pool = _pages(gen, reqs, -(-n // 64))
+    cache = qsa.latent_cache(pool, 64, rank)
+    latent = 2.0 ** -55 * (1 + torch.rand((reqs * n, rank), generator=gen, device="cuda"))
+    rotated = torch.zeros((reqs * n, 64), device="cuda")
+    rotated[:, 0] = torch.where(torch.arange(n, device="cuda").repeat(reqs) < 64, 0.0, 59.5)
+    qsa.qsa_latent_append(latent, rotated, *cache, btable, i32([0] * reqs), cu_tokens=i32([n * i for i in range(reqs + 1)]))
+    q = torch.zeros((rows, heads, rank + 64), device="cuda")
+    q[:, :, rank] = torch.tensor([1.0, 0.5, 0.984375, 0.0], device="cuda")
+    t2r = i32([i % reqs for i in range(rows)])
+    scale = float(np.log(2.0))
+    out = qsa.qsa_latent_decode(q.bfloat16(), *cache, btable, t2r, counts=i32([n] * rows), softmax_scale=scale)
+    assert (cache[2].view(-1)[torch.from_numpy(L.slots(btable.cpu().numpy(), 0, np.arange(n), 64, pool)).cuda()] == 2.0 ** -60).all()
+    _check_decode(out[:3], q[:3].bfloat16(), cache, btable, t2r[:3], counts=i32([n] * min(rows, 3)), scale=scale)
+    # every row has its request's result, however the work was shared out: each is within
+    # the bound above, with values above zero 2^-13 * 41.3 + 2^-7 + 2^-8 of it, twice under 2^-4
+    got = np64(out)
+    want = got[:reqs][np.arange(rows) % reqs]
+    assert (np.abs(got - want) <= 2.0 ** -4 * want).all() and (want > 0).all()
