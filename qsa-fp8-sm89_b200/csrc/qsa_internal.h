@@ -281,7 +281,7 @@ struct LatentDecodeParams {
   int64_t* total;     // tiles of all rows
   int2* begins;       // [groups] row and tile that each group begins with
   float* part_o;      // [2 groups, row_tiles, 64, rank] results of pieces of rows
-  float* part_lse;    // [2 groups, row_tiles, 64] their log2-sum-exp2, -inf for none
+  float* part_lse;    // [2 groups, row_tiles, 64] their log2-sum-exp2 less 30, -inf for none
   int* err;
   uint64_t wait_limit_ns;
 };

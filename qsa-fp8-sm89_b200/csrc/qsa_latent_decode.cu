@@ -29,12 +29,15 @@
 // and to steps of 2^-17 of it below. One scale for all tokens would lose what many
 // small weights add up to beside a few large ones (E4M3 ends at 2^-9). The sum of
 // weights takes the bf16 value, so that most of this rounding cancels in the
-// quotient: l = sum w_t / s_t, in fp32. With scales within 2^-60 .. 2^60, weights up to
-// 2^32 (below) and 2^31 tokens at most it stays under 2^(32 + 60 + 31) = 2^123.
+// quotient: l = sum w_t / s_t, in fp32. A row's largest weight is 1 to 2^60 (below), scales
+// are 2^-60 .. 2^60 and tokens 2^31 at most, so that l is 2^-60 to 2^151: it is held
+// times 2^-30, by the 1 / s that go into it, and results are brought back by as much
+// after their division. (A margin that keeps l itself in range, 2^32, was passed so
+// often that 32 contexts of 128 heads took 112 us instead of 99.)
 // (The conversions to E4M3 share a unit with 2^x that they kept 94 % busy: the terms
 // are cut out of the fp32 weights by integer operations instead.)
 // r is the largest score + log2 s of the first tile that has one. It moves, and O
-// with it, only when a tile passes it by 2^32; each set tells the other its r, tile
+// with it, only when a tile passes it by 2^60; each set tells the other its r, tile
 // by tile.
 //
 // Tiles of 64 tokens go in turn to two sets of warps, each with a ring, scores and
@@ -84,12 +87,13 @@ constexpr int kLdLoader0 = 8, kLdFenceWarp = 13, kLdWeighWarp = 14, kLdMmaWarp =
 constexpr int kLdThreads = 512;
 constexpr int64_t kLdDirectTiles = 8;  // tiles of a row that is not split
 constexpr float kLdOne = 8.f;    // log2 that bounds the largest weight of 32
-constexpr float kLdFar = 32.f;   // log2 by which a weight may pass the reference: the sum of weights has to stay in fp32
+constexpr float kLdFar = 60.f;   // log2 by which a weight may pass the reference
+constexpr float kLdSum = 0x1p-30f;  // what the sum of weights is held times
 constexpr float kLdNear = -110.f;  // log2 below it under which 32 weights get no smaller scale
 constexpr float kLowest = -3.402823466e38f;
 constexpr uint64_t kLdDrainNs = 1000000000ull;
 
-// Scales of a tile: s, log2 s, 1 / s, in two halves of 32 tokens that a lane pair
+// Scales of a tile: s, log2 s, kLdSum / s, in two halves of 32 tokens that a lane pair
 // reads at once, apart by a bank group.
 constexpr int kLdHalf = 36;
 struct LdMeta {
@@ -366,7 +370,7 @@ __global__ void __launch_bounds__(kLdThreads, 1) qsa_latent_decode_kernel(const 
           metas[m].s[at] = s;
           metas[m].lg[at] = slot < 0 ? -INFINITY : log2f(s);
           // a NaN token is a NaN in the weights of those that see it, and nothing in the others'
-          metas[m].inv[at] = slot < 0 || s != s ? 0.f : 1.0f / s;
+          metas[m].inv[at] = slot < 0 || s != s ? 0.f : kLdSum / s;
           __syncwarp();
           if (lane == 0) mbar_arrive(meta_full + m);
         }
@@ -799,6 +803,8 @@ __global__ void __launch_bounds__(kLdThreads, 1) qsa_latent_decode_kernel(const 
           for (int j = 0; j < 16; j += 4) {
             const float4 f = *reinterpret_cast<const float4*>(head_f + b + j);
             x[j] *= f.x, x[j + 1] *= f.y, x[j + 2] *= f.z, x[j + 3] *= f.w;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[j + i] *= kLdSum;
           }
           const int some = mine - b;
 #pragma unroll
