@@ -104,7 +104,7 @@ constexpr int kLdBarSet = 1, kLdBarAll = 3;  // named barriers: of a set (1, 2),
 
 // A block of 16 pairs' queries: words [rank / 16][32 lanes][4] for tensor memory (a
 // pair's first terms in lane 2 i, its second ones in 2 i + 1), bf16 [16][64] rotated
-// ones, float [16] what a product is to be multiplied by.
+// ones, float [16] what a product is to be multiplied by (-0: the query is not finite).
 constexpr int kLdBlockPairs = 16;
 __host__ __device__ constexpr int ld_block_bytes(int rank) { return 32 * rank + 16 * 128 + 256; }
 
@@ -777,6 +777,7 @@ __global__ void __launch_bounds__(kLdThreads, 1) qsa_latent_decode_kernel(const 
       const int piece = 2 * group + (now.from > 0 ? 0 : 1);
       if (live && !odd && set == 0) {
         l += head_f[pair];
+        if (__float_as_uint(km) == 0x80000000u && l != 0.f) l = __int_as_float(0x7fffffff);  // a query that is not finite
         head_f[pair] = l == 0.f ? 0.f : 1.0f / l;
         if (!now.whole && pair < mine)
           p.part_lse[((int64_t)piece * p.row_tiles + rt) * kLdPairs + pair] = l == 0.f ? -INFINITY : log2f(l) + r;
@@ -876,7 +877,15 @@ __global__ void __launch_bounds__(kLpreThreads) qsa_latent_prepare_kernel(const 
     a = min(max(a, -120), 120);
     const float up = __uint_as_float((uint32_t)(127 + a) << 23);
     float qs = pair < pairs ? __uint_as_float((uint32_t)(127 - a) << 23) * p.score_scale_log2 : 0.f;
-    if (t >= 0x7f80 || u >= 0x7f80) qs = __int_as_float(0x7fffffff);  // an infinity or NaN
+    qs += 0.f;  // no -0 but this one:
+    if (t >= 0x7f80 || u >= 0x7f80 || !(fabsf(qs) <= 3.402823466e38f)) {
+      // a pair that is NaN where it sees a token and zeros where it sees none: the factor
+      // -0 tells, and zeros for its values leave the masks of its scores as they are
+      qs = -0.f;
+#pragma unroll
+      for (int i = 0; i < kChunks; ++i) raw[i] = make_uint2(0u, 0u);
+      rot = 0;
+    }
 #pragma unroll
     for (int i = 0; i < kChunks; ++i) {
       const uint32_t v[2] = {raw[i].x, raw[i].y};

@@ -1195,3 +1195,41 @@ def test_latent_decode_tokens_of_the_least_scale_whose_scores_rise(rows, n, rank
     got = np64(out)
     want = got[:reqs][np.arange(rows) % reqs]
     assert (np.abs(got - want) <= 2.0 ** -4 * want).all() and (want > 0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("columns", [70, 3000])
+@pytest.mark.parametrize("heads", [3, 70])
+def test_latent_decode_queries_that_are_not_finite(heads, columns):
+    """NaN for a head that sees a token, zeros for one that sees none, and nothing of it
+    in the other heads: selections without a token, contexts without a page, trees whose
+    node sees nothing."""
+    import qsa_b200 as qsa
+
+    gen = _gen(61)
+    rows, rank = 4, 256
+    btable, pool = _pages(gen, rows, -(-columns // 16))
+    cache = _filled(gen, pool, 16, rank)
+    q = _queries(gen, rows, 1, heads, rank, 0.3)
+    clean = q.clone()
+    for r, (h, at, x) in enumerate([(0, 5, "nan"), (heads - 1, rank + 40, "inf"), (1, 0, "-inf"), (2, rank, "nan")]):
+        q[r, h, at] = float(x)
+    bad = torch.isnan(q - q).any(-1)
+    indices = torch.arange(columns, device="cuda", dtype=torch.int32).repeat(rows, 1)
+    indices[1] = -1
+    indices[2, 1:] = -1
+    out = qsa.qsa_latent_decode(q, *cache, btable, None, indices, softmax_scale=0.07)
+    seen = torch.tensor([True, False, True, True], device="cuda")
+    assert not out[1].any()
+    assert torch.equal(torch.isnan(out).any(-1), bad & seen[:, None]) and torch.equal(torch.isnan(out).all(-1), bad & seen[:, None])
+    ref = qsa.qsa_latent_decode(clean, *cache, btable, None, indices, softmax_scale=0.07)
+    assert torch.equal(out[~bad], ref[~bad])
+    gone = btable.clone()
+    gone[0] = -1
+    out = qsa.qsa_latent_decode(q, *cache, gone, softmax_scale=0.07)
+    assert not out[0].any() and torch.equal(torch.isnan(out).all(-1), bad & (torch.arange(rows, device="cuda") > 0)[:, None])
+    # two nodes that are all there is: the second one's bits are empty
+    nodes = torch.stack([q, q], 1).contiguous()
+    tree = torch.tensor([1, 0], dtype=torch.int32, device="cuda").repeat(rows, 1).view(rows, 2, 1).contiguous()
+    out = qsa.qsa_latent_decode(nodes, *cache, btable, counts=i32([2] * rows), tree=tree, softmax_scale=0.07)
+    assert not out[:, 1].any() and torch.equal(torch.isnan(out[:, 0]).all(-1), bad)
