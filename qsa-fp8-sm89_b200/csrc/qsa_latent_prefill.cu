@@ -147,7 +147,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kLpThreads, 1)
   uint64_t* drain = o_full + 2;
   uint32_t* tmem_at = reinterpret_cast<uint32_t*>(smem + L::kMisc);
   const uint32_t tries = tries_of(p.wait_limit_ns);
-  volatile int* odd_values = reinterpret_cast<volatile int*>(smem + L::kMisc + 12);  // values that were cleared
+  volatile int* stages_loaded = reinterpret_cast<volatile int*>(smem + L::kMisc + 8);  // as far as the loader has come
+  volatile int* odd_values = reinterpret_cast<volatile int*>(smem + L::kMisc + 12);    // values that were cleared
   LpBlock* found = reinterpret_cast<LpBlock*>(smem + L::kMisc + 16);
 
   const int at_block = (int)(blockIdx.x >> 1);
@@ -167,6 +168,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kLpThreads, 1)
     }
     mbar_init(q1_full, both);
     mbar_init(drain, 1);
+    *stages_loaded = 0;
     *odd_values = 0;
     *found = LpBlock{0, 0, 0, 0, -1, 0};  // a block past the last one
     fence_mbar_init();
@@ -315,6 +317,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kLpThreads, 1)
         failed = !wait_tries(empty + loaded % kStages, parity_of(loaded - kStages), tries);
         if (failed) break;
         load(loaded);
+        *stages_loaded = loaded;
       }
       const int n = loaded;
       // all copies have landed before the block leaves (the usual end: the products took them)
@@ -392,7 +395,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kLpThreads, 1)
       for (int j = whole; j < nk; ++j) {
         bool any = false;
         const int st = (j + kAhead) % kStages;
-        failed = !__all_sync(0xffffffffu, wait_tries(v_here + st, parity_of(j - whole), tries));
+        // the first comes when all whole tiles have gone through: the limit is for a time
+        // in which the loader has not brought another stage
+        for (int seen = __shfl_sync(0xffffffffu, *stages_loaded, 0);;) {
+          failed = !__all_sync(0xffffffffu, wait_tries(v_here + st, parity_of(j - whole), tries));
+          const int now = __shfl_sync(0xffffffffu, *stages_loaded, 0);
+          if (!failed || now == seen) break;
+          seen = now;
+        }
         if (failed) break;
         uint8_t* v = smem + L::kRing + st * L::kStage + L::kV;
 #pragma unroll 4

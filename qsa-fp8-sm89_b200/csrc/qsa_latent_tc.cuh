@@ -24,17 +24,19 @@ __device__ __forceinline__ bool bar_vote(int id, int count, bool pred) {
   return r != 0u;
 }
 
-// Bounded wait: false once `tries` looks at the barrier, of 20 ns or more each, have
-// not seen the phase end. It is this short because it stands in so many places: the
-// roles' code together is more than the instruction caches hold. (A try with a time to
-// sleep wakes up to 2 us after its barrier.)
+// Bounded wait: false once `tries` looks at the barrier have not seen the phase end. A
+// look that finds nothing took 4 us where a whole warp looks (the instruction itself
+// waits) and 0.1 us where one lane of a warp does. It is this short because it stands in
+// so many places. (A look with a time to sleep wakes up to 2 us after its barrier.) A wait
+// is for one step of the work, some microseconds; one that may take longer counts its
+// looks anew with each step.
 __device__ __forceinline__ bool wait_tries(uint64_t* bar, uint32_t parity, uint32_t tries) {
 #pragma unroll 1
   for (uint32_t i = 0; !mbar_try_wait(bar, parity); ++i)
     if (i >= tries) return false;
   return true;
 }
-// Tries that a limit in ns allows.
+// Tries that a limit in ns allows: they take a tenth of it to four times as long.
 __device__ __forceinline__ uint32_t tries_of(uint64_t limit_ns) { return (uint32_t)(limit_ns / 1024 < 0x7fffffffu ? limit_ns / 1024 : 0x7fffffffu); }
 
 // Descriptors of 128-byte swizzled operands whose 8-row groups lie 1024 bytes

@@ -1233,3 +1233,30 @@ def test_latent_decode_queries_that_are_not_finite(heads, columns):
     tree = torch.tensor([1, 0], dtype=torch.int32, device="cuda").repeat(rows, 1).view(rows, 2, 1).contiguous()
     out = qsa.qsa_latent_decode(nodes, *cache, btable, counts=i32([2] * rows), tree=tree, softmax_scale=0.07)
     assert not out[:, 1].any() and torch.equal(torch.isnan(out[:, 0]).all(-1), bad)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads,queries,keys", [(1, 100, 300005), (130, 300, 150005)])
+def test_latent_prefill_waits_are_for_a_step_and_not_for_a_block(heads, queries, keys, _wait_limit):
+    """A limit of 300 looks (30 us of one thread, 1.2 ms of a warp) is ample for every step
+    of a block, and less than a block over so many keys takes: 2 ms. Heads lie one behind
+    the other in the same memory."""
+    import qsa_b200 as qsa
+
+    gen = _gen(62)
+    base = torch.randn((keys + heads, 128), generator=gen, device="cuda").to(torch.bfloat16)
+    k = base.as_strided((keys, heads, 128), (128, 128, 1))
+    k_rope = torch.randn((keys, 64), generator=gen, device="cuda").to(torch.bfloat16)
+    q = torch.randn((queries, heads, 192), generator=gen, device="cuda").to(torch.bfloat16)
+    cu_q, cu_k = [0, queries], [0, keys]
+    call = lambda: qsa.qsa_latent_prefill(q, k, k_rope, k, i32(cu_q), i32(cu_k))
+    want = call()
+    _wait_limit.testing_set_wait_limit_ns(300 * 1024)
+    out = call()
+    torch.cuda.synchronize()
+    assert _wait_limit.device_error() == 0
+    assert torch.equal(out, want)
+    at, rows = sorted({0, heads // 2, heads - 1}), [0, queries // 2, queries - 1]
+    for i in rows:  # a query alone, over the keys that it sees
+        n = keys - (queries - 1 - i)
+        _check_prefill(out[i:i + 1, at], q[i:i + 1, at], k[:n, at], k_rope[:n], k[:n, at], [0, 1], [0, n], True, 192 ** -0.5)
