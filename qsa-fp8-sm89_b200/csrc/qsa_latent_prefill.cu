@@ -334,6 +334,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kLpThreads, 1)
         tc_fence_after();
         return true;
       };
+      // what the other CTA's threads tell of its shared memory
+      auto wait_pair = [&](uint64_t* bar, uint32_t parity) -> bool {
+        if (!__all_sync(0xffffffffu, cluster_wait_tries(bar, parity, tries))) return false;
+        tc_fence_after();
+        return true;
+      };
       auto scores = [&](int t, int st) {  // S_t = Q_t K^T
         const uint32_t a0 = desc_low(base_s) + (kSplit ? 0 : t) * 3 * (kLpChunk / 16);
         const uint32_t b0 = desc_low(base_s + L::kRing) + st * (L::kStage / 16);
@@ -363,8 +369,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kLpThreads, 1)
         for (int t = 0; t < 2 && !failed; ++t) {
           const int tiles = t == 0 ? nk0 : nk1, n = key_of(t, i) + kAhead, st = n % kStages;
           if (i < tiles && tiles > 0) {
-            failed = !wait(full + st, parity_of(n)) || (!kSplit && t == 1 && i < 0 && !wait(q1_full, 0u)) ||
-                     (n >= fix_from && !__all_sync(0xffffffffu, cluster_wait_tries(fixed + st, parity_of(n - fix_from), tries))) ||
+            failed = !wait_pair(full + st, parity_of(n)) || (!kSplit && t == 1 && i < 0 && !wait_pair(q1_full, 0u)) ||
+                     (n >= fix_from && !wait_pair(fixed + st, parity_of(n - fix_from))) ||
                      (i >= 0 && !weigh(t, i, st));
             if (failed) break;
             if (i + 1 < tiles) scores(t, st);

@@ -1260,3 +1260,23 @@ def test_latent_prefill_waits_are_for_a_step_and_not_for_a_block(heads, queries,
     for i in rows:  # a query alone, over the keys that it sees
         n = keys - (queries - 1 - i)
         _check_prefill(out[i:i + 1, at], q[i:i + 1, at], k[:n, at], k_rope[:n], k[:n, at], [0, 1], [0, n], True, 192 ** -0.5)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("entries,length", [(6, 1500)])
+def test_latent_prefill_gives_the_same_again_and_again(entries, length):
+    """Blocks of two CTAs that hand memory to one another, several on each SM in turn:
+    every call's bits are the first one's, and those are the formula's."""
+    import qsa_b200 as qsa
+
+    gen = _gen(63)
+    heads = 24
+    cu = [length * i for i in range(entries + 1)]
+    q, k, k_rope, v = _prompt(gen, cu[-1], cu[-1], heads, torch.bfloat16)
+    call = lambda: qsa.qsa_latent_prefill(q, k, k_rope, v, i32(cu))
+    want = call()
+    for _ in range(40):
+        assert torch.equal(call(), want)
+    n = min(length, 300)
+    at = [0, 7, heads - 1]
+    _check_prefill(want[:n, at], q[:n, at], k[:n, at], k_rope[:n], v[:n, at], [0, n], [0, n], True, 192 ** -0.5)
