@@ -392,6 +392,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kLpThreads, 1)
           tell(full + n % kStages, parity_of(n));
           if (n == 0 && queries1) tell(q1_full, 0u);
         }
+        // the products' arrivals here have come before the block leaves its memory
+        if (!mbar_wait_bounded(drain, 0u, kLpDrainNs)) failed = true;
       }
     } else if (warp >= kLpFixWarp) {
       // ====================== values that must not count ====================

@@ -1263,7 +1263,7 @@ def test_latent_prefill_waits_are_for_a_step_and_not_for_a_block(heads, queries,
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("entries,length", [(6, 1500)])
+@pytest.mark.parametrize("entries,length", [(6, 1500), (300, 5)])
 def test_latent_prefill_gives_the_same_again_and_again(entries, length):
     """Blocks of two CTAs that hand memory to one another, several on each SM in turn:
     every call's bits are the first one's, and those are the formula's."""
