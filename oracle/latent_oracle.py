@@ -111,7 +111,10 @@ def decode(q, codes, rope, scales, btable, t2r=None, indices=None, counts=None, 
     [nodes, heads, rank]; ``size``, the average of |value| by the same weights;
     ``score``, the largest sum of absolute terms of a score [nodes, heads];
     ``low``, the largest weight on the codes times the sum of |codes| over the
-    columns [nodes, heads, rank]."""
+    columns [nodes, heads, rank]; ``low32``, the same of each 32 columns, summed
+    over them; ``spread``, what independent relative errors of variance 1 of the
+    weights give the average: the sum of (weight (value - out))^2; ``steps``, the
+    same of errors of each 32 columns' largest weight on the codes."""
     rows, nodes, heads, _ = q.shape
     pages, page, rank = codes.shape
     lat, rot = values(codes, rope, scales)
@@ -154,7 +157,14 @@ def decode(q, codes, rope, scales, btable, t2r=None, indices=None, counts=None, 
         with np.errstate(invalid="ignore"):
             on_codes = np.where((p > 0) & np.isfinite(s), p * s, 0.0)  # of a head with a NaN weight nothing is compared
         low = on_codes.max(-1)[..., None] * codes_abs.sum(0)
-        res.append(dict(out=mix(p, c0), size=mix(p, np.abs(c0)), score=np.where(ok[:, None], terms, 0.0).max(-1), low=low))
+        cuts = np.flatnonzero(np.diff(np.flatnonzero(any_col) // 32, prepend=-1))  # where another 32 columns begin
+        largest = np.maximum.reduceat(on_codes, cuts, axis=-1)
+        low32 = np.einsum("nhb,bd->nhd", largest, np.add.reduceat(codes_abs, cuts, axis=0))
+        steps = np.einsum("nhb,bd->nhd", largest ** 2, np.add.reduceat(codes_abs ** 2, cuts, axis=0))
+        out, p0 = mix(p, c0), np.where(np.isnan(p), 0.0, p) ** 2
+        spread = np.einsum("nht,td->nhd", p0, c0 ** 2) - 2 * out * np.einsum("nht,td->nhd", p0, c0) + out ** 2 * p0.sum(-1)[..., None]
+        res.append(dict(out=out, size=mix(p, np.abs(c0)), score=np.where(ok[:, None], terms, 0.0).max(-1), low=low, low32=low32,
+                        spread=spread, steps=steps))
     return res
 
 

@@ -1280,3 +1280,88 @@ def test_latent_prefill_gives_the_same_again_and_again(entries, length):
     n = min(length, 300)
     at = [0, 7, heads - 1]
     _check_prefill(want[:n, at], q[:n, at], k[:n, at], k_rope[:n], v[:n, at], [0, n], [0, n], True, 192 ** -0.5)
+
+
+def test_oracle_steps_of_each_32_columns():
+    codes = np.zeros((5, 16, 128), np.uint8)
+    codes[..., 0] = 0x38  # 1.0
+    scales = np.ones((5, 16))
+    rope = np.zeros((5, 16, 64))
+    rope[2, 3, 0] = 1.0  # column 35
+    q = np.zeros((1, 1, 1, 192))
+    q[..., 128] = np.log(3.0)
+    w = L.decode(q, codes, rope, scales, np.arange(5)[None], counts=[70])[0]
+    total = 69 + 3
+    assert np.allclose(w["low32"][0, 0, 0], (32 * 1 + 32 * 3 + 6 * 1) / total) and np.allclose(w["low"][0, 0, 0], 70 * 3 / total)
+    assert np.allclose(w["spread"][0, 0], 0.0) and np.allclose(w["out"][0, 0, 0], 1.0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("spread", ["even", "scales", "scores", "far scales", "sink"])
+@pytest.mark.parametrize("heads,columns", [(12, 4000), (70, 700)])
+def test_latent_decode_loses_no_weight_beside_a_larger_one_of_other_columns(heads, columns, spread):
+    """The steps of small weights are those of the largest of their 32 columns, not of the
+    row: the bound of `_check_decode` with `low32` for `low`. And errors are no larger in
+    the mean square than independent roundings of weights and output to 8 bits make them,
+    each with a variance of 2^-16 / 3 at most relative to its value, steps of (2^-16)^2 / 3
+    of the 32 columns' largest weight, and 2^-13 of a score's terms, which moves each
+    token's weight for itself."""
+    import qsa_b200 as qsa
+
+    gen = _gen(64)
+    rows, rank = 2, 512
+    btable, pool = _pages(gen, rows, -(-columns // 64))
+    codes, rope, scales = _filled(gen, pool, 64, rank)
+    q = _queries(gen, rows, 1, heads, rank, 0.3)
+    if spread == "scales":
+        scales = torch.exp2((torch.randn((pool, 64), generator=gen, device="cuda") * 5).round() - 9)
+    elif spread == "scores":
+        q = (q * 30).to(torch.bfloat16)
+    elif spread == "far scales":
+        scales = torch.where(torch.rand((pool, 64), generator=gen, device="cuda") < 0.3, 2.0 ** -60, scales)
+    rope = (torch.randn(rope.shape, generator=gen, device="cuda") / scales[..., None]).to(torch.bfloat16)
+    if spread == "sink":  # one token with 2^14 times the weight of the others
+        rope[:] = 0
+        at = L.slots(btable.cpu().numpy(), 0, [columns // 2], 64, pool)[0]
+        q[..., rank:], q[..., :rank] = 0, q[..., :rank] * 0.25
+        q[..., rank] = 16.0
+        rope.view(-1, 64)[at, 0] = 14 * np.log(2.0) / 0.07 / 16 / float(scales.view(-1)[at])
+    counts = i32([columns, columns - 77])
+    out = qsa.qsa_latent_decode(q, codes, rope, scales, btable, counts=counts, softmax_scale=0.07)
+    host = [u8(codes), np64(rope), np64(scales), btable.cpu().numpy()]
+    want = L.decode(np64(q[:, None]), *host, counts=counts.cpu().numpy(), softmax_scale=0.07)
+    for r, w in enumerate(want):
+        err = np.abs(np64(out)[r] - w["out"][0])
+        score = w["score"][0][..., None]
+        bound = (2.0 ** -13 * score + 2.0 ** -7) * w["size"][0] + 2.0 ** -16 * w["low32"][0] + 2.0 ** -8 * np.abs(w["out"][0])
+        bad = ~(err <= bound + 2.0 ** -133)
+        assert not bad.any(), (r, np.argwhere(bad)[:4].tolist(), err[bad][:4], bound[bad][:4])
+        mean = 2.0 ** -16 / 3 * (w["out"][0] ** 2 + w["spread"][0]) + 2.0 ** -32 / 3 * w["steps"][0] + 2.0 ** -26 * score ** 2 * w["spread"][0]
+        assert (err ** 2).mean() <= mean.mean()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("heads,queries,keys", [(2, 300, 900), (80, 512, 512)])
+def test_latent_prefill_errors_are_those_of_its_roundings(heads, queries, keys, dtype):
+    """In the mean too: weights and output, each rounded to the type with a variance of
+    a third of the square of half a step, and 2^-15 of a score's terms, which moves each
+    weight for itself."""
+    import qsa_b200 as qsa
+
+    gen = _gen(65)
+    q, k, k_rope, v = _prompt(gen, queries, keys, heads, dtype)
+    out = qsa.qsa_latent_prefill(q, k, k_rope, v, i32([0, queries]), i32([0, keys]))
+    rel = ROUND[dtype][0]
+    for h in (0, heads - 1):
+        want, size, score, _ = L.prefill(np64(q[:, [h]]), np64(k[:, [h]]), np64(k_rope), np64(v[:, [h]]), [0, queries], [0, keys], True,
+                                         192 ** -0.5)
+        key = np.concatenate([np64(k[:, h]), np64(k_rope)], 1)
+        s = np64(q[:, h]) @ key.T * 192 ** -0.5
+        s = np.where(np.arange(keys)[None] <= np.arange(queries)[:, None] + keys - queries, s, -np.inf)
+        p = np.exp(s - s.max(1, keepdims=True))
+        p /= p.sum(1, keepdims=True)
+        err = np64(out[:, h]) - want[:, 0]
+        moved = p ** 2 @ np64(v[:, h]) ** 2
+        mean = rel ** 2 / 3 * (want[:, 0] ** 2 + moved) + 2.0 ** -30 * score ** 2 * moved
+        assert (err ** 2).mean() <= mean.mean()
