@@ -123,11 +123,11 @@ __device__ __forceinline__ uint2 quantise8(float (&v)[8], float s, float inv, bo
 #pragma unroll
     for (int d = 0; d < 8; ++d) v[d] = fabsf(v[d]) > FLT_MAX ? v[d] : divide(v[d], s, inv);
   } else {
-    const uint64_t by = pair(inv, inv), back = pair(-s, -s);  // divide()'s steps, two at a time
+    const uint64_t by = pair2(inv, inv), back = pair2(-s, -s);  // divide()'s steps, two at a time
 #pragma unroll
     for (int d = 0; d < 8; d += 2) {
-      const uint64_t x = pair(v[d], v[d + 1]), q = mul2(x, by);
-      unpair(fma2(fma2(q, back, x), by, q), v[d], v[d + 1]);
+      const uint64_t x = pair2(v[d], v[d + 1]), q = mul2(x, by);
+      unpair2(fma2(fma2(q, back, x), by, q), v[d], v[d + 1]);
     }
   }
   return make_uint2(to_e4m3(v), to_e4m3(v + 4));

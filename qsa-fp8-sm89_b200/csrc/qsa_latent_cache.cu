@@ -73,7 +73,7 @@ __global__ void __launch_bounds__(32 * kLcWarps) qsa_latent_append_kernel(const 
         latent_load4(static_cast<const __half*>(p.c_weight) + 128 * i + 4 * lane, w);
       else
         latent_load4(static_cast<const __nv_bfloat16*>(p.c_weight) + 128 * i + 4 * lane, w);
-      weight[i][0] = pair(w[0], w[1]), weight[i][1] = pair(w[2], w[3]);
+      weight[i][0] = pair2(w[0], w[1]), weight[i][1] = pair2(w[2], w[3]);
     }
   }
   float cs[kLcTokens], sn[kLcTokens];
@@ -95,7 +95,7 @@ __global__ void __launch_bounds__(32 * kLcWarps) qsa_latent_append_kernel(const 
     for (int i = 0; i < kChunks; ++i) {
       float x[4];
       latent_widen(words[k][i], x, T());
-      y[i][0] = pair(x[0], x[1]), y[i][1] = pair(x[2], x[3]);
+      y[i][0] = pair2(x[0], x[1]), y[i][1] = pair2(x[2], x[3]);
     }
     float u = latent_to_float(us[k]), v = latent_to_float(vs[k]);
 
@@ -104,7 +104,7 @@ __global__ void __launch_bounds__(32 * kLcWarps) qsa_latent_append_kernel(const 
 #pragma unroll
       for (int i = 0; i < kChunks; ++i) sums = fma2(y[i][1], y[i][1], fma2(y[i][0], y[i][0], sums));
       float sum, odd;
-      unpair(sums, sum, odd);
+      unpair2(sums, sum, odd);
       sum += odd;
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
@@ -117,7 +117,7 @@ __global__ void __launch_bounds__(32 * kLcWarps) qsa_latent_append_kernel(const 
 #pragma unroll
       for (int i = 0; i < kChunks; ++i)
 #pragma unroll
-        for (int j = 0; j < 2; ++j) y[i][j] = mul2(mul2(y[i][j], pair(r, r)), weight[i][j]);
+        for (int j = 0; j < 2; ++j) y[i][j] = mul2(mul2(y[i][j], pair2(r, r)), weight[i][j]);
     }
     float part[2] = {0.f, 0.f};
 #pragma unroll
@@ -125,7 +125,7 @@ __global__ void __launch_bounds__(32 * kLcWarps) qsa_latent_append_kernel(const 
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         float a, d;
-        unpair(y[i][j], a, d);
+        unpair2(y[i][j], a, d);
         part[j] = max3_nan(part[j], fabsf(a), fabsf(d));
       }
     // bits of values without a sign are in the values' order, those of a NaN above all
@@ -138,7 +138,7 @@ __global__ void __launch_bounds__(32 * kLcWarps) qsa_latent_append_kernel(const 
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           float a, d;
-          unpair(y[i][j], a, d);
+          unpair2(y[i][j], a, d);
           if (fabsf(a) <= 3.402823466e38f) of = fmaxf(of, fabsf(a));
           if (fabsf(d) <= 3.402823466e38f) of = fmaxf(of, fabsf(d));
         }
@@ -151,8 +151,8 @@ __global__ void __launch_bounds__(32 * kLcWarps) qsa_latent_append_kernel(const 
 #pragma unroll
     for (int i = 0; i < kChunks; ++i) {
       float2 lo, hi;
-      unpair(mul2(y[i][0], pair(inv, inv)), lo.x, lo.y);
-      unpair(mul2(y[i][1], pair(inv, inv)), hi.x, hi.y);
+      unpair2(mul2(y[i][0], pair2(inv, inv)), lo.x, lo.y);
+      unpair2(mul2(y[i][1], pair2(inv, inv)), hi.x, hi.y);
       const uint32_t codes = (uint32_t)__nv_cvt_float2_to_fp8x2(lo, __NV_SATFINITE, __NV_E4M3) |
                              (uint32_t)__nv_cvt_float2_to_fp8x2(hi, __NV_SATFINITE, __NV_E4M3) << 16;
       *reinterpret_cast<uint32_t*>(dst + 128 * i) = nan ? 0u : codes;

@@ -205,7 +205,7 @@ __global__ void __launch_bounds__(kLdThreads, 1) qsa_latent_decode_kernel(const 
   uint32_t* tmem_at = reinterpret_cast<uint32_t*>(smem + kLdMisc);
   const uint32_t tries = tries_of(p.wait_limit_ns);
   int* begin = reinterpret_cast<int*>(smem + kLdMisc + 16);          // row, tile
-  int64_t* share = reinterpret_cast<int64_t*>(smem + kLdMisc + 24);  // first unit, units
+  int64_t* share = reinterpret_cast<int64_t*>(smem + kLdMisc + 24);  // tiles
   LdMeta* metas = reinterpret_cast<LdMeta*>(smem + kLdMetaAt);
   float* head_f = reinterpret_cast<float*>(smem + kLdRow);
   float* pair_r = reinterpret_cast<float*>(smem + kLdRef);
@@ -258,9 +258,9 @@ __global__ void __launch_bounds__(kLdThreads, 1) qsa_latent_decode_kernel(const 
       const int2 b = p.begins[group];
       const int64_t total = *p.total, groups = min((int64_t)p.groups, total);
       begin[0] = b.x, begin[1] = b.y;
-      share[1] = group < groups ? total * (group + 1) / groups - total * group / groups : 0;
+      *share = group < groups ? total * (group + 1) / groups - total * group / groups : 0;
     } else {
-      share[1] = ld_tiles(p, group);
+      *share = ld_tiles(p, group);
     }
   }
   __syncwarp();
@@ -268,7 +268,7 @@ __global__ void __launch_bounds__(kLdThreads, 1) qsa_latent_decode_kernel(const 
   tc_fence_after();
   constexpr uint32_t tmem = 0;  // all of it is this block's
   LdWalk walk;
-  walk.row = begin[0], walk.from = begin[1], walk.left = share[1];
+  walk.row = begin[0], walk.from = begin[1], walk.left = *share;
   bool failed = false;
 
   if (warp >= kLdLoader0 && warp < kLdLoader0 + 4) {

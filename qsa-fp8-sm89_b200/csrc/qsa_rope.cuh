@@ -14,6 +14,7 @@
 #include <type_traits>
 
 #include "../../include/qsa_b200.h"
+#include "qsa_common.cuh"
 #include "qsa_internal.h"
 
 namespace qsa {
@@ -103,26 +104,6 @@ __device__ __forceinline__ void load_weight8(const void* weight, int dtype, Piec
   }
 }
 
-// Two fp32 operations an instruction; each half is rounded as by itself.
-__device__ __forceinline__ uint64_t pair(float a, float b) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};\n" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ void unpair(uint64_t v, float& a, float& b) {
-  asm("mov.b64 {%0, %1}, %2;\n" : "=f"(a), "=f"(b) : "l"(v));
-}
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("mul.rn.f32x2 %0, %1, %2;\n" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;\n" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-
 // x *= rsqrt(mean(x^2) + eps) * w over the half warp's 128 elements, for N rows
 // whose exchanges run side by side. Every lane goes through them; where `norms` is
 // false it keeps its rows.
@@ -134,11 +115,11 @@ __device__ __forceinline__ void rms_norm8(float (&x)[N][8], const float (&w)[8],
     uint64_t sum = 0;
 #pragma unroll
     for (int i = 0; i < 8; i += 2) {
-      const uint64_t v = pair(x[n][i], x[n][i + 1]);
+      const uint64_t v = pair2(x[n][i], x[n][i + 1]);
       sum = fma2(v, v, sum);
     }
     float even, odd;
-    unpair(sum, even, odd);
+    unpair2(sum, even, odd);
     s[n] = even + odd;
   }
 #pragma unroll
@@ -156,7 +137,7 @@ __device__ __forceinline__ void rms_norm8(float (&x)[N][8], const float (&w)[8],
     if (!norms) r = 1.f;
 #pragma unroll
     for (int i = 0; i < 8; i += 2)
-      unpair(mul2(mul2(pair(x[n][i], x[n][i + 1]), pair(r, r)), pair(w[i], w[i + 1])), x[n][i], x[n][i + 1]);
+      unpair2(mul2(mul2(pair2(x[n][i], x[n][i + 1]), pair2(r, r)), pair2(w[i], w[i + 1])), x[n][i], x[n][i + 1]);
   }
 }
 
@@ -210,10 +191,10 @@ __device__ __forceinline__ void turn_row(const float4& c, const float4& s, bool 
     if (turns && kTurn == kHalves) {
 #pragma unroll
       for (int i = 0; i < 4; i += 2) {
-        const uint64_t u = pair(x[i], x[i + 1]), v = pair(x[4 + i], x[5 + i]);
-        const uint64_t co = pair(cc[i], cc[i + 1]);
-        unpair(fma2(u, co, mul2(v, pair(-ss[i], -ss[i + 1]))), x[i], x[i + 1]);
-        unpair(fma2(v, co, mul2(u, pair(ss[i], ss[i + 1]))), x[4 + i], x[5 + i]);
+        const uint64_t u = pair2(x[i], x[i + 1]), v = pair2(x[4 + i], x[5 + i]);
+        const uint64_t co = pair2(cc[i], cc[i + 1]);
+        unpair2(fma2(u, co, mul2(v, pair2(-ss[i], -ss[i + 1]))), x[i], x[i + 1]);
+        unpair2(fma2(v, co, mul2(u, pair2(ss[i], ss[i + 1]))), x[4 + i], x[5 + i]);
       }
     } else if (turns) {
 #pragma unroll

@@ -1365,3 +1365,16 @@ def test_latent_prefill_errors_are_those_of_its_roundings(heads, queries, keys, 
         moved = p ** 2 @ np64(v[:, h]) ** 2
         mean = rel ** 2 / 3 * (want[:, 0] ** 2 + moved) + 2.0 ** -30 * score ** 2 * moved
         assert (err ** 2).mean() <= mean.mean()
+
+
+def test_device_helpers_have_one_definition():
+    """Headers that a source may include together define no helper twice."""
+    import re
+    from pathlib import Path
+
+    seen = {}
+    for path in sorted((Path(__file__).resolve().parents[1] / "qsa-fp8-sm89_b200" / "csrc").glob("*.cuh")):
+        for name, params in re.findall(r"__device__ __forceinline__ [\w:<>]+ (\w+)\(([^)]*)\)", path.read_text()):
+            types = re.sub(r"\b\w+\s*(?=,|$)", "", params).replace(" ", "")
+            assert seen.setdefault((name, types), path.name) == path.name, (name, path.name, seen[name, types])
+    assert ("fma2", "uint64_t,uint64_t,uint64_t") in seen
