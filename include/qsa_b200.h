@@ -497,7 +497,8 @@ QSA_B200_API int64_t qsa_b200_latent_decode_workspace_bytes(const qsa_b200_laten
  * qsa_b200_decode negative ones and ones on a page outside the table or the
  * cache) do not count, and what the cache holds there is not read, apart from
  * tokens that another node of the row sees. A node without a visible token
- * gives zeros. The workspace needs no clearing and may be reused by the next
+ * gives zeros; a head whose query has an infinity or NaN gives NaN where it sees
+ * a token. The workspace needs no clearing and may be reused by the next
  * call on the same stream. Needs 16-byte aligned tensors. Asynchronous on
  * `stream`. */
 QSA_B200_API int qsa_b200_latent_decode(const qsa_b200_latent_decode_args* args, void* workspace, size_t workspace_bytes,

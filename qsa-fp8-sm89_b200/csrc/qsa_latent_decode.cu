@@ -56,12 +56,14 @@
 // most two pieces of rows and any whole rows between. Pieces are joined by their
 // log-sums in a last kernel. Few short rows are a CTA each.
 //
-// Measured at a rank of 512: 8 contexts of 90001 to 131072 tokens, 16 heads, 164 us (3.5
-// TB/s; the main kernel 141); 32 of 4096 to 8192, 128 heads, 102 us (540 TFLOP/s); 16
+// Measured at a rank of 512: 8 contexts of 90001 to 131072 tokens, 16 heads, 163 us (3.5
+// TB/s; the main kernel 141); 32 of 4096 to 8192, 128 heads, 104 us (530 TFLOP/s); 16
 // trees of 24 nodes and 16 heads 108 us; 256 rows of 512 selected tokens, 32 heads, 59
-// us; 4 rows of 64 tokens 12.3 us. A tile takes a set some 3300 cycles of softmax, more
-// than twice what the same steps take in a loop by themselves: the roles' code is more
-// than the instruction caches hold.
+// us; 4 rows of 64 tokens 13 us. A tile takes a set some 3300 cycles of softmax, more
+// than twice what the same steps take in a loop by themselves. On the trees a warp's
+// time goes to loads and barrier looks (27 % of it), fixed latencies (18 %) and named
+// barriers (12 %), waits of the roles for one another among them; instructions that are
+// not there yet are 5 %.
 //
 // Every wait is bounded; a CTA that gives up records it in the device error word,
 // waits for its own copies and products, frees its tensor memory and returns.
@@ -85,7 +87,11 @@ constexpr int kLdLoader0 = 8, kLdFenceWarp = 13, kLdWeighWarp = 14, kLdMmaWarp =
 // of the fence with an idle one. The softmax takes registers that the others hand back:
 // 2 x 160 + 96 + 96 of the 4 x 128 that the block is launched with.
 constexpr int kLdThreads = 512;
-constexpr int64_t kLdDirectTiles = 8;  // tiles of a row that is not split
+// Tiles of a row that is not split, where there is an SM for each. One CTA a row against
+// rows shared out, 16 heads, us: 8 tiles, 1 row 18.4 and 15.8, 4 rows 18.0 and 16.6, 32
+// rows 18.2 and 21.6, 74 rows 18.8 and 19.4, 140 rows 20.5 and 30.9; 4 tiles, 1 row 13.7
+// and 14.7, 140 rows 15.5 and 24.4; 16 tiles, 1 row 27.5 and 18.2, 32 rows 27.4 and 23.6.
+constexpr int64_t kLdDirectTiles = 8;
 constexpr float kLdOne = 8.f;    // log2 that bounds the largest weight of 32
 constexpr float kLdFar = 60.f;   // log2 by which a weight may pass the reference
 constexpr float kLdSum = 0x1p-30f;  // what the sum of weights is held times
@@ -415,7 +421,7 @@ __global__ void __launch_bounds__(kLdThreads, 1) qsa_latent_decode_kernel(const 
           if (failed) break;
           const uint32_t d = tmem + kLdTmemS + set * kLdTile;
           int s = set ? slot[1] : slot[0];
-          // rolled: the roles' code together is more than the instruction caches hold
+          // rolled: the roles' code together is large
 #pragma unroll 1
           for (int c = 0; c < kChunks; ++c) {
             const uint32_t bd = ring + (set * kLdSlots + s) * (kLdSlot / 16);
@@ -839,8 +845,8 @@ __global__ void __launch_bounds__(kLdThreads, 1) qsa_latent_decode_kernel(const 
 
 // The queries as the products take them, 16 pairs a block and a pair a warp: q 2^a =
 // t0 + t1 / 16 in E4M3, with 2^a taking the largest latent query into [128, 256) as
-// far as the rotated ones stay far from bf16's end. The block past those shares out
-// the tiles.
+// far as the rotated ones stay far from bf16's end. A block before those shares out the
+// tiles where the rows are shared out.
 constexpr int kLpreThreads = 32 * kLdBlockPairs;
 template <int kChunks>
 __global__ void __launch_bounds__(kLpreThreads) qsa_latent_prepare_kernel(const __grid_constant__ LatentDecodeParams p) {

@@ -10,8 +10,12 @@
 // latency was what bounded the products, at 2250 cycles for a tile whose products
 // take 1280.
 //   S_t = Q_t K^T   256 x 128 x 192, both from shared memory
-//   O_t += P_t V    256 x 128 x 128, P (rounded to the inputs' type, the usual
-//                   choice: its sum is taken in fp32) over S in tensor memory
+//   O_t += P_t V    256 x 128 x 128, P over S in tensor memory, rounded to the
+//                   inputs' type: the products take nothing wider beside V, and a
+//                   second term would double them. Its sum takes the unrounded
+//                   weights: over values of either sign the rounded ones would
+//                   cancel little of it. Errors (rms, relative) are 0.0021 in bf16,
+//                   of which the output's own rounding is 0.0016; f16 0.00025, 0.0002.
 // t counts two such pairs of S and O, which take all 512 columns of tensor memory: the
 // softmax of one runs while the products of the other do, in the order
 // O_0(j) S_0(j+1) O_1(j) S_1(j+1). A block has 512 queries, 256 for each t, that share
@@ -31,8 +35,9 @@
 // them at the end (two warps look for them while the scores are under way).
 //
 // Between the CTAs: a thread of the odd one tells the even one's products what its
-// copies have brought. Where only tensor memory is handed over, ordered by the tcgen05
-// fences, arrivals are relaxed.
+// copies have brought (released and acquired at the cluster's scope), and stays until
+// the products' last arrivals have come. Where only tensor memory is handed over,
+// ordered by the tcgen05 fences, arrivals are relaxed.
 //
 // Measured: 16384 tokens, 16 heads, causal: 1.01 ms, 1370 TFLOP/s, a turn of t at 1760
 // cycles with 1280 of products: the softmax (125 for the scores, 840 to the first

@@ -129,12 +129,14 @@ def qsa_latent_decode(q, codes, rope, scales, btable, t2r=None, indices=None, *,
             ``nodes`` of its ``counts[r]`` tokens. Each sees the tokens before
             them and, of the nodes, those whose bit (j % 32 of word j // 32)
             is set; its own bit is an ancestor's like the others. None: a
-            chain, node i sees nodes 0 to i.
+            chain, node i sees nodes 0 to i. With one node it is not looked
+            at: that node sees all its tokens.
         softmax_scale: as of the expanded form, such as ``192 ** -0.5``.
         out: optional bf16 output ``[rows, (nodes,) heads, rank]``.
 
     Masked entries (as in ``qsa_decode``) do not count; a node without a
-    visible token gives zeros. Returns ``out``.
+    visible token gives zeros; a head whose query has an infinity or NaN gives
+    NaN where it sees a token. Returns ``out``.
     """
     if out is None:
         return _op("latent_decode")(q, codes, rope, scales, btable, t2r, indices, counts, tree, softmax_scale)
