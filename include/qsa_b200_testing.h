@@ -25,8 +25,7 @@ extern "C" {
  * process (0 restores the default of 1 s); returns the previous limit. The
  * latent kernels count looks at a barrier, one for each 1024 ns, of 0.1 us (one
  * thread's) to 4 us (a warp's): their waits last a tenth of the limit to four
- * times as long. A limit is for one step of a kernel, however long its sequences
- * are. A CTA whose wait runs out
+ * times as long, each for one step, however long the sequences are. A CTA whose wait runs out
  * records code 1 in the device error word (qsa_b200_device_error), waits
  * (with a limit of its own) for its copies and MMAs in flight, frees its
  * tensor memory and returns; its outputs are then undefined. Process-wide;

@@ -67,7 +67,8 @@ constexpr int kLpLoadWarp = 8, kLpMmaWarp = 9, kLpFixWarp = 10;
 constexpr int kLpHeads = 8;                   // heads whose blocks of an entry follow one another
 constexpr float kLpMost = 15.f;              // log2 of the largest weight
 constexpr float kLowest = -3.402823466e38f;
-constexpr uint64_t kLpDrainNs = 20000000ull;
+constexpr uint64_t kLpDrainNs = 20000000ull;  // for copies, whose announcement a failure can keep from coming
+constexpr uint64_t kLpDoneNs = 1000000000ull;  // for the products' last arrivals, which always come
 
 // Queries of a block, and shared memory: [Q tiles][3 chunks], then the stages. Stage n
 // brings what a turn needs: keys n (3 half chunks) and values n - kAhead (one chunk).
@@ -384,7 +385,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kLpThreads, 1)
           if (kSplit ? n < stages : t == 1) pair_commit(empty + st);  // the last to use it
         }
       pair_commit(drain);
-      if (!mbar_wait_bounded(drain, 0u, kLpDrainNs)) failed = true;
+      if (!mbar_wait_bounded(drain, 0u, kLpDoneNs)) failed = true;
     } else if (warp == kLpMmaWarp && nk > 0) {
       // ================== this CTA's copies, told to the products =================
       auto tell = [&](uint64_t* bar, uint32_t parity) {
@@ -398,7 +399,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kLpThreads, 1)
           if (n == 0 && queries1) tell(q1_full, 0u);
         }
         // the products' arrivals here have come before the block leaves its memory
-        if (!mbar_wait_bounded(drain, 0u, kLpDrainNs)) failed = true;
+        if (!mbar_wait_bounded(drain, 0u, kLpDoneNs)) failed = true;
       }
     } else if (warp >= kLpFixWarp) {
       // ====================== values that must not count ====================
